@@ -25,6 +25,9 @@ RQ_HMATH_SPLIT16, RQ_HMATH_FP32, RQ_HMATH_SPLIT16X3 = 0, 1, 2
 RQ_NOALLOC_SCRATCH_BYTES = 128 << 20
 RQ_CHOL_MAXBATCH = 64          # matrices per rq_chol_hinv_attempt call
 RQ_ACT_ORDER_MAXC = 65536      # widest rq_act_order_perm
+RQ_PACKED_MAXBITS = 9          # widest fields the products with packed weights take
+RQ_MOE_MAX_EXPERTS, RQ_MOE_MAX_TOP = 1024, 64
+RQ_SCORE_MAX_TOP = 64          # alternatives of rq_token_logprobs
 # g_update_mode -> (kernel mode of the in-block loop, kernel mode of the trailing update);
 # gptq_plus_utils.py:1190 (inner) and :1500 (outer)
 GMODES = {"frozen": (RQ_GMODE_FROZEN, RQ_GMODE_FROZEN),
@@ -34,6 +37,12 @@ GMODES = {"frozen": (RQ_GMODE_FROZEN, RQ_GMODE_FROZEN),
           "block_backward": (RQ_GMODE_SURROGATE_ONLINE, RQ_GMODE_FROZEN)}
 
 _P, _I, _L, _D = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_double
+
+class PackedExperts(ctypes.Structure):
+    """``rq_packed_experts``: one linear of every expert of a layer."""
+    _fields_ = [("qweight", _P), ("scales", _P), ("g_idx", _P), ("ldp", _L), ("lds", _L), ("stride_q", _L),
+                ("stride_scales", _L), ("nbits", _I), ("ngroups", _I), ("groupsize", _I)]
+
 
 # name -> (restype, argtypes); mirrors include/gptqplus_hip.h
 SIGNATURES = {
@@ -69,6 +78,14 @@ SIGNATURES = {
     "rq_hessian_reg_gemm": (_I, [_P, _L, _P, _I, _I, _I, _I, _P, _L, _P]),
     "rq_block_gd_step": (_I, [_P, _L, _I, _I, _I, _I, _P, _L, _P, _I, _I, _D, _D, _P, _P, _P, _I, _D,
                               _P, _L, _P, _L, _I, _P, _P, _P, _I, _I, _D, _D, _D, _P, _P]),
+    "rq_packed_linear": (_I, [_P, _I, _I, _L, _I, _P, _L, _I, _I, _P, _L, _I, _P, _I, _P, _P, _L, _P]),
+    "rq_packed_linear_grad_workspace_bytes": (_L, [_I, _I, _I]),
+    "rq_packed_linear_grad": (_I, [_P, _I, _I, _L, _I, _P, _L, _I, _I, _P, _L, _I, _P, _I, _P, _L, _P, _L, _P]),
+    "rq_packed_moe_workspace_bytes": (_L, [_I, _I, _I, _I, _I]),
+    "rq_packed_moe": (_I, [_P, _I, _I, _L, _I, _P, _L, _I, _I, _I, _I, _P, _P, _P, _P, _L, _P, _P, _P, _L, _P]),
+    "rq_token_logprobs_workspace_bytes": (_L, [_L, _I, _I]),
+    "rq_token_logprobs": (_I, [_P, _I, _L, _L, _I, _P, _L, _I, _P, _P, _P, _P, _P, _P, _L, _P]),
+    "rq_token_logprobs_grad": (_I, [_P, _I, _L, _L, _I, _P, _L, _P, _P, _P, _P, _L, _P]),
 }
 
 _lib = None

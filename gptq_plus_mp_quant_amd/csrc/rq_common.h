@@ -131,3 +131,13 @@ template <>
 __device__ __forceinline__ __hip_bfloat16 rq_cast<__hip_bfloat16>(float v) { return __float2bfloat16(v); }
 template <>
 __device__ __forceinline__ float rq_cast<float>(float v) { return v; }
+
+// A float as an unsigned key of the same order: -0 equals +0, every NaN is above +inf.
+__device__ __forceinline__ uint32_t rq_order_key(float v) {
+  if (v != v) return 0xFFFFFFFFu;
+  const uint32_t b = __float_as_uint(v == 0.0f ? 0.0f : v);
+  return (b & 0x80000000u) ? ~b : b | 0x80000000u;
+}
+__device__ __forceinline__ float rq_key_value(uint32_t k) {
+  return __uint_as_float((k & 0x80000000u) ? (k == 0xFFFFFFFFu ? 0x7FC00000u : k & 0x7FFFFFFFu) : ~k);
+}

@@ -13,6 +13,8 @@ form of the same information, on the GPU:
 * ``scales`` -- float32 [ngroups, R]: one row per scale group (per-channel: 1 group;
   static groups: the C/groupsize column groups; dynamic groups: one per block).
 * ``g_idx`` -- int32 [C]: the scale group of every natural column.
+* ``groupsize`` -- only where the groups are runs of natural columns (``g_idx[c] == c // groupsize``;
+  C for per-channel scales): lets ``packed_linear`` and ``packed_moe`` do without ``g_idx``.
 
 ``dequantize_packed`` (``rq_unpack_dequant``) rebuilds the layer weight bit for bit.
 ``save_packed`` / ``load_packed`` store entries and quantizer states with safetensors, so
@@ -37,7 +39,7 @@ def _nbits(bits: int, sym: bool) -> int:
 
 def export_packed(gptq) -> Dict[str, object]:
     """Pack a ``GPTQPlus`` after ``fasterquant``.  Returns ``{"qweight", "scales", "g_idx",
-    "nbits", "bits", "sym", "shape", "dtype"}``; raises if a code does not fit ``nbits``."""
+    "nbits", "bits", "sym", "shape", "dtype"}`` and, for runs of columns, ``"groupsize"``; raises if a code does not fit ``nbits``."""
     codes = getattr(gptq, "_codes_perm", None)
     if codes is None:
         raise RuntimeError("export_packed needs the codes of fasterquant (call it before free())")
@@ -46,27 +48,34 @@ def export_packed(gptq) -> Dict[str, object]:
     dev = codes.device
     nbits = _nbits(q.bits, bool(q.sym))
     invperm = gptq.invperm
+    groupsize = 0
     if gptq.qmode == nat.RQ_QMODE_CHANNEL:
         scales = gptq.scale_table.reshape(1, R)
         g_idx = torch.zeros(C, dtype=torch.int32, device=dev)
+        groupsize = C
     elif gptq.qmode == nat.RQ_QMODE_STATIC:
         # a scale table indexed by col_group[j] for the (permuted) column j: natural column c
         # reads col_group[invperm[c]] (GPTQ+ static groups give c // groupsize; classic GPTQ's
         # dynamic groups follow the permuted order)
         scales = gptq.scale_table
         g_idx = gptq.col_group[invperm] if invperm is not None else gptq.col_group
+        groupsize = gptq.groupsize_used if invperm is None or gptq.groups_natural else 0
     else:
         # dynamic groups: one scale per block of the (permuted) column order
         scales = gptq.dyn_scale
         j = invperm if invperm is not None else torch.arange(C, device=dev)
         g_idx = (j // gptq.blocksize_used).to(torch.int32)
+        groupsize = gptq.blocksize_used if invperm is None else 0
     flag = torch.zeros(1, dtype=torch.int32, device=dev)
     qweight = K.pack_codes(codes, nbits, invperm=invperm, range_flag=flag)
     if int(flag.item()):
         raise ValueError(f"a code does not fit {nbits} bits (NaN weight or inconsistent quantizer)")
-    return dict(qweight=qweight, scales=scales.contiguous(), g_idx=g_idx.contiguous(), nbits=nbits,
-                bits=int(q.bits), sym=bool(q.sym), shape=tuple(gptq.layer.weight.shape),
-                dtype=str(gptq.layer.weight.dtype).replace("torch.", ""))
+    entry = dict(qweight=qweight, scales=scales.contiguous(), g_idx=g_idx.contiguous(), nbits=nbits,
+                 bits=int(q.bits), sym=bool(q.sym), shape=tuple(gptq.layer.weight.shape),
+                 dtype=str(gptq.layer.weight.dtype).replace("torch.", ""))
+    if groupsize:
+        entry["groupsize"] = int(groupsize)
+    return entry
 
 
 def dequantize_packed(entry: Dict[str, object], dtype: Optional[torch.dtype] = None) -> torch.Tensor:
@@ -100,7 +109,7 @@ def save_packed(path: str, entries: Dict[str, Dict[str, object]],
     for name, e in entries.items():
         for key in ("qweight", "scales", "g_idx"):
             tensors[f"{name}.{key}"] = e[key].detach().contiguous().cpu()
-        meta[name] = json.dumps({k: e[k] for k in ("nbits", "bits", "sym", "shape", "dtype")})
+        meta[name] = json.dumps({k: e[k] for k in ("nbits", "bits", "sym", "shape", "dtype", "groupsize") if k in e})
     for name, q in (quantizers or {}).items():
         for key, t in quantizer_state(q).items():
             tensors[f"w_quantizers.{name}.{key}"] = t.cpu()

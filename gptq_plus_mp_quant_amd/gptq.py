@@ -172,6 +172,7 @@ class GPTQ:
         self.perm, self.invperm, self._codes_perm = perm, invperm, codes
         self.qmode, self.scale_table, self.col_group = qmode, scale_tab, col_group
         self.blocksize_used, self.groupsize_used = blocksize, groupsize
+        self.groups_natural = bool(static_groups)      # groups of natural, not permuted columns
         self.dyn_scale = None
         if int(nan_flag.item()):
             logging.warning("NaN in weights")

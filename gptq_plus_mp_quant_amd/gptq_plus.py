@@ -568,6 +568,7 @@ class GPTQPlus:
         self._codes_perm = codes
         self.qmode, self.scale_table, self.col_group, self.dyn_scale = qmode, scale_tab, col_group, dyn_scale
         self.blocksize_used, self.groupsize_used = blocksize, groupsize
+        self.groups_natural = True                     # a static group is a run of natural columns
         self.Hinv_all = Hinv_all if keep_hinv else None
         self.Hinv_init_all = Hinit_all if keep_hinv else None
         self.Z = Z if keep_hinv else None

@@ -1,0 +1,171 @@
+"""Running a quantised model from its packed entries.
+
+``export_packed`` leaves a linear as codes, scales and the scale group of every column.  The functions
+here compute with that form; the dequantized weight is never written out:
+
+* ``packed_linear(x, entry)`` -- ``x W^T`` (+ bias) for a few tokens; differentiable in ``x``.
+* ``packed_linear_backward(grad_y, entry)`` -- the gradient of ``x`` alone.
+* ``packed_moe(x, router, gate, up, down, top_k)`` -- a mixture-of-experts layer whose experts' linears
+  are packed, each of the three stacked over the experts by ``stack_packed``.
+
+W is scale times code as the entry holds them (``dequantize_packed`` rounds that product to the
+layer's type; the products here do not).  Sums are fp32 and the result is rounded once, to x's type.
+An entry's ``groupsize`` (``export_packed`` adds it where the groups are runs of columns) says that
+column c is in group ``c // groupsize``; without it every column's group is read from ``g_idx``.
+"""
+from __future__ import annotations
+
+from typing import Dict, Optional, Sequence
+
+import torch
+
+from . import _native as nat
+from . import kernels as K
+
+_FLOATS = (torch.float16, torch.bfloat16, torch.float32)
+
+
+def _checked(entry: Dict[str, object], batch: int):
+    """(qweight, nbits, scales, C, g_idx, groupsize) of an entry (batch = 1: stacked over experts)."""
+    q, scales, g_idx, nbits = entry["qweight"], entry["scales"], entry["g_idx"], int(entry["nbits"])
+    groupsize = int(entry.get("groupsize", 0))
+    for t, name, dtype in ((q, "qweight", torch.int32), (scales, "scales", torch.float32), (g_idx, "g_idx", torch.int32)):
+        if not (isinstance(t, torch.Tensor) and t.is_cuda):
+            nat.require_gpu(t, name)
+        if t.dtype != dtype:
+            raise ValueError(f"packed entry: {name} must be {dtype}")
+    if not 2 <= nbits <= nat.RQ_PACKED_MAXBITS:
+        raise NotImplementedError(f"packed weights of {nbits} bits: 2 to {nat.RQ_PACKED_MAXBITS} are supported")
+    if q.dim() != 2 + batch or scales.dim() != 2 + batch or g_idx.dim() != 1 + batch:
+        raise ValueError("packed entry: qweight [R, words], scales [ngroups, R] and g_idx [C] are expected"
+                         + (", each with a leading expert dimension (stack_packed)" if batch else ""))
+    C, R, ng = g_idx.shape[-1], q.shape[-2], scales.shape[-2]
+    if C == 0 or R == 0 or ng == 0 or q.shape[-1] * 32 < C * nbits or scales.shape[-1] != R:
+        raise ValueError("packed entry: the shapes of qweight, scales and g_idx do not belong together")
+    if batch and not (q.shape[0] == scales.shape[0] == g_idx.shape[0]):
+        raise ValueError("packed entry: qweight, scales and g_idx hold different numbers of experts")
+    if groupsize < 0 or (groupsize and ng > 1 and (C - 1) // groupsize >= ng):
+        raise ValueError(f"packed entry: groupsize {groupsize} does not fit {ng} groups of {C} columns")
+    if not (q.device == scales.device == g_idx.device):
+        raise ValueError("packed entry: qweight, scales and g_idx are on different devices")
+    if q.stride(-1) != 1 or scales.stride(-1) != 1 or (batch and q.stride(-2) < q.shape[-1]):
+        raise ValueError("packed entry: qweight and scales need unit column strides")
+    return q, nbits, scales, C, g_idx if g_idx.is_contiguous() else g_idx.contiguous(), groupsize
+
+
+def _tokens(x, width, device, name):
+    """x as [T, width] with unit column stride (copied only if its strides need it)."""
+    if not (isinstance(x, torch.Tensor) and x.is_cuda):
+        nat.require_gpu(x, name)
+    if x.dtype not in _FLOATS:
+        raise TypeError(f"{name}: unsupported dtype {x.dtype}; expected float16, bfloat16 or float32")
+    if x.dim() < 1 or x.shape[-1] != width:
+        raise ValueError(f"{name} must be [..., {width}], got {tuple(x.shape)}")
+    if x.device != device:
+        raise ValueError(f"{name} is on {x.device}, the packed weight on {device}")
+    x2 = x if x.dim() == 2 else x.reshape(-1, width)
+    if x2.stride(1) != 1 or (x2.stride(0) < width and x2.shape[0] > 1):
+        x2 = x2.contiguous()
+    elif x2.stride(0) < width:                   # one token: its row stride is never used
+        x2 = x2.as_strided((1, width), (width, 1))
+    return x2
+
+
+class _PackedLinear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, entry, bias):
+        ctx.entry = entry
+        return _forward(x, entry, bias)
+
+    @staticmethod
+    def backward(ctx, grad_y):
+        return packed_linear_backward(grad_y, ctx.entry), None, None
+
+
+def _forward(x, entry, bias):
+    q, nbits, scales, C, g_idx, groupsize = _checked(entry, 0)
+    x2 = _tokens(x, C, q.device, "x")
+    if bias is not None:
+        if bias.dtype != x.dtype or bias.shape != (q.shape[0],) or bias.device != x.device:
+            raise ValueError(f"bias must be {x.dtype} [{q.shape[0]}] on {x.device}")
+        bias = bias.contiguous()
+    y = K.packed_linear(x2, q, nbits, scales, C, g_idx, groupsize, bias)
+    return y if x.dim() == 2 else y.view(*x.shape[:-1], q.shape[0])
+
+
+def packed_linear(x: torch.Tensor, entry: Dict[str, object], bias: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``x [..., C]`` times the transpose of a packed weight, ``[..., R]`` in x's dtype (fp16, bf16 or
+    fp32); ``bias`` [R] of the same dtype is added before the rounding.  Any number of tokens; the
+    kernels are made for few (a decoding step, a short prompt).  Differentiable in ``x``; the weight
+    and the bias are constants (a bias that requires grad is refused)."""
+    if torch.is_grad_enabled():
+        if bias is not None and bias.requires_grad:
+            raise ValueError("packed_linear: the bias of a packed linear is a constant; detach it")
+        if isinstance(x, torch.Tensor) and x.requires_grad:
+            return _PackedLinear.apply(x, entry, bias)
+    return _forward(x, entry, bias)
+
+
+def packed_linear_backward(grad_y: torch.Tensor, entry: Dict[str, object]) -> torch.Tensor:
+    """The gradient of ``packed_linear``'s x: ``grad_y [..., R]`` times the packed weight, ``[..., C]`` in
+    grad_y's dtype.  The result does not change from run to run."""
+    q, nbits, scales, C, g_idx, groupsize = _checked(entry, 0)
+    g2 = _tokens(grad_y, q.shape[0], q.device, "grad_y")
+    gx = K.packed_linear_grad(g2, q, nbits, scales, C, g_idx, groupsize)
+    return gx if grad_y.dim() == 2 else gx.view(*grad_y.shape[:-1], C)
+
+
+def stack_packed(entries: Sequence[Dict[str, object]]) -> Dict[str, object]:
+    """One linear of every expert as one entry, for ``packed_moe``: qweight [E, R, words], scales
+    [E, ngroups, R], g_idx [E, C].  The experts' entries must agree in shape, bits and number of
+    groups."""
+    entries = list(entries)
+    if not entries:
+        raise ValueError("stack_packed: no entries")
+    first = entries[0]
+    for e in entries:
+        _checked(e, 0)
+        if int(e["nbits"]) != int(first["nbits"]) or e["qweight"].shape != first["qweight"].shape or \
+                e["scales"].shape != first["scales"].shape or e["g_idx"].shape != first["g_idx"].shape:
+            raise ValueError("stack_packed: the experts' entries differ in bits, shape or groups")
+    out = {k: torch.stack([e[k] for e in entries]) for k in ("qweight", "scales", "g_idx")}
+    sizes = {int(e.get("groupsize", 0)) for e in entries}
+    out.update(nbits=int(first["nbits"]), bits=first.get("bits"), sym=first.get("sym"), shape=tuple(first["shape"]),
+               dtype=first["dtype"], groupsize=sizes.pop() if len(sizes) == 1 else 0)
+    return out
+
+
+def packed_moe(x: torch.Tensor, router: torch.Tensor, gate: Dict[str, object], up: Dict[str, object],
+               down: Dict[str, object], top_k: int, norm_topk: bool = True, return_routing: bool = False):
+    """A mixture-of-experts layer for a few tokens: ``x [..., D]`` -> ``[..., D]`` in x's dtype.
+
+    ``router`` [E, D] (x's dtype) gives the logits; each token goes to its ``top_k`` largest (equal
+    logits: the lowest index), weighted by the softmax over all experts, divided by the chosen ones' sum
+    with ``norm_topk``; an expert is ``down(silu(gate(x)) * up(x))``.  ``gate`` / ``up`` (I x D) and ``down``
+    (D x I) are stacked entries, each with bits and groups of its own.  ``return_routing`` adds the
+    chosen ids (int32) and weights (fp32), ``[..., top_k]``.  At most 1024 experts, 64 chosen.  It has
+    no backward pass: an x that requires grad is refused."""
+    if torch.is_grad_enabled() and isinstance(x, torch.Tensor) and (x.requires_grad or router.requires_grad):
+        raise NotImplementedError("packed_moe has no backward pass: call it under torch.no_grad() or on detached tensors")
+    g, u, d = _checked(gate, 1), _checked(up, 1), _checked(down, 1)
+    E, I, _ = g[0].shape
+    D = g[3]
+    if u[0].shape[:2] != (E, I) or u[3] != D or d[0].shape[:2] != (E, D) or d[3] != I:
+        raise ValueError("packed_moe: gate and up must be [E, I x D] and down [E, D x I]")
+    if not (u[0].device == d[0].device == g[0].device):
+        raise ValueError("packed_moe: gate, up and down are on different devices")
+    x2 = _tokens(x, D, g[0].device, "x")
+    if not isinstance(router, torch.Tensor) or router.shape != (E, D) or router.dtype != x.dtype or router.device != x.device:
+        raise ValueError(f"packed_moe: router must be {x.dtype} [{E}, {D}] on {x.device}")
+    top_k = int(top_k)
+    if E > nat.RQ_MOE_MAX_EXPERTS or not 1 <= top_k <= min(E, nat.RQ_MOE_MAX_TOP):
+        raise ValueError(f"packed_moe: top_k {top_k} of {E} experts (at most {nat.RQ_MOE_MAX_TOP} of "
+                         f"{nat.RQ_MOE_MAX_EXPERTS})")
+    router = router if router.stride(1) == 1 and router.stride(0) >= D else router.contiguous()
+    args = [(q, nbits, scales, g_idx, groupsize) for q, nbits, scales, _, g_idx, groupsize in (g, u, d)]
+    y, ids, weights = K.packed_moe(x2, router, I, *args, top_k, norm_topk, return_routing)
+    y = y if x.dim() == 2 else y.view(x.shape)
+    if not return_routing:
+        return y
+    lead = x.shape[:-1]
+    return y, ids.view(*lead, top_k), weights.view(*lead, top_k)

@@ -1,0 +1,110 @@
+"""What a (quantised) model answers, from its logits: the log probability of given tokens, the entropy of
+every distribution and the most likely alternatives, in one pass over the logits, and the gradient of
+the logits.
+
+Perplexity is ``(-token_logprobs(logits, targets).logprob).mean().exp()``; a static saliency or a refreshed
+gradient starts from ``token_logprobs(...).logprob.sum().backward()``.
+"""
+from __future__ import annotations
+
+from typing import NamedTuple, Optional
+
+import torch
+
+from . import _native as nat
+from . import kernels as K
+
+_FLOATS = (torch.float16, torch.bfloat16, torch.float32)
+
+
+class TokenLogprobs(NamedTuple):
+    """``logprob`` and ``entropy`` fp32 ``[...]``; ``top_ids`` int64 and ``top_logprobs`` fp32
+    ``[..., top_k]``, the most likely first; ``stats`` fp32 ``[..., 3]`` for the backward pass (the row's
+    maximum, log sum exp(z - max), entropy)."""
+    logprob: torch.Tensor
+    entropy: torch.Tensor
+    top_ids: torch.Tensor
+    top_logprobs: torch.Tensor
+    stats: torch.Tensor
+
+
+def _rows(logits, targets):
+    if not (isinstance(logits, torch.Tensor) and logits.is_cuda):
+        nat.require_gpu(logits, "logits")
+    if logits.dtype not in _FLOATS:
+        raise TypeError(f"logits: unsupported dtype {logits.dtype}; expected float16, bfloat16 or float32")
+    if logits.dim() < 1 or logits.shape[-1] == 0:
+        raise ValueError("logits must be [..., V] with V > 0")
+    if not isinstance(targets, torch.Tensor) or targets.dtype != torch.int64 or targets.shape != logits.shape[:-1] or \
+            targets.device != logits.device:
+        raise ValueError(f"targets must be int64 {list(logits.shape[:-1])} on {logits.device}")
+    V = logits.shape[-1]
+    z = logits if logits.dim() == 2 else logits.reshape(-1, V)
+    if z.stride(1) != 1 or z.stride(0) < V:
+        z = z.contiguous()
+        if z.stride(0) < V:                      # one row: its stride is never used
+            z = z.as_strided((z.shape[0], V), (V, 1))
+    t = targets if targets.dim() == 1 else targets.reshape(-1)
+    return z, t if t.is_contiguous() else t.contiguous()
+
+
+def _forward(logits, targets, top_k, ignore_index):
+    z, t = _rows(logits, targets)
+    top_k = int(top_k)
+    if not 0 <= top_k <= min(nat.RQ_SCORE_MAX_TOP, z.shape[1]):
+        raise ValueError(f"top_k must be 0 to {min(nat.RQ_SCORE_MAX_TOP, z.shape[1])}, got {top_k}")
+    lp, H, ids, top, stats = K.token_logprobs(z, t, top_k, int(ignore_index))
+    if logits.dim() != 2:
+        lead = logits.shape[:-1]
+        lp, H = lp.view(lead), H.view(lead)
+        ids, top, stats = ids.view(*lead, top_k), top.view(*lead, top_k), stats.view(*lead, 3)
+    return TokenLogprobs(lp, H, ids, top, stats)
+
+
+class _TokenLogprobs(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, targets, top_k, ignore_index):
+        r = _forward(logits, targets, top_k, ignore_index)
+        ctx.save_for_backward(logits, targets, r.stats)
+        ctx.ignore_index = ignore_index
+        ctx.mark_non_differentiable(r.top_ids, r.top_logprobs, r.stats)
+        return tuple(r)
+
+    @staticmethod
+    def backward(ctx, grad_logprob, grad_entropy, *_):
+        logits, targets, stats = ctx.saved_tensors
+        return token_logprobs_backward(logits, targets, stats, grad_logprob, grad_entropy, ctx.ignore_index), None, None, None
+
+
+def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, top_k: int = 0, ignore_index: int = -100) -> TokenLogprobs:
+    """Score ``targets`` [...] (int64) under ``logits`` [..., V] (fp16, bf16 or fp32).
+
+    ``logprob`` is 0 where the target is ``ignore_index`` and NaN for another target outside the vocabulary.
+    ``top_k`` (0 to 64) alternatives are ordered by their logit, equal ones by their index.  Masked
+    logits (-inf, or the type's lowest value) have probability 0; a row with nothing but -inf has
+    logprob -inf, entropy 0 and no gradient; a row with a NaN or +inf is NaN.  ``logprob`` and
+    ``entropy`` are differentiable in ``logits``, ``top_logprobs`` is not."""
+    if torch.is_grad_enabled() and isinstance(logits, torch.Tensor) and logits.requires_grad:
+        return TokenLogprobs(*_TokenLogprobs.apply(logits, targets, top_k, ignore_index))
+    return _forward(logits, targets, top_k, ignore_index)
+
+
+def _row_grads(g, like, name):
+    if not isinstance(g, torch.Tensor) or g.dtype != torch.float32 or g.shape != like.shape[:-1] or g.device != like.device:
+        raise ValueError(f"{name} must be float32 {list(like.shape[:-1])} on {like.device}")
+    g = g if g.dim() == 1 else g.reshape(-1)
+    return g if g.is_contiguous() else g.contiguous()
+
+
+def token_logprobs_backward(logits: torch.Tensor, targets: torch.Tensor, stats: torch.Tensor, grad_logprob: torch.Tensor,
+                            grad_entropy: Optional[torch.Tensor] = None, ignore_index: int = -100) -> torch.Tensor:
+    """The gradient of ``logits`` from the gradients of ``logprob`` and (optionally) ``entropy``, in the
+    logits' dtype; ``stats`` is what ``token_logprobs`` returned for the same logits."""
+    z, t = _rows(logits, targets)
+    gl = _row_grads(grad_logprob, logits, "grad_logprob")
+    gh = None if grad_entropy is None else _row_grads(grad_entropy, logits, "grad_entropy")
+    if not isinstance(stats, torch.Tensor) or stats.dtype != torch.float32 or stats.shape != (*logits.shape[:-1], 3) or \
+            stats.device != logits.device:
+        raise ValueError(f"stats must be token_logprobs' float32 {list(logits.shape[:-1]) + [3]} on {logits.device}")
+    gz = K.token_logprobs_grad(z, t, int(ignore_index), stats if stats.is_contiguous() else stats.contiguous(), gl, gh)
+    return gz if logits.dim() == 2 else gz.view(logits.shape)

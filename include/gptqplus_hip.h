@@ -351,6 +351,75 @@ int rq_block_gd_step(float* Wp, int64_t ldw, int R, int R_s, int C, int i2, cons
                      double gate_floor, double gate_sharpness, double sine_amp, float* stats_parts,
                      void* stream);
 
+/* --- Working with packed weights -------------------------------------------------------------
+ * A packed weight is what rq_pack_codes wrote (qweight [R, ldp] words, nbits 2..9 here), scales
+ * [ngroups, lds] fp32 (row r's scale of group g at scales[g * lds + r]) and the group of each column:
+ * c / groupsize when groupsize > 0, else g_idx[c] (a column whose g_idx lies outside [0, ngroups)
+ * reads as NaN); one group needs neither.  The weight is s * q as it stands, not rounded to a layer's
+ * type.  No counterpart in the reference, which multiplies by the dequantized weight. */
+
+/* y[t, r] = sum_c x[t, c] * s[g(c), r] * q[r, c] (+ bias[r]): x [T, C] (row stride ldx), bias [R] or
+ * NULL and y [T, R] (row stride ldy) of type dtype.  fp32 sums, rounded once.  Any T; built for few. */
+int rq_packed_linear(const void* x, int dtype, int T, int64_t ldx, int C, const uint32_t* qweight,
+                     int64_t ldp, int nbits, int R, const float* scales, int64_t lds, int ngroups,
+                     const int32_t* g_idx, int groupsize, const void* bias, void* y, int64_t ldy,
+                     void* stream);
+
+/* grad_x[t, c] = sum_r grad_y[t, r] * s[g(c), r] * q[r, c]: the gradient of rq_packed_linear's x.
+ * workspace: rq_packed_linear_grad_workspace_bytes(T, R, C) bytes, any contents (partial sums, joined
+ * in a fixed order: results do not change from run to run). */
+int64_t rq_packed_linear_grad_workspace_bytes(int T, int R, int C);
+int rq_packed_linear_grad(const void* grad_y, int dtype, int T, int64_t ldg, int C,
+                          const uint32_t* qweight, int64_t ldp, int nbits, int R, const float* scales,
+                          int64_t lds, int ngroups, const int32_t* g_idx, int groupsize, void* grad_x,
+                          int64_t ldx, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* One linear of every expert: expert e's entry starts stride_q words, stride_scales floats and C
+ * g_idx entries after expert e - 1's. */
+typedef struct {
+  const uint32_t* qweight;
+  const float* scales;
+  const int32_t* g_idx;
+  int64_t ldp, lds, stride_q, stride_scales;
+  int nbits, ngroups, groupsize;
+} rq_packed_experts;
+
+/* A mixture-of-experts layer: logits = x router^T (x [T, D], router [E, D], both of type dtype), the K
+ * largest chosen (equal logits by their index; a NaN is above all), weighted by their softmax over all
+ * E logits (norm != 0: over the K), y = sum_k w_k down_k(silu(gate_k(x)) * up_k(x)), y [T, D] of type
+ * dtype.  gate and up are I x D, down is D x I; each may have its own nbits and groups.  E <= 1024,
+ * K <= 64.  ids_out / weights_out (optional, [T, K]): the chosen experts in order and their weights.
+ * workspace: rq_packed_moe_workspace_bytes bytes, any contents. */
+int64_t rq_packed_moe_workspace_bytes(int T, int D, int I, int E, int K);
+int rq_packed_moe(const void* x, int dtype, int T, int64_t ldx, int D, const void* router, int64_t ldr,
+                  int E, int K, int norm, int I, const rq_packed_experts* gate,
+                  const rq_packed_experts* up, const rq_packed_experts* down, void* y, int64_t ldy,
+                  int* ids_out, float* weights_out, void* workspace, int64_t workspace_bytes,
+                  void* stream);
+
+/* --- Scoring ------------------------------------------------------------------------------
+ * Per row of logits [N, V] (row stride ldz, type dtype): logprob[n] = log softmax(z)[targets[n]] (0
+ * where targets[n] == ignore_index, NaN for any other target outside [0, V)), entropy[n], and the
+ * top_k (<= 64) largest logits' indices and log probabilities, [N, top_k] in order (equal values by
+ * their index, NaN first).  stats [N, 3] receives the row's maximum, log sum exp(z - max) and entropy
+ * for rq_token_logprobs_grad.  A row with nothing but -inf has logprob and top_logprobs -inf and
+ * entropy 0; one with a NaN or +inf has NaN.  workspace: rq_token_logprobs_workspace_bytes(N, V,
+ * top_k) bytes, any contents (NULL where that is 0). */
+int64_t rq_token_logprobs_workspace_bytes(int64_t N, int V, int top_k);
+int rq_token_logprobs(const void* logits, int dtype, int64_t N, int64_t ldz, int V,
+                      const int64_t* targets, int64_t ignore_index, int top_k, float* logprob,
+                      float* entropy, int64_t* top_ids, float* top_logprobs, float* stats,
+                      void* workspace, int64_t workspace_bytes, void* stream);
+
+/* grad_logits[n, i] = gl[n] (delta(i, target) - p_i) - gh[n] p_i (log p_i + H): the gradient of
+ * logprob (grad_logprob [N], taken as 0 where the target is ignored) and entropy (grad_entropy [N] or
+ * NULL).  A row with nothing but -inf gets 0.  grad_logits [N, V], row stride ldd, type dtype; it may
+ * be the logits themselves (with ldd == ldz). */
+int rq_token_logprobs_grad(const void* logits, int dtype, int64_t N, int64_t ldz, int V,
+                           const int64_t* targets, int64_t ignore_index, const float* stats,
+                           const float* grad_logprob, const float* grad_entropy, void* grad_logits,
+                           int64_t ldd, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

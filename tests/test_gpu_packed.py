@@ -1,0 +1,423 @@
+"""packed_linear, its gradient and packed_moe against the formulas in 64 bits.
+
+Bounds: a sum's fp32 error over the sum of its terms' magnitudes (``sum_eps``), one rounding to the output's
+type, and for the gradient of 16-bit tensors the weight's rounding to 16 significant bits (two bf16
+pieces: 2^-16 of every term)."""
+import numpy as np
+import pytest
+import torch
+
+from gptq_plus_mp_quant_amd import (GPTQ, GPTQPlus, WeightQuantizer, dequantize_packed, export_packed, load_packed,
+                                    packed_linear, packed_linear_backward, packed_moe, save_packed, stack_packed)
+from tests._packed import ROUND, TINY, assert_within, make_entry, on, sum_eps
+from tests._util import rng, synth
+
+pytestmark = pytest.mark.gpu
+DEV = torch.device("cuda:0")
+F16, BF16, F32 = torch.float16, torch.bfloat16, torch.float32
+
+
+def randn(seed, *shape, dtype=F32, scale=1.0):
+    return (torch.from_numpy(rng(seed).standard_normal(shape, dtype=np.float32)) * scale).to(dtype)
+
+
+def check_linear(x, entry, W, bias=None, x_dev=None):
+    dt = x.dtype
+    y = packed_linear(x.to(DEV) if x_dev is None else x_dev, on(entry, DEV), bias=None if bias is None else bias.to(DEV))
+    assert y.dtype == dt
+    xd = x.double()
+    want = xd @ W.t() + (0 if bias is None else bias.double())
+    mag = xd.abs() @ W.abs().t() + (0 if bias is None else bias.double().abs())
+    assert_within(y, want, sum_eps(W.shape[1]) * mag + ROUND[dt] * want.abs() + TINY[dt], "y")
+    return y
+
+
+def check_grad(gy, entry, W, gy_dev=None):
+    dt = gy.dtype
+    gx = packed_linear_backward(gy.to(DEV) if gy_dev is None else gy_dev, on(entry, DEV))
+    assert gx.dtype == dt
+    gd = gy.double()
+    want, mag = gd @ W, gd.abs() @ W.abs()
+    pieces = 0.0 if dt == F32 else 2.0 ** -16
+    assert_within(gx, want, (sum_eps(W.shape[0]) + pieces) * mag + ROUND[dt] * want.abs() + TINY[dt], "gx")
+    return gx
+
+
+SHAPES = [(1, 1, 1), (1, 16, 128), (1, 17, 129), (2, 3, 7), (3, 64, 31), (5, 33, 520), (7, 130, 1365), (8, 1, 4096),
+          (15, 100, 96), (16, 15, 256), (17, 48, 384), (33, 65, 250), (64, 128, 512), (65, 31, 136), (130, 20, 200)]
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16, F32])
+@pytest.mark.parametrize("T,R,C", SHAPES)
+@pytest.mark.parametrize("nbits,groups", [(4, "channel"), (4, "128"), (5, "64"), (3, "order32")])
+def test_shapes(T, R, C, nbits, groups, dtype):
+    entry, W = make_entry(T * 7 + R + C, R, C, nbits, groups)
+    check_linear(randn(T + C, T, C, dtype=dtype), entry, W)
+    check_grad(randn(T + R, T, R, dtype=dtype), entry, W)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16, F32])
+@pytest.mark.parametrize("nbits", [2, 3, 4, 5, 6, 7, 8, 9])
+@pytest.mark.parametrize("groups", ["channel", "32", "128", "100", "8", "256", "order64"])
+def test_bits_and_groups(nbits, groups, dtype):
+    R, C = 70, 777
+    entry, W = make_entry(nbits, R, C, nbits, groups)
+    check_linear(randn(1, 9, C, dtype=dtype), entry, W, bias=randn(2, R, dtype=dtype))
+    check_grad(randn(3, 9, R, dtype=dtype), entry, W)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16, F32])
+@pytest.mark.parametrize("T", [1, 4, 40])
+def test_wide(T, dtype):
+    """Rows and columns past several tiles of every kernel."""
+    entry, W = make_entry(11, 1040, 2304, 4, "128")
+    check_linear(randn(1, T, 2304, dtype=dtype), entry, W)
+    check_grad(randn(2, T, 1040, dtype=dtype), entry, W)
+
+
+def test_outliers_and_scales():
+    """Activations 2^12 apart and scales 2^20 apart: the sums keep fp32's precision."""
+    entry, W = make_entry(5, 64, 1024, 4, "128")
+    entry["scales"][::2] *= 2.0 ** -20
+    W = W * torch.where(entry["g_idx"] % 2 == 0, 2.0 ** -20, 1.0).double()[None, :]
+    for dt in (F16, BF16, F32):
+        x = randn(3, 6, 1024)
+        x[:, ::97] *= 4096.0
+        check_linear(x.to(dt), entry, W)
+        check_grad(randn(4, 6, 64, dtype=dt), entry, W)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16, F32])
+def test_strides_and_views(dtype):
+    R, C = 50, 260
+    entry, W = make_entry(9, R, C, 5, "channel")
+    wide = randn(1, 12, C + 9, dtype=dtype)
+    for x in (wide[:, 1:C + 1], wide[::2, 5:C + 5], wide[:, :C].t().contiguous().t(), wide[3:4, :C].expand(4, C)):
+        dev = wide.to(DEV)
+        view = torch.as_strided(dev, x.shape, x.stride(), x.storage_offset()) if x.untyped_storage().data_ptr() == \
+            wide.untyped_storage().data_ptr() else x.to(DEV)
+        check_linear(x, entry, W, x_dev=view)
+    g = randn(2, 12, R + 3, dtype=dtype)
+    check_grad(g[:, 3:], entry, W, gy_dev=g.to(DEV)[:, 3:])
+    # leading dimensions, and a packed table with longer rows
+    x3 = randn(4, 2, 3, C, dtype=dtype)
+    y = packed_linear(x3.to(DEV), on(entry, DEV))
+    assert y.shape == (2, 3, R)
+    assert torch.equal(y.view(6, R), packed_linear(x3.view(6, C).to(DEV), on(entry, DEV)))
+    assert packed_linear(x3[0, 0].to(DEV), on(entry, DEV)).shape == (R,)
+    e = on(entry, DEV)
+    longer = torch.full((R, e["qweight"].shape[1] + 3), -1, dtype=torch.int32, device=DEV)
+    longer[:, 1:-2] = e["qweight"]
+    e["qweight"] = longer[:, 1:-2]
+    assert torch.equal(packed_linear(x3.to(DEV), e), y)
+    assert packed_linear(torch.empty((0, C), dtype=dtype, device=DEV), e).shape == (0, R)
+    assert packed_linear_backward(torch.empty((0, R), dtype=dtype, device=DEV), e).shape == (0, C)
+
+
+@pytest.mark.parametrize("groups", ["128", "order128"])
+@pytest.mark.parametrize("dtype", [F16, BF16, F32])
+def test_non_finite_inputs_stay_in_their_row(dtype, groups):
+    """An inf or NaN activation makes its own token's results what the formula gives (inf times a zero
+    code is NaN) and leaves the other tokens alone."""
+    entry, W = make_entry(21, 40, 300, 3, groups)
+    x = randn(1, 5, 300, dtype=dtype)
+    x[1, 7], x[2, 290], x[3, 299] = float("inf"), float("-inf"), float("nan")
+    check_linear(x, entry, W)
+    g = randn(2, 5, 40, dtype=dtype)
+    g[1, 0], g[3, 39], g[4, 20] = float("-inf"), float("inf"), float("nan")
+    check_grad(g, entry, W)
+
+
+def test_g_idx_out_of_range_reads_as_nan():
+    entry, _ = make_entry(4, 20, 64, 4, "order16")
+    e = on(entry, DEV)
+    e["g_idx"][5] = 4
+    e["g_idx"][6] = -1
+    y = packed_linear(torch.ones((2, 64), device=DEV), e)
+    gx = packed_linear_backward(torch.ones((2, 20), device=DEV), e)
+    assert bool(torch.isnan(y).all())
+    assert torch.isnan(gx).cpu().nonzero()[:, 1].tolist() == [5, 6, 5, 6]
+
+
+def test_same_results_every_time_and_on_another_stream():
+    entry, _ = make_entry(8, 300, 1500, 4, "128")
+    e = on(entry, DEV)
+    x, g = randn(1, 20, 1500, dtype=BF16).to(DEV), randn(2, 20, 300, dtype=BF16).to(DEV)
+    y, gx = packed_linear(x, e), packed_linear_backward(g, e)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        y2, gx2 = packed_linear(x, e), packed_linear_backward(g, e)
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(y, y2) and torch.equal(gx, gx2)
+
+
+def test_in_a_graph():
+    entry, _ = make_entry(8, 96, 512, 5, "channel")
+    e = on(entry, DEV)
+    x, g = randn(1, 3, 512, dtype=F16).to(DEV), randn(2, 3, 96, dtype=F16).to(DEV)
+    packed_linear(x, e), packed_linear_backward(g, e)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y, gx = packed_linear(x, e), packed_linear_backward(g, e)
+    for seed in range(3):
+        x.copy_(randn(10 + seed, 3, 512, dtype=F16))
+        g.copy_(randn(20 + seed, 3, 96, dtype=F16))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, packed_linear(x, e)) and torch.equal(gx, packed_linear_backward(g, e))
+
+
+@pytest.mark.parametrize("groups", ["channel", "32", "order32"])
+def test_autograd_and_differences(groups):
+    entry, W = make_entry(3, 24, 96, 4, groups)
+    e = on(entry, DEV)
+    x = randn(1, 2, 5, 96).to(DEV).requires_grad_()
+    g = randn(2, 2, 5, 24).to(DEV)
+    y = packed_linear(x, e)
+    (gx,) = torch.autograd.grad(y, x, g)
+    assert torch.equal(gx, packed_linear_backward(g, e))
+    # y is linear in x: a difference along v of any length gives <gx, v> up to the sums' rounding
+    v = randn(5, 2, 5, 96).to(DEV)
+    with torch.no_grad():
+        diff = ((packed_linear(x + v, e) - packed_linear(x - v, e)).double() * g.double()).sum() / 2
+        mag = float((x.abs().cpu().double() + v.abs().cpu().double()).view(10, 96).matmul(W.abs().t()).mul(
+            g.abs().cpu().double().view(10, 24)).sum())
+    assert abs(float(diff - (gx.double() * v.double()).sum())) <= 4 * sum_eps(96) * mag
+    with torch.no_grad():
+        assert not packed_linear(x, e).requires_grad
+
+
+def _quantised(cls, R, C, bits, sym, gs, act, static, seed=5):
+    X, W, s, grad = synth(seed, R, C, 2, 4, 64)
+    layer = torch.nn.Linear(C, R, bias=False).to(DEV, F16)
+    layer.weight.data.copy_(W.to(DEV))
+    g = GPTQPlus(layer, saliency=s, gradient=grad, num_groups=2, alpha=0.0, reference_loss=0.0) if cls is GPTQPlus else \
+        GPTQ(layer)
+    g.quantizer = WeightQuantizer()
+    g.quantizer.configure(bits, perchannel=True, sym=sym, mse=False)
+    for j in range(0, 4, 2):
+        g.add_batch(X[j:j + 2].to(DEV), None)
+    if cls is GPTQPlus:
+        g.finalize_hessian()
+        g.fasterquant(blocksize=64, percdamp=0.01, groupsize=gs, actorder=act, static_groups=static)
+    else:
+        g.fasterquant(percdamp=0.01, groupsize=gs, actorder=act, static_groups=static)
+    return g
+
+
+@pytest.mark.parametrize("cls,bits,sym,gs,act,static,size", [
+    (GPTQPlus, 4, False, -1, True, False, 320), (GPTQPlus, 3, True, 64, True, True, 64),
+    (GPTQPlus, 4, True, 64, False, False, 64), (GPTQPlus, 4, True, 64, True, False, None),
+    (GPTQ, 4, True, 64, True, True, 64), (GPTQ, 4, False, 64, True, False, None), (GPTQ, 8, False, 64, False, False, 64)])
+def test_exported_entries(cls, bits, sym, gs, act, static, size, tmp_path):
+    """What export_packed leaves, through a file, gives the product with the weight that
+    dequantize_packed rebuilds; groupsize is there exactly where the groups are runs of columns."""
+    g = _quantised(cls, 96, 320, bits, sym, gs, act, static)
+    e = export_packed(g)
+    assert e.get("groupsize") == size
+    if size:
+        assert torch.equal(e["g_idx"].cpu(), (torch.arange(320) // size).to(torch.int32))
+    save_packed(str(tmp_path / "p.safetensors"), {"m": e})
+    back = load_packed(str(tmp_path / "p.safetensors"), device=DEV)[0]["m"]
+    assert back.get("groupsize") == size
+    x = randn(7, 6, 320)
+    W = dequantize_packed(back, torch.float32).cpu().double()
+    y = packed_linear(x.to(DEV), back)
+    want, mag = x.double() @ W.t(), x.double().abs() @ W.abs().t()
+    assert_within(y, want, sum_eps(320) * mag + 2.0 ** -23 * mag, "y")
+    old = {k: v for k, v in back.items() if k != "groupsize"}              # a file without the size
+    assert_within(packed_linear(x.to(DEV), old), want, sum_eps(320) * mag + 2.0 ** -23 * mag, "y without groupsize")
+
+
+def test_refusals():
+    entry, _ = make_entry(1, 16, 64, 4, "32")
+    e = on(entry, DEV)
+    x = torch.zeros((2, 64), dtype=F16, device=DEV)
+
+    def bad(error, x=x, bias=None, **change):
+        with pytest.raises(error):
+            packed_linear(x, {**e, **change}, bias=bias)
+
+    bad(RuntimeError, x=x.cpu())
+    bad(RuntimeError, qweight=entry["qweight"])
+    bad(ValueError, x=x[:, :63])
+    bad(TypeError, x=x.double())
+    bad(ValueError, scales=e["scales"].half())
+    bad(ValueError, scales=e["scales"][:, :15])
+    bad(ValueError, qweight=e["qweight"][:, :7])
+    bad(ValueError, g_idx=e["g_idx"].long())
+    bad(ValueError, groupsize=16)
+    bad(ValueError, groupsize=-1)
+    bad(NotImplementedError, nbits=10)
+    bad(NotImplementedError, nbits=1)
+    bad(ValueError, bias=torch.zeros(15, dtype=F16, device=DEV))
+    bad(ValueError, bias=torch.zeros(16, device=DEV))
+    bad(ValueError, bias=torch.zeros(16, dtype=F16, device=DEV, requires_grad=True))
+    with pytest.raises(ValueError):
+        packed_linear_backward(x, e)
+    with pytest.raises(ValueError):
+        packed_linear(x, {**e, "qweight": e["qweight"][None], "scales": e["scales"][None], "g_idx": e["g_idx"][None]})
+
+
+# --- packed_moe -------------------------------------------------------------------------------
+
+
+def moe_case(seed, T, D, I, E, dtype, nbits=(4, 4, 4), groups=("128", "128", "128")):
+    parts = [make_entry(seed + k, R, C, nb, gr, batch=E) for k, (R, C, nb, gr) in
+             enumerate(zip((I, I, D), (D, D, I), nbits, groups))]
+    router = randn(seed + 9, E, D, dtype=dtype, scale=D ** -0.5)
+    return randn(seed + 8, T, D, dtype=dtype), router, parts
+
+
+def check_moe(x, router, parts, K, norm):
+    dt, (T, D), E = x.dtype, x.shape, router.shape[0]
+    y, ids, weights = packed_moe(x.to(DEV), router.to(DEV), *(on(e, DEV) for e, _ in parts), K, norm_topk=norm,
+                                 return_routing=True)
+    assert y.dtype == dt and y.shape == x.shape
+    xd, logits = x.double(), x.double() @ router.double().t()
+    best = torch.sort(logits, dim=-1, descending=True, stable=True)
+    p = torch.softmax(logits, -1).gather(1, best.indices[:, :K])
+    p = p / p.sum(-1, keepdim=True) if norm else p
+    got = ids.cpu().long()
+    # the chosen experts, up to logits closer than their sums' rounding
+    slack = sum_eps(D) * (xd.abs() @ router.double().abs().t()).amax(-1, keepdim=True)
+    assert bool(((logits.gather(1, got) - best.values[:, :K]).abs() <= 2 * slack).all())
+    assert all(len(set(row)) == K for row in got.tolist())
+    w_tol = (4 * slack + 2.0 ** -20) * p
+    assert_within(weights, p, w_tol, "weights")
+    Wg, Wu, Wd = (w for _, w in parts)
+    want, bound = torch.zeros((T, D), dtype=torch.float64), torch.zeros((T, D), dtype=torch.float64)
+    eps, eps2 = sum_eps(D), sum_eps(I_of(parts)) + 2.0 ** -16
+    for t in range(T):
+        for k in range(K):
+            ex = int(got[t, k])
+            a, b = Wg[ex] @ xd[t], Wu[ex] @ xd[t]
+            da, db = eps * (Wg[ex].abs() @ xd[t].abs()), eps * (Wu[ex].abs() @ xd[t].abs())
+            silu = a * torch.sigmoid(a)
+            h = silu * b
+            # |silu'| <= 1.1; 2^-20 for the fp32 activation itself
+            dh = 1.1 * da * (b.abs() + db) + silu.abs() * db + 2.0 ** -20 * h.abs()
+            o = Wd[ex] @ h
+            want[t] += p[t, k] * o
+            bound[t] += p[t, k] * (Wd[ex].abs() @ (dh + eps2 * h.abs())) + w_tol[t, k] * o.abs()
+    assert_within(y, want, bound + ROUND[dt] * want.abs() + TINY[dt], "y")
+
+
+def I_of(parts):
+    return parts[0][1].shape[1]
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16, F32])
+@pytest.mark.parametrize("T,D,I,E,K", [(1, 128, 96, 4, 1), (1, 256, 128, 8, 8), (3, 130, 70, 5, 2), (7, 96, 33, 16, 4),
+                                       (16, 256, 130, 3, 2), (20, 64, 64, 2, 1), (33, 128, 48, 70, 6), (70, 64, 40, 4, 3)])
+@pytest.mark.parametrize("norm", [True, False])
+def test_moe_shapes(T, D, I, E, K, norm, dtype):
+    check_moe(*moe_case(T + D, T, D, I, E, dtype), K, norm)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16, F32])
+@pytest.mark.parametrize("nbits,groups", [((4, 4, 4), ("channel",) * 3), ((5, 5, 5), ("128", "128", "64")),
+                                          ((3, 4, 8), ("32", "channel", "order16")), ((4, 4, 4), ("order64",) * 3),
+                                          ((9, 2, 6), ("channel", "128", "100")), ((8, 8, 3), ("order32", "order32", "8"))])
+def test_moe_bits_and_groups(nbits, groups, dtype):
+    """Mixed precision: each of the three linears may have bits and groups of its own."""
+    check_moe(*moe_case(4, 6, 260, 140, 6, dtype, nbits, groups), 3, True)
+
+
+def test_moe_every_token_to_one_expert():
+    """All tokens choose the same experts (the others are never touched), and one token none of them."""
+    x, router, parts = moe_case(6, 40, 128, 64, 9, BF16)
+    x = x.abs()
+    router[:] = -0.1
+    router[3], router[7] = 0.5, 0.4
+    x[11] = -x[11]
+    check_moe(x, router, parts, 2, True)
+
+
+def test_moe_ties_go_to_the_lowest_index():
+    x, router, parts = moe_case(2, 5, 64, 32, 12, F16)
+    router[:] = router[4]
+    _, ids, weights = packed_moe(x.to(DEV), router.to(DEV), *(on(e, DEV) for e, _ in parts), 5, return_routing=True)
+    assert ids.cpu().tolist() == [[0, 1, 2, 3, 4]] * 5
+    assert torch.allclose(weights.cpu(), torch.full((5, 5), 0.2), atol=1e-6, rtol=0)
+
+
+@pytest.mark.parametrize("K", [1, 3])
+def test_moe_non_finite_token(K):
+    """A NaN or inf token is NaN; the other tokens are as without it."""
+    x, router, parts = moe_case(3, 6, 128, 64, 5, BF16)
+    args = [on(e, DEV) for e, _ in parts]
+    clean = packed_moe(x.to(DEV), router.to(DEV), *args, K)
+    x[2, 5], x[4, 100] = float("nan"), float("inf")
+    y, ids, _ = packed_moe(x.to(DEV), router.to(DEV), *args, K, return_routing=True)
+    ids = ids.cpu()
+    assert bool((ids >= 0).all()) and bool((ids < 5).all())
+    assert bool(torch.isnan(y[2]).all())
+    keep = [0, 1, 3, 5]
+    assert torch.equal(y[keep], clean[keep])
+
+
+def test_moe_views_and_stack():
+    entries = [make_entry(30 + i, 48, 64, 4, "32")[0] for i in range(4)]
+    gate = stack_packed([on(e, DEV) for e in entries])
+    assert gate["qweight"].shape == (4, 48, 8) and gate["groupsize"] == 32
+    up = stack_packed([on(make_entry(50 + i, 48, 64, 4, "32")[0], DEV) for i in range(4)])
+    down = stack_packed([on(make_entry(70 + i, 64, 48, 5, "channel")[0], DEV) for i in range(4)])
+    wide = randn(1, 6, 70, dtype=F16).to(DEV)
+    router = randn(2, 4, 64, dtype=F16).to(DEV)
+    y = packed_moe(wide[:, 3:67], router, gate, up, down, 2)
+    assert torch.equal(y, packed_moe(wide[:, 3:67].contiguous(), router, gate, up, down, 2))
+    y3, ids, w = packed_moe(wide[:, 3:67].contiguous().view(2, 3, 64), router, gate, up, down, 2, return_routing=True)
+    assert torch.equal(y3.view(6, 64), y) and ids.shape == (2, 3, 2) and w.shape == (2, 3, 2)
+    assert packed_moe(wide[:0, 3:67], router, gate, up, down, 2).shape == (0, 64)
+    # one expert of one: its three packed linears in fp32
+    lone = [{**e, **{k: e[k][2:3] for k in ("qweight", "scales", "g_idx")}} for e in (gate, up, down)]
+    x1 = wide[:, 3:67].float().contiguous()
+    first = [{k: v[0] if isinstance(v, torch.Tensor) else v for k, v in e.items()} for e in lone]
+    a = packed_linear(x1, first[0])
+    want = packed_linear(torch.nn.functional.silu(a) * packed_linear(x1, first[1]), first[2])
+    got = packed_moe(x1, router[:1].float(), *lone, 1)
+    assert float((got - want).norm() / want.norm()) < 1e-5
+
+
+def test_moe_in_a_graph():
+    x, router, parts = moe_case(12, 4, 128, 64, 8, F16)
+    x, router, args = x.to(DEV), router.to(DEV), [on(e, DEV) for e, _ in parts]
+    packed_moe(x, router, *args, 2)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = packed_moe(x, router, *args, 2)
+    for seed in range(3):
+        x.copy_(randn(40 + seed, 4, 128, dtype=F16))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, packed_moe(x, router, *args, 2))
+
+
+def test_moe_refusals():
+    x, router, parts = moe_case(1, 2, 64, 32, 4, F16)
+    x, router = x.to(DEV), router.to(DEV)
+    gate, up, down = (on(e, DEV) for e, _ in parts)
+    with pytest.raises(ValueError):
+        packed_moe(x, router, gate, up, down, 5)
+    with pytest.raises(ValueError):
+        packed_moe(x, router, gate, up, down, 0)
+    with pytest.raises(ValueError):
+        packed_moe(x, router.float(), gate, up, down, 2)
+    with pytest.raises(ValueError):
+        packed_moe(x, router[:3], gate, up, down, 2)
+    with pytest.raises(ValueError):
+        packed_moe(x, router, gate, up, gate, 2)
+    with pytest.raises(ValueError):
+        packed_moe(x, router, gate, {k: v[0] if isinstance(v, torch.Tensor) else v for k, v in up.items()}, down, 2)
+    with pytest.raises(NotImplementedError):
+        packed_moe(x.requires_grad_(), router, gate, up, down, 2)
+    with pytest.raises(RuntimeError):
+        packed_moe(x.detach().cpu(), router, gate, up, down, 2)
+    with pytest.raises(ValueError):
+        stack_packed([])
+    with pytest.raises(ValueError):
+        stack_packed([on(make_entry(1, 16, 64, 4, "32")[0], DEV), on(make_entry(1, 16, 64, 5, "32")[0], DEV)])

@@ -130,6 +130,27 @@ def stream_of(device):
     return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
 
 
+try:
+    from torch._C import _cuda_getCurrentRawStream as _raw_stream_of
+except ImportError:                                  # a torch without the shortcut
+    def _raw_stream_of(index):
+        return torch.cuda.current_stream(index).cuda_stream
+
+
+def raw_stream(t):
+    """The current stream of a GPU tensor's device as an int, without making a Stream object (the
+    calls on single tokens, whose kernels take a few microseconds, are bound by the host)."""
+    return _raw_stream_of(t.get_device())
+
+
+def check(name, rc):
+    if rc != RQ_OK:
+        raise RuntimeError(f"{name} failed with status {rc}")
+
+
+DTYPE_CODES = {torch.float16: RQ_F16, torch.bfloat16: RQ_BF16, torch.float32: RQ_F32}
+
+
 def dtype_code(dt):
     if dt == torch.float16:
         return RQ_F16

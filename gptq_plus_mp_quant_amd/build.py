@@ -20,7 +20,8 @@ CSRC = PKG / "csrc"
 LIBDIR = PKG / "_lib"
 LIB = LIBDIR / "libgptqplus_hip.so"
 SOURCES = ["hessian.hip", "params.hip", "argsort.hip", "chol.hip", "terms.hip", "colloop.hip", "pack.hip",
-           "blockgd.hip", "plinear.hip", "pmoe.hip", "logprobs.hip"]
+           "blockgd.hip", "plinear.hip", "plinear_f16.hip", "plinear_bf16.hip",
+           "plinear_f32.hip", "pmoe.hip", "logprobs.hip"]
 
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 FLAGS = [

@@ -1,0 +1,251 @@
+// dx = dy W with a packed weight: the kernels and their launches for one element type.
+//
+// A workgroup takes 128 columns and 16 NT tokens over a range of rows; its waves take steps of 32 rows
+// in turn.  v_mfma_f32_16x16x32_bf16 with the tokens as A's rows (k: the step's rows) and the weight as
+// B: lane 16 q + j holds columns 8j..8j+7 of rows 8q..8q+7 (8 codes of each of 8 rows, read as they lie),
+// and product n of a step takes code n of each row, so that D's column j is the weight's column 8j + n.
+// The scale of column and row cannot wait until after the sum over rows:
+//   RUNS   all 128 columns are in one group: it multiplies dy, and the codes go in as they are
+//   SMALL  a lane's 8 columns are in one group (sizes that are multiples of 8): it multiplies the codes
+//   ANY    a scale for every weight
+// What a scale multiplied is an fp32 number, cut into bf16 pieces: two (2^-16 of it is lost; the 16-bit
+// types' results have 8 or 11 bits) or three (fp32, exact).  Products of pieces below 2^-24 are left out.
+#pragma once
+#include "packed_dot.h"
+
+namespace {
+
+// Pieces of dy and of the weight where each is cut (1: bf16 as it is).
+template <typename TX, int MODE> struct ColPieces;
+template <int MODE> struct ColPieces<__half, MODE> {
+  static constexpr int dy = 2, w = MODE == RQ_RUNS ? 1 : 2, keep = 3;
+};
+template <int MODE> struct ColPieces<__hip_bfloat16, MODE> {
+  static constexpr int dy = MODE == RQ_RUNS ? 2 : 1, w = MODE == RQ_RUNS ? 1 : 2, keep = 2;
+};
+template <int MODE> struct ColPieces<float, MODE> {
+  static constexpr int dy = 3, w = MODE == RQ_RUNS ? 1 : 3, keep = 3;
+};
+
+constexpr int COLS = 128, STEP = 32;
+
+// Words that hold columns c..c+7 of a row, shifted down to bit 0 (c a multiple of 8).
+template <int NB>
+struct Col8 {
+  static constexpr int NW = (24 + 8 * NB + 31) / 32, N = (8 * NB + 31) / 32;
+  uint32_t w[NW];
+};
+template <int NB>
+__device__ __forceinline__ int col_code(const uint32_t (&w)[Col8<NB>::NW], int n) {
+  const int b = n * NB, i = b >> 5, o = b & 31;
+  if (o + NB <= 32) return ((int)(w[i] << (32 - NB - o))) >> (32 - NB);
+  const uint32_t v = (uint32_t)((((uint64_t)w[i + 1 < Col8<NB>::NW ? i + 1 : i] << 32) | w[i]) >> o);
+  return ((int)(v << (32 - NB))) >> (32 - NB);
+}
+
+__device__ __forceinline__ void fp32_of(half8 v, floatx8& f) {
+#pragma unroll
+  for (int k = 0; k < 8; ++k) f[k] = (float)v[k];
+}
+__device__ __forceinline__ void fp32_of(bf16x8 v, floatx8& f) {
+#pragma unroll
+  for (int k = 0; k < 8; ++k) f[k] = (float)v[k];
+}
+__device__ __forceinline__ void fp32_of(floatx8 v, floatx8& f) { f = v; }
+
+constexpr int cols_waves(int nt) { return nt >= 4 ? 4 : 8; }
+
+template <typename TX, int NB, int MODE, int NT>
+__global__ __launch_bounds__(64 * cols_waves(NT)) void k_packed_cols(const TX* __restrict__ dy, int T, int64_t ldy,
+                                                                     RqPacked w, int steps_per, float* __restrict__ part,
+                                                                     TX* __restrict__ dx, int64_t ldx) {
+  constexpr int W = cols_waves(NT);
+  typedef ColPieces<TX, MODE> P;
+  typedef typename RqOperand<TX>::raw Raw;
+  __shared__ floatx4 join[W / 2][8 * NT][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, j = lane & 15, q = lane >> 4;
+  const int c0 = blockIdx.x * COLS, c = c0 + 8 * j, t0 = blockIdx.z * 16 * NT;
+  const int nc = min(8, w.C - c);                                  // the lane's columns (<= 0: none)
+  const int nsteps = (w.R + STEP - 1) / STEP;
+  const int sa = blockIdx.y * steps_per, sb = min(nsteps, sa + steps_per);
+  const int64_t bit = (int64_t)c * NB;
+  const int off = (int)(bit & 31), nw = nc > 0 ? (off + nc * NB + 31) >> 5 : 0;
+  const uint32_t* col = w.q + (bit >> 5);
+  int g[8];
+#pragma unroll
+  for (int k = 0; k < 8; ++k)
+    g[k] = MODE == RQ_RUNS ? rq_run_group(w, c0) : (MODE == RQ_SMALL && k) ? g[0] : k < nc ? rq_group_of(w, c + k) : 0;
+  const TX* tok[NT];
+#pragma unroll
+  for (int b = 0; b < NT; ++b) tok[b] = dy + (int64_t)min(t0 + 16 * b + j, T - 1) * ldy;
+
+  floatx4 acc[8][NT];
+#pragma unroll
+  for (int n = 0; n < 8; ++n)
+#pragma unroll
+    for (int b = 0; b < NT; ++b) acc[n][b] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+
+  for (int st = sa + wave; st < sb; st += W) {
+    const int r = st * STEP + 8 * q;                               // the lane's rows r..r+7
+    uint32_t wd[8][Col8<NB>::NW];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const uint32_t* p = col + (int64_t)min(r + k, w.R - 1) * w.ldp;
+#pragma unroll
+      for (int m = 0; m < Col8<NB>::NW; ++m) wd[k][m] = m < nw ? p[m] : 0u;
+    }
+    Raw raw[NT];
+    floatx8 sc;
+    const bool full = r + 8 <= w.R;
+#pragma unroll
+    for (int b = 0; b < NT; ++b) raw[b] = full ? rq_load_x<true>(tok[b] + r, 8) : rq_load_x<false>(tok[b] + r, w.R - r);
+    if (MODE != RQ_ANY) {
+      if (full && g[0] >= 0) {
+        sc = rq_load_as<floatx8>(w.scales + (int64_t)g[0] * w.lds + r);
+      } else {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) sc[k] = r + k < w.R ? rq_scale_of(w, g[0], r + k) : 0.0f;
+      }
+    }
+    bf16x8 d[NT][P::dy];
+#pragma unroll
+    for (int b = 0; b < NT; ++b) {
+      if constexpr (P::dy == 1) {
+        __builtin_memcpy(&d[b][0], &raw[b], 16);
+      } else {
+        floatx8 f;
+        fp32_of(raw[b], f);
+        if (MODE == RQ_RUNS) {
+#pragma unroll
+          for (int k = 0; k < 8; ++k) f[k] *= sc[k];
+        }
+        rq_operand<P::dy>(f, d[b]);
+      }
+    }
+    // an inf's product with a piece of 0 would be a NaN that the formula does not have
+    bf16x8 low[NT];
+    if constexpr (P::w > 1) {
+#pragma unroll
+      for (int b = 0; b < NT; ++b)
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const float v = (float)d[b][0][k];
+          low[b][k] = __builtin_fabsf(v) == INFINITY ? (__bf16)0.0f : d[b][0][k];
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {                                  // fields to bit 0, two's complement
+#pragma unroll
+      for (int m = 0; m < Col8<NB>::N; ++m) {
+        const uint32_t hi = m + 1 < Col8<NB>::NW ? wd[k][m + 1] : 0u;
+        uint32_t v = NB % 4 == 0 ? wd[k][m] : (uint32_t)((((uint64_t)hi << 32) | wd[k][m]) >> off);
+        wd[k][m] = v ^ rq_top_bits<NB>(m);
+      }
+    }
+#pragma unroll
+    for (int n = 0; n < 8; ++n) {
+      bf16x8 v[P::w];
+      if constexpr (P::w == 1) {
+#pragma unroll
+        for (int k = 0; k < 8; k += 2) rq_set2(v[0], k, (float)col_code<NB>(wd[k], n), (float)col_code<NB>(wd[k + 1], n));
+      } else {
+        floatx8 f;
+        if (MODE == RQ_ANY) {
+#pragma unroll
+          for (int k = 0; k < 8; ++k) sc[k] = r + k < w.R ? rq_scale_of(w, g[n], r + k) : 0.0f;
+        }
+#pragma unroll
+        for (int k = 0; k < 8; ++k) f[k] = sc[k] * (float)col_code<NB>(wd[k], n);
+        rq_operand<P::w>(f, v);
+      }
+#pragma unroll
+      for (int b = 0; b < NT; ++b)
+#pragma unroll
+        for (int pd = 0; pd < P::dy; ++pd)
+#pragma unroll
+          for (int pw = 0; pw < P::w; ++pw)
+            if (pd + pw < P::keep) {
+              if constexpr (P::w > 1) acc[n][b] = rq_mfma(pd == 0 && pw ? low[b] : d[b][pd], v[pw], acc[n][b]);
+              else acc[n][b] = rq_mfma(d[b][pd], v[pw], acc[n][b]);
+            }
+    }
+  }
+  // The waves' sums, halved together: always in the same order.
+#pragma unroll
+  for (int half = W / 2; half; half >>= 1) {
+    if (wave >= half && wave < 2 * half) {
+#pragma unroll
+      for (int n = 0; n < 8; ++n)
+#pragma unroll
+        for (int b = 0; b < NT; ++b) join[wave - half][n * NT + b][lane] = acc[n][b];
+    }
+    __syncthreads();
+    if (wave < half) {
+#pragma unroll
+      for (int n = 0; n < 8; ++n)
+#pragma unroll
+        for (int b = 0; b < NT; ++b) acc[n][b] += join[wave][n * NT + b][lane];
+    }
+    __syncthreads();
+  }
+  if (wave) return;
+#pragma unroll
+  for (int b = 0; b < NT; ++b)
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int t = t0 + 16 * b + 4 * q + k;
+      if (t >= T) continue;
+#pragma unroll
+      for (int n = 0; n < 8; ++n) {
+        if (n >= nc) continue;
+        if (part) part[((int64_t)blockIdx.y * T + t) * w.C + c + n] = acc[n][b][k];
+        else dx[(int64_t)t * ldx + c + n] = rq_cast<TX>(acc[n][b][k]);
+      }
+    }
+}
+
+template <typename TX>
+__global__ __launch_bounds__(256) void k_packed_join(const float* __restrict__ part, int nparts, int T, int C,
+                                                     TX* __restrict__ dx, int64_t ldx) {
+  const int c = blockIdx.x * 256 + threadIdx.x, t = blockIdx.y;
+  if (c >= C) return;
+  float s = 0.0f;
+  for (int p = 0; p < nparts; ++p) s += part[((int64_t)p * T + t) * C + c];
+  dx[(int64_t)t * ldx + c] = rq_cast<TX>(s);
+}
+
+template <typename TX, int NB, int MODE, int NT>
+void launch_cols(const TX* dy, int T, int64_t ldy, const RqPacked& w, const RqColSplit& sp, float* part, TX* dx, int64_t ldx,
+                 hipStream_t s) {
+  hipLaunchKernelGGL((k_packed_cols<TX, NB, MODE, NT>), dim3((w.C + COLS - 1) / COLS, sp.parts, (T + 16 * NT - 1) / (16 * NT)),
+                     dim3(64 * cols_waves(NT)), 0, s, dy, T, ldy, w, sp.steps_per, sp.parts > 1 ? part : nullptr, dx, ldx);
+}
+template <typename TX, int NB, int MODE>
+void linear_cols(const TX* dy, int T, int64_t ldy, const RqPacked& w, const RqColSplit& sp, float* part, TX* dx, int64_t ldx,
+                 hipStream_t s) {
+  constexpr int NT = RqOperand<TX>::pieces == 1 ? 4 : 2;        // fp32's pieces leave registers for two token tiles
+  if (T <= 16) launch_cols<TX, NB, MODE, 1>(dy, T, ldy, w, sp, part, dx, ldx, s);
+  else if (T <= 32) launch_cols<TX, NB, MODE, 2>(dy, T, ldy, w, sp, part, dx, ldx, s);
+  else launch_cols<TX, NB, MODE, NT>(dy, T, ldy, w, sp, part, dx, ldx, s);
+}
+
+}  // namespace
+
+template <typename TX>
+void rq_linear_cols(const TX* dy, int T, int64_t ldy, const RqPacked& w, int nbits, float* part, TX* dx, int64_t ldx,
+                    hipStream_t s) {
+  rq_with_nbits(nbits, [&](auto nb) {
+    constexpr int NB = decltype(nb)::value;
+    for (int64_t t0 = 0; t0 < T; t0 += RQ_COL_TOKENS) {
+      const int n = (int)(T - t0 < RQ_COL_TOKENS ? T - t0 : RQ_COL_TOKENS);
+      const RqColSplit sp = rq_col_split(n, w.R, w.C);
+      const TX* d = dy + t0 * ldy;
+      TX* out = dx + t0 * ldx;
+      if (w.ngroups == 1 || (w.groupsize > 0 && w.groupsize % COLS == 0)) linear_cols<TX, NB, RQ_RUNS>(d, n, ldy, w, sp, part, out, ldx, s);
+      else if (w.groupsize > 0 && w.groupsize % 8 == 0) linear_cols<TX, NB, RQ_SMALL>(d, n, ldy, w, sp, part, out, ldx, s);
+      else linear_cols<TX, NB, RQ_ANY>(d, n, ldy, w, sp, part, out, ldx, s);
+      if (sp.parts > 1)
+        hipLaunchKernelGGL(k_packed_join<TX>, dim3((w.C + 255) / 256, n), dim3(256), 0, s, part, sp.parts, n, w.C, out, ldx);
+    }
+  });
+}

@@ -526,74 +526,81 @@ def block_gd_step(Wp, R_s, i2, grad, perm, optimizer, step, lr, grad_clip, exp_a
 
 
 # --- working with packed weights; scoring ---------------------------------------------------
-def packed_linear(x, qweight, nbits, scales, C, g_idx=None, groupsize=0, bias=None):
+# Pointers go to these entry points as plain ints and the stream without a Stream object: a call on one
+# token is bound by the host.
+def _addr(t):
+    return None if t is None else t.data_ptr()
+
+
+def packed_linear(x, qweight, nbits, scales, T, R, C, ngroups, g_idx, groupsize=0, bias=None):
     """y [T, R] = x [T, C] times the transpose of a packed weight, in x's dtype; see rq_packed_linear."""
-    T, R = x.shape[0], qweight.shape[0]
-    y = torch.empty((T, R), dtype=x.dtype, device=x.device)
-    nat.call("rq_packed_linear", nat.ptr(x), nat.dtype_code(x.dtype), T, x.stride(0), C, nat.ptr(qweight),
-             qweight.stride(0), nbits, R, nat.ptr(scales), scales.stride(0), scales.shape[0], nat.ptr(g_idx), groupsize,
-             nat.ptr(bias), nat.ptr(y), R, _stream(x))
+    y = x.new_empty((T, R))
+    nat.check("rq_packed_linear", nat.load().rq_packed_linear(
+        x.data_ptr(), nat.DTYPE_CODES[x.dtype], T, x.stride(0), C, qweight.data_ptr(), qweight.stride(0), nbits, R,
+        scales.data_ptr(), scales.stride(0), ngroups, g_idx.data_ptr(), groupsize, _addr(bias), y.data_ptr(), R,
+        nat.raw_stream(x)))
     return y
 
 
-def packed_linear_grad(grad_y, qweight, nbits, scales, C, g_idx=None, groupsize=0):
+def packed_linear_grad(grad_y, qweight, nbits, scales, T, R, C, ngroups, g_idx, groupsize=0):
     """grad_x [T, C] = grad_y [T, R] times a packed weight; see rq_packed_linear_grad."""
-    T, R = grad_y.shape
-    gx = torch.empty((T, C), dtype=grad_y.dtype, device=grad_y.device)
-    nbytes = int(nat.load().rq_packed_linear_grad_workspace_bytes(T, R, C))
+    lib = nat.load()
+    gx = grad_y.new_empty((T, C))
+    nbytes = lib.rq_packed_linear_grad_workspace_bytes(T, R, C)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=grad_y.device)
-    nat.call("rq_packed_linear_grad", nat.ptr(grad_y), nat.dtype_code(grad_y.dtype), T, grad_y.stride(0), C,
-             nat.ptr(qweight), qweight.stride(0), nbits, R, nat.ptr(scales), scales.stride(0), scales.shape[0],
-             nat.ptr(g_idx), groupsize, nat.ptr(gx), C, nat.ptr(ws), nbytes, _stream(grad_y))
+    nat.check("rq_packed_linear_grad", lib.rq_packed_linear_grad(
+        grad_y.data_ptr(), nat.DTYPE_CODES[grad_y.dtype], T, grad_y.stride(0), C, qweight.data_ptr(), qweight.stride(0),
+        nbits, R, scales.data_ptr(), scales.stride(0), ngroups, g_idx.data_ptr(), groupsize, gx.data_ptr(), C,
+        ws.data_ptr(), nbytes, nat.raw_stream(grad_y)))
     return gx
 
 
-def _experts(qweight, nbits, scales, g_idx, groupsize):
-    return nat.PackedExperts(qweight.data_ptr(), scales.data_ptr(), g_idx.data_ptr() if g_idx is not None else None,
-                             qweight.stride(1), scales.stride(1), qweight.stride(0), scales.stride(0), nbits,
-                             scales.shape[1], groupsize)
+def _experts(qweight, nbits, scales, ngroups, g_idx, groupsize):
+    sq, ldp, _ = qweight.stride()
+    ss, lds, _ = scales.stride()
+    return nat.PackedExperts(qweight.data_ptr(), scales.data_ptr(), g_idx.data_ptr(), ldp, lds, sq, ss, nbits, ngroups,
+                             groupsize)
 
 
-def packed_moe(x, router, I, gate, up, down, top_k, norm_topk, want_routing=False):
+def packed_moe(x, router, T, D, I, E, gate, up, down, top_k, norm_topk, want_routing=False):
     """y [T, D] of a mixture-of-experts layer (and the chosen experts' int32 ids and fp32 weights
-    [T, top_k]); gate / up / down: (qweight [E, R, words], nbits, scales [E, ngroups, R], g_idx [E, C]
-    or None, groupsize); see rq_packed_moe."""
-    T, D = x.shape
-    E = router.shape[0]
-    y = torch.empty((T, D), dtype=x.dtype, device=x.device)
+    [T, top_k]); gate / up / down: (qweight [E, R, words], nbits, scales [E, ngroups, R], ngroups,
+    g_idx [E, C], groupsize); see rq_packed_moe."""
+    lib = nat.load()
+    y = x.new_empty((T, D))
     ids = torch.empty((T, top_k), dtype=torch.int32, device=x.device) if want_routing else None
     weights = torch.empty((T, top_k), dtype=_f32, device=x.device) if want_routing else None
-    nbytes = int(nat.load().rq_packed_moe_workspace_bytes(T, D, I, E, top_k))
+    nbytes = lib.rq_packed_moe_workspace_bytes(T, D, I, E, top_k)
     ws = torch.empty(max(nbytes, 0), dtype=torch.uint8, device=x.device)
-    g, u, d = _experts(*gate), _experts(*up), _experts(*down)
-    nat.call("rq_packed_moe", nat.ptr(x), nat.dtype_code(x.dtype), T, x.stride(0), D, nat.ptr(router), router.stride(0),
-             E, top_k, int(bool(norm_topk)), I, ctypes.byref(g), ctypes.byref(u), ctypes.byref(d), nat.ptr(y), D,
-             nat.ptr(ids), nat.ptr(weights), nat.ptr(ws), nbytes, _stream(x))
+    nat.check("rq_packed_moe", lib.rq_packed_moe(
+        x.data_ptr(), nat.DTYPE_CODES[x.dtype], T, x.stride(0), D, router.data_ptr(), router.stride(0), E, top_k,
+        1 if norm_topk else 0, I, ctypes.byref(_experts(*gate)), ctypes.byref(_experts(*up)), ctypes.byref(_experts(*down)),
+        y.data_ptr(), D, _addr(ids), _addr(weights), ws.data_ptr(), nbytes, nat.raw_stream(x)))
     return y, ids, weights
 
 
-def token_logprobs(logits, targets, top_k, ignore_index):
+def token_logprobs(logits, targets, N, V, top_k, ignore_index):
     """(logprob [N], entropy [N], top_ids [N, k], top_logprobs [N, k], stats [N, 3]); see
     rq_token_logprobs."""
-    N, V = logits.shape
+    lib = nat.load()
     dev = logits.device
     out = torch.empty((5 * N,), dtype=_f32, device=dev)
     logprob, entropy, stats = out[:N], out[N:2 * N], out[2 * N:].view(N, 3)
     ids = torch.empty((N, top_k), dtype=torch.int64, device=dev)
     top = torch.empty((N, top_k), dtype=_f32, device=dev)
-    nbytes = int(nat.load().rq_token_logprobs_workspace_bytes(N, V, top_k))
+    nbytes = lib.rq_token_logprobs_workspace_bytes(N, V, top_k)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes > 0 else None
-    nat.call("rq_token_logprobs", nat.ptr(logits), nat.dtype_code(logits.dtype), N, logits.stride(0), V,
-             nat.ptr(targets), ignore_index, top_k, nat.ptr(logprob), nat.ptr(entropy), nat.ptr(ids), nat.ptr(top),
-             nat.ptr(stats), nat.ptr(ws), nbytes, _stream(logits))
+    at = out.data_ptr()
+    nat.check("rq_token_logprobs", lib.rq_token_logprobs(
+        logits.data_ptr(), nat.DTYPE_CODES[logits.dtype], N, logits.stride(0), V, targets.data_ptr(), ignore_index, top_k,
+        at, at + 4 * N, ids.data_ptr(), top.data_ptr(), at + 8 * N, _addr(ws), nbytes, nat.raw_stream(logits)))
     return logprob, entropy, ids, top, stats
 
 
-def token_logprobs_grad(logits, targets, ignore_index, stats, grad_logprob, grad_entropy=None):
+def token_logprobs_grad(logits, targets, N, V, ignore_index, stats, grad_logprob, grad_entropy=None):
     """grad_logits [N, V] in the logits' dtype; see rq_token_logprobs_grad."""
-    N, V = logits.shape
-    gz = torch.empty((N, V), dtype=logits.dtype, device=logits.device)
-    nat.call("rq_token_logprobs_grad", nat.ptr(logits), nat.dtype_code(logits.dtype), N, logits.stride(0), V,
-             nat.ptr(targets), ignore_index, nat.ptr(stats), nat.ptr(grad_logprob), nat.ptr(grad_entropy), nat.ptr(gz),
-             V, _stream(logits))
+    gz = logits.new_empty((N, V))
+    nat.check("rq_token_logprobs_grad", nat.load().rq_token_logprobs_grad(
+        logits.data_ptr(), nat.DTYPE_CODES[logits.dtype], N, logits.stride(0), V, targets.data_ptr(), ignore_index,
+        stats.data_ptr(), grad_logprob.data_ptr(), _addr(grad_entropy), gz.data_ptr(), V, nat.raw_stream(logits)))
     return gz

@@ -22,53 +22,59 @@ import torch
 from . import _native as nat
 from . import kernels as K
 
-_FLOATS = (torch.float16, torch.bfloat16, torch.float32)
-
-
 def _checked(entry: Dict[str, object], batch: int):
-    """(qweight, nbits, scales, C, g_idx, groupsize) of an entry (batch = 1: stacked over experts)."""
-    q, scales, g_idx, nbits = entry["qweight"], entry["scales"], entry["g_idx"], int(entry["nbits"])
-    groupsize = int(entry.get("groupsize", 0))
-    for t, name, dtype in ((q, "qweight", torch.int32), (scales, "scales", torch.float32), (g_idx, "g_idx", torch.int32)):
-        if not (isinstance(t, torch.Tensor) and t.is_cuda):
-            nat.require_gpu(t, name)
-        if t.dtype != dtype:
-            raise ValueError(f"packed entry: {name} must be {dtype}")
+    """(qweight, nbits, scales, R, C, ngroups, g_idx, groupsize) of an entry (batch = 1: stacked over
+    experts)."""
+    q, scales, g_idx, nbits = entry["qweight"], entry["scales"], entry["g_idx"], entry["nbits"]
+    groupsize = entry.get("groupsize", 0)
+    if not (q.is_cuda and scales.is_cuda and g_idx.is_cuda):
+        for t, name in ((q, "qweight"), (scales, "scales"), (g_idx, "g_idx")):
+            nat.require_gpu(t, f"packed entry: {name}")
+    if q.dtype is not torch.int32 or scales.dtype is not torch.float32 or g_idx.dtype is not torch.int32:
+        raise ValueError("packed entry: qweight and g_idx must be int32, scales float32")
     if not 2 <= nbits <= nat.RQ_PACKED_MAXBITS:
         raise NotImplementedError(f"packed weights of {nbits} bits: 2 to {nat.RQ_PACKED_MAXBITS} are supported")
-    if q.dim() != 2 + batch or scales.dim() != 2 + batch or g_idx.dim() != 1 + batch:
+    qs, ss, gs = q.shape, scales.shape, g_idx.shape
+    if len(qs) != 2 + batch or len(ss) != 2 + batch or len(gs) != 1 + batch:
         raise ValueError("packed entry: qweight [R, words], scales [ngroups, R] and g_idx [C] are expected"
                          + (", each with a leading expert dimension (stack_packed)" if batch else ""))
-    C, R, ng = g_idx.shape[-1], q.shape[-2], scales.shape[-2]
-    if C == 0 or R == 0 or ng == 0 or q.shape[-1] * 32 < C * nbits or scales.shape[-1] != R:
+    R, words, ng, C = qs[-2], qs[-1], ss[-2], gs[-1]
+    if C == 0 or R == 0 or ng == 0 or words * 32 < C * nbits or ss[-1] != R:
         raise ValueError("packed entry: the shapes of qweight, scales and g_idx do not belong together")
-    if batch and not (q.shape[0] == scales.shape[0] == g_idx.shape[0]):
+    if batch and not qs[0] == ss[0] == gs[0]:
         raise ValueError("packed entry: qweight, scales and g_idx hold different numbers of experts")
     if groupsize < 0 or (groupsize and ng > 1 and (C - 1) // groupsize >= ng):
         raise ValueError(f"packed entry: groupsize {groupsize} does not fit {ng} groups of {C} columns")
-    if not (q.device == scales.device == g_idx.device):
+    dev = q.get_device()
+    if scales.get_device() != dev or g_idx.get_device() != dev:
         raise ValueError("packed entry: qweight, scales and g_idx are on different devices")
-    if q.stride(-1) != 1 or scales.stride(-1) != 1 or (batch and q.stride(-2) < q.shape[-1]):
+    qst, sst = q.stride(), scales.stride()
+    if qst[-1] != 1 or sst[-1] != 1 or (qst[-2] < words and R > 1) or (sst[-2] < R and ng > 1):
         raise ValueError("packed entry: qweight and scales need unit column strides")
-    return q, nbits, scales, C, g_idx if g_idx.is_contiguous() else g_idx.contiguous(), groupsize
+    return (q if qst[-2] >= words else q.contiguous(), nbits, scales if sst[-2] >= R else scales.contiguous(), R, C, ng,
+            g_idx if g_idx.is_contiguous() else g_idx.contiguous(), groupsize)
 
 
-def _tokens(x, width, device, name):
-    """x as [T, width] with unit column stride (copied only if its strides need it)."""
+def _tokens(x, width, q, name):
+    """x as [T, width] with unit column stride (copied only if its strides need it), and T."""
     if not (isinstance(x, torch.Tensor) and x.is_cuda):
         nat.require_gpu(x, name)
-    if x.dtype not in _FLOATS:
+    if x.dtype not in nat.DTYPE_CODES:
         raise TypeError(f"{name}: unsupported dtype {x.dtype}; expected float16, bfloat16 or float32")
-    if x.dim() < 1 or x.shape[-1] != width:
-        raise ValueError(f"{name} must be [..., {width}], got {tuple(x.shape)}")
-    if x.device != device:
-        raise ValueError(f"{name} is on {x.device}, the packed weight on {device}")
-    x2 = x if x.dim() == 2 else x.reshape(-1, width)
-    if x2.stride(1) != 1 or (x2.stride(0) < width and x2.shape[0] > 1):
-        x2 = x2.contiguous()
-    elif x2.stride(0) < width:                   # one token: its row stride is never used
-        x2 = x2.as_strided((1, width), (width, 1))
-    return x2
+    shape = x.shape
+    if len(shape) < 1 or shape[-1] != width:
+        raise ValueError(f"{name} must be [..., {width}], got {tuple(shape)}")
+    if x.get_device() != q.get_device():
+        raise ValueError(f"{name} is on {x.device}, the packed weight on {q.device}")
+    x2 = x if len(shape) == 2 else x.reshape(-1, width)
+    T = x2.shape[0]
+    s0, s1 = x2.stride()
+    if s1 != 1 or s0 < width:
+        if T > 1 or s1 != 1:
+            x2 = x2.contiguous()
+        if x2.stride(0) < width:                 # one token: its row stride is never used
+            x2 = x2.as_strided((T, width), (width, 1))
+    return x2, T
 
 
 class _PackedLinear(torch.autograd.Function):
@@ -83,14 +89,14 @@ class _PackedLinear(torch.autograd.Function):
 
 
 def _forward(x, entry, bias):
-    q, nbits, scales, C, g_idx, groupsize = _checked(entry, 0)
-    x2 = _tokens(x, C, q.device, "x")
+    q, nbits, scales, R, C, ng, g_idx, groupsize = _checked(entry, 0)
+    x2, T = _tokens(x, C, q, "x")
     if bias is not None:
-        if bias.dtype != x.dtype or bias.shape != (q.shape[0],) or bias.device != x.device:
-            raise ValueError(f"bias must be {x.dtype} [{q.shape[0]}] on {x.device}")
+        if bias.dtype != x.dtype or bias.shape != (R,) or bias.device != x.device:
+            raise ValueError(f"bias must be {x.dtype} [{R}] on {x.device}")
         bias = bias.contiguous()
-    y = K.packed_linear(x2, q, nbits, scales, C, g_idx, groupsize, bias)
-    return y if x.dim() == 2 else y.view(*x.shape[:-1], q.shape[0])
+    y = K.packed_linear(x2, q, nbits, scales, T, R, C, ng, g_idx, groupsize, bias)
+    return y if x.dim() == 2 else y.view(*x.shape[:-1], R)
 
 
 def packed_linear(x: torch.Tensor, entry: Dict[str, object], bias: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -109,9 +115,9 @@ def packed_linear(x: torch.Tensor, entry: Dict[str, object], bias: Optional[torc
 def packed_linear_backward(grad_y: torch.Tensor, entry: Dict[str, object]) -> torch.Tensor:
     """The gradient of ``packed_linear``'s x: ``grad_y [..., R]`` times the packed weight, ``[..., C]`` in
     grad_y's dtype.  The result does not change from run to run."""
-    q, nbits, scales, C, g_idx, groupsize = _checked(entry, 0)
-    g2 = _tokens(grad_y, q.shape[0], q.device, "grad_y")
-    gx = K.packed_linear_grad(g2, q, nbits, scales, C, g_idx, groupsize)
+    q, nbits, scales, R, C, ng, g_idx, groupsize = _checked(entry, 0)
+    g2, T = _tokens(grad_y, R, q, "grad_y")
+    gx = K.packed_linear_grad(g2, q, nbits, scales, T, R, C, ng, g_idx, groupsize)
     return gx if grad_y.dim() == 2 else gx.view(*grad_y.shape[:-1], C)
 
 
@@ -148,22 +154,25 @@ def packed_moe(x: torch.Tensor, router: torch.Tensor, gate: Dict[str, object], u
     if torch.is_grad_enabled() and isinstance(x, torch.Tensor) and (x.requires_grad or router.requires_grad):
         raise NotImplementedError("packed_moe has no backward pass: call it under torch.no_grad() or on detached tensors")
     g, u, d = _checked(gate, 1), _checked(up, 1), _checked(down, 1)
-    E, I, _ = g[0].shape
-    D = g[3]
-    if u[0].shape[:2] != (E, I) or u[3] != D or d[0].shape[:2] != (E, D) or d[3] != I:
+    E, I, D = g[0].shape[0], g[3], g[4]
+    if u[0].shape[0] != E or d[0].shape[0] != E or u[3] != I or u[4] != D or d[3] != D or d[4] != I:
         raise ValueError("packed_moe: gate and up must be [E, I x D] and down [E, D x I]")
-    if not (u[0].device == d[0].device == g[0].device):
+    if not u[0].get_device() == d[0].get_device() == g[0].get_device():
         raise ValueError("packed_moe: gate, up and down are on different devices")
-    x2 = _tokens(x, D, g[0].device, "x")
+    x2, T = _tokens(x, D, g[0], "x")
     if not isinstance(router, torch.Tensor) or router.shape != (E, D) or router.dtype != x.dtype or router.device != x.device:
         raise ValueError(f"packed_moe: router must be {x.dtype} [{E}, {D}] on {x.device}")
     top_k = int(top_k)
     if E > nat.RQ_MOE_MAX_EXPERTS or not 1 <= top_k <= min(E, nat.RQ_MOE_MAX_TOP):
         raise ValueError(f"packed_moe: top_k {top_k} of {E} experts (at most {nat.RQ_MOE_MAX_TOP} of "
                          f"{nat.RQ_MOE_MAX_EXPERTS})")
-    router = router if router.stride(1) == 1 and router.stride(0) >= D else router.contiguous()
-    args = [(q, nbits, scales, g_idx, groupsize) for q, nbits, scales, _, g_idx, groupsize in (g, u, d)]
-    y, ids, weights = K.packed_moe(x2, router, I, *args, top_k, norm_topk, return_routing)
+    r0, r1 = router.stride()
+    if r1 != 1 or r0 < D:
+        router = router.contiguous()
+        if router.stride(0) < D:
+            router = router.as_strided((E, D), (D, 1))
+    args = [(q, nbits, scales, ng, gi, gs) for q, nbits, scales, _, _, ng, gi, gs in (g, u, d)]
+    y, ids, weights = K.packed_moe(x2, router, T, D, I, E, *args, top_k, norm_topk, return_routing)
     y = y if x.dim() == 2 else y.view(x.shape)
     if not return_routing:
         return y

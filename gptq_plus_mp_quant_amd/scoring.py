@@ -14,8 +14,6 @@ import torch
 from . import _native as nat
 from . import kernels as K
 
-_FLOATS = (torch.float16, torch.bfloat16, torch.float32)
-
 
 class TokenLogprobs(NamedTuple):
     """``logprob`` and ``entropy`` fp32 ``[...]``; ``top_ids`` int64 and ``top_logprobs`` fp32
@@ -31,29 +29,31 @@ class TokenLogprobs(NamedTuple):
 def _rows(logits, targets):
     if not (isinstance(logits, torch.Tensor) and logits.is_cuda):
         nat.require_gpu(logits, "logits")
-    if logits.dtype not in _FLOATS:
+    if logits.dtype not in nat.DTYPE_CODES:
         raise TypeError(f"logits: unsupported dtype {logits.dtype}; expected float16, bfloat16 or float32")
-    if logits.dim() < 1 or logits.shape[-1] == 0:
+    shape = logits.shape
+    if len(shape) < 1 or shape[-1] == 0:
         raise ValueError("logits must be [..., V] with V > 0")
-    if not isinstance(targets, torch.Tensor) or targets.dtype != torch.int64 or targets.shape != logits.shape[:-1] or \
+    if not isinstance(targets, torch.Tensor) or targets.dtype is not torch.int64 or targets.shape != shape[:-1] or \
             targets.device != logits.device:
-        raise ValueError(f"targets must be int64 {list(logits.shape[:-1])} on {logits.device}")
-    V = logits.shape[-1]
-    z = logits if logits.dim() == 2 else logits.reshape(-1, V)
-    if z.stride(1) != 1 or z.stride(0) < V:
+        raise ValueError(f"targets must be int64 {list(shape[:-1])} on {logits.device}")
+    V = shape[-1]
+    z = logits if len(shape) == 2 else logits.reshape(-1, V)
+    s0, s1 = z.stride()
+    if s1 != 1 or s0 < V:
         z = z.contiguous()
         if z.stride(0) < V:                      # one row: its stride is never used
             z = z.as_strided((z.shape[0], V), (V, 1))
     t = targets if targets.dim() == 1 else targets.reshape(-1)
-    return z, t if t.is_contiguous() else t.contiguous()
+    return z, t if t.is_contiguous() else t.contiguous(), z.shape[0], V
 
 
 def _forward(logits, targets, top_k, ignore_index):
-    z, t = _rows(logits, targets)
+    z, t, N, V = _rows(logits, targets)
     top_k = int(top_k)
-    if not 0 <= top_k <= min(nat.RQ_SCORE_MAX_TOP, z.shape[1]):
-        raise ValueError(f"top_k must be 0 to {min(nat.RQ_SCORE_MAX_TOP, z.shape[1])}, got {top_k}")
-    lp, H, ids, top, stats = K.token_logprobs(z, t, top_k, int(ignore_index))
+    if not 0 <= top_k <= min(nat.RQ_SCORE_MAX_TOP, V):
+        raise ValueError(f"top_k must be 0 to {min(nat.RQ_SCORE_MAX_TOP, V)}, got {top_k}")
+    lp, H, ids, top, stats = K.token_logprobs(z, t, N, V, top_k, int(ignore_index))
     if logits.dim() != 2:
         lead = logits.shape[:-1]
         lp, H = lp.view(lead), H.view(lead)
@@ -100,11 +100,12 @@ def token_logprobs_backward(logits: torch.Tensor, targets: torch.Tensor, stats: 
                             grad_entropy: Optional[torch.Tensor] = None, ignore_index: int = -100) -> torch.Tensor:
     """The gradient of ``logits`` from the gradients of ``logprob`` and (optionally) ``entropy``, in the
     logits' dtype; ``stats`` is what ``token_logprobs`` returned for the same logits."""
-    z, t = _rows(logits, targets)
+    z, t, N, V = _rows(logits, targets)
     gl = _row_grads(grad_logprob, logits, "grad_logprob")
     gh = None if grad_entropy is None else _row_grads(grad_entropy, logits, "grad_entropy")
     if not isinstance(stats, torch.Tensor) or stats.dtype != torch.float32 or stats.shape != (*logits.shape[:-1], 3) or \
             stats.device != logits.device:
         raise ValueError(f"stats must be token_logprobs' float32 {list(logits.shape[:-1]) + [3]} on {logits.device}")
-    gz = K.token_logprobs_grad(z, t, int(ignore_index), stats if stats.is_contiguous() else stats.contiguous(), gl, gh)
+    gz = K.token_logprobs_grad(z, t, N, V, int(ignore_index), stats if stats.is_contiguous() else stats.contiguous(), gl,
+                               gh)
     return gz if logits.dim() == 2 else gz.view(logits.shape)

@@ -585,7 +585,7 @@ def token_logprobs(logits, targets, N, V, top_k, ignore_index):
     lib = nat.load()
     dev = logits.device
     out = torch.empty((5 * N,), dtype=_f32, device=dev)
-    logprob, entropy, stats = out[:N], out[N:2 * N], out[2 * N:].view(N, 3)
+    logprob, entropy, stats = out.split_with_sizes((N, N, 3 * N))
     ids = torch.empty((N, top_k), dtype=torch.int64, device=dev)
     top = torch.empty((N, top_k), dtype=_f32, device=dev)
     nbytes = lib.rq_token_logprobs_workspace_bytes(N, V, top_k)
@@ -594,7 +594,7 @@ def token_logprobs(logits, targets, N, V, top_k, ignore_index):
     nat.check("rq_token_logprobs", lib.rq_token_logprobs(
         logits.data_ptr(), nat.DTYPE_CODES[logits.dtype], N, logits.stride(0), V, targets.data_ptr(), ignore_index, top_k,
         at, at + 4 * N, ids.data_ptr(), top.data_ptr(), at + 8 * N, _addr(ws), nbytes, nat.raw_stream(logits)))
-    return logprob, entropy, ids, top, stats
+    return logprob, entropy, ids, top, stats.view(N, 3)
 
 
 def token_logprobs_grad(logits, targets, N, V, ignore_index, stats, grad_logprob, grad_entropy=None):

@@ -398,7 +398,7 @@ int rq_packed_moe(const void* x, int dtype, int T, int64_t ldx, int D, const voi
                   void* stream);
 
 /* --- Scoring ------------------------------------------------------------------------------
- * Per row of logits [N, V] (row stride ldz, type dtype): logprob[n] = log softmax(z)[targets[n]] (0
+ * Per row of logits [N, V] (V <= 2^30, row stride ldz, type dtype): logprob[n] = log softmax(z)[targets[n]] (0
  * where targets[n] == ignore_index, NaN for any other target outside [0, V)), entropy[n], and the
  * top_k (<= 64) largest logits' indices and log probabilities, [N, top_k] in order (equal values by
  * their index, NaN first).  stats [N, 3] receives the row's maximum, log sum exp(z - max) and entropy

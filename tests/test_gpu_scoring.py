@@ -83,7 +83,8 @@ def check_grad(z, t, ignore=-100, entropy=True, z_dev=None):
 @pytest.mark.parametrize("dtype", [F16, BF16, F32])
 @pytest.mark.parametrize("N,V,k", [(1, 1, 1), (1, 2, 2), (2, 3, 1), (3, 63, 20), (1, 64, 64), (4, 65, 64), (5, 500, 5),
                                    (1, 1000, 0), (1, 32003, 20), (7, 8191, 8), (2, 8193, 1), (300, 257, 4), (37, 32000, 20),
-                                   (1, 128256, 64), (3, 100001, 20), (1100, 2000, 3)])
+                                   (1, 128256, 64), (3, 100001, 20), (1100, 2000, 3),
+                                   (2, 300001, 20), (512, 8200, 9)])
 def test_shapes(N, V, k, dtype):
     z, t = randn(N + V, N, V, dtype=dtype, scale=3.0), ints(V, V, N)
     check(z, t, k)
@@ -93,7 +94,7 @@ def test_shapes(N, V, k, dtype):
 
 @pytest.mark.parametrize("dtype", [F16, BF16, F32])
 @pytest.mark.parametrize("order", ["up", "down", "equal", "late"])
-@pytest.mark.parametrize("N,V", [(1, 40000), (600, 5000)])
+@pytest.mark.parametrize("N,V", [(1, 40000), (600, 5000), (1, 270000)])
 def test_orders(N, V, order, dtype):
     """Rows in rising, falling and equal order, and with all that counts at the end: the hardest for
     a running maximum and for a list of candidates kept on the way."""
@@ -102,6 +103,15 @@ def test_orders(N, V, order, dtype):
         torch.arange(V) < V - 70, -30.0, base)}[order]
     z = row.to(dtype).expand(N, V).contiguous()
     check(z, ints(1, V, N), 20)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16, F32])
+@pytest.mark.parametrize("steps", [2, 5, 40])
+@pytest.mark.parametrize("N,V", [(3, 30000), (520, 4100)])
+def test_many_equal_values(N, V, steps, dtype):
+    """Few distinct values, so that the last places always go to the lowest of many equal indices."""
+    z = torch.round(randn(steps, N, V) * steps / 4).to(dtype)
+    check(z, ints(1, V, N), 33)
 
 
 @pytest.mark.parametrize("dtype", [F16, BF16, F32])

@@ -21,7 +21,7 @@ LIBDIR = PKG / "_lib"
 LIB = LIBDIR / "libgptqplus_hip.so"
 SOURCES = ["hessian.hip", "params.hip", "argsort.hip", "chol.hip", "terms.hip", "colloop.hip", "pack.hip",
            "blockgd.hip", "plinear.hip", "plinear_f16.hip", "plinear_bf16.hip",
-           "plinear_f32.hip", "pmoe.hip", "logprobs.hip"]
+           "plinear_f32.hip", "pmoe.hip", "pmoe_f16.hip", "pmoe_bf16.hip", "pmoe_f32.hip", "logprobs.hip"]
 
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 FLAGS = [

@@ -155,6 +155,49 @@ __device__ __forceinline__ void rq_operand(floatx8 x, bf16x8 (&v)[P]) {
   }
 }
 
+// A lane's tokens, one for each of NT tiles: rows of x.
+template <typename TX, int NT>
+struct RqTokens {
+  typedef typename RqOperand<TX>::raw raw;
+  typedef typename RqOperand<TX>::vec vec;
+  static constexpr int tiles = NT, pieces = RqOperand<TX>::pieces;
+  const TX* p[NT];
+  template <bool FULL>
+  __device__ __forceinline__ raw load(int b, int c, int n) const { return rq_load_x<FULL>(p[b] + c, n); }
+  __device__ __forceinline__ float element(int b, int c) const { return rq_load_elem(p[b] + c); }
+};
+// The same for fp32 values that were stored as P bf16 pieces, `plane` elements from one piece to the next.
+template <int P>
+struct RqPieceRow {
+  bf16x8 v[P];
+};
+template <int P>
+__device__ __forceinline__ void rq_operand(const RqPieceRow<P>& x, bf16x8 (&v)[P]) {
+#pragma unroll
+  for (int p = 0; p < P; ++p) v[p] = x.v[p];
+}
+template <int P>
+struct RqPieces {
+  typedef RqPieceRow<P> raw;
+  typedef bf16x8 vec;
+  static constexpr int tiles = 1, pieces = P;
+  const __hip_bfloat16* p;
+  int64_t plane;
+  template <bool FULL>
+  __device__ __forceinline__ raw load(int, int c, int n) const {
+    raw r;
+#pragma unroll
+    for (int k = 0; k < P; ++k) r.v[k] = rq_load_x<FULL>(p + k * plane + c, n);
+    return r;
+  }
+  __device__ __forceinline__ float element(int, int c) const {
+    float f = rq_load_elem(p + c);
+#pragma unroll
+    for (int k = 1; k < P; ++k) f += rq_load_elem(p + k * plane + c);
+    return f;
+  }
+};
+
 // The scales of group g and rows r..r+3, without a branch: a load that would pass the table's end is moved
 // back and its values shifted up (rows past the weight get some scale, and are never stored).  The table
 // holds at least four (rq_mode_of).
@@ -192,19 +235,19 @@ __device__ __forceinline__ void rq_load_runs(const RqPacked& w, const uint32_t* 
     f.sc[a] = rq_scales4(w, g, r0 + 16 * a + 4 * q);
   }
 }
-template <bool FULL, typename TX, int NT>
-__device__ __forceinline__ void rq_load_tokens(const TX* const (&xp)[NT], int C, int ch,
-                                               typename RqOperand<TX>::raw (&x)[NT][4]) {
+template <bool FULL, typename X>
+__device__ __forceinline__ void rq_load_tokens(const X& xs, int C, int ch, typename X::raw (&x)[X::tiles][4]) {
   const int c = ch * RQ_CHUNK + 32 * ((threadIdx.x & 63) >> 4);
 #pragma unroll
-  for (int b = 0; b < NT; ++b)
+  for (int b = 0; b < X::tiles; ++b)
 #pragma unroll
-    for (int s = 0; s < 4; ++s) x[b][s] = rq_load_x<FULL>(xp[b] + c + 8 * s, C - c - 8 * s);
+    for (int s = 0; s < 4; ++s) x[b][s] = xs.template load<FULL>(b, c + 8 * s, C - c - 8 * s);
 }
-template <typename TX, int NB, int RT, int NT, int P>
-__device__ __forceinline__ void rq_chunk_runs(RqRunsW<NB, RT>& f, const typename RqOperand<TX>::raw (&x)[NT][4],
-                                              floatx4 (&acc)[RT][NT]) {
-  typedef typename RqOperand<TX>::vec V;
+template <typename X, int NB, int RT>
+__device__ __forceinline__ void rq_chunk_runs(RqRunsW<NB, RT>& f, const typename X::raw (&x)[X::tiles][4],
+                                              floatx4 (&acc)[RT][X::tiles]) {
+  typedef typename X::vec V;
+  constexpr int NT = X::tiles, P = X::pieces;
   floatx4 part[RT][NT];
 #pragma unroll
   for (int a = 0; a < RT; ++a) {
@@ -235,13 +278,13 @@ __device__ __forceinline__ void rq_chunk_runs(RqRunsW<NB, RT>& f, const typename
 }
 
 // Chunks first, first + step, ... of rows [r0, r0 + 16 RT): acc[a][b] += the weight's rows
-// r0 + 16 a + 4q.. times the lane's token of tile b.  xp: the lane's token rows; a lane without a token is
-// given any other's (its sums go nowhere).  lds: scales of the workgroup's rows for ANY, laid out by
-// rq_stage_scales.
-template <typename TX, int NB, int MODE, int RT, int NT, int P>
-__device__ __forceinline__ void rq_rows_tokens(const RqPacked& w, int r0, const TX* const (&xp)[NT], int first,
-                                               int step, const float* lds, floatx4 (&acc)[RT][NT]) {
-  typedef typename RqOperand<TX>::vec V;
+// r0 + 16 a + 4q.. times the lane's token of tile b.  A lane without a token is given any other's (its sums
+// go nowhere).  lds: scales of the workgroup's rows for ANY, laid out by rq_stage_scales, or NULL.
+template <int NB, int MODE, int RT, typename X>
+__device__ __forceinline__ void rq_rows_tokens(const RqPacked& w, int r0, const X& xs, int first, int step,
+                                               const float* lds, floatx4 (&acc)[RT][X::tiles]) {
+  typedef typename X::vec V;
+  constexpr int NT = X::tiles, P = X::pieces;
   const int lane = threadIdx.x & 63, i = lane & 15, q = lane >> 4;
   const uint32_t* row[RT];
 #pragma unroll
@@ -249,30 +292,35 @@ __device__ __forceinline__ void rq_rows_tokens(const RqPacked& w, int r0, const 
   const int nfull = w.C / RQ_CHUNK, nch = (w.C + RQ_CHUNK - 1) / RQ_CHUNK;
   int ch = first;
   if constexpr (MODE == RQ_RUNS) {
-    // The words of D chunks are in flight, a chunk's place refilled as soon as it has been used.
-    constexpr int D = RT * (NB + 4) <= 18 ? 4 : 2;
+    // The words of D chunks and the tokens of DX are in flight, a chunk's place refilled as soon as it has
+    // been used.
+    constexpr int D = RT * (NB + 4) <= 18 ? 4 : 2, DX = NT == 1 && sizeof(typename X::raw) <= 16 ? 2 : 1;
     const int n = ch < nfull ? (nfull - ch + step - 1) / step : 0;     // full chunks of this wave
     RqRunsW<NB, RT> f[D];
+    typename X::raw x[DX][NT][4];
 #pragma unroll
     for (int u = 0; u < D; ++u)
       if (u < n) rq_load_runs<true>(w, row, r0, ch + u * step, f[u]);
+    if constexpr (DX == 2) {
+#pragma unroll
+      for (int u = 0; u < DX; ++u)
+        if (u < n) rq_load_tokens<true>(xs, w.C, ch + u * step, x[u]);
+    }
     for (int k = 0; k < n; k += D) {
 #pragma unroll
       for (int u = 0; u < D; ++u) {
         if (k + u < n) {
-          typename RqOperand<TX>::raw x[NT][4];
-          rq_load_tokens<true, TX, NT>(xp, w.C, ch + (k + u) * step, x);
-          rq_chunk_runs<TX, NB, RT, NT, P>(f[u], x, acc);
+          if constexpr (DX == 1) rq_load_tokens<true>(xs, w.C, ch + (k + u) * step, x[0]);
+          rq_chunk_runs<X, NB, RT>(f[u], x[u % DX], acc);
+          if (DX == 2 && k + u + DX < n) rq_load_tokens<true>(xs, w.C, ch + (k + u + DX) * step, x[u % DX]);
           if (k + u + D < n) rq_load_runs<true>(w, row, r0, ch + (k + u + D) * step, f[u]);
         }
       }
     }
-    if (nfull < nch && (nfull - first) % step == 0 && nfull >= first) {       // the ragged end is this wave's
-      RqRunsW<NB, RT> t;
-      typename RqOperand<TX>::raw x[NT][4];
-      rq_load_runs<false>(w, row, r0, nfull, t);
-      rq_load_tokens<false, TX, NT>(xp, w.C, nfull, x);
-      rq_chunk_runs<TX, NB, RT, NT, P>(t, x, acc);
+    if (nfull < nch && nfull >= first && (nfull - first) % step == 0) {       // the ragged end is this wave's
+      rq_load_runs<false>(w, row, r0, nfull, f[0]);
+      rq_load_tokens<false>(xs, w.C, nfull, x[0]);
+      rq_chunk_runs<X, NB, RT>(f[0], x[0], acc);
     }
   } else if constexpr (MODE == RQ_SMALL) {
     for (; ch < nch; ch += step) {
@@ -293,7 +341,7 @@ __device__ __forceinline__ void rq_rows_tokens(const RqPacked& w, int r0, const 
         V x[NT][P];
 #pragma unroll
         for (int b = 0; b < NT; ++b)
-          rq_operand(c + 8 <= w.C ? rq_load_x<true>(xp[b] + c, 8) : rq_load_x<false>(xp[b] + c, w.C - c), x[b]);
+          rq_operand(c + 8 <= w.C ? xs.template load<true>(b, c, 8) : xs.template load<false>(b, c, w.C - c), x[b]);
 #pragma unroll
         for (int a = 0; a < RT; ++a) {
           V codes;
@@ -328,7 +376,7 @@ __device__ __forceinline__ void rq_rows_tokens(const RqPacked& w, int r0, const 
         const int g = j < n ? rq_group_of(w, c + j) : 0;
         float xv[NT];
 #pragma unroll
-        for (int b = 0; b < NT; ++b) xv[b] = j < n ? rq_load_elem(xp[b] + c + j) : 0.0f;
+        for (int b = 0; b < NT; ++b) xv[b] = j < n ? xs.element(b, c + j) : 0.0f;
 #pragma unroll
         for (int a = 0; a < RT; ++a) {
           const float s = lds ? lds[((unsigned)g < (unsigned)w.ngroups ? g : w.ngroups) * (16 * RT) + 16 * a + i]

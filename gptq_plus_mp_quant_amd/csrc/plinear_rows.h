@@ -14,9 +14,9 @@ __global__ __launch_bounds__(rows_threads(RT, NT)) void k_packed_rows(const TX* 
   extern __shared__ __attribute__((aligned(16))) float lds[];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
   const int r0 = blockIdx.x * 16 * RT, t0 = blockIdx.y * 16 * NT;
-  const TX* xp[NT];
+  RqTokens<TX, NT> xs;
 #pragma unroll
-  for (int b = 0; b < NT; ++b) xp[b] = x + (int64_t)min(t0 + 16 * b + (lane & 15), T - 1) * ldx;
+  for (int b = 0; b < NT; ++b) xs.p[b] = x + (int64_t)min(t0 + 16 * b + (lane & 15), T - 1) * ldx;
   const bool staged = MODE == RQ_ANY && w.ngroups <= RQ_STAGED_GROUPS;
   if (staged) {
     rq_stage_scales(w, r0, 16 * RT, lds);
@@ -27,7 +27,7 @@ __global__ __launch_bounds__(rows_threads(RT, NT)) void k_packed_rows(const TX* 
   for (int a = 0; a < RT; ++a)
 #pragma unroll
     for (int b = 0; b < NT; ++b) acc[a][b] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
-  rq_rows_tokens<TX, NB, MODE, RT, NT, RqOperand<TX>::pieces>(w, r0, xp, wave, waves, staged ? lds : nullptr, acc);
+  rq_rows_tokens<NB, MODE, RT>(w, r0, xs, wave, waves, staged ? lds : nullptr, acc);
   if (staged) __syncthreads();
   floatx4* out = reinterpret_cast<floatx4*>(lds);
 #pragma unroll

@@ -3,169 +3,200 @@
 //   l = x router^T, the K largest of l chosen (equal logits by their index), w = softmax(l) of the chosen
 //   (divided by their sum when norm), y = sum_k w_k Wd_k (silu(Wg_k x) * (Wu_k x)).
 //
-// Router logits, products, the activation and the sum over experts are fp32; the one rounding to fewer
-// bits is the result's to x's type.
-#include "packed_bits.h"
+// Four launches: the router's logits; the routing, which sorts the chosen (token, expert) pairs into units of
+// up to 16 tokens of one expert; gate, up and the activation of every unit; down, summed over a token's
+// experts.  An expert that no token chose is not read, one that several chose is read once for 16 of them.
+// Router logits, sums, the activation and the sum over experts are fp32 (the activation in bf16 pieces that
+// carry 16 bits or all 24); the one rounding to fewer bits is the result's to x's type.
+#include "packed_dot.h"
+#include "pmoe_types.h"
 
 namespace {
-
-constexpr int RW = 4;                 // rows per wave
-constexpr int MAX_E = 1024, MAX_K = 64;
-constexpr int TOKENS = 64;            // tokens per pass over the experts
-
-// The experts' weights: expert e's entry is w with its pointers moved by e strides.
-struct RqExperts {
-  RqPacked w;
-  int64_t sq, ss, sg;                 // strides of q, scales, g_idx from one expert to the next
-};
-__device__ __forceinline__ RqPacked expert(const RqExperts& x, int e) {
-  RqPacked w = x.w;
-  w.q += x.sq * e;
-  w.scales += x.ss * e;
-  if (w.g_idx) w.g_idx += x.sg * e;
-  return w;
-}
-
-// acc[i] += sum_c xv[c] * W[r0 + i, c] of the lane's columns
-template <int NB, typename TX>
-__device__ __forceinline__ void rows_dot(const RqPacked& w, const TX* __restrict__ x, int r0, float (&acc)[RW]) {
-  for (int c = (threadIdx.x & 63) * 8; c < w.C; c += 512) {
-    const int nc = min(8, w.C - c);
-    float xv[8];
-    int g[8];
-#pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      xv[k] = k < nc ? rq_load_elem(x + c + k) : 0.0f;
-      g[k] = rq_group_of(w, c + (k < nc ? k : 0));
-    }
-#pragma unroll
-    for (int i = 0; i < RW; ++i) {
-      const int r = min(r0 + i, w.R - 1);
-      int code[8];
-      rq_codes8<NB>(w.q + (int64_t)r * w.ldp, c, nc, code);
-#pragma unroll
-      for (int k = 0; k < 8; ++k)
-        acc[i] = __builtin_fmaf(xv[k], k < nc ? rq_scale_of(w, g[k], r) * (float)code[k] : 0.0f, acc[i]);
-    }
-  }
-}
 
 __device__ __forceinline__ float wave_sum(float v) {
 #pragma unroll
   for (int m = 32; m; m >>= 1) v += __shfl_xor(v, m);
   return v;
 }
+__device__ __forceinline__ int lanes_before(uint64_t mask) {
+  return __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0));
+}
 
+// A wave takes one expert and 8 tokens, 8 columns a lane.
+constexpr int ROUTER_TOKENS = 8;
 template <typename TX>
-__global__ __launch_bounds__(256) void k_moe_router(const TX* __restrict__ x, int64_t ldx, int D,
+__global__ __launch_bounds__(256) void k_moe_router(const TX* __restrict__ x, int64_t ldx, int T, int D,
                                                     const TX* __restrict__ router, int64_t ldr, int E,
                                                     float* __restrict__ logits) {
-  const int e = blockIdx.x * 4 + (threadIdx.x >> 6), t = blockIdx.y;
+  const int e = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63, t0 = blockIdx.y * ROUTER_TOKENS;
   if (e >= E) return;
-  float s = 0.0f;
-  for (int c = threadIdx.x & 63; c < D; c += 64)
-    s = __builtin_fmaf(rq_load_elem(x + (int64_t)t * ldx + c), rq_load_elem(router + (int64_t)e * ldr + c), s);
-  s = wave_sum(s);
-  if ((threadIdx.x & 63) == 0) logits[(int64_t)t * E + e] = s;
+  const TX* r = router + (int64_t)e * ldr;
+  const int nt = min(ROUTER_TOKENS, T - t0);
+  float s[ROUTER_TOKENS] = {};
+  auto add = [&](auto full, int c, int n) {
+    constexpr bool FULL = decltype(full)::value;
+    const auto w = rq_load_x<FULL>(r + c, n);
+#pragma unroll
+    for (int t = 0; t < ROUTER_TOKENS; ++t) {
+      if (t >= nt) break;
+      const auto v = rq_load_x<FULL>(x + (int64_t)(t0 + t) * ldx + c, n);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) s[t] = __builtin_fmaf((float)v[k], (float)w[k], s[t]);
+    }
+  };
+  const int whole = D / 512 * 512;
+#pragma unroll 2
+  for (int c = 8 * lane; c < whole; c += 512) add(std::true_type{}, c, 8);
+  if (whole < D) add(std::false_type{}, whole + 8 * lane, D - whole - 8 * lane);
+#pragma unroll
+  for (int t = 0; t < ROUTER_TOKENS; ++t) {
+    const float v = wave_sum(s[t]);
+    if (lane == 0 && t < nt) logits[(int64_t)(t0 + t) * E + e] = v;
+  }
 }
 
-// One wave per token: an expert's rank is the number of experts before it, so the ranks are a
-// permutation whatever the logits hold.
-__global__ __launch_bounds__(64) void k_moe_route(const float* __restrict__ logits, int E, int K, int norm,
-                                                  int* __restrict__ ids, float* __restrict__ weights,
-                                                  int* __restrict__ ids_out, float* __restrict__ weights_out) {
-  __shared__ float l[MAX_E];
-  __shared__ float chosen[MAX_K];
-  const int t = blockIdx.x, lane = threadIdx.x;
-  float m = -INFINITY;
-  for (int e = lane; e < E; e += 64) {
-    const float v = logits[(int64_t)t * E + e];
-    l[e] = v;
-    m = rq_nan_max(m, v);
+// One workgroup.  A wave takes a token: the K-th largest order key is found bit by bit from the number of
+// experts that reach a value (whatever the logits hold, exactly K are chosen); they are ranked among
+// themselves.  Then a wave takes an expert: its pairs in ascending order, cut into units.
+__global__ __launch_bounds__(1024) void k_moe_route(const float* __restrict__ logits, int T, int E, int K, int norm,
+                                                    float* __restrict__ weights, int* __restrict__ nunits,
+                                                    RqUnit* __restrict__ units, int* __restrict__ ids_out,
+                                                    float* __restrict__ weights_out) {
+  __shared__ int ids[MOE_TOKENS * MOE_MAX_K];
+  __shared__ int first[MOE_MAX_E];                   // the expert's first unit, once they are counted
+  __shared__ uint64_t picked[16][MOE_MAX_K];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  constexpr int EL = MOE_MAX_E / 64;
+  for (int t = wave; t < T; t += 16) {
+    const float* l = logits + (int64_t)t * E;
+    float v[EL];
+    uint32_t key[EL];
+    float m = -INFINITY;
+#pragma unroll
+    for (int u = 0; u < EL; ++u) {
+      if (64 * u >= E) break;
+      const int e = 64 * u + lane;
+      v[u] = e < E ? l[e] : -INFINITY;
+      key[u] = e < E ? rq_order_key(v[u]) : 0;       // below every logit's
+      m = rq_nan_max(m, v[u]);
+    }
+    uint32_t least = 0;
+    for (int bit = 31; bit >= 0; --bit) {
+      const uint32_t tried = least | (1u << bit);
+      int reach = 0;
+#pragma unroll
+      for (int u = 0; u < EL; ++u) {
+        if (64 * u >= E) break;
+        reach += __popcll(__ballot(key[u] >= tried));
+      }
+      if (reach >= K) least = tried;
+      if (reach == K) break;
+    }
+    // all above the K-th largest, and of those equal to it the first
+    int above = 0;
+#pragma unroll
+    for (int u = 0; u < EL; ++u) {
+      if (64 * u >= E) break;
+      above += __popcll(__ballot(key[u] > least));
+    }
+    int at = 0, equal = 0;
+#pragma unroll
+    for (int u = 0; u < EL; ++u) {
+      if (64 * u >= E) break;
+      const uint64_t eq = __ballot(key[u] == least);
+      const bool take = key[u] > least || (key[u] == least && equal + lanes_before(eq) < K - above);
+      const uint64_t mask = __ballot(take);
+      if (take) picked[wave][at + lanes_before(mask)] = ((uint64_t)key[u] << 32) | (uint32_t)~(uint32_t)(64 * u + lane);
+      at += __popcll(mask);
+      equal += __popcll(eq);
+    }
+    for (int o = 32; o; o >>= 1) m = rq_nan_max(m, __shfl_xor(m, o));
+    float s = 0.0f;
+#pragma unroll
+    for (int u = 0; u < EL; ++u) {
+      if (64 * u >= E) break;
+      s += expf(v[u] - m);                           // 0 past the last expert
+    }
+    s = wave_sum(s);
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    const uint64_t mine = lane < K ? picked[wave][lane] : 0;
+    int place = 0;
+    for (int j = 0; j < K; ++j) place += picked[wave][j] > mine ? 1 : 0;
+    const float p = lane < K ? expf(rq_key_value((uint32_t)(mine >> 32)) - m) : 0.0f;
+    const float total = norm ? wave_sum(p) : s;
+    if (lane < K) {
+      const int e = (int)~(uint32_t)mine;
+      ids[t * K + place] = e;
+      weights[t * K + place] = p / total;
+      if (ids_out) ids_out[t * K + place] = e;
+      if (weights_out) weights_out[t * K + place] = p / total;
+    }
+    __builtin_amdgcn_wave_barrier();
   }
-  for (int o = 32; o; o >>= 1) m = rq_nan_max(m, __shfl_xor(m, o));
   __syncthreads();
-  float s = 0.0f;
-  for (int e = lane; e < E; e += 64) {
-    const uint32_t mine = rq_order_key(l[e]);
-    const float p = expf(l[e] - m);
-    s += p;
-    int rank = 0;
-    for (int j = 0; j < E; ++j) {
-      const uint32_t other = rq_order_key(l[j]);
-      rank += (other > mine) || (other == mine && j < e);
-    }
-    if (rank < K) {
-      ids[t * K + rank] = e;
-      if (ids_out) ids_out[t * K + rank] = e;
-      chosen[rank] = p;
-    }
+  const int pairs = T * K;
+  for (int e = wave; e < E; e += 16) {               // units of every expert
+    int n = 0;
+    for (int p = 0; p < pairs; p += 64) n += __popcll(__ballot(p + lane < pairs && ids[p + lane] == e));
+    if (lane == 0) first[e] = (n + 15) / 16;
   }
-  s = wave_sum(s);
   __syncthreads();
-  const float p = lane < K ? chosen[lane] : 0.0f;
-  const float total = norm ? wave_sum(p) : s;
-  if (lane < K) {
-    weights[t * K + lane] = p / total;
-    if (weights_out) weights_out[t * K + lane] = p / total;
-  }
-}
-
-// What a gate / up launch leaves: the gate's product, or its activation times the up product.
-enum { MOE_GATE = 0, MOE_UP = 1 };
-
-template <typename TX, int NB>
-__global__ __launch_bounds__(256) void k_moe_in(const TX* __restrict__ x, int64_t ldx, RqExperts ex, int K,
-                                                const int* __restrict__ ids, int mode, float* __restrict__ h) {
-  const int pair = blockIdx.y, r0 = (blockIdx.x * 4 + (threadIdx.x >> 6)) * RW;
-  if (r0 >= ex.w.R) return;
-  const RqPacked w = expert(ex, ids[pair]);
-  float acc[RW] = {};
-  rows_dot<NB>(w, x + (int64_t)(pair / K) * ldx, r0, acc);
+  if (wave == 0) {                                   // to the number of units before it
+    int before = 0;
+    for (int e = 0; e < E; e += 64) {
+      const int mine = e + lane < E ? first[e + lane] : 0;
+      int sum = mine;
 #pragma unroll
-  for (int i = 0; i < RW; ++i) {
-    const float v = wave_sum(acc[i]);
-    if ((threadIdx.x & 63) == 0 && r0 + i < w.R) {
-      float* at = h + (int64_t)pair * w.R + r0 + i;
-      if (mode == MOE_GATE) *at = v;
-      else *at = *at / (1.0f + expf(-*at)) * v;
+      for (int o = 1; o < 64; o <<= 1) {
+        const int below = __shfl_up(sum, o);
+        sum += lane >= o ? below : 0;
+      }
+      if (e + lane < E) first[e + lane] = before + sum - mine;
+      before += __shfl(sum, 63);
     }
+    if (lane == 0) *nunits = before;
   }
-}
-
-template <typename TX, int NB>
-__global__ __launch_bounds__(256) void k_moe_out(const float* __restrict__ h, RqExperts ex, int K,
-                                                 const int* __restrict__ ids, const float* __restrict__ weights,
-                                                 TX* __restrict__ y, int64_t ldy) {
-  const int t = blockIdx.y, r0 = (blockIdx.x * 4 + (threadIdx.x >> 6)) * RW;
-  if (r0 >= ex.w.R) return;
-  float acc[RW] = {};
-  for (int k = 0; k < K; ++k) {
-    const int pair = t * K + k;
-    float one[RW] = {};
-    rows_dot<NB>(expert(ex, ids[pair]), h + (int64_t)pair * ex.w.C, r0, one);
-#pragma unroll
-    for (int i = 0; i < RW; ++i) acc[i] = __builtin_fmaf(weights[pair], one[i], acc[i]);
-  }
-#pragma unroll
-  for (int i = 0; i < RW; ++i) {
-    const float v = wave_sum(acc[i]);
-    if ((threadIdx.x & 63) == 0 && r0 + i < ex.w.R) y[(int64_t)t * ldy + r0 + i] = rq_cast<TX>(v);
+  __syncthreads();
+  for (int e = wave; e < E; e += 16) {
+    int n = 0;
+    for (int p = 0; p < pairs; p += 64) {
+      const bool is = p + lane < pairs && ids[p + lane] == e;
+      const uint64_t mask = __ballot(is);
+      const int at = n + lanes_before(mask);
+      if (is) units[first[e] + at / 16].pairs[at % 16] = p + lane;
+      n += __popcll(mask);
+    }
+    if (n == 0) continue;
+    const int full = (n - 1) / 16;                   // every unit but the last is full
+    if (lane <= full) {
+      units[first[e] + lane].expert = e;
+      units[first[e] + lane].n = lane < full ? 16 : n - 16 * full;
+    }
+    // the places past the last unit's tokens take the expert's first pair
+    int pair0 = -1;
+    for (int p = 0; p < pairs && pair0 < 0; p += 64) {
+      const uint64_t mask = __ballot(p + lane < pairs && ids[p + lane] == e);
+      if (mask) pair0 = p + __ffsll((unsigned long long)mask) - 1;
+    }
+    if (lane < 16 && lane >= n - 16 * full) units[first[e] + full].pairs[lane] = pair0;
   }
 }
 
 inline int64_t up256(int64_t n) { return (n + 255) / 256 * 256; }
 struct Layout {
-  int64_t logits, ids, weights, h, total;
+  int64_t logits, weights, nunits, units, gate, h, total;
 };
 inline Layout layout(int T, int I, int E, int K) {
-  const int64_t n = T < TOKENS ? T : TOKENS;
+  const int64_t n = T < MOE_TOKENS ? T : MOE_TOKENS;
   Layout l;
   l.logits = 0;
-  l.ids = l.logits + up256(n * E * 4);
-  l.weights = l.ids + up256(n * K * 4);
-  l.h = l.weights + up256(n * K * 4);
-  l.total = l.h + up256(n * K * I * 4);
+  l.weights = l.logits + up256(n * E * 4);
+  l.nunits = l.weights + up256(n * K * 4);
+  l.units = l.nunits + 256;
+  l.gate = l.units + up256((int64_t)rq_units((int)n, E, K) * (int64_t)sizeof(RqUnit));
+  l.h = l.gate + up256(n * K * I * 4);
+  l.total = l.h + up256(n * K * I * 2 * 3);
   return l;
 }
 inline RqExperts experts(const rq_packed_experts* p, int R, int C) {
@@ -176,7 +207,7 @@ inline RqExperts experts(const rq_packed_experts* p, int R, int C) {
 }  // namespace
 
 extern "C" int64_t rq_packed_moe_workspace_bytes(int T, int D, int I, int E, int K) {
-  if (T < 0 || D <= 0 || I <= 0 || E <= 0 || E > MAX_E || K <= 0 || K > MAX_K || K > E) return RQ_EINVAL;
+  if (T < 0 || D <= 0 || I <= 0 || E <= 0 || E > MOE_MAX_E || K <= 0 || K > MOE_MAX_K || K > E) return RQ_EINVAL;
   return layout(T, I, E, K).total;
 }
 
@@ -196,29 +227,21 @@ extern "C" int rq_packed_moe(const void* x, int dtype, int T, int64_t ldx, int D
   const Layout l = layout(T, I, E, K);
   char* ws = (char*)workspace;
   float* logits = (float*)(ws + l.logits);
-  int* ids = (int*)(ws + l.ids);
   float* weights = (float*)(ws + l.weights);
-  float* h = (float*)(ws + l.h);
+  int* nunits = (int*)(ws + l.nunits);
+  RqUnit* units = (RqUnit*)(ws + l.units);
   const bool known = rq_with_dtype(dtype, [&](auto* p) {
     typedef typename std::remove_pointer<decltype(p)>::type TX;
-    for (int t0 = 0; t0 < T; t0 += TOKENS) {
-      const int n = T - t0 < TOKENS ? T - t0 : TOKENS;
-      const TX* xt = (const TX*)x + (int64_t)t0 * ldx;
-      const dim3 in((I + 4 * RW - 1) / (4 * RW), n * K), out((D + 4 * RW - 1) / (4 * RW), n);
-      hipLaunchKernelGGL(k_moe_router<TX>, dim3((E + 3) / 4, n), dim3(256), 0, s, xt, ldx, D, (const TX*)router, ldr, E,
-                         logits);
-      hipLaunchKernelGGL(k_moe_route, dim3(n), dim3(64), 0, s, logits, E, K, norm, ids, weights,
-                         ids_out ? ids_out + (int64_t)t0 * K : nullptr, weights_out ? weights_out + (int64_t)t0 * K : nullptr);
-      rq_with_nbits(gate->nbits, [&](auto nb) {
-        hipLaunchKernelGGL((k_moe_in<TX, decltype(nb)::value>), in, dim3(256), 0, s, xt, ldx, g, K, ids, MOE_GATE, h);
-      });
-      rq_with_nbits(up->nbits, [&](auto nb) {
-        hipLaunchKernelGGL((k_moe_in<TX, decltype(nb)::value>), in, dim3(256), 0, s, xt, ldx, u, K, ids, MOE_UP, h);
-      });
-      rq_with_nbits(down->nbits, [&](auto nb) {
-        hipLaunchKernelGGL((k_moe_out<TX, decltype(nb)::value>), out, dim3(256), 0, s, h, d, K, ids, weights,
-                           (TX*)y + (int64_t)t0 * ldy, ldy);
-      });
+    for (int64_t t0 = 0; t0 < T; t0 += MOE_TOKENS) {
+      const int n = (int)(T - t0 < MOE_TOKENS ? T - t0 : MOE_TOKENS);
+      const TX* xt = (const TX*)x + t0 * ldx;
+      const RqMoe m{n, D, I, E, K, norm, nunits, units, weights, (float*)(ws + l.gate), (__hip_bfloat16*)(ws + l.h)};
+      hipLaunchKernelGGL(k_moe_router<TX>, dim3((E + 3) / 4, (n + ROUTER_TOKENS - 1) / ROUTER_TOKENS), dim3(256), 0, s, xt,
+                         ldx, n, D, (const TX*)router, ldr, E, logits);
+      hipLaunchKernelGGL(k_moe_route, dim3(1), dim3(1024), 0, s, logits, n, E, K, norm, weights, nunits, units,
+                         ids_out ? ids_out + t0 * K : nullptr, weights_out ? weights_out + t0 * K : nullptr);
+      rq_moe_in<TX>(xt, ldx, g, gate->nbits, u, up->nbits, m, s);
+      rq_moe_out<TX>(d, down->nbits, m, (TX*)y + t0 * ldy, ldy, s);
     }
   });
   if (!known) return RQ_EINVAL;

@@ -1,0 +1,53 @@
+// A mixture-of-experts layer for a few tokens: what its launches share.  Each element type's kernels (one
+// for every bit width) are a translation unit of their own.
+#pragma once
+#include "packed_bits.h"
+
+constexpr int MOE_MAX_E = 1024, MOE_MAX_K = 64;
+constexpr int MOE_TOKENS = 64;            // tokens per pass over the experts
+
+// The experts' weights: expert e's entry is w with its pointers moved by e strides.
+struct RqExperts {
+  RqPacked w;
+  int64_t sq, ss, sg;                     // strides of q, scales, g_idx from one expert to the next
+};
+__device__ __forceinline__ RqPacked rq_expert(const RqExperts& x, int e) {
+  RqPacked w = x.w;
+  w.q += x.sq * e;
+  w.scales += x.ss * e;
+  if (w.g_idx) w.g_idx += x.sg * e;
+  return w;
+}
+
+// Up to 16 tokens of one expert: what a tile of the matrix cores takes.  pairs: token * K + place among the
+// token's experts, ascending; past n the first again.
+struct RqUnit {
+  int expert, n, pairs[16];
+};
+// Units that T tokens with K experts each can make at most.
+inline int rq_units(int T, int E, int K) {
+  const int pairs = T * K, all = E + pairs / 16;
+  return pairs < all ? pairs : all;
+}
+
+// Pieces of the activation between the two products: fp32 in bf16 planes, two where the result is rounded
+// to 16 bits (2^-16 is lost), three for fp32 (exact).
+template <typename TX>
+constexpr int rq_moe_pieces() { return sizeof(TX) == 4 ? 3 : 2; }
+
+struct RqMoe {
+  int T, D, I, E, K, norm;
+  const int* nunits;                      // 1
+  const RqUnit* units;                    // rq_units
+  const float* weights;                   // T * K
+  float* gate;                            // T * K * I: the gate's product where up has other bits or groups
+  __hip_bfloat16* h;                      // pieces planes of T * K * I
+};
+
+// h = weight * silu(gate x) * (up x) of every pair, in pieces.
+template <typename TX>
+void rq_moe_in(const TX* x, int64_t ldx, const RqExperts& gate, int gate_bits, const RqExperts& up, int up_bits,
+               const RqMoe& m, hipStream_t s);
+// y = the sum over a token's pairs of down h.
+template <typename TX>
+void rq_moe_out(const RqExperts& down, int bits, const RqMoe& m, TX* y, int64_t ldy, hipStream_t s);

@@ -13,7 +13,17 @@ struct RqPacked {
   int64_t lds;
   const int32_t* g_idx;   // [C] or NULL
   int R, C, ngroups, groupsize;
+  uint32_t run_magic;     // ceil(2^32 / (groupsize / 32)) for rq_run_group; 0: one group, 1: groups of 32
 };
+
+// The weight an entry point was given.  run_magic divides by groupsize / 32 (group sizes that are multiples of
+// 32): n * magic >> 32 is n / d while n * d < 2^32.
+inline RqPacked rq_packed(const uint32_t* q, int64_t ldp, const float* scales, int64_t lds, const int32_t* g_idx, int R,
+                          int C, int ngroups, int groupsize) {
+  const uint32_t d = ngroups > 1 && groupsize > 0 && groupsize % 32 == 0 ? (uint32_t)groupsize / 32 : 0;
+  const uint32_t magic = d == 0 ? 0 : d == 1 ? 1 : (uint32_t)(((1ull << 32) + d - 1) / d);
+  return RqPacked{q, ldp, scales, lds, g_idx, R, C, ngroups, groupsize, magic};
+}
 
 // The group of column c, -1 where g_idx names none (its scale then reads as NaN, never out of bounds).
 __device__ __forceinline__ int rq_group_of(const RqPacked& w, int c) {
@@ -25,8 +35,8 @@ __device__ __forceinline__ float rq_scale_of(const RqPacked& w, int g, int r) {
   return g < 0 ? __builtin_nanf("") : w.scales[(int64_t)g * w.lds + r];
 }
 
-// The nc <= 8 codes of columns [c, c + nc), c a multiple of 8; the rest read as 0.  No word past the
-// row's last field is read.
+// The nc <= 8 codes of columns [c, c + nc), c a multiple of 8; the rest read as 0.  No word past the last of these
+// fields is read (row's first where nc <= 0 and c = 0): the loads are moved back, not masked.
 template <int NB>
 __device__ __forceinline__ void rq_codes8(const uint32_t* __restrict__ row, int c, int nc, int (&code)[8]) {
   constexpr int half = 1 << (NB - 1);
@@ -38,7 +48,7 @@ __device__ __forceinline__ void rq_codes8(const uint32_t* __restrict__ row, int 
   const int nw = (off + nc * NB + 31) >> 5;
   uint32_t w[NW + 1];
 #pragma unroll
-  for (int k = 0; k < NW; ++k) w[k] = k < nw ? p[k] : 0u;
+  for (int k = 0; k < NW; ++k) w[k] = p[max(min(k, nw - 1), 0)];
   w[NW] = 0u;
 #pragma unroll
   for (int k = 0; k < NW; ++k) w[k] = (uint32_t)((((uint64_t)w[k + 1] << 32) | w[k]) >> off);

@@ -56,15 +56,9 @@ __device__ __forceinline__ V rq_load_as(const T* p) {
   return v;
 }
 
-// Small integers (|v| <= 256, exact in every type) to the operand's type.
-__device__ __forceinline__ void rq_set2(half8& v, int k, float a, float b) {
-  v[k] = (_Float16)a;
-  v[k + 1] = (_Float16)b;
-}
-__device__ __forceinline__ void rq_set2(bf16x8& v, int k, float a, float b) {
-  v[k] = (__bf16)a;
-  v[k + 1] = (__bf16)b;
-}
+// Codes over rq_unit (integers up to 256 or sixteenths up to 8: exact in every type) to the operand's type.
+__device__ __forceinline__ void rq_convert(floatx8 f, half8& v) { v = __builtin_convertvector(f, half8); }
+__device__ __forceinline__ void rq_convert(floatx8 f, bf16x8& v) { v = __builtin_convertvector(f, bf16x8); }
 
 // Word k of the pattern that has the top bit of every field set: codes are stored offset by
 // 2^(NB-1), and flipping that bit makes them two's complement.
@@ -90,23 +84,45 @@ __device__ __forceinline__ int rq_signed_code(const uint32_t (&w)[NB], int j) {
   const uint32_t v = (uint32_t)((((uint64_t)w[i + 1 < NB ? i + 1 : i] << 32) | w[i]) >> o);
   return ((int)(v << (32 - NB))) >> (32 - NB);
 }
-template <typename V, int NB>
-__device__ __forceinline__ V rq_codes_operand(const uint32_t (&w)[NB], int s) {
-  V v;
+// 4-bit codes have an instruction of their own, a signed nibble over 16 at the low end of a byte: with the odd
+// nibbles shifted down once, 14 instructions make eight operands (20 and more with bit fields).
+template <int NB>
+constexpr float rq_unit() { return NB == 4 ? 16.0f : 1.0f; }
+__device__ __forceinline__ uint32_t rq_odd_nibbles(uint32_t w) {
+  uint32_t y = w >> 4;
+  asm("" : "+v"(y));               // or the shift is joined with the byte's again
+  return y;
+}
+__device__ __forceinline__ float rq_nibble(uint32_t w, uint32_t odd, int n) {
+  return __builtin_amdgcn_cvt_off_f32_i4((n & 1 ? odd : w) >> (8 * (n >> 1)));
+}
+// Codes 8s..8s+7 of 32 over rq_unit.
+template <int NB>
+__device__ __forceinline__ floatx8 rq_codes_of(const uint32_t (&w)[NB], int s) {
+  floatx8 f;
+  if constexpr (NB == 4) {
+    const uint32_t odd = rq_odd_nibbles(w[s]);
 #pragma unroll
-  for (int k = 0; k < 8; k += 2)
-    rq_set2(v, k, (float)rq_signed_code<NB>(w, 8 * s + k), (float)rq_signed_code<NB>(w, 8 * s + k + 1));
-  return v;
+    for (int k = 0; k < 8; ++k) f[k] = rq_nibble(w[s], odd, k);
+  } else {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) f[k] = (float)rq_signed_code<NB>(w, 8 * s + k);
+  }
+  return f;
 }
 
-// Eight x of a token as they are loaded (FULL: all eight exist; else the first n, the rest 0), and the
-// operand's pieces made of them.
+// Eight x of a token as they are loaded (FULL: all eight exist; else the first n, which may be none, the rest 0),
+// and the operand's pieces made of them.  Loads past the row's end are moved back to its last element, whose
+// place is p[n - 1], and their values dropped: a mask for every element would take the scalar registers.
 template <bool FULL>
 __device__ __forceinline__ half8 rq_load_x(const __half* p, int n) {
   if (FULL) return rq_load_as<half8>(p);
   half8 v;
 #pragma unroll
-  for (int k = 0; k < 8; ++k) v[k] = k < n ? rq_load_as<_Float16>(p + k) : (_Float16)0.0f;
+  for (int k = 0; k < 8; ++k) {
+    const _Float16 e = rq_load_as<_Float16>(p + min(k, n - 1));
+    v[k] = k < n ? e : (_Float16)0.0f;
+  }
   return v;
 }
 template <bool FULL>
@@ -114,7 +130,10 @@ __device__ __forceinline__ bf16x8 rq_load_x(const __hip_bfloat16* p, int n) {
   if (FULL) return rq_load_as<bf16x8>(p);
   bf16x8 v;
 #pragma unroll
-  for (int k = 0; k < 8; ++k) v[k] = k < n ? rq_load_as<__bf16>(p + k) : (__bf16)0.0f;
+  for (int k = 0; k < 8; ++k) {
+    const __bf16 e = rq_load_as<__bf16>(p + min(k, n - 1));
+    v[k] = k < n ? e : (__bf16)0.0f;
+  }
   return v;
 }
 template <bool FULL>
@@ -122,7 +141,10 @@ __device__ __forceinline__ floatx8 rq_load_x(const float* p, int n) {
   if (FULL) return rq_load_as<floatx8>(p);
   floatx8 v;
 #pragma unroll
-  for (int k = 0; k < 8; ++k) v[k] = k < n ? p[k] : 0.0f;
+  for (int k = 0; k < 8; ++k) {
+    const float e = p[min(k, n - 1)];
+    v[k] = k < n ? e : 0.0f;
+  }
   return v;
 }
 __device__ __forceinline__ void rq_operand(half8 x, half8 (&v)[1]) { v[0] = x; }
@@ -161,11 +183,14 @@ struct RqTokens {
   typedef typename RqOperand<TX>::raw raw;
   typedef typename RqOperand<TX>::vec vec;
   static constexpr int tiles = NT, pieces = RqOperand<TX>::pieces;
+  static constexpr bool arranged = false;
   const TX* p[NT];
   template <bool FULL>
   __device__ __forceinline__ raw load(int b, int c, int n) const { return rq_load_x<FULL>(p[b] + c, n); }
   __device__ __forceinline__ float element(int b, int c) const { return rq_load_elem(p[b] + c); }
 };
+// Where column c of a row lies when its chunks are arranged: columns 32q + 8s.. of a chunk at 32s + 8q.
+__device__ __forceinline__ int rq_arranged(int c) { return (c & ~127) + (c >> 3 & 3) * 32 + (c >> 5 & 3) * 8 + (c & 7); }
 // The same for fp32 values that were stored as P bf16 pieces, `plane` elements from one piece to the next.
 template <int P>
 struct RqPieceRow {
@@ -176,11 +201,14 @@ __device__ __forceinline__ void rq_operand(const RqPieceRow<P>& x, bf16x8 (&v)[P
 #pragma unroll
   for (int p = 0; p < P; ++p) v[p] = x.v[p];
 }
-template <int P>
+// ARRANGED: within every chunk of 128 columns the 4 x 4 blocks of 8 lie transposed (rq_arranged), as the lanes
+// of the codes want them, and the last chunk is filled up with zeros.
+template <int P, bool ARRANGED>
 struct RqPieces {
   typedef RqPieceRow<P> raw;
   typedef bf16x8 vec;
   static constexpr int tiles = 1, pieces = P;
+  static constexpr bool arranged = ARRANGED;
   const __hip_bfloat16* p;
   int64_t plane;
   template <bool FULL>
@@ -198,57 +226,97 @@ struct RqPieces {
   }
 };
 
-// The scales of group g and rows r..r+3, without a branch: a load that would pass the table's end is moved
-// back and its values shifted up (rows past the weight get some scale, and are never stored).  The table
-// holds at least four (rq_mode_of).
-__device__ __forceinline__ floatx4 rq_scales4(const RqPacked& w, int g, int r) {
+// The scales of group g and rows r..r+3 (rows past the weight get some scale, and are never stored).  A load
+// that would pass the table's end is moved back, and rq_scales4_of shifts its values up; where R is a
+// multiple of 4 only rows past the weight are ever moved.  The table holds at least four (rq_mode_of).
+__device__ __forceinline__ floatx4 rq_load_scales4(const RqPacked& w, int g, int r) {
   const int64_t at = (int64_t)g * w.lds + r, last = (int64_t)(w.ngroups - 1) * w.lds + w.R - 4;
-  const floatx4 v = rq_load_as<floatx4>(w.scales + (at < last ? at : last));
-  const int d = at > last ? (int)(at - last) : 0;
-  return floatx4{d == 0 ? v[0] : d == 1 ? v[1] : d == 2 ? v[2] : v[3], d == 0 ? v[1] : d == 1 ? v[2] : v[3],
-                 d == 0 ? v[2] : v[3], v[3]};
+  return rq_load_as<floatx4>(w.scales + (at < last ? at : last));
+}
+__device__ __forceinline__ floatx4 rq_scales4_of(const RqPacked& w, int g, int r, floatx4 v) {
+  if ((w.R & 3) == 0) return v;
+  const int64_t d = (int64_t)g * w.lds + r - ((int64_t)(w.ngroups - 1) * w.lds + w.R - 4);
+  return floatx4{d <= 0 ? v[0] : d == 1 ? v[1] : d == 2 ? v[2] : v[3], d <= 0 ? v[1] : d == 1 ? v[2] : v[3],
+                 d <= 0 ? v[2] : v[3], v[3]};
 }
 
-__device__ __forceinline__ int rq_run_group(const RqPacked& w, int c) { return w.ngroups == 1 ? 0 : c / w.groupsize; }
+// The group of column c where groups are runs of a multiple of 32 columns (or there is one).
+__device__ __forceinline__ int rq_run_group(const RqPacked& w, int c) {
+  const uint32_t n = (uint32_t)c >> 5;
+  return w.run_magic > 1 ? (int)__umulhi(n, w.run_magic) : w.run_magic ? (int)n : 0;
+}
 
-// What a lane needs of a chunk of 128 columns with RUNS: its words and scales, and its tokens' x.
+// The words of columns c..c+31 of a row (c a multiple of 32); the row's last word again where it has none there,
+// for columns whose x is 0.
+template <int NB>
+__device__ __forceinline__ void rq_words(const uint32_t* row, int c, int C, uint32_t (&w)[NB]) {
+  const int64_t first = (int64_t)(c >> 5) * NB, last = ((int64_t)C * NB + 31) / 32 - 1;
+#pragma unroll
+  for (int k = 0; k < NB; ++k) w[k] = row[first + k < last ? first + k : last];
+}
+
+// What a lane needs of a chunk of 128 columns with RUNS: its words and scales, and its tokens' x.  Row tiles
+// go over NM weights of one shape, tile a being rows r0 + 16 (a / NM) of weight a mod NM.
 template <int NB, int RT>
 struct RqRunsW {
   uint32_t wd[RT][NB];
   floatx4 sc[RT];
 };
-template <bool FULL, int NB, int RT>
-__device__ __forceinline__ void rq_load_runs(const RqPacked& w, const uint32_t* const (&row)[RT], int r0, int ch,
+template <bool FULL, int NB, int RT, int NM>
+__device__ __forceinline__ void rq_load_runs(const RqPacked (&w)[NM], const uint32_t* const (&row)[RT], int r0, int ch,
                                              RqRunsW<NB, RT>& f) {
   const int q = (threadIdx.x & 63) >> 4, c = ch * RQ_CHUNK + 32 * q;
-  const int g = rq_run_group(w, ch * RQ_CHUNK);
 #pragma unroll
   for (int a = 0; a < RT; ++a) {
-    const uint32_t* p = row[a] + (int64_t)(c >> 5) * NB;
     if (FULL) {
-      __builtin_memcpy(f.wd[a], p, 4 * NB);
+      __builtin_memcpy(f.wd[a], row[a] + (int64_t)(c >> 5) * NB, 4 * NB);
     } else {
-      const int words = c < w.C ? (min(32, w.C - c) * NB + 31) >> 5 : 0;
-#pragma unroll
-      for (int k = 0; k < NB; ++k) f.wd[a][k] = k < words ? p[k] : 0u;
+      rq_words<NB>(row[a], c, w[0].C, f.wd[a]);
     }
-    f.sc[a] = rq_scales4(w, g, r0 + 16 * a + 4 * q);
+    f.sc[a] = rq_load_scales4(w[a % NM], rq_run_group(w[a % NM], ch * RQ_CHUNK), r0 + 16 * (a / NM) + 4 * q);
   }
 }
+// Step s loads columns 32s + 8q of the chunk, 64 bytes (of a 16-bit type) in a row of each token, and rq_to_runs
+// brings them to the lanes of the codes that they go with (columns 32q + 8s, which loaded as they are would
+// touch four times as many lines of the cache).
 template <bool FULL, typename X>
 __device__ __forceinline__ void rq_load_tokens(const X& xs, int C, int ch, typename X::raw (&x)[X::tiles][4]) {
-  const int c = ch * RQ_CHUNK + 32 * ((threadIdx.x & 63) >> 4);
+  const int q = (threadIdx.x & 63) >> 4, c = ch * RQ_CHUNK + 8 * q;
 #pragma unroll
   for (int b = 0; b < X::tiles; ++b)
 #pragma unroll
-    for (int s = 0; s < 4; ++s) x[b][s] = xs.template load<FULL>(b, c + 8 * s, C - c - 8 * s);
+    for (int s = 0; s < 4; ++s) x[b][s] = xs.template load<FULL>(b, c + 32 * s, C - c - 32 * s);
 }
-template <typename X, int NB, int RT>
-__device__ __forceinline__ void rq_chunk_runs(RqRunsW<NB, RT>& f, const typename X::raw (&x)[X::tiles][4],
-                                              floatx4 (&acc)[RT][X::tiles]) {
+// The 4 x 4 transpose of a step's quarter q of the wave and the step, 32 bits at a time.
+template <typename T>
+__device__ __forceinline__ void rq_to_runs(T (&x)[4]) {
+  static_assert(sizeof(T) % 4 == 0);
+  constexpr int N = sizeof(T) / 4;
+  uint32_t r[4][N];
+  __builtin_memcpy(r, x, sizeof(x));
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    const auto a = __builtin_amdgcn_permlane32_swap(r[0][k], r[2][k], false, false);
+    const auto b = __builtin_amdgcn_permlane32_swap(r[1][k], r[3][k], false, false);
+    const auto c = __builtin_amdgcn_permlane16_swap(a[0], b[0], false, false);
+    const auto d = __builtin_amdgcn_permlane16_swap(a[1], b[1], false, false);
+    r[0][k] = c[0];
+    r[1][k] = c[1];
+    r[2][k] = d[0];
+    r[3][k] = d[1];
+  }
+  __builtin_memcpy(x, r, sizeof(x));
+}
+template <typename X, int NB, int RT, int NM>
+__device__ __forceinline__ void rq_chunk_runs(const RqPacked (&w)[NM], int r0, int ch, RqRunsW<NB, RT>& f,
+                                              typename X::raw (&x)[X::tiles][4], floatx4 (&acc)[RT][X::tiles]) {
   typedef typename X::vec V;
   constexpr int NT = X::tiles, P = X::pieces;
   floatx4 part[RT][NT];
+  if constexpr (!X::arranged) {
+#pragma unroll
+    for (int b = 0; b < NT; ++b) rq_to_runs(x[b]);
+  }
 #pragma unroll
   for (int a = 0; a < RT; ++a) {
     rq_to_signed<NB>(f.wd[a]);
@@ -262,65 +330,92 @@ __device__ __forceinline__ void rq_chunk_runs(RqRunsW<NB, RT>& f, const typename
     for (int b = 0; b < NT; ++b) rq_operand(x[b][s], xo[b]);
 #pragma unroll
     for (int a = 0; a < RT; ++a) {
-      const V codes = rq_codes_operand<V, NB>(f.wd[a], s);
+      V codes;
+      rq_convert(rq_codes_of<NB>(f.wd[a], s), codes);
 #pragma unroll
       for (int b = 0; b < NT; ++b)
 #pragma unroll
         for (int p = 0; p < P; ++p) part[a][b] = rq_mfma(codes, xo[b][p], part[a][b]);
     }
   }
+  const int r = r0 + 4 * ((threadIdx.x & 63) >> 4);
 #pragma unroll
-  for (int a = 0; a < RT; ++a)
+  for (int a = 0; a < RT; ++a) {
+    const RqPacked& wa = w[a % NM];
+    const floatx4 sc = rq_scales4_of(wa, rq_run_group(wa, ch * RQ_CHUNK), r + 16 * (a / NM), f.sc[a]) * rq_unit<NB>();
 #pragma unroll
     for (int b = 0; b < NT; ++b)
 #pragma unroll
-      for (int k = 0; k < 4; ++k) acc[a][b][k] = __builtin_fmaf(f.sc[a][k], part[a][b][k], acc[a][b][k]);
+      for (int k = 0; k < 4; ++k) acc[a][b][k] = __builtin_fmaf(sc[k], part[a][b][k], acc[a][b][k]);
+  }
 }
 
-// Chunks first, first + step, ... of rows [r0, r0 + 16 RT): acc[a][b] += the weight's rows
-// r0 + 16 a + 4q.. times the lane's token of tile b.  A lane without a token is given any other's (its sums
+// The wave's index as a scalar: what is computed from it needs no exec mask.
+__device__ __forceinline__ int rq_wave() { return __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6); }
+
+// Chunks first, first + step, ...: acc[a][b] += rows 4q.. of row tile a times the lane's token of tile b.  A lane without a token is given any other's (its sums
 // go nowhere).  lds: scales of the workgroup's rows for ANY, laid out by rq_stage_scales, or NULL.
-template <int NB, int MODE, int RT, typename X>
-__device__ __forceinline__ void rq_rows_tokens(const RqPacked& w, int r0, const X& xs, int first, int step,
+template <int NB, int MODE, int RT, int NM, typename X>
+__device__ __forceinline__ void rq_rows_tokens(const RqPacked (&w)[NM], int r0, const X& xs, int first, int step,
                                                const float* lds, floatx4 (&acc)[RT][X::tiles]) {
   typedef typename X::vec V;
   constexpr int NT = X::tiles, P = X::pieces;
   const int lane = threadIdx.x & 63, i = lane & 15, q = lane >> 4;
   const uint32_t* row[RT];
 #pragma unroll
-  for (int a = 0; a < RT; ++a) row[a] = w.q + (int64_t)min(r0 + 16 * a + i, w.R - 1) * w.ldp;
-  const int nfull = w.C / RQ_CHUNK, nch = (w.C + RQ_CHUNK - 1) / RQ_CHUNK;
+  for (int a = 0; a < RT; ++a) row[a] = w[a % NM].q + (int64_t)min(r0 + 16 * (a / NM) + i, w[a % NM].R - 1) * w[a % NM].ldp;
+  const int C = w[0].C, nfull = C / RQ_CHUNK, nch = (C + RQ_CHUNK - 1) / RQ_CHUNK;
   int ch = first;
   if constexpr (MODE == RQ_RUNS) {
     // The words of D chunks and the tokens of DX are in flight, a chunk's place refilled as soon as it has
-    // been used.
-    constexpr int D = RT * (NB + 4) <= 18 ? 4 : 2, DX = NT == 1 && sizeof(typename X::raw) <= 16 ? 2 : 1;
+    // been used.  No load of the loop is conditional: a wait then counts the later loads that may stay
+    // in flight, where a branch around one would make it wait for all of them.
+    constexpr int D = NT * P * NM == 1 && NB <= 5 ? 4 : 2, DX = NT == 1 && sizeof(typename X::raw) <= 16 ? 2 : 1;
     const int n = ch < nfull ? (nfull - ch + step - 1) / step : 0;     // full chunks of this wave
     RqRunsW<NB, RT> f[D];
     typename X::raw x[DX][NT][4];
+    auto words = [&](int k, RqRunsW<NB, RT>& to) { rq_load_runs<true>(w, row, r0, ch + k * step, to); };
+    auto tokens = [&](int k, typename X::raw (&to)[NT][4]) { rq_load_tokens<true>(xs, C, ch + k * step, to); };
+    auto compute = [&](int k, RqRunsW<NB, RT>& of, typename X::raw (&xk)[NT][4]) {
+      if constexpr (DX == 1) tokens(k, xk);
+      rq_chunk_runs<X, NB, RT, NM>(w, r0, ch + k * step, of, xk, acc);
+    };
+    int k = 0;
+    if (n >= D) {
 #pragma unroll
-    for (int u = 0; u < D; ++u)
-      if (u < n) rq_load_runs<true>(w, row, r0, ch + u * step, f[u]);
-    if constexpr (DX == 2) {
+      for (int u = 0; u < D; ++u) words(u, f[u]);
+      if constexpr (DX == 2) {
+        tokens(0, x[0]);
+        tokens(1, x[1]);
+      }
+      for (; k + 2 * D <= n; k += D) {
 #pragma unroll
-      for (int u = 0; u < DX; ++u)
-        if (u < n) rq_load_tokens<true>(xs, w.C, ch + u * step, x[u]);
-    }
-    for (int k = 0; k < n; k += D) {
-#pragma unroll
-      for (int u = 0; u < D; ++u) {
-        if (k + u < n) {
-          if constexpr (DX == 1) rq_load_tokens<true>(xs, w.C, ch + (k + u) * step, x[0]);
-          rq_chunk_runs<X, NB, RT>(f[u], x[u % DX], acc);
-          if (DX == 2 && k + u + DX < n) rq_load_tokens<true>(xs, w.C, ch + (k + u + DX) * step, x[u % DX]);
-          if (k + u + D < n) rq_load_runs<true>(w, row, r0, ch + (k + u + D) * step, f[u]);
+        for (int u = 0; u < D; ++u) {
+          compute(k + u, f[u], x[u % DX]);
+          if constexpr (DX == 2) tokens(k + u + 2, x[u % 2]);
+          words(k + u + D, f[u]);
         }
       }
+#pragma unroll
+      for (int u = 0; u < D; ++u) {
+        compute(k + u, f[u], x[u % DX]);
+        if (DX == 2 && u + 2 < D) tokens(k + u + 2, x[u % 2]);
+      }
+      k += D;
     }
+#pragma unroll
+    for (int u = 0; u < D - 1; ++u)
+      if (k + u < n) words(k + u, f[u]);
+#pragma unroll
+    for (int u = 0; u < D - 1; ++u)
+      if (k + u < n) {
+        if constexpr (DX == 2) tokens(k + u, x[0]);
+        compute(k + u, f[u], x[0]);
+      }
     if (nfull < nch && nfull >= first && (nfull - first) % step == 0) {       // the ragged end is this wave's
       rq_load_runs<false>(w, row, r0, nfull, f[0]);
-      rq_load_tokens<false>(xs, w.C, nfull, x[0]);
-      rq_chunk_runs<X, NB, RT>(f[0], x[0], acc);
+      rq_load_tokens<false>(xs, C, nfull, x[0]);
+      rq_chunk_runs<X, NB, RT, NM>(w, r0, nfull, f[0], x[0], acc);
     }
   } else if constexpr (MODE == RQ_SMALL) {
     for (; ch < nch; ch += step) {
@@ -331,23 +426,26 @@ __device__ __forceinline__ void rq_rows_tokens(const RqPacked& w, int r0, const 
 #pragma unroll
         for (int a = 0; a < RT; ++a) {
           const int c = c0 + 32 * s + 8 * q;
-          rq_codes8<NB>(row[a], c < w.C ? c : 0, c < w.C ? min(8, w.C - c) : 0, code[s][a]);
+          rq_codes8<NB>(row[a], c < C ? c : 0, c < C ? min(8, C - c) : 0, code[s][a]);
         }
 #pragma unroll
       for (int s = 0; s < 4; ++s) {
         const int c = c0 + 32 * s + 8 * q;
-        if (c0 + 32 * s >= w.C) break;
-        const int g = rq_run_group(w, c0 + 32 * s);
+        if (c0 + 32 * s >= C) break;
         V x[NT][P];
 #pragma unroll
         for (int b = 0; b < NT; ++b)
-          rq_operand(c + 8 <= w.C ? xs.template load<true>(b, c, 8) : xs.template load<false>(b, c, w.C - c), x[b]);
+          rq_operand(c + 8 <= C ? xs.template load<true>(b, c, 8) : xs.template load<false>(b, c, C - c), x[b]);
 #pragma unroll
         for (int a = 0; a < RT; ++a) {
           V codes;
+          floatx8 f;
 #pragma unroll
-          for (int k = 0; k < 8; k += 2) rq_set2(codes, k, (float)code[s][a][k], (float)code[s][a][k + 1]);
-          const floatx4 sc = rq_scales4(w, g, r0 + 16 * a + 4 * q);
+          for (int k = 0; k < 8; ++k) f[k] = (float)code[s][a][k];
+          rq_convert(f, codes);
+          const RqPacked& wa = w[a % NM];
+          const int g = rq_run_group(wa, c0 + 32 * s), r = r0 + 16 * (a / NM) + 4 * q;
+          const floatx4 sc = rq_scales4_of(wa, g, r, rq_load_scales4(wa, g, r));
 #pragma unroll
           for (int b = 0; b < NT; ++b) {
             floatx4 part = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -361,26 +459,24 @@ __device__ __forceinline__ void rq_rows_tokens(const RqPacked& w, int r0, const 
     }
   } else {
     for (; ch < nch; ch += step) {
-      const int c = ch * RQ_CHUNK + 32 * q, n = min(32, w.C - c);     // the lane's columns (n <= 0: none)
+      const int c = ch * RQ_CHUNK + 32 * q, n = min(32, C - c);     // the lane's columns (n <= 0: none)
       uint32_t wd[RT][NB];
 #pragma unroll
       for (int a = 0; a < RT; ++a) {
-        const uint32_t* p = row[a] + (int64_t)(c >> 5) * NB;
-        const int words = n > 0 ? (n * NB + 31) >> 5 : 0;
-#pragma unroll
-        for (int k = 0; k < NB; ++k) wd[a][k] = k < words ? p[k] : 0u;
+        rq_words<NB>(row[a], c, C, wd[a]);
         rq_to_signed<NB>(wd[a]);
       }
 #pragma unroll
       for (int j = 0; j < 32; ++j) {
-        const int g = j < n ? rq_group_of(w, c + j) : 0;
         float xv[NT];
 #pragma unroll
         for (int b = 0; b < NT; ++b) xv[b] = j < n ? xs.element(b, c + j) : 0.0f;
 #pragma unroll
         for (int a = 0; a < RT; ++a) {
-          const float s = lds ? lds[((unsigned)g < (unsigned)w.ngroups ? g : w.ngroups) * (16 * RT) + 16 * a + i]
-                              : rq_scale_of(w, g, min(r0 + 16 * a + i, w.R - 1));
+          const RqPacked& wa = w[a % NM];
+          const int g = j < n ? rq_group_of(wa, c + j) : 0;
+          const float s = lds ? lds[((unsigned)g < (unsigned)wa.ngroups ? g : wa.ngroups) * (16 * RT) + 16 * a + i]
+                              : rq_scale_of(wa, g, min(r0 + 16 * (a / NM) + i, wa.R - 1));
           const float wv = j < n ? s * (float)rq_signed_code<NB>(wd[a], j) : 0.0f;
 #pragma unroll
           for (int b = 0; b < NT; ++b) acc[a][b] = __builtin_amdgcn_mfma_f32_16x16x4f32(wv, xv[b], acc[a][b], 0, 0, 0);
@@ -404,6 +500,7 @@ constexpr int RQ_STAGED_GROUPS = 127;       // groups whose scales a workgroup s
 // Which of the three serves a weight.
 inline int rq_mode_of(const RqPacked& w) {
   if ((int64_t)(w.ngroups - 1) * w.lds + w.R < 4) return RQ_ANY;
+  if (w.groupsize > 0 && (int64_t)(w.C / 32 + 1) * (w.groupsize / 32 + 1) >= 1ll << 32 && w.ngroups > 1) return RQ_ANY;
   if (w.ngroups == 1 || (w.groupsize > 0 && w.groupsize % RQ_CHUNK == 0)) return RQ_RUNS;
   return w.groupsize > 0 && w.groupsize % 32 == 0 ? RQ_SMALL : RQ_ANY;
 }

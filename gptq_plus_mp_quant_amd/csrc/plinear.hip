@@ -11,7 +11,7 @@ extern "C" int rq_packed_linear(const void* x, int x_dtype, int T, int64_t ldx, 
                                 int64_t ldp, int nbits, int R, const float* scales, int64_t lds, int ngroups,
                                 const int32_t* g_idx, int groupsize, const void* bias, void* y, int64_t ldy,
                                 void* stream) {
-  const RqPacked w{qweight, ldp, scales, lds, g_idx, R, C, ngroups, groupsize};
+  const RqPacked w = rq_packed(qweight, ldp, scales, lds, g_idx, R, C, ngroups, groupsize);
   if (T < 0 || rq_packed_check(w, nbits) != RQ_OK) return RQ_EINVAL;
   if (T == 0) return RQ_OK;
   if (!x || !y || ldx < C || ldy < R) return RQ_EINVAL;
@@ -38,7 +38,7 @@ extern "C" int rq_packed_linear_grad(const void* grad_y, int dtype, int T, int64
                                      int64_t ldp, int nbits, int R, const float* scales, int64_t lds, int ngroups,
                                      const int32_t* g_idx, int groupsize, void* grad_x, int64_t ldx, void* workspace,
                                      int64_t workspace_bytes, void* stream) {
-  const RqPacked w{qweight, ldp, scales, lds, g_idx, R, C, ngroups, groupsize};
+  const RqPacked w = rq_packed(qweight, ldp, scales, lds, g_idx, R, C, ngroups, groupsize);
   if (T < 0 || rq_packed_check(w, nbits) != RQ_OK) return RQ_EINVAL;
   if (T == 0) return RQ_OK;
   if (!grad_y || !grad_x || ldg < R || ldx < C) return RQ_EINVAL;

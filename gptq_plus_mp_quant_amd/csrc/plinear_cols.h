@@ -42,6 +42,17 @@ __device__ __forceinline__ int col_code(const uint32_t (&w)[Col8<NB>::NW], int n
   const uint32_t v = (uint32_t)((((uint64_t)w[i + 1 < Col8<NB>::NW ? i + 1 : i] << 32) | w[i]) >> o);
   return ((int)(v << (32 - NB))) >> (32 - NB);
 }
+// Code n of each of 8 rows, over rq_unit (odd: the rows' odd nibbles, for 4 bits).
+template <int NB>
+__device__ __forceinline__ floatx8 col_codes(const uint32_t (&w)[8][Col8<NB>::NW], const uint32_t (&odd)[8], int n) {
+  floatx8 f;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    if constexpr (NB == 4) f[k] = rq_nibble(w[k][0], odd[k], n);
+    else f[k] = (float)col_code<NB>(w[k], n);
+  }
+  return f;
+}
 
 __device__ __forceinline__ void fp32_of(half8 v, floatx8& f) {
 #pragma unroll
@@ -63,14 +74,15 @@ __global__ __launch_bounds__(64 * cols_waves(NT)) void k_packed_cols(const TX* _
   typedef ColPieces<TX, MODE> P;
   typedef typename RqOperand<TX>::raw Raw;
   __shared__ floatx4 join[W / 2][8 * NT][64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, j = lane & 15, q = lane >> 4;
+  const int lane = threadIdx.x & 63, wave = rq_wave(), j = lane & 15, q = lane >> 4;
   const int c0 = blockIdx.x * COLS, c = c0 + 8 * j, t0 = blockIdx.z * 16 * NT;
   const int nc = min(8, w.C - c);                                  // the lane's columns (<= 0: none)
   const int nsteps = (w.R + STEP - 1) / STEP;
   const int sa = blockIdx.y * steps_per, sb = min(nsteps, sa + steps_per);
   const int64_t bit = (int64_t)c * NB;
   const int off = (int)(bit & 31), nw = nc > 0 ? (off + nc * NB + 31) >> 5 : 0;
-  const uint32_t* col = w.q + (bit >> 5);
+  // A lane past the last column reads the row's first word; words past a row's last field are not read.
+  const uint32_t* col = w.q + (nc > 0 ? bit >> 5 : 0);
   int g[8];
 #pragma unroll
   for (int k = 0; k < 8; ++k)
@@ -85,41 +97,45 @@ __global__ __launch_bounds__(64 * cols_waves(NT)) void k_packed_cols(const TX* _
 #pragma unroll
     for (int b = 0; b < NT; ++b) acc[n][b] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
 
-  for (int st = sa + wave; st < sb; st += W) {
-    const int r = st * STEP + 8 * q;                               // the lane's rows r..r+7
+  struct Step {
     uint32_t wd[8][Col8<NB>::NW];
+    Raw dy[NT];
+    floatx8 sc;
+  };
+  // FULL: all 32 rows exist; else rows past the last read as dy = 0 and any row's words.
+  auto load = [&](auto full, int st, Step& f) {
+    constexpr bool FULL = decltype(full)::value;
+    const int r = st * STEP + 8 * q;                               // the lane's rows r..r+7
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
-      const uint32_t* p = col + (int64_t)min(r + k, w.R - 1) * w.ldp;
+      const uint32_t* p = col + (int64_t)(FULL ? r + k : min(r + k, w.R - 1)) * w.ldp;
 #pragma unroll
-      for (int m = 0; m < Col8<NB>::NW; ++m) wd[k][m] = m < nw ? p[m] : 0u;
+      for (int m = 0; m < Col8<NB>::NW; ++m) f.wd[k][m] = p[max(min(m, nw - 1), 0)];
     }
-    Raw raw[NT];
-    floatx8 sc;
-    const bool full = r + 8 <= w.R;
 #pragma unroll
-    for (int b = 0; b < NT; ++b) raw[b] = full ? rq_load_x<true>(tok[b] + r, 8) : rq_load_x<false>(tok[b] + r, w.R - r);
+    for (int b = 0; b < NT; ++b) f.dy[b] = rq_load_x<FULL>(tok[b] + r, w.R - r);
     if (MODE != RQ_ANY) {
-      if (full && g[0] >= 0) {
-        sc = rq_load_as<floatx8>(w.scales + (int64_t)g[0] * w.lds + r);
+      const float* s = w.scales + (int64_t)g[0] * w.lds + r;
+      if (FULL) {
+        f.sc = rq_load_as<floatx8>(s);
       } else {
 #pragma unroll
-        for (int k = 0; k < 8; ++k) sc[k] = r + k < w.R ? rq_scale_of(w, g[0], r + k) : 0.0f;
+        for (int k = 0; k < 8; ++k) f.sc[k] = r + k < w.R ? s[k] : 0.0f;
       }
     }
+  };
+  auto compute = [&](int st, Step& f) {
+    const int r = st * STEP + 8 * q;
     bf16x8 d[NT][P::dy];
 #pragma unroll
     for (int b = 0; b < NT; ++b) {
       if constexpr (P::dy == 1) {
-        __builtin_memcpy(&d[b][0], &raw[b], 16);
+        __builtin_memcpy(&d[b][0], &f.dy[b], 16);
       } else {
-        floatx8 f;
-        fp32_of(raw[b], f);
-        if (MODE == RQ_RUNS) {
-#pragma unroll
-          for (int k = 0; k < 8; ++k) f[k] *= sc[k];
-        }
-        rq_operand<P::dy>(f, d[b]);
+        floatx8 v;
+        fp32_of(f.dy[b], v);
+        if (MODE == RQ_RUNS) v *= f.sc * rq_unit<NB>();
+        rq_operand<P::dy>(v, d[b]);
       }
     }
     // an inf's product with a piece of 0 would be a NaN that the formula does not have
@@ -133,42 +149,61 @@ __global__ __launch_bounds__(64 * cols_waves(NT)) void k_packed_cols(const TX* _
           low[b][k] = __builtin_fabsf(v) == INFINITY ? (__bf16)0.0f : d[b][0][k];
         }
     }
+    uint32_t odd[8];
 #pragma unroll
     for (int k = 0; k < 8; ++k) {                                  // fields to bit 0, two's complement
 #pragma unroll
       for (int m = 0; m < Col8<NB>::N; ++m) {
-        const uint32_t hi = m + 1 < Col8<NB>::NW ? wd[k][m + 1] : 0u;
-        uint32_t v = NB % 4 == 0 ? wd[k][m] : (uint32_t)((((uint64_t)hi << 32) | wd[k][m]) >> off);
-        wd[k][m] = v ^ rq_top_bits<NB>(m);
+        const uint32_t hi = m + 1 < Col8<NB>::NW ? f.wd[k][m + 1] : 0u;
+        const uint32_t v = NB % 4 == 0 ? f.wd[k][m] : (uint32_t)((((uint64_t)hi << 32) | f.wd[k][m]) >> off);
+        f.wd[k][m] = v ^ rq_top_bits<NB>(m);
       }
+      odd[k] = NB == 4 ? rq_odd_nibbles(f.wd[k][0]) : 0u;
     }
 #pragma unroll
     for (int n = 0; n < 8; ++n) {
+      const floatx8 codes = col_codes<NB>(f.wd, odd, n);
       bf16x8 v[P::w];
       if constexpr (P::w == 1) {
-#pragma unroll
-        for (int k = 0; k < 8; k += 2) rq_set2(v[0], k, (float)col_code<NB>(wd[k], n), (float)col_code<NB>(wd[k + 1], n));
+        rq_convert(codes, v[0]);
       } else {
-        floatx8 f;
+        floatx8 sc = f.sc;
         if (MODE == RQ_ANY) {
 #pragma unroll
           for (int k = 0; k < 8; ++k) sc[k] = r + k < w.R ? rq_scale_of(w, g[n], r + k) : 0.0f;
         }
-#pragma unroll
-        for (int k = 0; k < 8; ++k) f[k] = sc[k] * (float)col_code<NB>(wd[k], n);
-        rq_operand<P::w>(f, v);
+        rq_operand<P::w>(sc * rq_unit<NB>() * codes, v);
       }
 #pragma unroll
-      for (int b = 0; b < NT; ++b)
+      for (int pd = 0; pd < P::dy; ++pd)
 #pragma unroll
-        for (int pd = 0; pd < P::dy; ++pd)
+        for (int pw = 0; pw < P::w; ++pw)
+          if (pd + pw < P::keep) {
 #pragma unroll
-          for (int pw = 0; pw < P::w; ++pw)
-            if (pd + pw < P::keep) {
+            for (int b = 0; b < NT; ++b) {
               if constexpr (P::w > 1) acc[n][b] = rq_mfma(pd == 0 && pw ? low[b] : d[b][pd], v[pw], acc[n][b]);
               else acc[n][b] = rq_mfma(d[b][pd], v[pw], acc[n][b]);
             }
+          }
     }
+  };
+  // A step's loads are in flight while the one before is computed.
+  const int sf = min(sb, w.R / STEP);                              // up to here steps are full
+  Step now, then;
+  int st = sa + wave;
+  if (st < sf) {
+    load(std::true_type{}, st, now);
+    for (; st + W < sf; st += W) {
+      load(std::true_type{}, st + W, then);
+      compute(st, now);
+      now = then;
+    }
+    compute(st, now);
+    st += W;
+  }
+  if (st < sb) {
+    load(std::false_type{}, st, now);
+    compute(st, now);
   }
   // The waves' sums, halved together: always in the same order.
 #pragma unroll
@@ -195,11 +230,22 @@ __global__ __launch_bounds__(64 * cols_waves(NT)) void k_packed_cols(const TX* _
     for (int k = 0; k < 4; ++k) {
       const int t = t0 + 16 * b + 4 * q + k;
       if (t >= T) continue;
+      floatx8 v;
 #pragma unroll
-      for (int n = 0; n < 8; ++n) {
-        if (n >= nc) continue;
-        if (part) part[((int64_t)blockIdx.y * T + t) * w.C + c + n] = acc[n][b][k];
-        else dx[(int64_t)t * ldx + c + n] = rq_cast<TX>(acc[n][b][k]);
+      for (int n = 0; n < 8; ++n) v[n] = acc[n][b][k];
+      if (part) {
+        float* to = part + ((int64_t)blockIdx.y * T + t) * w.C + c;
+        if (nc >= 8) {
+          __builtin_memcpy(to, &v, 32);
+        } else {
+#pragma unroll
+          for (int n = 0; n < 8; ++n)
+            if (n < nc) to[n] = v[n];
+        }
+      } else {
+#pragma unroll
+        for (int n = 0; n < 8; ++n)
+          if (n < nc) dx[(int64_t)t * ldx + c + n] = rq_cast<TX>(v[n]);
       }
     }
 }

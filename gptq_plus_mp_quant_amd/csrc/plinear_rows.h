@@ -12,7 +12,7 @@ template <typename TX, int NB, int MODE, int RT, int NT>
 __global__ __launch_bounds__(rows_threads(RT, NT)) void k_packed_rows(const TX* __restrict__ x, int T, int64_t ldx, RqPacked w,
                                                       const TX* __restrict__ bias, TX* __restrict__ y, int64_t ldy) {
   extern __shared__ __attribute__((aligned(16))) float lds[];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+  const int lane = threadIdx.x & 63, wave = rq_wave(), waves = blockDim.x >> 6;
   const int r0 = blockIdx.x * 16 * RT, t0 = blockIdx.y * 16 * NT;
   RqTokens<TX, NT> xs;
 #pragma unroll
@@ -27,7 +27,7 @@ __global__ __launch_bounds__(rows_threads(RT, NT)) void k_packed_rows(const TX* 
   for (int a = 0; a < RT; ++a)
 #pragma unroll
     for (int b = 0; b < NT; ++b) acc[a][b] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
-  rq_rows_tokens<NB, MODE, RT>(w, r0, xs, wave, waves, staged ? lds : nullptr, acc);
+  rq_rows_tokens<NB, MODE, RT, 1>({w}, r0, xs, wave, waves, staged ? lds : nullptr, acc);
   if (staged) __syncthreads();
   floatx4* out = reinterpret_cast<floatx4*>(lds);
 #pragma unroll
@@ -77,7 +77,10 @@ void linear_rows(const TX* x, int T, int64_t ldx, const RqPacked& w, const TX* b
   constexpr int RT4 = RqOperand<TX>::pieces == 1 ? 2 : 1;       // fp32's pieces leave registers for one row tile
   switch (rq_mode_of(w)) {
     case RQ_RUNS:
-      if (T <= 16) launch_rows<TX, NB, RQ_RUNS, 1, 1>(x, T, ldx, w, bias, y, ldy, s);
+      // Two row tiles a wave share their tokens' loads; taken where they still make a workgroup for every CU
+      // (8192 x 28672 4-bit bf16, 1 / 16 tokens: 42 / 71 us with one, 35 / 49 with two).
+      if (T <= 16 && w.R >= 8192) launch_rows<TX, NB, RQ_RUNS, 2, 1>(x, T, ldx, w, bias, y, ldy, s);
+      else if (T <= 16) launch_rows<TX, NB, RQ_RUNS, 1, 1>(x, T, ldx, w, bias, y, ldy, s);
       else if (T <= 32) launch_rows<TX, NB, RQ_RUNS, 1, 2>(x, T, ldx, w, bias, y, ldy, s);
       else launch_rows<TX, NB, RQ_RUNS, RT4, 4>(x, T, ldx, w, bias, y, ldy, s);
       break;

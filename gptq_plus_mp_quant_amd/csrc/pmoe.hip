@@ -8,7 +8,6 @@
 // experts.  An expert that no token chose is not read, one that several chose is read once for 16 of them.
 // Router logits, sums, the activation and the sum over experts are fp32 (the activation in bf16 pieces that
 // carry 16 bits or all 24); the one rounding to fewer bits is the result's to x's type.
-#include "packed_dot.h"
 #include "pmoe_types.h"
 
 namespace {
@@ -22,14 +21,14 @@ __device__ __forceinline__ int lanes_before(uint64_t mask) {
   return __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0));
 }
 
-// A wave takes one expert and 8 tokens, 8 columns a lane.
+// A workgroup takes one expert and 8 tokens; its waves take 512 columns in turn, 8 a lane.
 constexpr int ROUTER_TOKENS = 8;
 template <typename TX>
 __global__ __launch_bounds__(256) void k_moe_router(const TX* __restrict__ x, int64_t ldx, int T, int D,
                                                     const TX* __restrict__ router, int64_t ldr, int E,
                                                     float* __restrict__ logits) {
-  const int e = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63, t0 = blockIdx.y * ROUTER_TOKENS;
-  if (e >= E) return;
+  __shared__ float join[4][ROUTER_TOKENS];
+  const int e = blockIdx.x, lane = threadIdx.x & 63, wave = rq_wave(), t0 = blockIdx.y * ROUTER_TOKENS;
   const TX* r = router + (int64_t)e * ldr;
   const int nt = min(ROUTER_TOKENS, T - t0);
   float s[ROUTER_TOKENS] = {};
@@ -46,12 +45,18 @@ __global__ __launch_bounds__(256) void k_moe_router(const TX* __restrict__ x, in
   };
   const int whole = D / 512 * 512;
 #pragma unroll 2
-  for (int c = 8 * lane; c < whole; c += 512) add(std::true_type{}, c, 8);
-  if (whole < D) add(std::false_type{}, whole + 8 * lane, D - whole - 8 * lane);
+  for (int c = 512 * wave; c < whole; c += 2048) add(std::true_type{}, c + 8 * lane, 8);
+  if (whole < D && whole / 512 % 4 == wave) add(std::false_type{}, whole + 8 * lane, D - whole - 8 * lane);
 #pragma unroll
   for (int t = 0; t < ROUTER_TOKENS; ++t) {
+    if (t >= nt) break;
     const float v = wave_sum(s[t]);
-    if (lane == 0 && t < nt) logits[(int64_t)(t0 + t) * E + e] = v;
+    if (lane == 0) join[wave][t] = v;
+  }
+  __syncthreads();
+  if ((int)threadIdx.x < nt) {
+    const int t = threadIdx.x;
+    logits[(int64_t)(t0 + t) * E + e] = (join[0][t] + join[1][t]) + (join[2][t] + join[3][t]);
   }
 }
 
@@ -60,7 +65,7 @@ __global__ __launch_bounds__(256) void k_moe_router(const TX* __restrict__ x, in
 // themselves.  Then a wave takes an expert: its pairs in ascending order, cut into units.
 __global__ __launch_bounds__(1024) void k_moe_route(const float* __restrict__ logits, int T, int E, int K, int norm,
                                                     float* __restrict__ weights, int* __restrict__ nunits,
-                                                    RqUnit* __restrict__ units, int* __restrict__ ids_out,
+                                                    RqUnit* __restrict__ units, int most, int* __restrict__ ids_out,
                                                     float* __restrict__ weights_out) {
   __shared__ int ids[MOE_TOKENS * MOE_MAX_K];
   __shared__ int first[MOE_MAX_E];                   // the expert's first unit, once they are counted
@@ -76,8 +81,9 @@ __global__ __launch_bounds__(1024) void k_moe_route(const float* __restrict__ lo
     for (int u = 0; u < EL; ++u) {
       if (64 * u >= E) break;
       const int e = 64 * u + lane;
-      v[u] = e < E ? l[e] : -INFINITY;
-      key[u] = e < E ? rq_order_key(v[u]) : 0;       // below every logit's
+      const float logit = l[min(e, E - 1)];
+      v[u] = e < E ? logit : -INFINITY;
+      key[u] = e < E ? rq_order_key(logit) : 0;      // below every logit's
       m = rq_nan_max(m, v[u]);
     }
     uint32_t least = 0;
@@ -136,6 +142,41 @@ __global__ __launch_bounds__(1024) void k_moe_route(const float* __restrict__ lo
   }
   __syncthreads();
   const int pairs = T * K;
+  if (pairs <= 64) {
+    // Few pairs, one a lane: the pairs of its expert before it, all of its expert's, and the units of lower
+    // experts are counted over the others.
+    if (wave) return;
+    const int e = lane < pairs ? ids[lane] : -1;
+    int before = 0, n = 0, pair0 = lane;
+    for (int j = pairs - 1; j >= 0; --j) {
+      const bool same = __builtin_amdgcn_readlane(e, j) == e;
+      before += same && j < lane ? 1 : 0;
+      n += same ? 1 : 0;
+      pair0 = same ? j : pair0;
+    }
+    const bool leads = lane < pairs && before == 0;
+    const int mine = leads ? (n + 15) / 16 : 0;
+    int lower = 0, all = 0;
+    for (int j = 0; j < pairs; ++j) {
+      const int ej = __builtin_amdgcn_readlane(e, j), uj = __builtin_amdgcn_readlane(mine, j);
+      lower += ej < e ? uj : 0;
+      all += uj;
+    }
+    if (lane < pairs) {
+      RqUnit& u = units[lower + before / 16];
+      u.pairs[before % 16] = lane;
+      if (before % 16 == 0) {
+        u.expert = e;
+        u.n = min(16, n - before);
+      }
+      // the last of an expert's pairs fills the places past it
+      if (before == n - 1)
+        for (int k = before % 16 + 1; k < 16; ++k) u.pairs[k] = pair0;
+    }
+    if (lane == 0) *nunits = all;
+    for (int k = all + lane; k < most; k += 64) units[k].n = 0;
+    return;
+  }
   for (int e = wave; e < E; e += 16) {               // units of every expert
     int n = 0;
     for (int p = 0; p < pairs; p += 64) n += __popcll(__ballot(p + lane < pairs && ids[p + lane] == e));
@@ -156,6 +197,7 @@ __global__ __launch_bounds__(1024) void k_moe_route(const float* __restrict__ lo
       before += __shfl(sum, 63);
     }
     if (lane == 0) *nunits = before;
+    for (int k = before + lane; k < most; k += 64) units[k].n = 0;
   }
   __syncthreads();
   for (int e = wave; e < E; e += 16) {
@@ -196,11 +238,11 @@ inline Layout layout(int T, int I, int E, int K) {
   l.units = l.nunits + 256;
   l.gate = l.units + up256((int64_t)rq_units((int)n, E, K) * (int64_t)sizeof(RqUnit));
   l.h = l.gate + up256(n * K * I * 4);
-  l.total = l.h + up256(n * K * I * 2 * 3);
+  l.total = l.h + up256(n * K * ((I + 127) / 128 * 128) * 2 * 3);
   return l;
 }
 inline RqExperts experts(const rq_packed_experts* p, int R, int C) {
-  return RqExperts{RqPacked{p->qweight, p->ldp, p->scales, p->lds, p->g_idx, R, C, p->ngroups, p->groupsize},
+  return RqExperts{rq_packed(p->qweight, p->ldp, p->scales, p->lds, p->g_idx, R, C, p->ngroups, p->groupsize),
                    p->stride_q, p->stride_scales, C};
 }
 
@@ -235,10 +277,13 @@ extern "C" int rq_packed_moe(const void* x, int dtype, int T, int64_t ldx, int D
     for (int64_t t0 = 0; t0 < T; t0 += MOE_TOKENS) {
       const int n = (int)(T - t0 < MOE_TOKENS ? T - t0 : MOE_TOKENS);
       const TX* xt = (const TX*)x + t0 * ldx;
-      const RqMoe m{n, D, I, E, K, norm, nunits, units, weights, (float*)(ws + l.gate), (__hip_bfloat16*)(ws + l.h)};
-      hipLaunchKernelGGL(k_moe_router<TX>, dim3((E + 3) / 4, (n + ROUTER_TOKENS - 1) / ROUTER_TOKENS), dim3(256), 0, s, xt,
+      const RqMoe m{n, D, I, E, K, norm, nunits, units, weights, (float*)(ws + l.gate), (__hip_bfloat16*)(ws + l.h),
+                    rq_moe_out_mode(d.w) == RQ_RUNS ? (I + 127) / 128 * 128 : I,
+                    rq_moe_out_mode(d.w) == RQ_RUNS};
+      hipLaunchKernelGGL(k_moe_router<TX>, dim3(E, (n + ROUTER_TOKENS - 1) / ROUTER_TOKENS), dim3(256), 0, s, xt,
                          ldx, n, D, (const TX*)router, ldr, E, logits);
       hipLaunchKernelGGL(k_moe_route, dim3(1), dim3(1024), 0, s, logits, n, E, K, norm, weights, nunits, units,
+                         rq_units(n, E, K),
                          ids_out ? ids_out + t0 * K : nullptr, weights_out ? weights_out + t0 * K : nullptr);
       rq_moe_in<TX>(xt, ldx, g, gate->nbits, u, up->nbits, m, s);
       rq_moe_out<TX>(d, down->nbits, m, (TX*)y + t0 * ldy, ldy, s);

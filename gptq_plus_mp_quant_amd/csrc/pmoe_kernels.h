@@ -1,54 +1,56 @@
 // The two products of a mixture-of-experts layer on the matrix cores (packed_dot.h), for one element type.
 #pragma once
-#include "packed_dot.h"
 #include "pmoe_types.h"
 
 namespace {
 
 enum { MOE_BOTH = 0, MOE_GATE = 1, MOE_UP = 2 };
 
-// Grid (row tiles, units).  BOTH: the first half of the waves takes 16 rows of gate, the second the same rows of
-// up, chunks of 128 columns in turn; joined through LDS, in their order.  GATE leaves the gate's product in
-// fp32, UP takes it from there (weights of different bits or groups).
-template <typename TX, int NB, int MODE>
-__global__ __launch_bounds__(512) void k_moe_in(const TX* __restrict__ x, int64_t ldx, RqExperts gate, RqExperts up,
+// Grid (row tiles, units): 16 rows, chunks of 128 columns to the waves in turn, joined through LDS in their order.
+// BOTH: a wave multiplies the rows of gate and of up by the tokens it has loaded once.  GATE leaves the gate's
+// product in fp32, UP takes it from there (weights of different bits or groups).
+template <typename TX, int NB, int MODE, int NM>
+__global__ __launch_bounds__(512, 4) void k_moe_in(const TX* __restrict__ x, int64_t ldx, RqExperts first, RqExperts second,
                                                 int what, RqMoe m) {
-  __shared__ floatx4 join[8][64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
-  if ((int)blockIdx.y >= *m.nunits) return;
+  __shared__ floatx4 join[NM][8][64];
+  const int lane = threadIdx.x & 63, wave = rq_wave(), waves = blockDim.x >> 6;
   const RqUnit& u = m.units[blockIdx.y];
-  const int r0 = blockIdx.x * 16, pair = u.pairs[lane & 15];
+  const int r0 = blockIdx.x * 16, pair = u.pairs[lane & 15], expert = u.expert;
+  if (u.n == 0) return;
   RqTokens<TX, 1> xs;
   xs.p[0] = x + (int64_t)(pair / m.K) * ldx;
-  const int each = what == MOE_BOTH ? waves / 2 : waves;
-  const RqPacked w = rq_expert(what == MOE_UP || wave >= each ? up : gate, u.expert);
-  floatx4 acc[1][1] = {{{0.0f, 0.0f, 0.0f, 0.0f}}};
-  rq_rows_tokens<NB, MODE, 1>(w, r0, xs, wave % each, each, nullptr, acc);
-  join[wave][lane] = acc[0][0];
+  RqPacked w[NM];
+  w[0] = rq_expert(first, expert);
+  if constexpr (NM == 2) w[1] = rq_expert(second, expert);
+  floatx4 acc[NM][1];
+#pragma unroll
+  for (int a = 0; a < NM; ++a) acc[a][0] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+  rq_rows_tokens<NB, MODE, NM, NM>(w, r0, xs, wave, waves, nullptr, acc);
+#pragma unroll
+  for (int a = 0; a < NM; ++a) join[a][wave][lane] = acc[a][0];
   __syncthreads();
   if (wave || (lane & 15) >= u.n) return;
-  floatx4 a = join[0][lane];
-  for (int k = 1; k < each; ++k) a += join[k][lane];
+  floatx4 a = join[0][0][lane], b = join[NM - 1][0][lane];
+  for (int k = 1; k < waves; ++k) {
+    a += join[0][k][lane];
+    b += join[NM - 1][k][lane];
+  }
   const int r = r0 + 4 * (lane >> 4);
   float* g = m.gate + (int64_t)pair * m.I + r;
-  floatx4 b;
   if (what == MOE_GATE) {
 #pragma unroll
     for (int k = 0; k < 4; ++k)
       if (r + k < m.I) g[k] = a[k];
     return;
   }
-  if (what == MOE_BOTH) {
-    b = join[each][lane];
-    for (int k = 1; k < each; ++k) b += join[each + k][lane];
-  } else {
-    b = a;
+  if (what == MOE_UP) {
 #pragma unroll
     for (int k = 0; k < 4; ++k) a[k] = r + k < m.I ? g[k] : 0.0f;
   }
   constexpr int P = rq_moe_pieces<TX>();
-  const int64_t plane = (int64_t)m.T * m.K * m.I;
-  __hip_bfloat16* h = m.h + (int64_t)pair * m.I + r;
+  const int64_t plane = (int64_t)m.T * m.K * m.ldh;
+  __hip_bfloat16* row = m.h + (int64_t)pair * m.ldh;
+  __hip_bfloat16* h = row + (m.arranged ? rq_arranged(r) : r);                // r is a multiple of 4
   const float p = m.weights[pair];
   floatx8 v = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
@@ -60,30 +62,105 @@ __global__ __launch_bounds__(512) void k_moe_in(const TX* __restrict__ x, int64_
 #pragma unroll
     for (int k = 0; k < 4; ++k)
       if (r + k < m.I) __builtin_memcpy(h + q * plane + k, (const char*)&o[q] + 2 * k, 2);
+  if (r0 + 16 >= m.I && m.arranged) {                  // the last rows' workgroup fills the last chunk up
+    for (int c = m.I + (lane >> 4); c < m.ldh; c += 4)
+#pragma unroll
+      for (int q = 0; q < P; ++q) row[q * plane + rq_arranged(c)] = __hip_bfloat16(0.0f);
+  }
 }
 
 // Grid (row tiles): 16 rows of down for every unit.  Chunk c of expert e goes to wave (c + e) mod W, whatever else
-// is in the batch, and a wave adds its units' sums to its own copy of the workgroup's results in LDS, in the
+// is in the batch, and a wave adds every chunk's sums to its own copy of the workgroup's results in LDS, in the
 // order of the experts: a token's result does not depend on the other tokens.
-template <typename TX, int NB, int MODE, int W>
-__global__ __launch_bounds__(64 * W) void k_moe_out(RqExperts down, RqMoe m, TX* __restrict__ y, int64_t ldy) {
-  constexpr int P = rq_moe_pieces<TX>();
-  extern __shared__ __attribute__((aligned(16))) floatx4 sums[];       // [W][T][4]: 16 rows of a token
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, q = lane >> 4;
-  const int r0 = blockIdx.x * 16, n = *m.nunits;
+// RUNS: the loads of the next D chunks, of whatever units, are in flight.
+constexpr int OUT_WAVES = 8;
+template <typename TX, int NB, int MODE>
+__global__ __launch_bounds__(64 * OUT_WAVES) void k_moe_out(RqExperts down, RqMoe m, TX* __restrict__ y, int64_t ldy) {
+  constexpr int P = rq_moe_pieces<TX>(), W = OUT_WAVES;
+  extern __shared__ __attribute__((aligned(16))) floatx4 sums[];       // [W][T][4]: 16 rows of a token; then the units
+  RqUnit* units = reinterpret_cast<RqUnit*>(sums + W * m.T * 4);
+  const int lane = threadIdx.x & 63, wave = rq_wave(), i = lane & 15, q = lane >> 4;
+  const int r0 = blockIdx.x * 16, n = __builtin_amdgcn_readfirstlane(*m.nunits);
+  for (int k = threadIdx.x; k < m.T * 4 * W; k += 64 * W) sums[k] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+  for (int k = threadIdx.x; k < n * (int)(sizeof(RqUnit) / 4); k += 64 * W)
+    reinterpret_cast<int*>(units)[k] = reinterpret_cast<const int*>(m.units)[k];
+  __syncthreads();
   floatx4* mine = sums + wave * m.T * 4;
-  for (int k = lane; k < m.T * 4; k += 64) mine[k] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
-  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-  __builtin_amdgcn_wave_barrier();
-  for (int k = 0; k < n; ++k) {
-    const RqUnit& u = m.units[k];
-    const int pair = u.pairs[i];
-    RqPieces<P> xs;
-    xs.p = m.h + (int64_t)pair * m.I;
-    xs.plane = (int64_t)m.T * m.K * m.I;
-    floatx4 acc[1][1] = {{{0.0f, 0.0f, 0.0f, 0.0f}}};
-    rq_rows_tokens<NB, MODE, 1>(rq_expert(down, u.expert), r0, xs, (wave + W - u.expert % W) % W, W, nullptr, acc);
-    if (i < u.n) mine[pair / m.K * 4 + q] += acc[0][0];
+  const int nch = (down.w.C + RQ_CHUNK - 1) / RQ_CHUNK;
+  auto expert_of = [&](int k) { return __builtin_amdgcn_readfirstlane(units[k].expert); };
+  auto begin = [&](int k) { return (wave + W - expert_of(k) % W) % W; };       // the wave's first chunk of a unit
+  if constexpr (MODE == RQ_RUNS) {
+    typedef RqPieces<P, true> X;
+    constexpr int D = 3;
+    // The wave's chunks in order: unit k, chunk c.
+    struct Place {
+      int k, c;
+    };
+    auto next = [&](Place p) {
+      p.c += W;
+      while (p.k < n && p.c >= nch) {
+        ++p.k;
+        if (p.k < n) p.c = begin(p.k);
+      }
+      return p;
+    };
+    struct Flight {
+      RqRunsW<NB, 1> f;
+      typename X::raw x[1][4];
+      int pair, places, c;                 // places: tokens of the unit, 0 past the last chunk
+    };
+    Place ahead{0, 0};
+    if (n > 0) ahead.c = begin(0) - W;
+    ahead = next(ahead);
+    const Place first = ahead;
+    // Past the end the first chunk is loaded again and nothing is made of it: no load is conditional.
+    auto load = [&](Flight& t) {
+      const bool is = ahead.k < n;
+      const Place p = is ? ahead : first;
+      const RqUnit& u = units[p.k];
+      t.pair = u.pairs[i];
+      t.places = is ? __builtin_amdgcn_readfirstlane(u.n) : 0;
+      t.c = p.c;
+      X xs;
+      xs.p = m.h + (int64_t)t.pair * m.ldh;
+      xs.plane = (int64_t)m.T * m.K * m.ldh;
+      const RqPacked w[1] = {rq_expert(down, expert_of(p.k))};
+      const uint32_t* row[1] = {w[0].q + (int64_t)min(r0 + i, w[0].R - 1) * w[0].ldp};
+      // A lane past the row's last column, where h is 0, loads the last words again.
+      const int c = min(p.c * RQ_CHUNK + 32 * q, w[0].C - 32);
+      __builtin_memcpy(t.f.wd[0], row[0] + (int64_t)(c >> 5) * NB, 4 * NB);
+      t.f.sc[0] = rq_load_scales4(w[0], rq_run_group(w[0], p.c * RQ_CHUNK), r0 + 4 * q);
+      rq_load_tokens<true>(xs, w[0].C, p.c, t.x);
+      ahead = is ? next(ahead) : ahead;
+    };
+    if (first.k < n) {
+      Flight t[D];
+#pragma unroll
+      for (int u = 0; u < D; ++u) load(t[u]);
+      const RqPacked w[1] = {down.w};      // for the groups of rows and columns
+      for (;;) {
+#pragma unroll
+        for (int u = 0; u < D; ++u) {
+          if (t[u].places == 0) goto done;
+          floatx4 acc[1][1] = {{{0.0f, 0.0f, 0.0f, 0.0f}}};
+          rq_chunk_runs<X, NB, 1, 1>(w, r0, t[u].c, t[u].f, t[u].x, acc);
+          if (i < t[u].places) mine[t[u].pair / m.K * 4 + q] += acc[0][0];
+          load(t[u]);
+        }
+      }
+    done:;
+    }
+  } else {
+    for (int k = 0; k < n; ++k) {
+      const int pair = units[k].pairs[i];
+      RqPieces<P, false> xs;
+      xs.p = m.h + (int64_t)pair * m.ldh;
+      xs.plane = (int64_t)m.T * m.K * m.ldh;
+      const RqPacked w[1] = {rq_expert(down, expert_of(k))};
+      floatx4 acc[1][1] = {{{0.0f, 0.0f, 0.0f, 0.0f}}};
+      rq_rows_tokens<NB, MODE, 1, 1>(w, r0, xs, begin(k), W, nullptr, acc);
+      if (i < units[k].n) mine[pair / m.K * 4 + q] += acc[0][0];
+    }
   }
   __syncthreads();
   for (int e = threadIdx.x; e < m.T * 4; e += 64 * W) {
@@ -97,8 +174,8 @@ __global__ __launch_bounds__(64 * W) void k_moe_out(RqExperts down, RqMoe m, TX*
 }
 
 template <typename F>
-inline void with_mode(const RqPacked& w, F&& f) {
-  switch (rq_mode_of(w)) {
+inline void with_mode(int mode, F&& f) {
+  switch (mode) {
     case RQ_RUNS: f(std::integral_constant<int, RQ_RUNS>{}); break;
     case RQ_SMALL: f(std::integral_constant<int, RQ_SMALL>{}); break;
     default: f(std::integral_constant<int, RQ_ANY>{}); break;
@@ -111,33 +188,30 @@ template <typename TX>
 void rq_moe_in(const TX* x, int64_t ldx, const RqExperts& gate, int gate_bits, const RqExperts& up, int up_bits,
                const RqMoe& m, hipStream_t s) {
   const dim3 grid((m.I + 15) / 16, rq_units(m.T, m.E, m.K)), block(512);
-  auto launch = [&](const RqExperts& of, int bits, int what) {
+  auto launch = [&](const RqExperts& of, int bits, int what, auto both) {
+    constexpr int NM = decltype(both)::value ? 2 : 1;
     rq_with_nbits(bits, [&](auto nb) {
-      with_mode(of.w, [&](auto mode) {
-        hipLaunchKernelGGL((k_moe_in<TX, decltype(nb)::value, decltype(mode)::value>), grid, block, 0, s, x, ldx, gate, up,
+      with_mode(rq_mode_of(of.w), [&](auto mode) {
+        hipLaunchKernelGGL((k_moe_in<TX, decltype(nb)::value, decltype(mode)::value, NM>), grid, block, 0, s, x, ldx, of, up,
                            what, m);
       });
     });
   };
   if (gate_bits == up_bits && rq_mode_of(gate.w) == rq_mode_of(up.w)) {
-    launch(gate, gate_bits, MOE_BOTH);
+    launch(gate, gate_bits, MOE_BOTH, std::true_type{});
   } else {
-    launch(gate, gate_bits, MOE_GATE);
-    launch(up, up_bits, MOE_UP);
+    launch(gate, gate_bits, MOE_GATE, std::false_type{});
+    launch(up, up_bits, MOE_UP, std::false_type{});
   }
 }
 
 template <typename TX>
 void rq_moe_out(const RqExperts& down, int bits, const RqMoe& m, TX* y, int64_t ldy, hipStream_t s) {
   rq_with_nbits(bits, [&](auto nb) {
-    with_mode(down.w, [&](auto mode) {
-      constexpr int NB = decltype(nb)::value, MODE = decltype(mode)::value;
-      const dim3 grid((m.D + 15) / 16);
-      // the copies of the results fit 32 KB of LDS
-      if (m.T <= 32)
-        hipLaunchKernelGGL((k_moe_out<TX, NB, MODE, 16>), grid, dim3(1024), 16 * m.T * 64, s, down, m, y, ldy);
-      else
-        hipLaunchKernelGGL((k_moe_out<TX, NB, MODE, 8>), grid, dim3(512), 8 * m.T * 64, s, down, m, y, ldy);
+    with_mode(rq_moe_out_mode(down.w), [&](auto mode) {
+      hipLaunchKernelGGL((k_moe_out<TX, decltype(nb)::value, decltype(mode)::value>), dim3((m.D + 15) / 16),
+                         dim3(64 * OUT_WAVES),
+                         OUT_WAVES * m.T * 64 + rq_units(m.T, m.E, m.K) * (int)sizeof(RqUnit), s, down, m, y, ldy);
     });
   });
 }

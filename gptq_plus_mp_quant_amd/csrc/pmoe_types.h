@@ -1,7 +1,7 @@
 // A mixture-of-experts layer for a few tokens: what its launches share.  Each element type's kernels (one
 // for every bit width) are a translation unit of their own.
 #pragma once
-#include "packed_bits.h"
+#include "packed_dot.h"
 
 constexpr int MOE_MAX_E = 1024, MOE_MAX_K = 64;
 constexpr int MOE_TOKENS = 64;            // tokens per pass over the experts
@@ -20,7 +20,7 @@ __device__ __forceinline__ RqPacked rq_expert(const RqExperts& x, int e) {
 }
 
 // Up to 16 tokens of one expert: what a tile of the matrix cores takes.  pairs: token * K + place among the
-// token's experts, ascending; past n the first again.
+// token's experts, ascending; past n the first again.  Units past the last have n = 0.
 struct RqUnit {
   int expert, n, pairs[16];
 };
@@ -35,13 +35,22 @@ inline int rq_units(int T, int E, int K) {
 template <typename TX>
 constexpr int rq_moe_pieces() { return sizeof(TX) == 4 ? 3 : 2; }
 
+// How down is read: h may be filled up to whole chunks, so RUNS needs no ragged end as long as rows are whole
+// words of 32 columns; other rows go 8 columns at a time.
+inline int rq_moe_out_mode(const RqPacked& down) {
+  const int mode = rq_mode_of(down);
+  return mode == RQ_RUNS && down.C % 32 ? RQ_SMALL : mode;
+}
+
 struct RqMoe {
   int T, D, I, E, K, norm;
   const int* nunits;                      // 1
   const RqUnit* units;                    // rq_units
   const float* weights;                   // T * K
   float* gate;                            // T * K * I: the gate's product where up has other bits or groups
-  __hip_bfloat16* h;                      // pieces planes of T * K * I
+  __hip_bfloat16* h;                      // pieces planes of T * K * ldh
+  int ldh;                                // I; where h lies arranged (rq_arranged, for a down of RUNS), whole chunks
+  bool arranged;
 };
 
 // h = weight * silu(gate x) * (up x) of every pair, in pieces.

@@ -66,10 +66,15 @@ __device__ __forceinline__ void fp32_of(floatx8 v, floatx8& f) { f = v; }
 
 constexpr int cols_waves(int nt) { return nt >= 4 ? 4 : 8; }
 
+// Waves of a SIMD that the registers are cut for: with RUNS four token tiles fit 256 (14336 x 4096 4-bit bf16,
+// 64 tokens: 30 us, 37 with one wave a SIMD and 280); the other modes would spill (4096 x 4096 along an order: 54 for
+// 45).
+constexpr int cols_occupancy(int mode, int nt) { return mode == RQ_RUNS && nt >= 4 ? 2 : 1; }
+
 template <typename TX, int NB, int MODE, int NT>
-__global__ __launch_bounds__(64 * cols_waves(NT)) void k_packed_cols(const TX* __restrict__ dy, int T, int64_t ldy,
-                                                                     RqPacked w, int steps_per, float* __restrict__ part,
-                                                                     TX* __restrict__ dx, int64_t ldx) {
+__global__ __launch_bounds__(64 * cols_waves(NT), cols_occupancy(MODE, NT)) void k_packed_cols(
+    const TX* __restrict__ dy, int T, int64_t ldy, RqPacked w, int steps_per, float* __restrict__ part, TX* __restrict__ dx,
+    int64_t ldx) {
   constexpr int W = cols_waves(NT);
   typedef ColPieces<TX, MODE> P;
   typedef typename RqOperand<TX>::raw Raw;

@@ -227,9 +227,9 @@ __global__ __launch_bounds__(1024) void k_moe_route(const float* __restrict__ lo
 
 inline int64_t up256(int64_t n) { return (n + 255) / 256 * 256; }
 struct Layout {
-  int64_t logits, weights, nunits, units, gate, h, total;
+  int64_t logits, weights, nunits, units, gate, h, parts, total;
 };
-inline Layout layout(int T, int I, int E, int K) {
+inline Layout layout(int T, int D, int I, int E, int K) {
   const int64_t n = T < MOE_TOKENS ? T : MOE_TOKENS;
   Layout l;
   l.logits = 0;
@@ -238,7 +238,8 @@ inline Layout layout(int T, int I, int E, int K) {
   l.units = l.nunits + 256;
   l.gate = l.units + up256((int64_t)rq_units((int)n, E, K) * (int64_t)sizeof(RqUnit));
   l.h = l.gate + up256(n * K * I * 4);
-  l.total = l.h + up256(n * K * ((I + 127) / 128 * 128) * 2 * 3);
+  l.parts = l.h + up256(n * K * (((int64_t)I + 127) / 128 * 128) * 2 * 3);
+  l.total = l.parts + up256((int64_t)rq_moe_parts(D) * n * D * 4);
   return l;
 }
 inline RqExperts experts(const rq_packed_experts* p, int R, int C) {
@@ -250,7 +251,7 @@ inline RqExperts experts(const rq_packed_experts* p, int R, int C) {
 
 extern "C" int64_t rq_packed_moe_workspace_bytes(int T, int D, int I, int E, int K) {
   if (T < 0 || D <= 0 || I <= 0 || E <= 0 || E > MOE_MAX_E || K <= 0 || K > MOE_MAX_K || K > E) return RQ_EINVAL;
-  return layout(T, I, E, K).total;
+  return layout(T, D, I, E, K).total;
 }
 
 extern "C" int rq_packed_moe(const void* x, int dtype, int T, int64_t ldx, int D, const void* router, int64_t ldr, int E,
@@ -266,7 +267,7 @@ extern "C" int rq_packed_moe(const void* x, int dtype, int T, int64_t ldx, int D
   if (T == 0) return RQ_OK;
   if (!x || !router || !y || ldx < D || ldr < D || ldy < D || !workspace || workspace_bytes < need) return RQ_EINVAL;
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-  const Layout l = layout(T, I, E, K);
+  const Layout l = layout(T, D, I, E, K);
   char* ws = (char*)workspace;
   float* logits = (float*)(ws + l.logits);
   float* weights = (float*)(ws + l.weights);
@@ -279,7 +280,7 @@ extern "C" int rq_packed_moe(const void* x, int dtype, int T, int64_t ldx, int D
       const TX* xt = (const TX*)x + t0 * ldx;
       const RqMoe m{n, D, I, E, K, norm, nunits, units, weights, (float*)(ws + l.gate), (__hip_bfloat16*)(ws + l.h),
                     rq_moe_out_mode(d.w) == RQ_RUNS ? (I + 127) / 128 * 128 : I,
-                    rq_moe_out_mode(d.w) == RQ_RUNS};
+                    rq_moe_out_mode(d.w) == RQ_RUNS, (float*)(ws + l.parts)};
       hipLaunchKernelGGL(k_moe_router<TX>, dim3(E, (n + ROUTER_TOKENS - 1) / ROUTER_TOKENS), dim3(256), 0, s, xt,
                          ldx, n, D, (const TX*)router, ldr, E, logits);
       hipLaunchKernelGGL(k_moe_route, dim3(1), dim3(1024), 0, s, logits, n, E, K, norm, weights, nunits, units,

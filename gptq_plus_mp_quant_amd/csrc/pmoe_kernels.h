@@ -22,9 +22,7 @@ __global__ __launch_bounds__(512, 4) void k_moe_in(const TX* __restrict__ x, int
   RqPacked w[NM];
   w[0] = rq_expert(first, expert);
   if constexpr (NM == 2) w[1] = rq_expert(second, expert);
-  floatx4 acc[NM][1];
-#pragma unroll
-  for (int a = 0; a < NM; ++a) acc[a][0] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+  floatx4 acc[NM][1] = {};
   rq_rows_tokens<NB, MODE, NM, NM>(w, r0, xs, wave, waves, nullptr, acc);
 #pragma unroll
   for (int a = 0; a < NM; ++a) join[a][wave][lane] = acc[a][0];
@@ -62,7 +60,7 @@ __global__ __launch_bounds__(512, 4) void k_moe_in(const TX* __restrict__ x, int
 #pragma unroll
     for (int k = 0; k < 4; ++k)
       if (r + k < m.I) __builtin_memcpy(h + q * plane + k, (const char*)&o[q] + 2 * k, 2);
-  if (r0 + 16 >= m.I && m.arranged) {                  // the last rows' workgroup fills the last chunk up
+  if (r0 + 16 >= m.I && m.arranged) {       // the last rows' workgroup fills the last chunk up
     for (int c = m.I + (lane >> 4); c < m.ldh; c += 4)
 #pragma unroll
       for (int q = 0; q < P; ++q) row[q * plane + rq_arranged(c)] = __hip_bfloat16(0.0f);
@@ -73,31 +71,31 @@ __global__ __launch_bounds__(512, 4) void k_moe_in(const TX* __restrict__ x, int
 // is in the batch, and a wave adds every chunk's sums to its own copy of the workgroup's results in LDS, in the
 // order of the experts: a token's result does not depend on the other tokens.
 // RUNS: the loads of the next D chunks, of whatever units, are in flight.
-constexpr int OUT_WAVES = 8;
-template <typename TX, int NB, int MODE>
-__global__ __launch_bounds__(64 * OUT_WAVES) void k_moe_out(RqExperts down, RqMoe m, TX* __restrict__ y, int64_t ldy) {
-  constexpr int P = rq_moe_pieces<TX>(), W = OUT_WAVES;
-  extern __shared__ __attribute__((aligned(16))) floatx4 sums[];       // [W][T][4]: 16 rows of a token; then the units
-  RqUnit* units = reinterpret_cast<RqUnit*>(sums + W * m.T * 4);
+template <typename TX, int NB, int MODE, int RT>
+__global__ __launch_bounds__(64 * MOE_OUT_WAVES) void k_moe_out(RqExperts down, RqMoe m, TX* __restrict__ y, int64_t ldy) {
+  constexpr int P = rq_moe_pieces<TX>(), W = MOE_OUT_WAVES, R4 = 4 * RT;
+  extern __shared__ __attribute__((aligned(16))) floatx4 sums[];       // [W][T][R4]: the rows of a token; then the units
+  RqUnit* units = reinterpret_cast<RqUnit*>(sums + W * m.T * R4);
   const int lane = threadIdx.x & 63, wave = rq_wave(), i = lane & 15, q = lane >> 4;
-  const int r0 = blockIdx.x * 16, n = __builtin_amdgcn_readfirstlane(*m.nunits);
-  for (int k = threadIdx.x; k < m.T * 4 * W; k += 64 * W) sums[k] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+  const int r0 = blockIdx.x * 16 * RT, n = __builtin_amdgcn_readfirstlane(*m.nunits);
+  for (int k = threadIdx.x; k < m.T * R4 * W; k += 64 * W) sums[k] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
   for (int k = threadIdx.x; k < n * (int)(sizeof(RqUnit) / 4); k += 64 * W)
     reinterpret_cast<int*>(units)[k] = reinterpret_cast<const int*>(m.units)[k];
   __syncthreads();
-  floatx4* mine = sums + wave * m.T * 4;
+  floatx4* mine = sums + wave * m.T * R4;
+  const int all = W * gridDim.y, self = wave + W * blockIdx.y;         // of the waves that share the rows
   const int nch = (down.w.C + RQ_CHUNK - 1) / RQ_CHUNK;
   auto expert_of = [&](int k) { return __builtin_amdgcn_readfirstlane(units[k].expert); };
-  auto begin = [&](int k) { return (wave + W - expert_of(k) % W) % W; };       // the wave's first chunk of a unit
+  auto begin = [&](int k) { return (self + all - expert_of(k) % all) % all; };       // the wave's first chunk of a unit
   if constexpr (MODE == RQ_RUNS) {
     typedef RqPieces<P, true> X;
-    constexpr int D = 3;
+    constexpr int D = RT == 1 ? 3 : 2;
     // The wave's chunks in order: unit k, chunk c.
     struct Place {
       int k, c;
     };
     auto next = [&](Place p) {
-      p.c += W;
+      p.c += all;
       while (p.k < n && p.c >= nch) {
         ++p.k;
         if (p.k < n) p.c = begin(p.k);
@@ -105,12 +103,12 @@ __global__ __launch_bounds__(64 * OUT_WAVES) void k_moe_out(RqExperts down, RqMo
       return p;
     };
     struct Flight {
-      RqRunsW<NB, 1> f;
+      RqRunsW<NB, RT> f;
       typename X::raw x[1][4];
       int pair, places, c;                 // places: tokens of the unit, 0 past the last chunk
     };
     Place ahead{0, 0};
-    if (n > 0) ahead.c = begin(0) - W;
+    if (n > 0) ahead.c = begin(0) - all;
     ahead = next(ahead);
     const Place first = ahead;
     // Past the end the first chunk is loaded again and nothing is made of it: no load is conditional.
@@ -125,11 +123,14 @@ __global__ __launch_bounds__(64 * OUT_WAVES) void k_moe_out(RqExperts down, RqMo
       xs.p = m.h + (int64_t)t.pair * m.ldh;
       xs.plane = (int64_t)m.T * m.K * m.ldh;
       const RqPacked w[1] = {rq_expert(down, expert_of(p.k))};
-      const uint32_t* row[1] = {w[0].q + (int64_t)min(r0 + i, w[0].R - 1) * w[0].ldp};
       // A lane past the row's last column, where h is 0, loads the last words again.
       const int c = min(p.c * RQ_CHUNK + 32 * q, w[0].C - 32);
-      __builtin_memcpy(t.f.wd[0], row[0] + (int64_t)(c >> 5) * NB, 4 * NB);
-      t.f.sc[0] = rq_load_scales4(w[0], rq_run_group(w[0], p.c * RQ_CHUNK), r0 + 4 * q);
+#pragma unroll
+      for (int a = 0; a < RT; ++a) {
+        const uint32_t* row = w[0].q + (int64_t)min(r0 + 16 * a + i, w[0].R - 1) * w[0].ldp;
+        __builtin_memcpy(t.f.wd[a], row + (int64_t)(c >> 5) * NB, 4 * NB);
+        t.f.sc[a] = rq_load_scales4(w[0], rq_run_group(w[0], p.c * RQ_CHUNK), r0 + 16 * a + 4 * q);
+      }
       rq_load_tokens<true>(xs, w[0].C, p.c, t.x);
       ahead = is ? next(ahead) : ahead;
     };
@@ -142,9 +143,12 @@ __global__ __launch_bounds__(64 * OUT_WAVES) void k_moe_out(RqExperts down, RqMo
 #pragma unroll
         for (int u = 0; u < D; ++u) {
           if (t[u].places == 0) goto done;
-          floatx4 acc[1][1] = {{{0.0f, 0.0f, 0.0f, 0.0f}}};
-          rq_chunk_runs<X, NB, 1, 1>(w, r0, t[u].c, t[u].f, t[u].x, acc);
-          if (i < t[u].places) mine[t[u].pair / m.K * 4 + q] += acc[0][0];
+          floatx4 acc[RT][1] = {};
+          rq_chunk_runs<X, NB, RT, 1>(w, r0, t[u].c, t[u].f, t[u].x, acc);
+          if (i < t[u].places) {
+#pragma unroll
+            for (int a = 0; a < RT; ++a) mine[t[u].pair / m.K * R4 + 4 * a + q] += acc[a][0];
+          }
           load(t[u]);
         }
       }
@@ -157,20 +161,36 @@ __global__ __launch_bounds__(64 * OUT_WAVES) void k_moe_out(RqExperts down, RqMo
       xs.p = m.h + (int64_t)pair * m.ldh;
       xs.plane = (int64_t)m.T * m.K * m.ldh;
       const RqPacked w[1] = {rq_expert(down, expert_of(k))};
-      floatx4 acc[1][1] = {{{0.0f, 0.0f, 0.0f, 0.0f}}};
-      rq_rows_tokens<NB, MODE, 1, 1>(w, r0, xs, begin(k), W, nullptr, acc);
-      if (i < units[k].n) mine[pair / m.K * 4 + q] += acc[0][0];
+      floatx4 acc[RT][1] = {};
+      rq_rows_tokens<NB, MODE, RT, 1>(w, r0, xs, begin(k), all, nullptr, acc);
+      if (i < units[k].n) {
+#pragma unroll
+        for (int a = 0; a < RT; ++a) mine[pair / m.K * R4 + 4 * a + q] += acc[a][0];
+      }
     }
   }
   __syncthreads();
-  for (int e = threadIdx.x; e < m.T * 4; e += 64 * W) {
-    const int t = e >> 2, r = r0 + 4 * (e & 3);
+  for (int e = threadIdx.x; e < m.T * R4; e += 64 * W) {
+    const int t = e / R4, r = r0 + 4 * (e % R4);
     floatx4 v = sums[e];
-    for (int k = 1; k < W; ++k) v += sums[k * m.T * 4 + e];
+    for (int k = 1; k < W; ++k) v += sums[k * m.T * R4 + e];
 #pragma unroll
-    for (int k = 0; k < 4; ++k)
-      if (r + k < m.D) y[(int64_t)t * ldy + r + k] = rq_cast<TX>(v[k]);
+    for (int k = 0; k < 4; ++k) {
+      if (r + k >= m.D) continue;
+      if (gridDim.y > 1) m.parts[((int64_t)blockIdx.y * m.T + t) * m.D + r + k] = v[k];
+      else y[(int64_t)t * ldy + r + k] = rq_cast<TX>(v[k]);
+    }
   }
+}
+// The sums of the workgroups that share rows, in their order.
+template <typename TX>
+__global__ __launch_bounds__(256) void k_moe_join(const float* __restrict__ parts, int n, int T, int D, TX* __restrict__ y,
+                                                  int64_t ldy) {
+  const int r = blockIdx.x * 256 + threadIdx.x, t = blockIdx.y;
+  if (r >= D) return;
+  float v = parts[(int64_t)t * D + r];
+  for (int k = 1; k < n; ++k) v += parts[((int64_t)k * T + t) * D + r];
+  y[(int64_t)t * ldy + r] = rq_cast<TX>(v);
 }
 
 template <typename F>
@@ -187,13 +207,16 @@ inline void with_mode(int mode, F&& f) {
 template <typename TX>
 void rq_moe_in(const TX* x, int64_t ldx, const RqExperts& gate, int gate_bits, const RqExperts& up, int up_bits,
                const RqMoe& m, hipStream_t s) {
-  const dim3 grid((m.I + 15) / 16, rq_units(m.T, m.E, m.K)), block(512);
+  const dim3 grid((m.I + 15) / 16, rq_units(m.T, m.E, m.K));
+  // Eight waves share the columns, four where there are workgroups enough without (8 experts of 4096 x 7168, 32
+  // tokens: 107 us for 111).
+  const dim3 block(grid.x * grid.y >= 2048 ? 256 : 512);
   auto launch = [&](const RqExperts& of, int bits, int what, auto both) {
     constexpr int NM = decltype(both)::value ? 2 : 1;
     rq_with_nbits(bits, [&](auto nb) {
       with_mode(rq_mode_of(of.w), [&](auto mode) {
-        hipLaunchKernelGGL((k_moe_in<TX, decltype(nb)::value, decltype(mode)::value, NM>), grid, block, 0, s, x, ldx, of, up,
-                           what, m);
+        hipLaunchKernelGGL((k_moe_in<TX, decltype(nb)::value, decltype(mode)::value, NM>), grid, block, 0, s, x, ldx, of,
+                           up, what, m);
       });
     });
   };
@@ -209,9 +232,18 @@ template <typename TX>
 void rq_moe_out(const RqExperts& down, int bits, const RqMoe& m, TX* y, int64_t ldy, hipStream_t s) {
   rq_with_nbits(bits, [&](auto nb) {
     with_mode(rq_moe_out_mode(down.w), [&](auto mode) {
-      hipLaunchKernelGGL((k_moe_out<TX, decltype(nb)::value, decltype(mode)::value>), dim3((m.D + 15) / 16),
-                         dim3(64 * OUT_WAVES),
-                         OUT_WAVES * m.T * 64 + rq_units(m.T, m.E, m.K) * (int)sizeof(RqUnit), s, down, m, y, ldy);
+      auto go = [&](auto rt, int parts) {
+        constexpr int RT = decltype(rt)::value;
+        hipLaunchKernelGGL((k_moe_out<TX, decltype(nb)::value, decltype(mode)::value, RT>),
+                           dim3((m.D + 16 * RT - 1) / (16 * RT), parts), dim3(64 * MOE_OUT_WAVES),
+                           rq_moe_out_lds(m, RT), s, down, m, y, ldy);
+        if (parts > 1)
+          hipLaunchKernelGGL(k_moe_join<TX>, dim3((m.D + 255) / 256, m.T), dim3(256), 0, s, m.parts, parts, m.T, m.D, y, ldy);
+      };
+      if constexpr (decltype(mode)::value == RQ_RUNS) {
+        if (rq_moe_dense(m)) return go(std::integral_constant<int, MOE_OUT_ROWS>{}, rq_moe_parts(m.D));
+      }
+      go(std::integral_constant<int, 1>{}, 1);
     });
   });
 }

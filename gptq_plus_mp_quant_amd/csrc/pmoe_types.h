@@ -51,7 +51,24 @@ struct RqMoe {
   __hip_bfloat16* h;                      // pieces planes of T * K * ldh
   int ldh;                                // I; where h lies arranged (rq_arranged, for a down of RUNS), whole chunks
   bool arranged;
+  float* parts;                           // rq_moe_parts planes of T * D
 };
+// The product with down for many pairs takes four row tiles a wave for a load of h, which is several times the
+// weights' bytes where an expert has many tokens; workgroups share rows until there is one for every CU, and a launch
+// of its own adds them up.  From 32 pairs on that is faster (one row tile / four, the whole layer: 8 experts of 4096 x
+// 7168 at 5 bits, 2 of them a token, 8 tokens 172 / 178 us, 16 tokens 206 / 193, 64 tokens 340 / 286; 128 of 2048 x 768
+// at 4 bits, 8 a token, 4 tokens 63 / 58, 16 tokens 134 / 108), as long as the sums of all tokens fit LDS.
+constexpr int MOE_OUT_WAVES = 8, MOE_OUT_ROWS = 4;
+inline int rq_moe_parts(int D) {
+  const int tiles = (D + 16 * MOE_OUT_ROWS - 1) / (16 * MOE_OUT_ROWS), parts = (256 + tiles - 1) / tiles;
+  return parts < 8 ? parts : 8;
+}
+inline int rq_moe_out_lds(const RqMoe& m, int rows) {
+  return MOE_OUT_WAVES * m.T * 64 * rows + rq_units(m.T, m.E, m.K) * (int)sizeof(RqUnit);
+}
+inline bool rq_moe_dense(const RqMoe& m) {
+  return m.T * m.K >= 32 && rq_moe_out_lds(m, MOE_OUT_ROWS) <= 160 * 1024;
+}
 
 // h = weight * silu(gate x) * (up x) of every pair, in pieces.
 template <typename TX>

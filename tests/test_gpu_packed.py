@@ -302,6 +302,9 @@ def check_moe(x, router, parts, K, norm):
             o = Wd[ex] @ h
             want[t] += p[t, k] * o
             bound[t] += p[t, k] * (Wd[ex].abs() @ (dh + eps2 * h.abs())) + w_tol[t, k] * o.abs()
+    if dt == F16:  # sums past the type's range round to infinity; as near to its end as the bound, they may
+        past = (want.abs() - bound >= 65520.0) | ((want.abs() + bound >= 65520.0) & torch.isinf(y.cpu()))
+        want = torch.where(past, want.sign() * float("inf"), want)
     assert_within(y, want, bound + ROUND[dt] * want.abs() + TINY[dt], "y")
 
 
@@ -421,3 +424,38 @@ def test_moe_refusals():
         stack_packed([])
     with pytest.raises(ValueError):
         stack_packed([on(make_entry(1, 16, 64, 4, "32")[0], DEV), on(make_entry(1, 16, 64, 5, "32")[0], DEV)])
+
+
+@pytest.mark.parametrize("T", [3, 40])
+@pytest.mark.parametrize("nbits", [2, 3, 4, 5, 6, 7, 8, 9])
+@pytest.mark.parametrize("I", [32, 96, 140, 160])
+def test_moe_widths_that_are_not_whole_chunks(I, nbits, T):
+    """down's rows end inside a chunk of 128 columns (and, 140, inside a word's 32), with few and many pairs."""
+    dtype = (F16, BF16, F32)[(I // 4 + nbits) % 3]
+    check_moe(*moe_case(I + nbits, T, 200, I, 3, dtype, (nbits,) * 3, ("channel", "128", ("channel", "128")[nbits % 2])), 2, True)
+
+
+@pytest.mark.parametrize("T,D,I,E,K", [(16, 72, 256, 5, 2), (33, 520, 384, 4, 1), (64, 130, 128, 16, 4), (100, 64, 640, 8, 3)])
+@pytest.mark.parametrize("dtype", [F16, BF16, F32])
+def test_moe_many_pairs(T, D, I, E, K, dtype):
+    """Workgroups that share rows of down, several units an expert, more tokens than a pass takes."""
+    check_moe(*moe_case(T + I, T, D, I, E, dtype, (5, 5, 4), ("128", "128", "128")), K, False)
+
+
+def test_moe_most_experts():
+    """As many experts and choices as there can be: the units fill most of the shared memory."""
+    check_moe(*moe_case(5, 64, 32, 32, 1024, F32, (4, 4, 4), ("channel",) * 3), 64, True)
+
+
+def test_moe_many_pairs_keep_to_themselves():
+    """The same rows give the same bits again, and a NaN token leaves the others' as they were."""
+    x, router, parts = moe_case(21, 48, 256, 384, 6, BF16)
+    x, router, args = x.to(DEV), router.to(DEV), [on(e, DEV) for e, _ in parts]
+    clean = packed_moe(x, router, *args, 2)
+    assert torch.equal(clean, packed_moe(x, router, *args, 2))
+    x[7, 3] = float("nan")
+    y = packed_moe(x, router, *args, 2)
+    assert bool(torch.isnan(y[7]).all())
+    keep = [t for t in range(48) if t != 7]
+    # the NaN token's experts have other companions now, in another order of units
+    assert torch.allclose(y[keep].float(), clean[keep].float(), rtol=2.0 ** -7, atol=1e-6)

@@ -187,7 +187,6 @@ struct RqTokens {
   const TX* p[NT];
   template <bool FULL>
   __device__ __forceinline__ raw load(int b, int c, int n) const { return rq_load_x<FULL>(p[b] + c, n); }
-  __device__ __forceinline__ float element(int b, int c) const { return rq_load_elem(p[b] + c); }
 };
 // Where column c of a row lies when its chunks are arranged: columns 32q + 8s.. of a chunk at 32s + 8q.
 __device__ __forceinline__ int rq_arranged(int c) { return (c & ~127) + (c >> 3 & 3) * 32 + (c >> 5 & 3) * 8 + (c & 7); }
@@ -218,13 +217,38 @@ struct RqPieces {
     for (int k = 0; k < P; ++k) r.v[k] = rq_load_x<FULL>(p + k * plane + c, n);
     return r;
   }
-  __device__ __forceinline__ float element(int, int c) const {
-    float f = rq_load_elem(p + c);
-#pragma unroll
-    for (int k = 1; k < P; ++k) f += rq_load_elem(p + k * plane + c);
-    return f;
-  }
 };
+
+// A lane's eight x of any kind as fp32.
+template <typename V>
+__device__ __forceinline__ void rq_floats(const V& x, floatx8& f) { f = __builtin_convertvector(x, floatx8); }
+template <int P>
+__device__ __forceinline__ void rq_floats(const RqPieceRow<P>& x, floatx8& f) {
+  rq_floats(x.v[0], f);
+#pragma unroll
+  for (int p = 1; p < P; ++p) {
+    floatx8 more;
+    rq_floats(x.v[p], more);
+    f += more;
+  }
+}
+// The groups of the first n (FULL: all eight) of columns c..c+7; past them that of the row's last column.
+template <bool FULL>
+__device__ __forceinline__ void rq_groups8(const RqPacked& w, int c, int n, int (&g)[8]) {
+  if (w.ngroups > 1 && w.groupsize == 0) {
+    if (FULL) {
+      __builtin_memcpy(g, w.g_idx + c, 32);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) g[j] = w.g_idx[c + min(j, n - 1)];
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) g[j] = (unsigned)g[j] < (unsigned)w.ngroups ? g[j] : -1;
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) g[j] = rq_group_of(w, c + (FULL ? j : min(j, n - 1)));
+  }
+}
 
 // The scales of group g and rows r..r+3 (rows past the weight get some scale, and are never stored).  A load
 // that would pass the table's end is moved back, and rq_scales4_of shifts its values up; where R is a
@@ -353,6 +377,12 @@ __device__ __forceinline__ void rq_chunk_runs(const RqPacked (&w)[NM], int r0, i
 // The wave's index as a scalar: what is computed from it needs no exec mask.
 __device__ __forceinline__ int rq_wave() { return __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6); }
 
+// A wave's LDS accesses before it are done and seen by the wave's later ones.
+__device__ __forceinline__ void rq_wave_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
 // Chunks first, first + step, ...: acc[a][b] += rows 4q.. of row tile a times the lane's token of tile b.  A lane without a token is given any other's (its sums
 // go nowhere).  lds: scales of the workgroup's rows for ANY, laid out by rq_stage_scales, or NULL.
 template <int NB, int MODE, int RT, int NM, typename X>
@@ -459,7 +489,7 @@ __device__ __forceinline__ void rq_rows_tokens(const RqPacked (&w)[NM], int r0, 
     }
   } else {
     for (; ch < nch; ch += step) {
-      const int c = ch * RQ_CHUNK + 32 * q, n = min(32, C - c);     // the lane's columns (n <= 0: none)
+      const int c = ch * RQ_CHUNK + 32 * q;                         // the lane's 32 columns
       uint32_t wd[RT][NB];
 #pragma unroll
       for (int a = 0; a < RT; ++a) {
@@ -467,35 +497,48 @@ __device__ __forceinline__ void rq_rows_tokens(const RqPacked (&w)[NM], int r0, 
         rq_to_signed<NB>(wd[a]);
       }
 #pragma unroll
-      for (int j = 0; j < 32; ++j) {
-        float xv[NT];
+      for (int k = 0; k < 4; ++k) {
+        const int ck = c + 8 * k, nk = C - ck;                      // eight of them, or the nk that exist
+        floatx8 xv[NT];
+        int g[NM][8];
+        if ((ch + 1) * RQ_CHUNK <= C) {
 #pragma unroll
-        for (int b = 0; b < NT; ++b) xv[b] = j < n ? xs.element(b, c + j) : 0.0f;
+          for (int b = 0; b < NT; ++b) rq_floats(xs.template load<true>(b, ck, 8), xv[b]);
 #pragma unroll
-        for (int a = 0; a < RT; ++a) {
-          const RqPacked& wa = w[a % NM];
-          const int g = j < n ? rq_group_of(wa, c + j) : 0;
-          const float s = lds ? lds[((unsigned)g < (unsigned)wa.ngroups ? g : wa.ngroups) * (16 * RT) + 16 * a + i]
-                              : rq_scale_of(wa, g, min(r0 + 16 * (a / NM) + i, wa.R - 1));
-          const float wv = j < n ? s * (float)rq_signed_code<NB>(wd[a], j) : 0.0f;
+          for (int m = 0; m < NM; ++m) rq_groups8<true>(w[m], ck, 8, g[m]);
+        } else {
 #pragma unroll
-          for (int b = 0; b < NT; ++b) acc[a][b] = __builtin_amdgcn_mfma_f32_16x16x4f32(wv, xv[b], acc[a][b], 0, 0, 0);
+          for (int b = 0; b < NT; ++b) rq_floats(xs.template load<false>(b, ck, nk), xv[b]);
+#pragma unroll
+          for (int m = 0; m < NM; ++m) rq_groups8<false>(w[m], ck, nk, g[m]);
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+#pragma unroll
+          for (int a = 0; a < RT; ++a) {
+            const RqPacked& wa = w[a % NM];
+            const int ga = g[a % NM][j];
+            const float s = lds ? lds[(ga < 0 ? wa.ngroups : ga) * (16 * RT) + 16 * a + i]
+                                : rq_scale_of(wa, ga, min(r0 + 16 * (a / NM) + i, wa.R - 1));
+            const float wv = j < nk ? s * (float)rq_signed_code<NB>(wd[a], 8 * k + j) : 0.0f;
+#pragma unroll
+            for (int b = 0; b < NT; ++b) acc[a][b] = __builtin_amdgcn_mfma_f32_16x16x4f32(wv, xv[b][j], acc[a][b], 0, 0, 0);
+          }
         }
       }
     }
   }
 }
 
-// The workgroup's scales for ANY, group by group, and a group of NaN for columns without one.  The caller
-// waits at a barrier before they are read.
-__device__ __forceinline__ void rq_stage_scales(const RqPacked& w, int r0, int rows, float* lds) {
-  const int total = (w.ngroups + 1) * rows;
-  for (int k = threadIdx.x; k < total; k += blockDim.x) {
-    const int g = k / rows, r = r0 + k % rows;
-    lds[k] = g == w.ngroups ? __builtin_nanf("") : w.scales[(int64_t)g * w.lds + min(r, w.R - 1)];
+// Scales for ANY in LDS, group by group, and a group of NaN for columns without one: rows r0..r0+15 of row tile
+// `tile` of `tiles`, by the threads first, first + step, ...  The caller waits before they are read.
+__device__ __forceinline__ void rq_stage_scales(const RqPacked& w, int r0, int tile, int tiles, int first, int step, float* lds) {
+  for (int k = first; k < (w.ngroups + 1) * 16; k += step) {
+    const int g = k >> 4, r = r0 + (k & 15);
+    lds[g * 16 * tiles + 16 * tile + (k & 15)] = g == w.ngroups ? __builtin_nanf("") : w.scales[(int64_t)g * w.lds + min(r, w.R - 1)];
   }
 }
-constexpr int RQ_STAGED_GROUPS = 127;       // groups whose scales a workgroup stages (8 KB for 16 rows)
+constexpr int RQ_STAGED_GROUPS = 1023;      // groups whose scales a workgroup stages (64 KB for 16 rows)
 
 // Which of the three serves a weight.
 inline int rq_mode_of(const RqPacked& w) {

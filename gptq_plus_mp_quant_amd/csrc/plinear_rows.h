@@ -19,7 +19,7 @@ __global__ __launch_bounds__(rows_threads(RT, NT)) void k_packed_rows(const TX* 
   for (int b = 0; b < NT; ++b) xs.p[b] = x + (int64_t)min(t0 + 16 * b + (lane & 15), T - 1) * ldx;
   const bool staged = MODE == RQ_ANY && w.ngroups <= RQ_STAGED_GROUPS;
   if (staged) {
-    rq_stage_scales(w, r0, 16 * RT, lds);
+    for (int a = 0; a < RT; ++a) rq_stage_scales(w, r0 + 16 * a, a, RT, threadIdx.x, blockDim.x, lds);
     __syncthreads();
   }
   floatx4 acc[RT][NT];

@@ -13,6 +13,7 @@ template <typename TX, int NB, int MODE, int NM>
 __global__ __launch_bounds__(512, 4) void k_moe_in(const TX* __restrict__ x, int64_t ldx, RqExperts first, RqExperts second,
                                                 int what, RqMoe m) {
   __shared__ floatx4 join[NM][8][64];
+  extern __shared__ __attribute__((aligned(16))) float scales[];
   const int lane = threadIdx.x & 63, wave = rq_wave(), waves = blockDim.x >> 6;
   const RqUnit& u = m.units[blockIdx.y];
   const int r0 = blockIdx.x * 16, pair = u.pairs[lane & 15], expert = u.expert;
@@ -23,7 +24,13 @@ __global__ __launch_bounds__(512, 4) void k_moe_in(const TX* __restrict__ x, int
   w[0] = rq_expert(first, expert);
   if constexpr (NM == 2) w[1] = rq_expert(second, expert);
   floatx4 acc[NM][1] = {};
-  rq_rows_tokens<NB, MODE, NM, NM>(w, r0, xs, wave, waves, nullptr, acc);
+  const bool staged = MODE == RQ_ANY && rq_moe_in_lds(first.w, second.w) > 0;
+  if (staged) {
+#pragma unroll
+    for (int a = 0; a < NM; ++a) rq_stage_scales(w[a], r0, a, NM, threadIdx.x, blockDim.x, scales);
+    __syncthreads();
+  }
+  rq_rows_tokens<NB, MODE, NM, NM>(w, r0, xs, wave, waves, staged ? scales : nullptr, acc);
 #pragma unroll
   for (int a = 0; a < NM; ++a) join[a][wave][lane] = acc[a][0];
   __syncthreads();
@@ -72,7 +79,8 @@ __global__ __launch_bounds__(512, 4) void k_moe_in(const TX* __restrict__ x, int
 // order of the experts: a token's result does not depend on the other tokens.
 // RUNS: the loads of the next D chunks, of whatever units, are in flight.
 template <typename TX, int NB, int MODE, int RT>
-__global__ __launch_bounds__(64 * MOE_OUT_WAVES) void k_moe_out(RqExperts down, RqMoe m, TX* __restrict__ y, int64_t ldy) {
+__global__ __launch_bounds__(64 * MOE_OUT_WAVES) void k_moe_out(RqExperts down, RqMoe m, bool staged,
+                                                                 TX* __restrict__ y, int64_t ldy) {
   constexpr int P = rq_moe_pieces<TX>(), W = MOE_OUT_WAVES, R4 = 4 * RT;
   extern __shared__ __attribute__((aligned(16))) floatx4 sums[];       // [W][T][R4]: the rows of a token; then the units
   RqUnit* units = reinterpret_cast<RqUnit*>(sums + W * m.T * R4);
@@ -155,6 +163,8 @@ __global__ __launch_bounds__(64 * MOE_OUT_WAVES) void k_moe_out(RqExperts down, 
     done:;
     }
   } else {
+    // a wave's own scales, expert by expert
+    float* scales = MODE == RQ_ANY && staged ? reinterpret_cast<float*>(units + n) + wave * (down.w.ngroups + 1) * 16 : nullptr;
     for (int k = 0; k < n; ++k) {
       const int pair = units[k].pairs[i];
       RqPieces<P, false> xs;
@@ -162,7 +172,13 @@ __global__ __launch_bounds__(64 * MOE_OUT_WAVES) void k_moe_out(RqExperts down, 
       xs.plane = (int64_t)m.T * m.K * m.ldh;
       const RqPacked w[1] = {rq_expert(down, expert_of(k))};
       floatx4 acc[RT][1] = {};
-      rq_rows_tokens<NB, MODE, RT, 1>(w, r0, xs, begin(k), all, nullptr, acc);
+      if (begin(k) >= nch) continue;
+      if (scales) {
+        rq_wave_sync();
+        rq_stage_scales(w[0], r0, 0, 1, lane, 64, scales);
+        rq_wave_sync();
+      }
+      rq_rows_tokens<NB, MODE, RT, 1>(w, r0, xs, begin(k), all, scales, acc);
       if (i < units[k].n) {
 #pragma unroll
         for (int a = 0; a < RT; ++a) mine[pair / m.K * R4 + 4 * a + q] += acc[a][0];
@@ -215,8 +231,8 @@ void rq_moe_in(const TX* x, int64_t ldx, const RqExperts& gate, int gate_bits, c
     constexpr int NM = decltype(both)::value ? 2 : 1;
     rq_with_nbits(bits, [&](auto nb) {
       with_mode(rq_mode_of(of.w), [&](auto mode) {
-        hipLaunchKernelGGL((k_moe_in<TX, decltype(nb)::value, decltype(mode)::value, NM>), grid, block, 0, s, x, ldx, of,
-                           up, what, m);
+        hipLaunchKernelGGL((k_moe_in<TX, decltype(nb)::value, decltype(mode)::value, NM>), grid, block,
+                           decltype(mode)::value == RQ_ANY ? rq_moe_in_lds(of.w, up.w) : 0, s, x, ldx, of, up, what, m);
       });
     });
   };
@@ -234,9 +250,10 @@ void rq_moe_out(const RqExperts& down, int bits, const RqMoe& m, TX* y, int64_t 
     with_mode(rq_moe_out_mode(down.w), [&](auto mode) {
       auto go = [&](auto rt, int parts) {
         constexpr int RT = decltype(rt)::value;
+        const int scales = decltype(mode)::value == RQ_ANY ? rq_moe_out_scales(down.w) : 0;
         hipLaunchKernelGGL((k_moe_out<TX, decltype(nb)::value, decltype(mode)::value, RT>),
                            dim3((m.D + 16 * RT - 1) / (16 * RT), parts), dim3(64 * MOE_OUT_WAVES),
-                           rq_moe_out_lds(m, RT), s, down, m, y, ldy);
+                           rq_moe_out_lds(m, RT) + scales, s, down, m, scales > 0, y, ldy);
         if (parts > 1)
           hipLaunchKernelGGL(k_moe_join<TX>, dim3((m.D + 255) / 256, m.T), dim3(256), 0, s, m.parts, parts, m.T, m.D, y, ldy);
       };

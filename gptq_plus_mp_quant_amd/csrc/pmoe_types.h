@@ -70,6 +70,14 @@ inline bool rq_moe_dense(const RqMoe& m) {
   return m.T * m.K >= 32 && rq_moe_out_lds(m, MOE_OUT_ROWS) <= 160 * 1024;
 }
 
+// LDS for the scales of groups that are no runs of columns (bytes, 0 where there are too many groups): gate's and up's of a
+// workgroup's rows, and down's of each wave's expert.  Gathered from memory they cost several times the product.
+__host__ __device__ inline int rq_moe_in_lds(const RqPacked& gate, const RqPacked& up) {
+  const int most = gate.ngroups > up.ngroups ? gate.ngroups : up.ngroups;
+  return most < 256 ? (most + 1) * 128 : 0;
+}
+inline int rq_moe_out_scales(const RqPacked& down) { return down.ngroups < 64 ? (down.ngroups + 1) * 64 * MOE_OUT_WAVES : 0; }
+
 // h = weight * silu(gate x) * (up x) of every pair, in pieces.
 template <typename TX>
 void rq_moe_in(const TX* x, int64_t ldx, const RqExperts& gate, int gate_bits, const RqExperts& up, int up_bits,

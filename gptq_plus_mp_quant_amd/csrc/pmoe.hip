@@ -63,6 +63,8 @@ __global__ __launch_bounds__(256) void k_moe_router(const TX* __restrict__ x, in
 // One workgroup.  A wave takes a token: the K-th largest order key is found bit by bit from the number of
 // experts that reach a value (whatever the logits hold, exactly K are chosen); they are ranked among
 // themselves.  Then a wave takes an expert: its pairs in ascending order, cut into units.
+// EL: experts a lane holds (its loops are unrolled; 32 tokens to 2 of 8 experts: 8 us, 11 with 16).
+template <int EL>
 __global__ __launch_bounds__(1024) void k_moe_route(const float* __restrict__ logits, int T, int E, int K, int norm,
                                                     float* __restrict__ weights, int* __restrict__ nunits,
                                                     RqUnit* __restrict__ units, int most, int* __restrict__ ids_out,
@@ -71,7 +73,6 @@ __global__ __launch_bounds__(1024) void k_moe_route(const float* __restrict__ lo
   __shared__ int first[MOE_MAX_E];                   // the expert's first unit, once they are counted
   __shared__ uint64_t picked[16][MOE_MAX_K];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  constexpr int EL = MOE_MAX_E / 64;
   for (int t = wave; t < T; t += 16) {
     const float* l = logits + (int64_t)t * E;
     float v[EL];
@@ -142,42 +143,21 @@ __global__ __launch_bounds__(1024) void k_moe_route(const float* __restrict__ lo
   }
   __syncthreads();
   const int pairs = T * K;
-  if (pairs <= 64) {
-    // Few pairs, one a lane: the pairs of its expert before it, all of its expert's, and the units of lower
-    // experts are counted over the others.
-    if (wave) return;
-    const int e = lane < pairs ? ids[lane] : -1;
-    int before = 0, n = 0, pair0 = lane;
-    for (int j = pairs - 1; j >= 0; --j) {
-      const bool same = __builtin_amdgcn_readlane(e, j) == e;
-      before += same && j < lane ? 1 : 0;
-      n += same ? 1 : 0;
-      pair0 = same ? j : pair0;
+  // Few pairs: one a lane of the first wave, and the lanes of its expert by ten ballots.
+  const bool few = pairs <= 64;
+  const int own = few && lane < pairs ? ids[lane] : MOE_MAX_E;
+  uint64_t same = ~0ull;
+  if (few && wave == 0) {
+#pragma unroll
+    for (int bit = 0; (1 << bit) <= MOE_MAX_E; ++bit) {
+      const uint64_t set = __ballot(own >> bit & 1);
+      same &= own >> bit & 1 ? set : ~set;
     }
-    const bool leads = lane < pairs && before == 0;
-    const int mine = leads ? (n + 15) / 16 : 0;
-    int lower = 0, all = 0;
-    for (int j = 0; j < pairs; ++j) {
-      const int ej = __builtin_amdgcn_readlane(e, j), uj = __builtin_amdgcn_readlane(mine, j);
-      lower += ej < e ? uj : 0;
-      all += uj;
-    }
-    if (lane < pairs) {
-      RqUnit& u = units[lower + before / 16];
-      u.pairs[before % 16] = lane;
-      if (before % 16 == 0) {
-        u.expert = e;
-        u.n = min(16, n - before);
-      }
-      // the last of an expert's pairs fills the places past it
-      if (before == n - 1)
-        for (int k = before % 16 + 1; k < 16; ++k) u.pairs[k] = pair0;
-    }
-    if (lane == 0) *nunits = all;
-    for (int k = all + lane; k < most; k += 64) units[k].n = 0;
-    return;
+    for (int e = lane; e < E; e += 64) first[e] = 0;
+    rq_wave_sync();
+    if (lane < pairs) first[own] = (__popcll(same) + 15) / 16;
   }
-  for (int e = wave; e < E; e += 16) {               // units of every expert
+  for (int e = few ? E : wave; e < E; e += 16) {     // units of every expert
     int n = 0;
     for (int p = 0; p < pairs; p += 64) n += __popcll(__ballot(p + lane < pairs && ids[p + lane] == e));
     if (lane == 0) first[e] = (n + 15) / 16;
@@ -200,6 +180,20 @@ __global__ __launch_bounds__(1024) void k_moe_route(const float* __restrict__ lo
     for (int k = before + lane; k < most; k += 64) units[k].n = 0;
   }
   __syncthreads();
+  if (few) {
+    if (wave || lane >= pairs) return;
+    const int n = __popcll(same), before = __popcll(same & ((1ull << lane) - 1));
+    RqUnit& u = units[first[own] + before / 16];
+    u.pairs[before % 16] = lane;
+    if (before % 16 == 0) {
+      u.expert = own;
+      u.n = min(16, n - before);
+    }
+    // the expert's last pair fills the places past it with its first
+    if (before == n - 1)
+      for (int k = before % 16 + 1; k < 16; ++k) u.pairs[k] = __ffsll((unsigned long long)same) - 1;
+    return;
+  }
   for (int e = wave; e < E; e += 16) {
     int n = 0;
     for (int p = 0; p < pairs; p += 64) {
@@ -283,9 +277,14 @@ extern "C" int rq_packed_moe(const void* x, int dtype, int T, int64_t ldx, int D
                     rq_moe_out_mode(d.w) == RQ_RUNS, (float*)(ws + l.parts)};
       hipLaunchKernelGGL(k_moe_router<TX>, dim3(E, (n + ROUTER_TOKENS - 1) / ROUTER_TOKENS), dim3(256), 0, s, xt,
                          ldx, n, D, (const TX*)router, ldr, E, logits);
-      hipLaunchKernelGGL(k_moe_route, dim3(1), dim3(1024), 0, s, logits, n, E, K, norm, weights, nunits, units,
-                         rq_units(n, E, K),
-                         ids_out ? ids_out + t0 * K : nullptr, weights_out ? weights_out + t0 * K : nullptr);
+      auto route = [&](auto el) {
+        hipLaunchKernelGGL(k_moe_route<decltype(el)::value>, dim3(1), dim3(1024), 0, s, logits, n, E, K, norm, weights, nunits,
+                           units, rq_units(n, E, K), ids_out ? ids_out + t0 * K : nullptr,
+                           weights_out ? weights_out + t0 * K : nullptr);
+      };
+      if (E <= 64) route(std::integral_constant<int, 1>{});
+      else if (E <= 256) route(std::integral_constant<int, 4>{});
+      else route(std::integral_constant<int, MOE_MAX_E / 64>{});
       rq_moe_in<TX>(xt, ldx, g, gate->nbits, u, up->nbits, m, s);
       rq_moe_out<TX>(d, down->nbits, m, (TX*)y + t0 * ldy, ldy, s);
     }

@@ -15,7 +15,8 @@
 // The alternatives cost the pass nothing but the maxima: the top_k-th largest of the lanes' maxima is a bar
 // that at least top_k logits reach and, the lanes being many more than top_k, few others.  Each lane also
 // leaves a maximum for every block of its loads, and the few blocks that reach the bar are read again (from
-// the caches) for the logits that do: 2048 rows of 128256 bf16 with 5 alternatives take 139 us, 117 without.
+// the caches) for the logits that do.  2048 rows of 128256 bf16 with 5 alternatives take 129 us, 525 MB read: 4.1 TB/s,
+// where a copy of that size reaches 5.0 (read and written).
 // A row's segments are joined by one wave: in the workgroup that has the whole row, or by k_logprob_join
 // where a row is cut over many workgroups.
 #include "packed_dot.h"
@@ -23,7 +24,7 @@
 namespace {
 
 constexpr int MAX_TOP = 64, MAX_V = 1 << 30;
-constexpr int LIST = 320;                  // candidates a wave holds: 256 of half a load and what stays
+constexpr int LIST = 320;                  // candidates a wave holds
 constexpr float LOG2E = 1.4426950408889634f;
 
 constexpr float LN2 = 0.6931471805599453f;
@@ -51,6 +52,18 @@ __device__ __forceinline__ int lane_rank(uint64_t key, int n) {
 #pragma unroll 4
   for (int j = 0; j < n; ++j) place += lane_value(key, j) > key ? 1 : 0;
   return place;
+}
+
+// A value that at least k <= 64 of the lanes' reach, the k-th largest or what is left of it when no more do.
+__device__ __forceinline__ uint32_t kth_largest(uint32_t mine, int k) {
+  uint32_t least = 0;
+  for (int bit = 31; bit >= 0; --bit) {
+    const uint32_t tried = least | (1u << bit);
+    const int reach = __popcll(__ballot(mine >= tried));
+    if (reach >= k) least = tried;
+    if (reach == k) break;
+  }
+  return least;
 }
 
 struct Stat {
@@ -146,25 +159,33 @@ __device__ __forceinline__ void finish_row(const TX* __restrict__ row, int V, in
     stats[3 * n + 2] = H;
   }
   if (!top) return;
-  // A value is among the top only if it reaches the top-th largest of the parts' best.
+  // A value is among the top only if it reaches the top-th largest of the parts' best values.
   uint64_t floor_key = 0;
   if (nparts > 8) {
     uint64_t best = 0;
-    if (nparts <= 64) best = lane < nparts ? parts.key(lane, 0) : 0;
-    else
-      for (int p = lane; p < nparts; p += 64) {
-        const uint64_t o = parts.key(p, 0);
-        best = o > best ? o : best;
-      }
-    const uint64_t is = __ballot(lane_rank(best, min(nparts, 64)) == top - 1 && best != 0);
-    if (is) floor_key = lane_value(best, __ffsll((unsigned long long)is) - 1);
+    for (int p = lane; p < nparts; p += 64) {
+      const uint64_t o = parts.key(p, 0);
+      best = o > best ? o : best;
+    }
+    const uint32_t least = kth_largest((uint32_t)(best >> 32), top);
+    floor_key = (uint64_t)least << 32;
+    // Where more of them are equal the exact key is found, or every part's list would pass.
+    if (__popcll(__ballot((uint32_t)(best >> 32) >= least)) > top) {
+      const uint64_t is = __ballot(lane_rank(best, 64) == top - 1 && best != 0);
+      if (is) floor_key = lane_value(best, __ffsll((unsigned long long)is) - 1);
+    }
   }
   int count = 0;
   for (int p0 = 0; p0 < nparts; p0 += 64) {
-    uint64_t next = p0 + lane < nparts ? parts.key(p0 + lane, 0) : 0;
+    constexpr int AHEAD = 4;
+    uint64_t next[AHEAD];
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u) next[u] = p0 + lane < nparts && u < top ? parts.key(p0 + lane, u) : 0;
     for (int k = 0; k < top; ++k) {
-      const uint64_t key = next;
-      next = p0 + lane < nparts && k + 1 < top ? parts.key(p0 + lane, k + 1) : 0;
+      const uint64_t key = next[0];
+#pragma unroll
+      for (int u = 0; u + 1 < AHEAD; ++u) next[u] = next[u + 1];
+      next[AHEAD - 1] = p0 + lane < nparts && k + AHEAD < top ? parts.key(p0 + lane, k + AHEAD) : 0;
       const bool take = key != 0 && key >= floor_key;
       const uint64_t mask = __ballot(take);
       if (!mask) break;                              // the parts' lists are in order
@@ -288,19 +309,14 @@ __device__ __forceinline__ Stat scan_segment(const Scan<TX>& sc, float* most) {
 
 // A float that at least k <= 64 of the workgroup's logits reach: the k-th largest of 64 maxima, each over one
 // lane of every wave (order keys).  About 64 ln(64 / (64 - k)) logits reach it: 5 for k = 5, 24 for 20, 300
-// for 64.  (The k-th largest of all lanes' maxima lets fewer pass, and took 5 us longer to find.)
+// for 64.  (The k-th largest of all lanes' maxima lets fewer pass, and took 5 us
+// longer to find.)
 __device__ __forceinline__ float bar_of(const uint32_t* keys, int k) {
   const int lane = threadIdx.x & 63;
   uint32_t mine = keys[lane];
 #pragma unroll
   for (int u = 1; u < W; ++u) mine = max(mine, keys[64 * u + lane]);
-  uint32_t least = 0;
-  for (int bit = 31; bit >= 0; --bit) {
-    const uint32_t tried = least | (1u << bit);
-    const int reach = __popcll(__ballot(mine >= tried));
-    if (reach >= k) least = tried;
-    if (reach == k) break;
-  }
+  const uint32_t least = kth_largest(mine, k);
   return rq_key_value(min(max(least, 0x007FFFFFu), 0xFF800000u));       // from -inf to inf, which NaNs reach too
 }
 
@@ -334,33 +350,48 @@ __device__ __forceinline__ void collect(const Scan<TX>& sc, const float* most, b
 #pragma unroll
         for (int u = 1; u < U; ++u)
           if (u == u0) x = in[u];
-        // Of the values equal to the bar the first top suffice (a lane's eight lie before the next lane's).
-        int before = 0;
+        float f[8];
+        uint32_t takes = 0, equals = 0;              // of the lane's eight
 #pragma unroll
-        for (int k = 0; k < 8; ++k) before += lanes_before(__ballot((float)x[k] == bar && at + k < c1));
-#pragma unroll 1
-        for (int h = 0; h < 8; h += 4) {
-          if (count > LIST - 256) {
+        for (int k = 0; k < 8; ++k) {
+          f[k] = (float)x[k];
+          takes |= at + k < c1 && !(f[k] < bar) ? 1u << k : 0u;
+          equals |= f[k] == bar ? 1u << k : 0u;
+        }
+        equals &= takes;
+        if (__any(equals != 0)) {
+          // Of the values equal to the bar the first top suffice (a lane's eight lie before the next lane's).
+          int before = 0;
+#pragma unroll
+          for (int k = 0; k < 8; ++k) before += lanes_before(__ballot(equals >> k & 1));
+#pragma unroll
+          for (int k = 0; k < 8; ++k)
+            if (equals >> k & 1)
+              if (before++ >= top) takes &= ~(1u << k);
+        }
+        // One of each lane at a time: mostly one is all.
+        while (__any(takes != 0)) {
+          if (count > LIST - 64) {
             keep_top(list, count, top, c1);
-            count = min(count, top);
+            count = top;
             const float last = rq_key_value((uint32_t)(list[top - 1] >> 32));
-            if (count == top && last > bar) {
+            if (last > bar) {
               bar = last;
               strict = false;
-              before = 0;                  // unknown for the new one: all of this load's are taken
+#pragma unroll
+              for (int k = 0; k < 8; ++k)
+                if (f[k] < bar) takes &= ~(1u << k);
             }
           }
+          const bool take = takes != 0;
+          const int k0 = __ffs(takes) - 1;
+          float v = f[0];
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const float f = (float)(h ? x[4 + k] : x[k]);
-            const bool equal = f == bar;
-            const bool take = at + h + k < c1 && !(f < bar) && !(equal && before >= top);
-            before += equal ? 1 : 0;
-            const uint64_t mask = __ballot(take);
-            if (!mask) continue;
-            if (take) list[count + lanes_before(mask)] = top_key(f, at + h + k);
-            count += __popcll(mask);
-          }
+          for (int k = 1; k < 8; ++k) v = k == k0 ? f[k] : v;
+          const uint64_t mask = __ballot(take);
+          if (take) list[count + lanes_before(mask)] = top_key(v, at + k0);
+          count += __popcll(mask);
+          takes &= takes - 1;                        // 0 stays 0
           wave_fence();
         }
         // top values that reach the bar are held: equal ones of later loads come after them
@@ -446,7 +477,7 @@ __global__ __launch_bounds__(64) void k_logprob_join(const TX* __restrict__ z, i
 
 // How a row is cut: into one workgroup's 4 segments where the rows alone fill the GPU or are short; fewer rows
 // over more workgroups, down to 2048 columns a wave, and a second launch joins them (one row of 128256 bf16,
-// 20 alternatives: 13 + 6.6 us; one workgroup of 16 waves took 30).
+// 20 alternatives: 11.5 + 6.6 us, a chain of latencies; one workgroup of 16 waves took 30).
 struct Split {
   int segs, cols;
 };
@@ -459,7 +490,8 @@ constexpr int64_t ROWS_PER_LAUNCH = 1 << 20;
 
 // --- the gradient ---------------------------------------------------------------------------
 // A workgroup takes rounds of 8192 columns of a row, 4 x 8 a thread: read once, written once.  z and dz may
-// be the same memory (a thread reads what it writes first).
+// be the same memory (a thread reads what it writes first).  1024 rows of 128256 bf16: 108 us for 525 MB,
+// 4.9 TB/s, a copy's rate; 12 rows of 32003 fp32 4.8 us, a launch.
 constexpr int GRAD_COLS = 8192;
 
 template <typename TX>

@@ -18,9 +18,11 @@ from __future__ import annotations
 from typing import Dict, Optional, Sequence
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _native as nat
 from . import kernels as K
+
 
 def _checked(entry: Dict[str, object], batch: int):
     """(qweight, nbits, scales, R, C, ngroups, g_idx, groupsize) of an entry (batch = 1: stacked over
@@ -84,6 +86,7 @@ class _PackedLinear(torch.autograd.Function):
         return _forward(x, entry, bias)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, grad_y):
         return packed_linear_backward(grad_y, ctx.entry), None, None
 

@@ -10,6 +10,7 @@ from __future__ import annotations
 from typing import NamedTuple, Optional
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _native as nat
 from . import kernels as K
@@ -71,6 +72,7 @@ class _TokenLogprobs(torch.autograd.Function):
         return tuple(r)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, grad_logprob, grad_entropy, *_):
         logits, targets, stats = ctx.saved_tensors
         return token_logprobs_backward(logits, targets, stats, grad_logprob, grad_entropy, ctx.ignore_index), None, None, None

@@ -459,3 +459,12 @@ def test_moe_many_pairs_keep_to_themselves():
     keep = [t for t in range(48) if t != 7]
     # the NaN token's experts have other companions now, in another order of units
     assert torch.allclose(y[keep].float(), clean[keep].float(), rtol=2.0 ** -7, atol=1e-6)
+
+
+def test_second_derivatives_are_refused():
+    """The gradients come from kernels that no graph follows: a gradient of them is an error, not a zero."""
+    entry, _ = make_entry(3, 32, 64, 4, "32")
+    x = randn(1, 2, 64).to(DEV).requires_grad_()
+    g, = torch.autograd.grad(packed_linear(x, on(entry, DEV)).square().sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError):
+        g.sum().backward()

@@ -25,14 +25,14 @@ inline RqPacked rq_packed(const uint32_t* q, int64_t ldp, const float* scales, i
   return RqPacked{q, ldp, scales, lds, g_idx, R, C, ngroups, groupsize, magic};
 }
 
-// The group of column c, -1 where g_idx names none (its scale then reads as NaN, never out of bounds).
-__device__ __forceinline__ int rq_group_of(const RqPacked& w, int c) {
+// The group of column c, ngroups where g_idx names none (its scale then reads as NaN, never out of bounds).
+__device__ __forceinline__ uint32_t rq_group_of(const RqPacked& w, int c) {
   if (w.ngroups == 1) return 0;
-  const int g = w.groupsize > 0 ? c / w.groupsize : w.g_idx[c];
-  return (unsigned)g < (unsigned)w.ngroups ? g : -1;
+  return min((uint32_t)(w.groupsize > 0 ? c / w.groupsize : w.g_idx[c]), (uint32_t)w.ngroups);
 }
-__device__ __forceinline__ float rq_scale_of(const RqPacked& w, int g, int r) {
-  return g < 0 ? __builtin_nanf("") : w.scales[(int64_t)g * w.lds + r];
+__device__ __forceinline__ float rq_scale_of(const RqPacked& w, uint32_t g, int r) {
+  const float s = w.scales[(int64_t)(g < (uint32_t)w.ngroups ? g : 0) * w.lds + r];
+  return g < (uint32_t)w.ngroups ? s : __builtin_nanf("");
 }
 
 // The nc <= 8 codes of columns [c, c + nc), c a multiple of 8; the rest read as 0.  No word past the last of these

@@ -234,16 +234,16 @@ __device__ __forceinline__ void rq_floats(const RqPieceRow<P>& x, floatx8& f) {
 }
 // The groups of the first n (FULL: all eight) of columns c..c+7; past them that of the row's last column.
 template <bool FULL>
-__device__ __forceinline__ void rq_groups8(const RqPacked& w, int c, int n, int (&g)[8]) {
+__device__ __forceinline__ void rq_groups8(const RqPacked& w, int c, int n, uint32_t (&g)[8]) {
   if (w.ngroups > 1 && w.groupsize == 0) {
     if (FULL) {
       __builtin_memcpy(g, w.g_idx + c, 32);
     } else {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) g[j] = w.g_idx[c + min(j, n - 1)];
+      for (int j = 0; j < 8; ++j) g[j] = (uint32_t)w.g_idx[c + min(j, n - 1)];
     }
 #pragma unroll
-    for (int j = 0; j < 8; ++j) g[j] = (unsigned)g[j] < (unsigned)w.ngroups ? g[j] : -1;
+    for (int j = 0; j < 8; ++j) g[j] = min(g[j], (uint32_t)w.ngroups);
   } else {
 #pragma unroll
     for (int j = 0; j < 8; ++j) g[j] = rq_group_of(w, c + (FULL ? j : min(j, n - 1)));
@@ -496,36 +496,34 @@ __device__ __forceinline__ void rq_rows_tokens(const RqPacked (&w)[NM], int r0, 
         rq_words<NB>(row[a], c, C, wd[a]);
         rq_to_signed<NB>(wd[a]);
       }
+      auto columns = [&](auto full) {
+        constexpr bool FULL = decltype(full)::value;                // else columns past the last have w = x = 0
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const int ck = c + 8 * k, nk = C - ck;                      // eight of them, or the nk that exist
-        floatx8 xv[NT];
-        int g[NM][8];
-        if ((ch + 1) * RQ_CHUNK <= C) {
+        for (int k = 0; k < 4; ++k) {
+          const int ck = c + 8 * k, nk = C - ck;                    // eight columns, or the nk that exist
+          floatx8 xv[NT];
+          uint32_t g[NM][8];
 #pragma unroll
-          for (int b = 0; b < NT; ++b) rq_floats(xs.template load<true>(b, ck, 8), xv[b]);
+          for (int b = 0; b < NT; ++b) rq_floats(xs.template load<FULL>(b, ck, nk), xv[b]);
 #pragma unroll
-          for (int m = 0; m < NM; ++m) rq_groups8<true>(w[m], ck, 8, g[m]);
-        } else {
+          for (int m = 0; m < NM; ++m) rq_groups8<FULL>(w[m], ck, nk, g[m]);
 #pragma unroll
-          for (int b = 0; b < NT; ++b) rq_floats(xs.template load<false>(b, ck, nk), xv[b]);
+          for (int j = 0; j < 8; ++j) {
 #pragma unroll
-          for (int m = 0; m < NM; ++m) rq_groups8<false>(w[m], ck, nk, g[m]);
-        }
+            for (int a = 0; a < RT; ++a) {
+              const RqPacked& wa = w[a % NM];
+              const uint32_t ga = g[a % NM][j];
+              const float s = lds ? lds[ga * (16 * RT) + 16 * a + i]
+                                  : rq_scale_of(wa, ga, min(r0 + 16 * (a / NM) + i, wa.R - 1));
+              const float v = s * (float)rq_signed_code<NB>(wd[a], 8 * k + j), wv = FULL || j < nk ? v : 0.0f;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-#pragma unroll
-          for (int a = 0; a < RT; ++a) {
-            const RqPacked& wa = w[a % NM];
-            const int ga = g[a % NM][j];
-            const float s = lds ? lds[(ga < 0 ? wa.ngroups : ga) * (16 * RT) + 16 * a + i]
-                                : rq_scale_of(wa, ga, min(r0 + 16 * (a / NM) + i, wa.R - 1));
-            const float wv = j < nk ? s * (float)rq_signed_code<NB>(wd[a], 8 * k + j) : 0.0f;
-#pragma unroll
-            for (int b = 0; b < NT; ++b) acc[a][b] = __builtin_amdgcn_mfma_f32_16x16x4f32(wv, xv[b][j], acc[a][b], 0, 0, 0);
+              for (int b = 0; b < NT; ++b) acc[a][b] = __builtin_amdgcn_mfma_f32_16x16x4f32(wv, xv[b][j], acc[a][b], 0, 0, 0);
+            }
           }
         }
-      }
+      };
+      if ((ch + 1) * RQ_CHUNK <= C) columns(std::true_type{});
+      else columns(std::false_type{});
     }
   }
 }

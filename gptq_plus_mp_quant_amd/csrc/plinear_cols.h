@@ -88,7 +88,7 @@ __global__ __launch_bounds__(64 * cols_waves(NT), cols_occupancy(MODE, NT)) void
   const int off = (int)(bit & 31), nw = nc > 0 ? (off + nc * NB + 31) >> 5 : 0;
   // A lane past the last column reads the row's first word; words past a row's last field are not read.
   const uint32_t* col = w.q + (nc > 0 ? bit >> 5 : 0);
-  int g[8];
+  uint32_t g[8];
 #pragma unroll
   for (int k = 0; k < 8; ++k)
     g[k] = MODE == RQ_RUNS ? rq_run_group(w, c0) : (MODE == RQ_SMALL && k) ? g[0] : k < nc ? rq_group_of(w, c + k) : 0;
@@ -129,7 +129,8 @@ __global__ __launch_bounds__(64 * cols_waves(NT), cols_occupancy(MODE, NT)) void
       }
     }
   };
-  auto compute = [&](int st, Step& f) {
+  auto compute = [&](auto full, int st, Step& f) {
+    constexpr bool FULL = decltype(full)::value;
     const int r = st * STEP + 8 * q;
     bf16x8 d[NT][P::dy];
 #pragma unroll
@@ -175,7 +176,11 @@ __global__ __launch_bounds__(64 * cols_waves(NT), cols_occupancy(MODE, NT)) void
         floatx8 sc = f.sc;
         if (MODE == RQ_ANY) {
 #pragma unroll
-          for (int k = 0; k < 8; ++k) sc[k] = r + k < w.R ? rq_scale_of(w, g[n], r + k) : 0.0f;
+          for (int k = 0; k < 8; ++k) sc[k] = rq_scale_of(w, g[n], FULL ? r + k : min(r + k, w.R - 1));
+          if (!FULL) {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) sc[k] = r + k < w.R ? sc[k] : 0.0f;
+          }
         }
         rq_operand<P::w>(sc * rq_unit<NB>() * codes, v);
       }
@@ -200,15 +205,15 @@ __global__ __launch_bounds__(64 * cols_waves(NT), cols_occupancy(MODE, NT)) void
     load(std::true_type{}, st, now);
     for (; st + W < sf; st += W) {
       load(std::true_type{}, st + W, then);
-      compute(st, now);
+      compute(std::true_type{}, st, now);
       now = then;
     }
-    compute(st, now);
+    compute(std::true_type{}, st, now);
     st += W;
   }
   if (st < sb) {
     load(std::false_type{}, st, now);
-    compute(st, now);
+    compute(std::false_type{}, st, now);
   }
   // The waves' sums, halved together: always in the same order.
 #pragma unroll

@@ -1,5 +1,5 @@
-// Rows of a packed weight times tokens on the matrix cores: 16 rows x 16 tokens a tile, no LDS on the
-// way.
+// Rows of a packed weight times tokens on the matrix cores: 16 rows x 16 tokens a tile, words and tokens
+// straight to registers (a weight is used once, and LDS would only add a trip).
 //
 // v_mfma_f32_16x16x32: lane l = 16 q + i holds A[i][8q..8q+7] and B[8q..8q+7][i] and receives
 // D[4q..4q+3][i].  A row of A is a row of the weight, a column of B a token.  Which columns of the weight
@@ -383,8 +383,9 @@ __device__ __forceinline__ void rq_wave_sync() {
   __builtin_amdgcn_wave_barrier();
 }
 
-// Chunks first, first + step, ...: acc[a][b] += rows 4q.. of row tile a times the lane's token of tile b.  A lane without a token is given any other's (its sums
-// go nowhere).  lds: scales of the workgroup's rows for ANY, laid out by rq_stage_scales, or NULL.
+// Chunks first, first + step, ...: acc[a][b] += rows 4q.. of row tile a times the lane's token of tile b.  A lane
+// without a token is given any other's (its sums go nowhere).  lds: scales of the rows for ANY, laid out by
+// rq_stage_scales, or NULL.
 template <int NB, int MODE, int RT, int NM, typename X>
 __device__ __forceinline__ void rq_rows_tokens(const RqPacked (&w)[NM], int r0, const X& xs, int first, int step,
                                                const float* lds, floatx4 (&acc)[RT][X::tiles]) {

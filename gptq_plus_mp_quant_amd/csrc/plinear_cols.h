@@ -10,6 +10,10 @@
 //   ANY    a scale for every weight
 // What a scale multiplied is an fp32 number, cut into bf16 pieces: two (2^-16 of it is lost; the 16-bit
 // types' results have 8 or 11 bits) or three (fp32, exact).  Products of pieces below 2^-24 are left out.
+// Rows are split over workgroups until there are 512, whose sums a second launch joins in their order.
+// Measured: 4096 x 4096 5-bit fp16, 8 tokens 9.1 + 4.1 us, latency; 14336 x 4096 4-bit bf16, 64 tokens 30 + 5.3 us, where
+// the conversions of codes and of dy on the vector units and two pieces' matrix instructions (7.5 GFLOP twice)
+// overlap in part, with two waves a SIMD.
 #pragma once
 #include "packed_dot.h"
 

@@ -3,7 +3,7 @@
 //   l = x router^T, the K largest of l chosen (equal logits by their index), w = softmax(l) of the chosen
 //   (divided by their sum when norm), y = sum_k w_k Wd_k (silu(Wg_k x) * (Wu_k x)).
 //
-// Four launches: the router's logits; the routing, which sorts the chosen (token, expert) pairs into units of
+// Four launches, five for many tokens: the router's logits; the routing, which sorts the chosen (token, expert) pairs into units of
 // up to 16 tokens of one expert; gate, up and the activation of every unit; down, summed over a token's
 // experts.  An expert that no token chose is not read, one that several chose is read once for 16 of them.
 // Router logits, sums, the activation and the sum over experts are fp32 (the activation in bf16 pieces that
@@ -21,7 +21,8 @@ __device__ __forceinline__ int lanes_before(uint64_t mask) {
   return __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0));
 }
 
-// A workgroup takes one expert and 8 tokens; its waves take 512 columns in turn, 8 a lane.
+// A workgroup takes one expert and 8 tokens; its waves take 512 columns in turn, 8 a lane (a router of 128 x 2048, 1 token
+// 3 us; of 8 x 4096, 32 tokens 6 us: latency).
 constexpr int ROUTER_TOKENS = 8;
 template <typename TX>
 __global__ __launch_bounds__(256) void k_moe_router(const TX* __restrict__ x, int64_t ldx, int T, int D,

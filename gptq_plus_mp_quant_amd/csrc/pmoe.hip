@@ -3,23 +3,14 @@
 //   l = x router^T, the K largest of l chosen (equal logits by their index), w = softmax(l) of the chosen
 //   (divided by their sum when norm), y = sum_k w_k Wd_k (silu(Wg_k x) * (Wu_k x)).
 //
-// Four launches, five for many tokens: the router's logits; the routing, which sorts the chosen (token, expert) pairs into units of
-// up to 16 tokens of one expert; gate, up and the activation of every unit; down, summed over a token's
+// Four launches, three for one token, five for many: the router's logits; the routing, which sorts the chosen
+// (token, expert) pairs into units of up to 16 tokens of one expert (one token's needs no launch); gate, up and the activation of every unit; down, summed over a token's
 // experts.  An expert that no token chose is not read, one that several chose is read once for 16 of them.
 // Router logits, sums, the activation and the sum over experts are fp32 (the activation in bf16 pieces that
 // carry 16 bits or all 24); the one rounding to fewer bits is the result's to x's type.
 #include "pmoe_types.h"
 
 namespace {
-
-__device__ __forceinline__ float wave_sum(float v) {
-#pragma unroll
-  for (int m = 32; m; m >>= 1) v += __shfl_xor(v, m);
-  return v;
-}
-__device__ __forceinline__ int lanes_before(uint64_t mask) {
-  return __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0));
-}
 
 // A workgroup takes one expert and 8 tokens; its waves take 512 columns in turn, 8 a lane (a router of 128 x 2048, 1 token
 // 3 us; of 8 x 4096, 32 tokens 6 us: latency).
@@ -51,7 +42,7 @@ __global__ __launch_bounds__(256) void k_moe_router(const TX* __restrict__ x, in
 #pragma unroll
   for (int t = 0; t < ROUTER_TOKENS; ++t) {
     if (t >= nt) break;
-    const float v = wave_sum(s[t]);
+    const float v = rq_wave_sum(s[t]);
     if (lane == 0) join[wave][t] = v;
   }
   __syncthreads();
@@ -61,9 +52,8 @@ __global__ __launch_bounds__(256) void k_moe_router(const TX* __restrict__ x, in
   }
 }
 
-// One workgroup.  A wave takes a token: the K-th largest order key is found bit by bit from the number of
-// experts that reach a value (whatever the logits hold, exactly K are chosen); they are ranked among
-// themselves.  Then a wave takes an expert: its pairs in ascending order, cut into units.
+// One workgroup.  A wave takes a token: its experts are chosen (rq_choose) and ranked among themselves.  Then a
+// wave takes an expert: its pairs in ascending order, cut into units.
 // EL: experts a lane holds (its loops are unrolled; 32 tokens to 2 of 8 experts: 8 us, 11 with 16).
 template <int EL>
 __global__ __launch_bounds__(1024) void k_moe_route(const float* __restrict__ logits, int T, int E, int K, int norm,
@@ -75,64 +65,30 @@ __global__ __launch_bounds__(1024) void k_moe_route(const float* __restrict__ lo
   __shared__ uint64_t picked[16][MOE_MAX_K];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   for (int t = wave; t < T; t += 16) {
-    const float* l = logits + (int64_t)t * E;
-    float v[EL];
-    uint32_t key[EL];
-    float m = -INFINITY;
+    RqChoice<EL> c;
+    rq_choose<EL>(logits + (int64_t)t * E, E, K, c);
+    int at = 0;
 #pragma unroll
     for (int u = 0; u < EL; ++u) {
-      if (64 * u >= E) break;
-      const int e = 64 * u + lane;
-      const float logit = l[min(e, E - 1)];
-      v[u] = e < E ? logit : -INFINITY;
-      key[u] = e < E ? rq_order_key(logit) : 0;      // below every logit's
-      m = rq_nan_max(m, v[u]);
+      if (u >= c.used) break;
+      if (c.taken[u] >> lane & 1)
+        picked[wave][at + rq_lanes_before(c.taken[u])] = ((uint64_t)c.key[u] << 32) | (uint32_t)~(uint32_t)(64 * u + lane);
+      at += __popcll(c.taken[u]);
     }
-    uint32_t least = 0;
-    for (int bit = 31; bit >= 0; --bit) {
-      const uint32_t tried = least | (1u << bit);
-      int reach = 0;
-#pragma unroll
-      for (int u = 0; u < EL; ++u) {
-        if (64 * u >= E) break;
-        reach += __popcll(__ballot(key[u] >= tried));
-      }
-      if (reach >= K) least = tried;
-      if (reach == K) break;
-    }
-    // all above the K-th largest, and of those equal to it the first
-    int above = 0;
-#pragma unroll
-    for (int u = 0; u < EL; ++u) {
-      if (64 * u >= E) break;
-      above += __popcll(__ballot(key[u] > least));
-    }
-    int at = 0, equal = 0;
-#pragma unroll
-    for (int u = 0; u < EL; ++u) {
-      if (64 * u >= E) break;
-      const uint64_t eq = __ballot(key[u] == least);
-      const bool take = key[u] > least || (key[u] == least && equal + lanes_before(eq) < K - above);
-      const uint64_t mask = __ballot(take);
-      if (take) picked[wave][at + lanes_before(mask)] = ((uint64_t)key[u] << 32) | (uint32_t)~(uint32_t)(64 * u + lane);
-      at += __popcll(mask);
-      equal += __popcll(eq);
-    }
-    for (int o = 32; o; o >>= 1) m = rq_nan_max(m, __shfl_xor(m, o));
     float s = 0.0f;
 #pragma unroll
     for (int u = 0; u < EL; ++u) {
-      if (64 * u >= E) break;
-      s += expf(v[u] - m);                           // 0 past the last expert
+      if (u >= c.used) break;
+      s += expf(c.v[u] - c.m);                           // 0 past the last expert
     }
-    s = wave_sum(s);
+    s = rq_wave_sum(s);
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     __builtin_amdgcn_wave_barrier();
     const uint64_t mine = lane < K ? picked[wave][lane] : 0;
     int place = 0;
     for (int j = 0; j < K; ++j) place += picked[wave][j] > mine ? 1 : 0;
-    const float p = lane < K ? expf(rq_key_value((uint32_t)(mine >> 32)) - m) : 0.0f;
-    const float total = norm ? wave_sum(p) : s;
+    const float p = lane < K ? expf(rq_key_value((uint32_t)(mine >> 32)) - c.m) : 0.0f;
+    const float total = norm ? rq_wave_sum(p) : s;
     if (lane < K) {
       const int e = (int)~(uint32_t)mine;
       ids[t * K + place] = e;
@@ -200,7 +156,7 @@ __global__ __launch_bounds__(1024) void k_moe_route(const float* __restrict__ lo
     for (int p = 0; p < pairs; p += 64) {
       const bool is = p + lane < pairs && ids[p + lane] == e;
       const uint64_t mask = __ballot(is);
-      const int at = n + lanes_before(mask);
+      const int at = n + rq_lanes_before(mask);
       if (is) units[first[e] + at / 16].pairs[at % 16] = p + lane;
       n += __popcll(mask);
     }
@@ -275,7 +231,9 @@ extern "C" int rq_packed_moe(const void* x, int dtype, int T, int64_t ldx, int D
       const TX* xt = (const TX*)x + t0 * ldx;
       const RqMoe m{n, D, I, E, K, norm, nunits, units, weights, (float*)(ws + l.gate), (__hip_bfloat16*)(ws + l.h),
                     rq_moe_out_mode(d.w) == RQ_RUNS ? (I + 127) / 128 * 128 : I,
-                    rq_moe_out_mode(d.w) == RQ_RUNS, (float*)(ws + l.parts)};
+                    rq_moe_out_mode(d.w) == RQ_RUNS, (float*)(ws + l.parts),
+                    n == 1 && E <= 64 * MOE_CHOICE ? logits : nullptr, ids_out ? ids_out + t0 * K : nullptr,
+                    weights_out ? weights_out + t0 * K : nullptr};
       hipLaunchKernelGGL(k_moe_router<TX>, dim3(E, (n + ROUTER_TOKENS - 1) / ROUTER_TOKENS), dim3(256), 0, s, xt,
                          ldx, n, D, (const TX*)router, ldr, E, logits);
       auto route = [&](auto el) {
@@ -283,7 +241,9 @@ extern "C" int rq_packed_moe(const void* x, int dtype, int T, int64_t ldx, int D
                            units, rq_units(n, E, K), ids_out ? ids_out + t0 * K : nullptr,
                            weights_out ? weights_out + t0 * K : nullptr);
       };
-      if (E <= 64) route(std::integral_constant<int, 1>{});
+      // One token's experts are few enough to be chosen where they are needed.
+      if (m.logits) {
+      } else if (E <= 64) route(std::integral_constant<int, 1>{});
       else if (E <= 256) route(std::integral_constant<int, 4>{});
       else route(std::integral_constant<int, MOE_MAX_E / 64>{});
       rq_moe_in<TX>(xt, ldx, g, gate->nbits, u, up->nbits, m, s);

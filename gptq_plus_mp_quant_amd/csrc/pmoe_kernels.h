@@ -6,11 +6,72 @@ namespace {
 
 enum { MOE_BOTH = 0, MOE_GATE = 1, MOE_UP = 2 };
 
+// Unit u of one token: the u-th of its experts in their order, which every wave chooses for itself (a launch of its
+// own for that took 5.6 us, and waits for it before and after).  The first row tile's workgroups leave the units
+// for the second product, the first one of them the routing.
+struct Lone {
+  int expert;
+  float weight;
+};
+__device__ __forceinline__ Lone lone_unit(const RqMoe& m, int unit) {
+  const int lane = threadIdx.x & 63;
+  RqChoice<MOE_CHOICE> c;
+  rq_choose<MOE_CHOICE>(m.logits, m.E, m.K, c);
+  float sum = 0.0f;
+  float p[MOE_CHOICE];
+#pragma unroll
+  for (int k = 0; k < MOE_CHOICE; ++k) {
+    p[k] = k < c.used ? expf(c.v[k] - c.m) : 0.0f;   // 0 past the last expert
+    sum += m.norm && !(c.taken[k] >> lane & 1) ? 0.0f : p[k];
+  }
+  sum = rq_wave_sum(sum);
+  Lone one = {0, 0.0f};
+  int before = 0;
+#pragma unroll
+  for (int k = 0; k < MOE_CHOICE; ++k) {
+    const bool taken = c.taken[k] >> lane & 1;
+    const uint64_t is = __ballot(taken && before + rq_lanes_before(c.taken[k]) == unit);
+    if (is) {
+      const int at = __ffsll((unsigned long long)is) - 1;
+      one.expert = __builtin_amdgcn_readfirstlane(64 * k + at);
+      one.weight = __shfl(p[k], at) / sum;
+    }
+    before += __popcll(c.taken[k]);
+  }
+  if (blockIdx.x || threadIdx.x >= 64) return one;
+  RqUnit& u = m.units[unit];
+  if (lane < 16) u.pairs[lane] = unit;
+  if (lane == 0) {
+    u.expert = one.expert;
+    u.n = 1;
+    if (unit == 0) *m.nunits = m.K;
+  }
+  if (unit == 0 && (m.ids_out || m.weights_out)) {
+#pragma unroll
+    for (int k = 0; k < MOE_CHOICE; ++k) {
+      int place = 0;                                 // chosen experts with larger logits, or equal ones before it
+#pragma unroll
+      for (int j = 0; j < MOE_CHOICE; ++j)
+        for (uint64_t left = c.taken[j]; left; left &= left - 1) {
+          const int other = __ffsll((unsigned long long)left) - 1;
+          const uint32_t key = (uint32_t)__builtin_amdgcn_readlane((int)c.key[j], other);
+          place += key > c.key[k] || (key == c.key[k] && 64 * j + other < 64 * k + lane) ? 1 : 0;
+        }
+      if (c.taken[k] >> lane & 1) {
+        if (m.ids_out) m.ids_out[place] = 64 * k + lane;
+        if (m.weights_out) m.weights_out[place] = p[k] / sum;
+      }
+    }
+  }
+  return one;
+}
+
 // Grid (row tiles, units): 16 rows, chunks of 128 columns to the waves in turn, joined through LDS in their order.
 // BOTH: a wave multiplies the rows of gate and of up by the tokens it has loaded once.  GATE leaves the gate's
 // product in fp32, UP takes it from there (weights of different bits or groups).
 // 128 registers a lane, two workgroups a CU.  Bound by the weights' bytes: 8 experts of 4096 x 7168 at 5 bits, 32 tokens
-// 109 us for 294 MB, 2.7 TB/s, the tokens' loads beside them; 8 of 2048 x 768 at 4 bits, 1 token 9.5 us, latency.  Two row
+// 109 us for 294 MB, 2.7 TB/s, the tokens' loads beside them; 8 of 2048 x 768 at 4 bits, 1 token 12.7 us, 3 of them
+// its choice of experts: latency.  Two row
 // tiles a wave, which halve the tokens' loads, need 256 registers: 125 us.
 template <typename TX, int NB, int MODE, int NM>
 __global__ __launch_bounds__(512, 4) void k_moe_in(const TX* __restrict__ x, int64_t ldx, RqExperts first, RqExperts second,
@@ -18,9 +79,23 @@ __global__ __launch_bounds__(512, 4) void k_moe_in(const TX* __restrict__ x, int
   __shared__ floatx4 join[NM][8][64];
   extern __shared__ __attribute__((aligned(16))) float scales[];
   const int lane = threadIdx.x & 63, wave = rq_wave(), waves = blockDim.x >> 6;
-  const RqUnit& u = m.units[blockIdx.y];
-  const int r0 = blockIdx.x * 16, pair = u.pairs[lane & 15], expert = u.expert;
-  if (u.n == 0) return;
+  const int r0 = blockIdx.x * 16;
+  int pair, expert, n;
+  float p;
+  if (m.logits) {
+    const Lone one = lone_unit(m, blockIdx.y);
+    pair = blockIdx.y;
+    expert = one.expert;
+    n = 1;
+    p = one.weight;
+  } else {
+    const RqUnit& u = m.units[blockIdx.y];
+    n = u.n;
+    if (n == 0) return;
+    pair = u.pairs[lane & 15];
+    expert = u.expert;
+    p = m.weights[pair];
+  }
   RqTokens<TX, 1> xs;
   xs.p[0] = x + (int64_t)(pair / m.K) * ldx;
   RqPacked w[NM];
@@ -37,7 +112,7 @@ __global__ __launch_bounds__(512, 4) void k_moe_in(const TX* __restrict__ x, int
 #pragma unroll
   for (int a = 0; a < NM; ++a) join[a][wave][lane] = acc[a][0];
   __syncthreads();
-  if (wave || (lane & 15) >= u.n) return;
+  if (wave || (lane & 15) >= n) return;
   floatx4 a = join[0][0][lane], b = join[NM - 1][0][lane];
   for (int k = 1; k < waves; ++k) {
     a += join[0][k][lane];
@@ -59,7 +134,6 @@ __global__ __launch_bounds__(512, 4) void k_moe_in(const TX* __restrict__ x, int
   const int64_t plane = (int64_t)m.T * m.K * m.ldh;
   __hip_bfloat16* row = m.h + (int64_t)pair * m.ldh;
   __hip_bfloat16* h = row + (m.arranged ? rq_arranged(r) : r);                // r is a multiple of 4
-  const float p = m.weights[pair];
   floatx8 v = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
   for (int k = 0; k < 4; ++k) v[k] = p * (a[k] / (1.0f + expf(-a[k])) * b[k]);

@@ -5,6 +5,7 @@
 
 constexpr int MOE_MAX_E = 1024, MOE_MAX_K = 64;
 constexpr int MOE_TOKENS = 64;            // tokens per pass over the experts
+constexpr int MOE_CHOICE = 4;             // times 64: experts of one token that the first product chooses from
 
 // The experts' weights: expert e's entry is w with its pointers moved by e strides.
 struct RqExperts {
@@ -30,6 +31,65 @@ inline int rq_units(int T, int E, int K) {
   return pairs < all ? pairs : all;
 }
 
+__device__ __forceinline__ float rq_wave_sum(float v) {
+#pragma unroll
+  for (int m = 32; m; m >>= 1) v += __shfl_xor(v, m);
+  return v;
+}
+__device__ __forceinline__ int rq_lanes_before(uint64_t mask) {
+  return __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0));
+}
+// The K experts of one token's logits; a wave, lane i with experts i, 64 + i, ...  The K-th largest order key is
+// found bit by bit from the number of experts that reach a value; all above it are taken, and of those equal to
+// it the first: whatever the logits hold, exactly K.
+template <int EL>
+struct RqChoice {
+  float v[EL], m;
+  uint32_t key[EL];
+  uint64_t taken[EL];                     // of experts 64 u..64 u + 63
+  int used;                               // ceil(E / 64)
+};
+template <int EL>
+__device__ __forceinline__ void rq_choose(const float* l, int E, int K, RqChoice<EL>& c) {
+  const int lane = threadIdx.x & 63;
+  c.used = (E + 63) / 64;
+  c.m = -INFINITY;
+#pragma unroll
+  for (int u = 0; u < EL; ++u) {
+    c.taken[u] = 0;
+    c.v[u] = -INFINITY;
+    c.key[u] = 0;
+    if (u >= c.used) continue;
+    const int e = 64 * u + lane;
+    const float logit = l[min(e, E - 1)];
+    c.v[u] = e < E ? logit : -INFINITY;
+    c.key[u] = e < E ? rq_order_key(logit) : 0;      // below every logit's
+    c.m = rq_nan_max(c.m, c.v[u]);
+  }
+  uint32_t least = 0;
+  for (int bit = 31; bit >= 0; --bit) {
+    const uint32_t tried = least | (1u << bit);
+    int reach = 0;
+#pragma unroll
+    for (int u = 0; u < EL; ++u)
+      if (u < c.used) reach += __popcll(__ballot(c.key[u] >= tried));
+    if (reach >= K) least = tried;
+    if (reach == K) break;
+  }
+  int above = 0, equal = 0;
+#pragma unroll
+  for (int u = 0; u < EL; ++u)
+    if (u < c.used) above += __popcll(__ballot(c.key[u] > least));
+#pragma unroll
+  for (int u = 0; u < EL; ++u) {
+    if (u >= c.used) continue;
+    const uint64_t eq = __ballot(c.key[u] == least);
+    c.taken[u] = __ballot(c.key[u] > least || (c.key[u] == least && equal + rq_lanes_before(eq) < K - above));
+    equal += __popcll(eq);
+  }
+  for (int o = 32; o; o >>= 1) c.m = rq_nan_max(c.m, __shfl_xor(c.m, o));
+}
+
 // Pieces of the activation between the two products: fp32 in bf16 planes, two where the result is rounded
 // to 16 bits (2^-16 is lost), three for fp32 (exact).
 template <typename TX>
@@ -44,14 +104,17 @@ inline int rq_moe_out_mode(const RqPacked& down) {
 
 struct RqMoe {
   int T, D, I, E, K, norm;
-  const int* nunits;                      // 1
-  const RqUnit* units;                    // rq_units
+  int* nunits;                            // 1
+  RqUnit* units;                          // rq_units
   const float* weights;                   // T * K
   float* gate;                            // T * K * I: the gate's product where up has other bits or groups
   __hip_bfloat16* h;                      // pieces planes of T * K * ldh
   int ldh;                                // I; where h lies arranged (rq_arranged, for a down of RUNS), whole chunks
   bool arranged;
   float* parts;                           // rq_moe_parts planes of T * D
+  const float* logits;                    // of the one token whose experts the first product chooses, or NULL
+  int* ids_out;                           // then: NULL or K
+  float* weights_out;
 };
 // The product with down for many pairs takes four row tiles a wave for a load of h, which is several times the
 // weights' bytes where an expert has many tokens; workgroups share rows until there is one for every CU, and a launch

@@ -24,6 +24,11 @@ from . import _native as nat
 from . import kernels as K
 
 
+def _rows_apart(t):
+    """A single row whose stride, which no element needs, is shorter than the row."""
+    return t.clone(memory_format=torch.contiguous_format)
+
+
 def _checked(entry: Dict[str, object], batch: int):
     """(qweight, nbits, scales, R, C, ngroups, g_idx, groupsize) of an entry (batch = 1: stacked over
     experts)."""
@@ -53,7 +58,7 @@ def _checked(entry: Dict[str, object], batch: int):
     qst, sst = q.stride(), scales.stride()
     if qst[-1] != 1 or sst[-1] != 1 or (qst[-2] < words and R > 1) or (sst[-2] < R and ng > 1):
         raise ValueError("packed entry: qweight and scales need unit column strides")
-    return (q if qst[-2] >= words else q.contiguous(), nbits, scales if sst[-2] >= R else scales.contiguous(), R, C, ng,
+    return (q if qst[-2] >= words else _rows_apart(q), nbits, scales if sst[-2] >= R else _rows_apart(scales), R, C, ng,
             g_idx if g_idx.is_contiguous() else g_idx.contiguous(), groupsize)
 
 

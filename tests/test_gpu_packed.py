@@ -468,3 +468,38 @@ def test_second_derivatives_are_refused():
     g, = torch.autograd.grad(packed_linear(x, on(entry, DEV)).square().sum(), x, create_graph=True)
     with pytest.raises(RuntimeError):
         g.sum().backward()
+
+
+@pytest.mark.parametrize("T", [1, 65])
+@pytest.mark.parametrize("norm", [True, False])
+@pytest.mark.parametrize("E,K", [(1, 1), (3, 3), (64, 5), (65, 64), (200, 7), (256, 64), (257, 6)])
+def test_moe_one_token_at_a_time(E, K, norm, T):
+    """A lone token (the last pass of 65 as well) at every number of experts, up to all of them chosen."""
+    check_moe(*moe_case(E + K, T, 64, 48, E, (F16, BF16, F32)[E % 3], (4, 4, 4), ("32", "32", "channel")), K, norm)
+
+
+def test_moe_one_token_ties_and_mixed_bits():
+    x, router, parts = moe_case(7, 1, 64, 32, 100, F16, (3, 4, 5), ("32", "channel", "order16"))
+    router[:] = router[4]
+    router[90] = 2 * router[4] * torch.sign(router[4] @ x[0])
+    _, ids, weights = packed_moe(x.to(DEV), router.to(DEV), *(on(e, DEV) for e, _ in parts), 5, return_routing=True)
+    rest = [e for e in range(100) if e != 90]
+    assert ids.cpu().tolist() == [[90] + rest[:4]]
+    router[:, :] = 0.0
+    check_moe(x, router, parts, 3, True)
+    x[0, 3] = float("nan")
+    y, ids, _ = packed_moe(x.to(DEV), router.to(DEV), *(on(e, DEV) for e, _ in parts), 3, return_routing=True)
+    assert bool(torch.isnan(y).all()) and bool((ids >= 0).all()) and bool((ids < 100).all())
+
+
+def test_single_row_with_a_short_stride():
+    """One row's stride is never used: scales that are a transposed column, a weight of one row."""
+    entry, W = make_entry(5, 40, 64, 4, "channel")
+    e = on(entry, DEV)
+    e["scales"] = e["scales"].as_strided((1, 40), (1, 1))
+    check_linear(randn(1, 3, 64, dtype=F16), e, W)
+    entry, W = make_entry(6, 1, 64, 4, "32")
+    e = on(entry, DEV)
+    e["qweight"] = e["qweight"].as_strided((1, 8), (1, 1))
+    check_linear(randn(2, 3, 64, dtype=F16), e, W)
+    check_grad(randn(3, 3, 1, dtype=F16), e, W)

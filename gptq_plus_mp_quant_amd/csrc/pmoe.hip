@@ -4,8 +4,9 @@
 //   (divided by their sum when norm), y = sum_k w_k Wd_k (silu(Wg_k x) * (Wu_k x)).
 //
 // Four launches, three for one token, five for many: the router's logits; the routing, which sorts the chosen
-// (token, expert) pairs into units of up to 16 tokens of one expert (one token's needs no launch); gate, up and the activation of every unit; down, summed over a token's
-// experts.  An expert that no token chose is not read, one that several chose is read once for 16 of them.
+// (token, expert) pairs into units of up to 16 tokens of one expert (one token's needs no launch); gate, up and
+// the activation of every unit; down, summed over a token's experts.  An expert that no token chose is not read,
+// one that several chose is read once for 16 of them.
 // Router logits, sums, the activation and the sum over experts are fp32 (the activation in bf16 pieces that
 // carry 16 bits or all 24); the one rounding to fewer bits is the result's to x's type.
 #include "pmoe_types.h"
@@ -241,11 +242,11 @@ extern "C" int rq_packed_moe(const void* x, int dtype, int T, int64_t ldx, int D
                            units, rq_units(n, E, K), ids_out ? ids_out + t0 * K : nullptr,
                            weights_out ? weights_out + t0 * K : nullptr);
       };
-      // One token's experts are few enough to be chosen where they are needed.
-      if (m.logits) {
-      } else if (E <= 64) route(std::integral_constant<int, 1>{});
-      else if (E <= 256) route(std::integral_constant<int, 4>{});
-      else route(std::integral_constant<int, MOE_MAX_E / 64>{});
+      if (!m.logits) {                               // else they are chosen where they are needed
+        if (E <= 64) route(std::integral_constant<int, 1>{});
+        else if (E <= 256) route(std::integral_constant<int, 4>{});
+        else route(std::integral_constant<int, MOE_MAX_E / 64>{});
+      }
       rq_moe_in<TX>(xt, ldx, g, gate->nbits, u, up->nbits, m, s);
       rq_moe_out<TX>(d, down->nbits, m, (TX*)y + t0 * ldy, ldy, s);
     }

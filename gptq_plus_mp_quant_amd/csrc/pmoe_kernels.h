@@ -71,8 +71,7 @@ __device__ __forceinline__ Lone lone_unit(const RqMoe& m, int unit) {
 // product in fp32, UP takes it from there (weights of different bits or groups).
 // 128 registers a lane, two workgroups a CU.  Bound by the weights' bytes: 8 experts of 4096 x 7168 at 5 bits, 32 tokens
 // 109 us for 294 MB, 2.7 TB/s, the tokens' loads beside them; 8 of 2048 x 768 at 4 bits, 1 token 12.7 us, 3 of them
-// its choice of experts: latency.  Two row
-// tiles a wave, which halve the tokens' loads, need 256 registers: 125 us.
+// its choice of experts: latency.  Two row tiles a wave, which halve the tokens' loads, need 256 registers: 125 us.
 template <typename TX, int NB, int MODE, int NM>
 __global__ __launch_bounds__(512, 4) void k_moe_in(const TX* __restrict__ x, int64_t ldx, RqExperts first, RqExperts second,
                                                 int what, RqMoe m) {

@@ -503,3 +503,18 @@ def test_single_row_with_a_short_stride():
     e["qweight"] = e["qweight"].as_strided((1, 8), (1, 1))
     check_linear(randn(2, 3, 64, dtype=F16), e, W)
     check_grad(randn(3, 3, 1, dtype=F16), e, W)
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("T", [2, 20])
+def test_more_groups_than_are_staged(T, dtype):
+    """Scales are read from memory where a workgroup's do not fit its share of LDS."""
+    for groups, C in (("order8", 8400), ("8", 8232)):
+        entry, W = make_entry(C, 24, C, 4, groups)
+        check_linear(randn(T, T, C, dtype=dtype), entry, W)
+        check_grad(randn(T + 1, T, 24, dtype=dtype), entry, W)
+
+
+@pytest.mark.parametrize("T", [1, 24])
+def test_moe_more_groups_than_are_staged(T):
+    check_moe(*moe_case(T, T, 2080, 560, 3, BF16, (4, 4, 4), ("order8", "order8", "order8")), 2, True)

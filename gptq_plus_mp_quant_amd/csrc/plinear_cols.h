@@ -8,12 +8,13 @@
 //   RUNS   all 128 columns are in one group: it multiplies dy, and the codes go in as they are
 //   SMALL  a lane's 8 columns are in one group (sizes that are multiples of 8): it multiplies the codes
 //   ANY    a scale for every weight
-// What a scale multiplied is an fp32 number, cut into bf16 pieces: two (2^-16 of it is lost; the 16-bit
-// types' results have 8 or 11 bits) or three (fp32, exact).  Products of pieces below 2^-24 are left out.
+// What a scale multiplied is an fp32 number and is cut into three bf16 pieces, exactly, whatever dy's type: sums
+// that cancel keep fp32's precision.  Where both sides are cut, products that come to at most 2^-22 of a term (2^-24
+// mostly) are left out.
 // Rows are split over workgroups until there are 512, whose sums a second launch joins in their order.
-// Measured: 4096 x 4096 5-bit fp16, 8 tokens 9.1 + 4.1 us, latency; 14336 x 4096 4-bit bf16, 64 tokens 30 + 5.3 us, where
-// the conversions of codes and of dy on the vector units and two pieces' matrix instructions (7.5 GFLOP twice)
-// overlap in part, with two waves a SIMD.
+// Measured: 4096 x 4096 5-bit fp16, 8 tokens 9.1 + 4.1 us, latency; 14336 x 4096 4-bit bf16, 64 tokens 33 + 5.3 us (30.6 with
+// two pieces), where the conversions of codes and of dy on the vector units and three pieces' matrix instructions (7.5
+// GFLOP each) overlap in part, with two waves a SIMD.
 #pragma once
 #include "packed_dot.h"
 
@@ -22,14 +23,15 @@ namespace {
 // Pieces of dy and of the weight where each is cut (1: bf16 as it is).
 template <typename TX, int MODE> struct ColPieces;
 template <int MODE> struct ColPieces<__half, MODE> {
-  static constexpr int dy = 2, w = MODE == RQ_RUNS ? 1 : 2, keep = 3;
+  static constexpr int dy = MODE == RQ_RUNS ? 3 : 2, w = MODE == RQ_RUNS ? 1 : 3;
 };
 template <int MODE> struct ColPieces<__hip_bfloat16, MODE> {
-  static constexpr int dy = MODE == RQ_RUNS ? 2 : 1, w = MODE == RQ_RUNS ? 1 : 2, keep = 2;
+  static constexpr int dy = MODE == RQ_RUNS ? 3 : 1, w = MODE == RQ_RUNS ? 1 : 3;
 };
 template <int MODE> struct ColPieces<float, MODE> {
-  static constexpr int dy = 3, w = MODE == RQ_RUNS ? 1 : 3, keep = 3;
+  static constexpr int dy = 3, w = MODE == RQ_RUNS ? 1 : 3;
 };
+constexpr int PIECES_KEPT = 3;             // products of pieces i and j with i + j below this
 
 constexpr int COLS = 128, STEP = 32;
 
@@ -192,7 +194,7 @@ __global__ __launch_bounds__(64 * cols_waves(NT), cols_occupancy(MODE, NT)) void
       for (int pd = 0; pd < P::dy; ++pd)
 #pragma unroll
         for (int pw = 0; pw < P::w; ++pw)
-          if (pd + pw < P::keep) {
+          if (pd + pw < PIECES_KEPT) {
 #pragma unroll
             for (int b = 0; b < NT; ++b) {
               if constexpr (P::w > 1) acc[n][b] = rq_mfma(pd == 0 && pw ? low[b] : d[b][pd], v[pw], acc[n][b]);

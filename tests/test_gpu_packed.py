@@ -9,6 +9,7 @@ import torch
 
 from gptq_plus_mp_quant_amd import (GPTQ, GPTQPlus, WeightQuantizer, dequantize_packed, export_packed, load_packed,
                                     packed_linear, packed_linear_backward, packed_moe, save_packed, stack_packed)
+from oracle.packing import pack_rows
 from tests._packed import ROUND, TINY, assert_within, make_entry, on, sum_eps
 from tests._util import rng, synth
 
@@ -518,3 +519,41 @@ def test_more_groups_than_are_staged(T, dtype):
 @pytest.mark.parametrize("T", [1, 24])
 def test_moe_more_groups_than_are_staged(T):
     check_moe(*moe_case(T, T, 2080, 560, 3, BF16, (4, 4, 4), ("order8", "order8", "order8")), 2, True)
+
+
+# --- 32 bits throughout ------------------------------------------------------------------------
+
+
+def by_hand(codes, scales, g_idx, nbits, groupsize=None):
+    """An entry from codes [R, C], scales [ngroups, R] and groups [C], and its weight in float64."""
+    R, C = codes.shape
+    entry = dict(qweight=torch.from_numpy(pack_rows(codes, nbits).view(np.int32)), scales=torch.from_numpy(scales),
+                 g_idx=torch.from_numpy(g_idx.astype(np.int32)), nbits=nbits, bits=nbits, sym=True, shape=(R, C), dtype="float16")
+    if groupsize:
+        entry["groupsize"] = groupsize
+    return entry, torch.from_numpy(scales.astype(np.float64)[g_idx].T * codes)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16, F32])
+@pytest.mark.parametrize("T", [5, 20, 40])
+@pytest.mark.parametrize("nbits,groups", [(4, "channel"), (5, "128"), (4, "32"), (5, "order32")])
+def test_gradient_keeps_32_bits(nbits, groups, T, dtype):
+    """Two rows whose products cancel to the last bit of fp32 (codes and scales are three times as large in
+    one): what is left shows every rounding to fewer bits on the way.  Allowed, in units of 2^-24 of the
+    terms' magnitudes: two for the products of dy, scale and code, two for each of the sums over at most six
+    pairs of pieces."""
+    r, C = rng(T + nbits), 384
+    size = C if groups == "channel" else int(groups.replace("order", ""))
+    order = r.permutation(C) if groups.startswith("order") else np.arange(C)
+    g_idx = np.argsort(order) // size
+    codes = r.choice([-2, -1, 1, 2], size=(1, C))
+    codes = np.concatenate([3 * codes, -codes])
+    a, b = 1.375, 1.25
+    s0 = (r.uniform(0.5, 1.0, size=C // size) * 0.25).astype(np.float32)
+    scales = np.stack([s0, (3 * s0 * np.float32(a) / np.float32(b)).astype(np.float32)], 1)
+    entry, W = by_hand(codes, scales, g_idx, nbits, None if groups.startswith("order") else size)
+    gy = torch.from_numpy(r.integers(1, 16, size=(T, 1)) * np.array([[a, b]])).to(dtype)     # exact in every type
+    gx = packed_linear_backward(gy.to(DEV), on(entry, DEV))
+    want, mag = gy.double() @ W, gy.double().abs() @ W.abs()
+    assert float((want.abs() / mag).max()) < 2.0 ** -23
+    assert_within(gx, want, 14 * 2.0 ** -24 * mag + ROUND[dtype] * want.abs() + TINY[dtype], "gx")

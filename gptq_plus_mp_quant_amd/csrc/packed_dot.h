@@ -149,30 +149,23 @@ __device__ __forceinline__ floatx8 rq_load_x(const float* p, int n) {
 }
 __device__ __forceinline__ void rq_operand(half8 x, half8 (&v)[1]) { v[0] = x; }
 __device__ __forceinline__ void rq_operand(bf16x8 x, bf16x8 (&v)[1]) { v[0] = x; }
-// fp32 in bf16 pieces.  Three: cut off by truncation, 8 + 8 + 8 bits, exact (canonicalising keeps a NaN's
-// mark in its upper half).  Two: the first rounded to nearest, so the second leaves at most 2^-16 of the
-// value.  An infinite first piece leaves 0 over.
+// fp32 in bf16 pieces, each cut off by truncation: three carry 8 + 8 + 8 bits, exactly; two an fp16 number's 11
+// (canonicalising keeps a NaN's mark in its upper half).  An infinite first piece leaves 0 over.
 template <int P>
 __device__ __forceinline__ void rq_operand(floatx8 x, bf16x8 (&v)[P]) {
 #pragma unroll
   for (int k = 0; k < 8; ++k) {
-    if constexpr (P == 2) {
-      v[0][k] = (__bf16)x[k];
-      const float hi = (float)v[0][k];
-      v[1][k] = (__bf16)(__builtin_fabsf(hi) == INFINITY ? 0.0f : x[k] - hi);
-    } else {
-      float r = __builtin_canonicalizef(x[k]);
-      const bool inf = __builtin_fabsf(r) == INFINITY;
+    float r = __builtin_canonicalizef(x[k]);
+    const bool inf = __builtin_fabsf(r) == INFINITY;
 #pragma unroll
-      for (int p = 0; p < P; ++p) {
-        const uint32_t b = __float_as_uint(r) & 0xFFFF0000u;
-        const uint16_t top = (uint16_t)(b >> 16);
-        __bf16 h;
-        __builtin_memcpy(&h, &top, 2);
-        v[p][k] = h;
-        r -= __uint_as_float(b);
-        if (p == 0 && inf) r = 0.0f;
-      }
+    for (int p = 0; p < P; ++p) {
+      const uint32_t b = __float_as_uint(r) & 0xFFFF0000u;
+      const uint16_t top = (uint16_t)(b >> 16);
+      __bf16 h;
+      __builtin_memcpy(&h, &top, 2);
+      v[p][k] = h;
+      r -= __uint_as_float(b);
+      if (p == 0 && inf) r = 0.0f;
     }
   }
 }

@@ -7,8 +7,8 @@
 // (token, expert) pairs into units of up to 16 tokens of one expert (one token's needs no launch); gate, up and
 // the activation of every unit; down, summed over a token's experts.  An expert that no token chose is not read,
 // one that several chose is read once for 16 of them.
-// Router logits, sums, the activation and the sum over experts are fp32 (the activation in bf16 pieces that
-// carry 16 bits or all 24); the one rounding to fewer bits is the result's to x's type.
+// Router logits, sums, the activation and the sum over experts are fp32 (the activation in three bf16 pieces that
+// carry all 24 bits); the one rounding to fewer bits is the result's to x's type.
 #include "pmoe_types.h"
 
 namespace {
@@ -190,7 +190,7 @@ inline Layout layout(int T, int D, int I, int E, int K) {
   l.units = l.nunits + 256;
   l.gate = l.units + up256((int64_t)rq_units((int)n, E, K) * (int64_t)sizeof(RqUnit));
   l.h = l.gate + up256(n * K * I * 4);
-  l.parts = l.h + up256(n * K * (((int64_t)I + 127) / 128 * 128) * 2 * 3);
+  l.parts = l.h + up256(n * K * (((int64_t)I + 127) / 128 * 128) * 2 * MOE_PIECES);
   l.total = l.parts + up256((int64_t)rq_moe_parts(D) * n * D * 4);
   return l;
 }

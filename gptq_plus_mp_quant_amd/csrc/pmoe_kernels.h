@@ -129,7 +129,7 @@ __global__ __launch_bounds__(512, 4) void k_moe_in(const TX* __restrict__ x, int
 #pragma unroll
     for (int k = 0; k < 4; ++k) a[k] = r + k < m.I ? g[k] : 0.0f;
   }
-  constexpr int P = rq_moe_pieces<TX>();
+  constexpr int P = MOE_PIECES;
   const int64_t plane = (int64_t)m.T * m.K * m.ldh;
   __hip_bfloat16* row = m.h + (int64_t)pair * m.ldh;
   __hip_bfloat16* h = row + (m.arranged ? rq_arranged(r) : r);                // r is a multiple of 4
@@ -154,13 +154,13 @@ __global__ __launch_bounds__(512, 4) void k_moe_in(const TX* __restrict__ x, int
 // whatever else is in the batch, and a wave adds every chunk's sums to its own copy of the workgroup's results in
 // LDS, in the order of the experts: a token's result depends on how many tokens there are, not on which.
 // RUNS: the loads of the next D chunks, of whatever units, are in flight.
-// h, in two pieces, is 8 KB a chunk of 16 tokens, six times a row tile's words: with one row tile a wave 107 us for 8
-// experts of 7168 x 4096 at 5 bits (147 MB) and 32 tokens, with four 70 us and 4.8 us to join the parts.  8 of 768 x 2048 at
-// 4 bits, 1 token: 10.7 us, latency.
+// h, in three pieces, is 12 KB a chunk of 16 tokens, ten times a row tile's words: with four row tiles a wave 80 us and
+// 4.8 us to join the parts for 8 experts of 7168 x 4096 at 5 bits (147 MB) and 32 tokens.  8 of 768 x 2048 at 4 bits, 1
+// token: 12.6 us, latency.
 template <typename TX, int NB, int MODE, int RT>
 __global__ __launch_bounds__(64 * MOE_OUT_WAVES) void k_moe_out(RqExperts down, RqMoe m, bool staged,
                                                                  TX* __restrict__ y, int64_t ldy) {
-  constexpr int P = rq_moe_pieces<TX>(), W = MOE_OUT_WAVES, R4 = 4 * RT;
+  constexpr int P = MOE_PIECES, W = MOE_OUT_WAVES, R4 = 4 * RT;
   extern __shared__ __attribute__((aligned(16))) floatx4 sums[];       // [W][T][R4]: the rows of a token; then the units
   RqUnit* units = reinterpret_cast<RqUnit*>(sums + W * m.T * R4);
   const int lane = threadIdx.x & 63, wave = rq_wave(), i = lane & 15, q = lane >> 4;

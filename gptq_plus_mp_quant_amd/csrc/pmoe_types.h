@@ -90,10 +90,10 @@ __device__ __forceinline__ void rq_choose(const float* l, int E, int K, RqChoice
   for (int o = 32; o; o >>= 1) c.m = rq_nan_max(c.m, __shfl_xor(c.m, o));
 }
 
-// Pieces of the activation between the two products: fp32 in bf16 planes, two where the result is rounded
-// to 16 bits (2^-16 is lost), three for fp32 (exact).
-template <typename TX>
-constexpr int rq_moe_pieces() { return sizeof(TX) == 4 ? 3 : 2; }
+// Pieces of the activation between the two products: an fp32 number in three bf16 planes, exactly, whatever x's type
+// (kept in fp32 and cut where it is loaded it takes two thirds of the bytes, and longer: 128 experts of 2048 x 768, 1
+// token 30.2 us for 27.0, 8 of 4096 x 7168, 8 tokens 190 for 178).
+constexpr int MOE_PIECES = 3;
 
 // How down is read: h may be filled up to whole chunks, so RUNS needs no ragged end as long as rows are whole
 // words of 32 columns; other rows go 8 columns at a time.
@@ -108,7 +108,7 @@ struct RqMoe {
   RqUnit* units;                          // rq_units
   const float* weights;                   // T * K
   float* gate;                            // T * K * I: the gate's product where up has other bits or groups
-  __hip_bfloat16* h;                      // pieces planes of T * K * ldh
+  __hip_bfloat16* h;                      // MOE_PIECES planes of T * K * ldh
   int ldh;                                // I; where h lies arranged (rq_arranged, for a down of RUNS), whole chunks
   bool arranged;
   float* parts;                           // rq_moe_parts planes of T * D
@@ -118,10 +118,11 @@ struct RqMoe {
 };
 // The product with down for many pairs takes four row tiles a wave for a load of h, which is several times the
 // weights' bytes where an expert has many tokens; workgroups share rows until there is one for every CU, and a launch
-// of its own adds them up.  From 32 pairs on that is faster (one row tile / four, the whole layer: 8 experts of 4096 x
-// 7168 at 5 bits, 2 of them a token, 8 tokens 172 / 178 us, 16 tokens 206 / 193, 64 tokens 340 / 286; 128 of 2048 x 768
-// at 4 bits, 8 a token, 4 tokens 63 / 58, 16 tokens 134 / 108), as long as the sums of all tokens fit LDS.
-constexpr int MOE_OUT_WAVES = 8, MOE_OUT_ROWS = 4;
+// of its own adds them up.  From 96 pairs' chunks of 128 columns on that is faster, as long as the sums of all tokens fit
+// LDS (one row tile / four, the whole layer in us: 8 experts of 4096 x 7168 at 5 bits, 2 of them a token, 1 token 62.3 /
+// 59.1, 8 tokens 179 / 155, 64 tokens 384 / 280; 128 of 2048 x 768 at 4 bits, 8 a token, 1 token 26.8 / 28.8, 2 tokens
+// 41.0 / 39.2, 16 tokens 144 / 105; 16 of 512 x 1024 at 8 bits, 2 a token, 4 tokens 29.5 / 35.6).
+constexpr int MOE_OUT_WAVES = 8, MOE_OUT_ROWS = 4, MOE_DENSE_CHUNKS = 96;
 inline int rq_moe_parts(int D) {
   const int tiles = (D + 16 * MOE_OUT_ROWS - 1) / (16 * MOE_OUT_ROWS), parts = (256 + tiles - 1) / tiles;
   return parts < 8 ? parts : 8;
@@ -130,7 +131,7 @@ inline int rq_moe_out_lds(const RqMoe& m, int rows) {
   return MOE_OUT_WAVES * m.T * 64 * rows + rq_units(m.T, m.E, m.K) * (int)sizeof(RqUnit);
 }
 inline bool rq_moe_dense(const RqMoe& m) {
-  return m.T * m.K >= 32 && rq_moe_out_lds(m, MOE_OUT_ROWS) <= 160 * 1024;
+  return (int64_t)m.T * m.K * ((m.I + 127) / 128) >= MOE_DENSE_CHUNKS && rq_moe_out_lds(m, MOE_OUT_ROWS) <= 160 * 1024;
 }
 
 // LDS for the scales of groups that are no runs of columns (bytes, 0 where there are too many groups): gate's and up's of a

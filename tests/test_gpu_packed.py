@@ -557,3 +557,48 @@ def test_gradient_keeps_32_bits(nbits, groups, T, dtype):
     want, mag = gy.double() @ W, gy.double().abs() @ W.abs()
     assert float((want.abs() / mag).max()) < 2.0 ** -23
     assert_within(gx, want, 14 * 2.0 ** -24 * mag + ROUND[dtype] * want.abs() + TINY[dtype], "gx")
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16, F32])
+@pytest.mark.parametrize("T", [1, 5, 40])
+@pytest.mark.parametrize("I,groups", [(2, "channel"), (64, "channel"), (64, "order32"), (96, "32")])
+def test_moe_activation_keeps_32_bits(I, groups, T, dtype):
+    """Two columns of the activation that are one and three times the same, which down cancels: everything
+    before the activation is exact (few bits, scales that are powers of two), so the result is off by the
+    activation's own rounding, one unit of 2^-24, and two for each of the six pieces' products in the sum."""
+    r, D, E = rng(T + I), 32, 3
+
+    def stacked(parts):
+        entry = dict(parts[0][0])
+        entry.update({k: torch.stack([e[k] for e, _ in parts]) for k in ("qweight", "scales", "g_idx")})
+        return entry, torch.stack([w for _, w in parts])
+
+    def one(codes, scale, C):
+        size = C if groups == "channel" else int(groups.replace("order", ""))
+        g_idx = np.arange(C) // size if size < C else np.zeros(C, dtype=np.int64)
+        if groups.startswith("order"):
+            g_idx = g_idx[::-1].copy()
+        scales = np.full((int(g_idx.max()) + 1, codes.shape[0]), scale, dtype=np.float32)
+        return by_hand(codes, scales, g_idx, 4, None if groups.startswith("order") else size)
+
+    def expert():
+        gate, up, down = (np.zeros(s, dtype=np.int64) for s in ((I, D), (I, D), (D, I)))
+        gate[:2] = r.integers(-7, 8, size=(1, D))
+        up[:1] = r.integers(-2, 3, size=(1, D))
+        up[1] = 3 * up[0]
+        v = r.choice([-2, -1, 1, 2], size=D)
+        down[:, 0], down[:, 1] = 3 * v, -v
+        return one(gate, 2.0 ** -6, D), one(up, 2.0 ** -3, D), one(down, 2.0 ** -2, I)
+
+    parts = [stacked(p) for p in zip(*(expert() for _ in range(E)))]
+    x = torch.from_numpy(r.integers(-15, 16, size=(T, D)) / 4.0).to(dtype)
+    router = randn(T, E, D, dtype=dtype)
+    y, ids, w = packed_moe(x.to(DEV), router.to(DEV), *(on(e, DEV) for e, _ in parts), 1, return_routing=True)
+    assert torch.equal(w.cpu(), torch.ones(T, 1))
+    Wg, Wu, Wd = (p[1][ids.cpu().long()[:, 0]] for p in parts)
+    xd = x.double()[:, :, None]
+    gate, up = Wg @ xd, Wu @ xd
+    h = gate * torch.sigmoid(gate) * up
+    want, mag = (Wd @ h)[:, :, 0], (Wd.abs() @ h.abs())[:, :, 0]
+    assert float(mag.max()) > 0.1 and float(want.abs().max()) <= 1e-12 * float(mag.max())
+    assert_within(y, torch.zeros_like(want), 13 * 2.0 ** -24 * mag + TINY[dtype], "y")

@@ -255,9 +255,11 @@ __device__ __forceinline__ Stat scan_segment(const Scan<TX>& sc, float* most) {
 #pragma unroll
     for (int k = 0; k < 8; ++k) v.m = fmaxf(v.m, (float)in[u][k]);
   // Exponents are f log2e - shift with shift = fl(m log2e), one fma: the sums are off by the factor
-  // 2^(m log2e - shift), which is taken out at the end.  Where m log2e overflows (wide: the type's lowest
-  // value as a mask of everything so far, or +inf) they are (f - m) log2e.
-  auto is_wide = [](float m) { return m != -INFINITY && __builtin_fabsf(m) > 2e38f; };
+  // 2^(m log2e - shift), which is taken out at the end.  It is within 2^(+-1/16) up to |shift| = WIDE; beyond (wide: masks
+  // of a large negative number in everything so far, the type's lowest value among them, or +inf) exponents are
+  // (f - m) log2e.
+  constexpr float WIDE = 0x1p20f;
+  auto is_wide = [](float at) { return __builtin_fabsf(at) > WIDE; };
   float shift = v.m == -INFINITY ? 0.0f : v.m * LOG2E;
   float block = -INFINITY;
   int round = 0;
@@ -275,7 +277,15 @@ __device__ __forceinline__ Stat scan_segment(const Scan<TX>& sc, float* most) {
       for (int k = 1; k < 8; ++k) big = fmaxf(big, f[k]);
       block = fmaxf(block, big);
       if (big > v.m) {                     // the maximum grows
-        const float grown = big * LOG2E, D = __builtin_amdgcn_fmed3f(shift - grown, LOW, 0.0f);
+        const float grown = big * LOG2E;
+        // far: from what the sums' exponents were taken from to what they are taken from now.  One of them is wide only
+        // if -shift or grown is (a lane without a maximum so far has shift 0 and sums of 0).
+        float far = shift - grown;
+        if (__any(__builtin_fmaxf(-shift, grown) > WIDE)) {
+          if (is_wide(shift)) far = is_wide(grown) ? (v.m - big) * LOG2E : __builtin_fmaf(v.m, LOG2E, -grown);
+          else if (is_wide(grown)) far = __builtin_fmaf(-big, LOG2E, shift);
+        }
+        const float D = __builtin_amdgcn_fmed3f(far, LOW, 1.0f);
         const float scale = v.m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(D);
         v.a = scale * (v.a + D * v.s);
         v.s *= scale;
@@ -287,9 +297,9 @@ __device__ __forceinline__ Stat scan_segment(const Scan<TX>& sc, float* most) {
         v.s += e;
         v.a = __builtin_fmaf(e, __builtin_amdgcn_fmed3f(x, LOW, 1.0f), v.a);
       };
-      if (__any(is_wide(v.m))) {
+      if (__any(is_wide(shift))) {
 #pragma unroll
-        for (int k = 0; k < 8; ++k) add(is_wide(v.m) ? (f[k] - v.m) * LOG2E : __builtin_fmaf(f[k], LOG2E, -shift));
+        for (int k = 0; k < 8; ++k) add(is_wide(shift) ? (f[k] - v.m) * LOG2E : __builtin_fmaf(f[k], LOG2E, -shift));
       } else {
 #pragma unroll
         for (int k = 0; k < 8; ++k) add(__builtin_fmaf(f[k], LOG2E, -shift));
@@ -300,7 +310,7 @@ __device__ __forceinline__ Stat scan_segment(const Scan<TX>& sc, float* most) {
       block = -INFINITY;
     }
   }
-  const float off = v.m == -INFINITY || is_wide(v.m) ? 0.0f : __builtin_fmaf(v.m, LOG2E, -shift);
+  const float off = v.m == -INFINITY || is_wide(shift) ? 0.0f : __builtin_fmaf(v.m, LOG2E, -shift);
   const float back = __builtin_amdgcn_exp2f(-off);
   v.a = back * (v.a - off * v.s);
   v.s *= back;

@@ -273,3 +273,38 @@ def test_refusals():
     for args in ((z, t, s[:2], g), (z, t, s, g[:2]), (z, t, s, g.double()), (z, t, s, g, g[:1]), (z, t, s.half(), g)):
         with pytest.raises(ValueError):
             token_logprobs_backward(*args)
+
+
+@pytest.mark.parametrize("dtype,mask", [(F16, -3e4), (F16, -6e4), *((d, m) for d in (BF16, F32) for m in (
+    -1e6, -2.0 ** 21, -1e8, -1e9, -1e10, -1e20, -1e30, -1.7e38))])
+@pytest.mark.parametrize("N,V", [(6, 50), (6, 4099), (6, 70001), (600, 4500)])
+def test_finite_masks(N, V, mask, dtype):
+    """Masks by any large negative number, as attention and sampling code uses them: in part of a row, in all
+    but three places of it, before and after what counts, and in the whole row."""
+    z = randn(V, N, V, dtype=dtype, scale=3.0)
+    z[0::6, :] = mask
+    for k, c in enumerate((V // 3, V // 2, V - 2)):
+        z[0::6, c] = float(k)
+    z[1::6, :V // 2] = mask
+    z[2::6, V // 2:] = mask
+    z[3::6, :] = mask
+    z[4::6][torch.from_numpy(rng(V + 1).random((z[4::6].shape[0], V)) < 0.7)] = mask
+    t = torch.tensor([V // 2, V - 1, 1, 7, 3, 0]).repeat(N // 6)
+    r = check(z, t, 9)
+    assert bool((r.logprob[3::6] + math.log(V)).abs().max() < 1e-5) and bool((r.entropy[3::6] - math.log(V)).abs().max() < 1e-5)
+    if N == 6:
+        check_grad(z, t)
+
+
+@pytest.mark.parametrize("at", [-2.0 ** 30, -2.0 ** 22, -2.0 ** 20, -2.0 ** 18, 2.0 ** 18, 2.0 ** 20, 2.0 ** 22, 2.0 ** 30])
+@pytest.mark.parametrize("order", ["up", "down", "mixed"])
+def test_logits_far_from_zero(order, at):
+    """A distribution of logits that lie far from zero, a few units in their last place apart."""
+    N, V = 5, 9001
+    step = max(abs(at) * 2.0 ** -23, 2.0 ** -6)
+    k = ints(3, 24, N, V)
+    k = k if order == "mixed" else k.sort(dim=-1, descending=order == "down").values
+    z = (at + step * k.double()).float()
+    assert torch.equal(z.double(), at + step * k.double())
+    check(z, ints(4, V, N), 5)
+    check_grad(z, ints(4, V, N))

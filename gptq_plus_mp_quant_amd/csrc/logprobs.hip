@@ -5,7 +5,7 @@
 //   logprob = d_target - log s        H = log s - (sum_i exp(d_i) d_i) / s        p_i = exp(d_i - log s)
 //   dz_i = gl (delta_{i,target} - p_i) - gh p_i (log p_i + H)
 // Differences from m are formed first, so masks of the type's lowest value cost no precision; a term
-// with exp(d_i) = 0 is 0 whatever d_i is (-inf among them).  A row with nothing left (m = -inf) has
+// with exp(d_i) = 0 is 0 whatever d_i is (-inf among them).  A row with nothing but -inf (m = -inf, s = 0) has
 // logprob -inf, H = 0 and no gradient.  A NaN or +inf logit makes its row NaN.
 // All statistics are fp32.  Equal values are ordered by their index, NaN above everything.
 //
@@ -143,7 +143,7 @@ __device__ __forceinline__ void finish_row(const TX* __restrict__ row, int V, in
   Stat v = {-INFINITY, 0.0f, 0.0f};
   for (int p = lane; p < nparts; p += 64) v = join(v, parts.stat(p));
   v = wave_join(v);
-  const bool empty = v.m == -INFINITY;
+  const bool empty = v.m == -INFINITY && v.s == 0.0f;      // the maximum passes NaNs over, the sum does not
   const float ls = empty ? 0.0f : logf(v.s);
   const float H = empty ? 0.0f : ls - LN2 * (v.a / v.s);
   if (lane == 0) {

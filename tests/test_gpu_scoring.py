@@ -308,3 +308,32 @@ def test_logits_far_from_zero(order, at):
     assert torch.equal(z.double(), at + step * k.double())
     check(z, ints(4, V, N), 5)
     check_grad(z, ints(4, V, N))
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16, F32])
+@pytest.mark.parametrize("N,V", [(5, 1), (5, 40), (5, 5003), (5, 70001), (600, 40), (515, 5003), (515, 20011)])
+def test_rows_with_nothing_finite(N, V, dtype):
+    """All NaN, and NaN beside nothing but -inf, are NaN in all results and in the gradient; -inf alone is a
+    row with nothing left."""
+    z = randn(V, N, V, dtype=dtype)
+    kinds = torch.arange(N) % 5
+    z[kinds == 0] = float("nan")
+    z[kinds == 1] = -INF
+    z[(kinds == 1).nonzero()[:, 0], V // 2] = float("nan")
+    z[kinds == 2] = -INF
+    z[kinds == 3] = -INF
+    z[(kinds == 3).nonzero()[:, 0], V - 1] = INF
+    t, k = ints(1, V, N), min(4, V)
+    r = token_logprobs(z.to(DEV), t.to(DEV), top_k=k)
+    g = token_logprobs_backward(z.to(DEV), t.to(DEV), r.stats, torch.ones(N, device=DEV), torch.ones(N, device=DEV))
+    for kind in (0, 1, 3):
+        for x in (r.logprob, r.entropy, r.top_logprobs, g):
+            assert bool(torch.isnan(x[kinds == kind]).all()), kind
+    assert bool((r.logprob[kinds == 2] == -INF).all()) and bool((r.entropy[kinds == 2] == 0).all())
+    assert bool((r.top_logprobs[kinds == 2] == -INF).all()) and bool((g[kinds == 2] == 0).all())
+    assert bool(torch.isfinite(g[kinds == 4]).all()) and bool(torch.isfinite(r.logprob[kinds == 4]).all())
+    at = V // 2
+    first = [at] + [i for i in range(k) if i != at]
+    ids = r.top_ids.cpu()
+    for kind, want in ((0, list(range(k))), (1, first[:k]), (2, list(range(k))), (3, ([V - 1] + list(range(k)))[:k])):
+        assert bool((ids[kinds == kind] == torch.tensor(want)).all()), kind

@@ -579,22 +579,20 @@ def packed_moe(x, router, T, D, I, E, gate, up, down, top_k, norm_topk, want_rou
     return y, ids, weights
 
 
-def token_logprobs(logits, targets, N, V, top_k, ignore_index):
-    """(logprob [N], entropy [N], top_ids [N, k], top_logprobs [N, k], stats [N, 3]); see
-    rq_token_logprobs."""
+def token_logprobs(logits, targets, N, V, top_k, ignore_index, lead):
+    """(logprob, entropy, top_ids, top_logprobs, stats) of N = prod(lead) rows: lead, lead, [*lead, k] twice and
+    [*lead, 3], none a view of another (so that each may be edited in place); see rq_token_logprobs."""
     lib = nat.load()
-    dev = logits.device
-    out = torch.empty((5 * N,), dtype=_f32, device=dev)
-    logprob, entropy, stats = out.split_with_sizes((N, N, 3 * N))
-    ids = torch.empty((N, top_k), dtype=torch.int64, device=dev)
-    top = torch.empty((N, top_k), dtype=_f32, device=dev)
+    logprob = logits.new_empty(lead, dtype=_f32)
+    entropy, stats = torch.empty_like(logprob), logprob.new_empty((*lead, 3))
+    ids, top = targets.new_empty((*lead, top_k)), logprob.new_empty((*lead, top_k))
     nbytes = lib.rq_token_logprobs_workspace_bytes(N, V, top_k)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes > 0 else None
-    at = out.data_ptr()
+    ws = logprob.new_empty(nbytes, dtype=torch.uint8) if nbytes > 0 else None
     nat.check("rq_token_logprobs", lib.rq_token_logprobs(
         logits.data_ptr(), nat.DTYPE_CODES[logits.dtype], N, logits.stride(0), V, targets.data_ptr(), ignore_index, top_k,
-        at, at + 4 * N, ids.data_ptr(), top.data_ptr(), at + 8 * N, _addr(ws), nbytes, nat.raw_stream(logits)))
-    return logprob, entropy, ids, top, stats.view(N, 3)
+        logprob.data_ptr(), entropy.data_ptr(), ids.data_ptr(), top.data_ptr(), stats.data_ptr(), _addr(ws), nbytes,
+        nat.raw_stream(logits)))
+    return logprob, entropy, ids, top, stats
 
 
 def token_logprobs_grad(logits, targets, N, V, ignore_index, stats, grad_logprob, grad_entropy=None):

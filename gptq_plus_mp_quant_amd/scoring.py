@@ -54,12 +54,7 @@ def _forward(logits, targets, top_k, ignore_index):
     top_k = int(top_k)
     if not 0 <= top_k <= min(nat.RQ_SCORE_MAX_TOP, V):
         raise ValueError(f"top_k must be 0 to {min(nat.RQ_SCORE_MAX_TOP, V)}, got {top_k}")
-    lp, H, ids, top, stats = K.token_logprobs(z, t, N, V, top_k, int(ignore_index))
-    if logits.dim() != 2:
-        lead = logits.shape[:-1]
-        lp, H = lp.view(lead), H.view(lead)
-        ids, top, stats = ids.view(*lead, top_k), top.view(*lead, top_k), stats.view(*lead, 3)
-    return TokenLogprobs(lp, H, ids, top, stats)
+    return TokenLogprobs(*K.token_logprobs(z, t, N, V, top_k, int(ignore_index), logits.shape[:-1]))
 
 
 class _TokenLogprobs(torch.autograd.Function):

@@ -337,3 +337,24 @@ def test_rows_with_nothing_finite(N, V, dtype):
     ids = r.top_ids.cpu()
     for kind, want in ((0, list(range(k))), (1, first[:k]), (2, list(range(k))), (3, ([V - 1] + list(range(k)))[:k])):
         assert bool((ids[kinds == kind] == torch.tensor(want)).all()), kind
+
+
+@pytest.mark.parametrize("lead", [(6,), (2, 3)])
+def test_results_can_be_edited_in_place(lead):
+    """Masking the log probabilities in place before they are summed, with a gradient as without one."""
+    z, t = randn(16, *lead, 90).to(DEV), ints(17, 90, *lead).to(DEV)
+    keep = (ints(18, 2, *lead) == 1).to(DEV).float()
+    want = token_logprobs(z, t, top_k=2).logprob * keep
+    a, b = z.clone().requires_grad_(), z.clone().requires_grad_()
+    (token_logprobs(a, t).logprob * keep).sum().backward()
+    r = token_logprobs(b, t, top_k=2)
+    r.logprob.mul_(keep)
+    with torch.no_grad():
+        r.entropy.zero_()
+        r.top_logprobs.zero_()
+    assert torch.equal(r.logprob.detach(), want)
+    r.logprob.sum().backward()
+    assert torch.equal(a.grad, b.grad)
+    r = token_logprobs(z, t, top_k=2)
+    r.logprob.mul_(keep)
+    assert torch.equal(r.logprob, want) and bool((r.entropy > 0).all())

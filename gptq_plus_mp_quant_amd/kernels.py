@@ -532,9 +532,10 @@ def _addr(t):
     return None if t is None else t.data_ptr()
 
 
-def packed_linear(x, qweight, nbits, scales, T, R, C, ngroups, g_idx, groupsize=0, bias=None):
-    """y [T, R] = x [T, C] times the transpose of a packed weight, in x's dtype; see rq_packed_linear."""
-    y = x.new_empty((T, R))
+def packed_linear(x, qweight, nbits, scales, T, R, C, ngroups, g_idx, groupsize, bias, lead):
+    """y [*lead, R] = x [T, C] times the transpose of a packed weight, in x's dtype; see rq_packed_linear.  T =
+    prod(lead): the result is made in its final shape, for a view could not be edited in place under autograd."""
+    y = x.new_empty((*lead, R))
     nat.check("rq_packed_linear", nat.load().rq_packed_linear(
         x.data_ptr(), nat.DTYPE_CODES[x.dtype], T, x.stride(0), C, qweight.data_ptr(), qweight.stride(0), nbits, R,
         scales.data_ptr(), scales.stride(0), ngroups, g_idx.data_ptr(), groupsize, _addr(bias), y.data_ptr(), R,
@@ -542,10 +543,10 @@ def packed_linear(x, qweight, nbits, scales, T, R, C, ngroups, g_idx, groupsize=
     return y
 
 
-def packed_linear_grad(grad_y, qweight, nbits, scales, T, R, C, ngroups, g_idx, groupsize=0):
-    """grad_x [T, C] = grad_y [T, R] times a packed weight; see rq_packed_linear_grad."""
+def packed_linear_grad(grad_y, qweight, nbits, scales, T, R, C, ngroups, g_idx, groupsize, lead):
+    """grad_x [*lead, C] = grad_y [T, R] times a packed weight, T = prod(lead); see rq_packed_linear_grad."""
     lib = nat.load()
-    gx = grad_y.new_empty((T, C))
+    gx = grad_y.new_empty((*lead, C))
     nbytes = lib.rq_packed_linear_grad_workspace_bytes(T, R, C)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=grad_y.device)
     nat.check("rq_packed_linear_grad", lib.rq_packed_linear_grad(

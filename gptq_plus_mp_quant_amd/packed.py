@@ -103,8 +103,7 @@ def _forward(x, entry, bias):
         if bias.dtype != x.dtype or bias.shape != (R,) or bias.device != x.device:
             raise ValueError(f"bias must be {x.dtype} [{R}] on {x.device}")
         bias = bias.contiguous()
-    y = K.packed_linear(x2, q, nbits, scales, T, R, C, ng, g_idx, groupsize, bias)
-    return y if x.dim() == 2 else y.view(*x.shape[:-1], R)
+    return K.packed_linear(x2, q, nbits, scales, T, R, C, ng, g_idx, groupsize, bias, x.shape[:-1])
 
 
 def packed_linear(x: torch.Tensor, entry: Dict[str, object], bias: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -125,8 +124,7 @@ def packed_linear_backward(grad_y: torch.Tensor, entry: Dict[str, object]) -> to
     grad_y's dtype.  The result does not change from run to run."""
     q, nbits, scales, R, C, ng, g_idx, groupsize = _checked(entry, 0)
     g2, T = _tokens(grad_y, R, q, "grad_y")
-    gx = K.packed_linear_grad(g2, q, nbits, scales, T, R, C, ng, g_idx, groupsize)
-    return gx if grad_y.dim() == 2 else gx.view(*grad_y.shape[:-1], C)
+    return K.packed_linear_grad(g2, q, nbits, scales, T, R, C, ng, g_idx, groupsize, grad_y.shape[:-1])
 
 
 def stack_packed(entries: Sequence[Dict[str, object]]) -> Dict[str, object]:

@@ -602,3 +602,18 @@ def test_moe_activation_keeps_32_bits(I, groups, T, dtype):
     want, mag = (Wd @ h)[:, :, 0], (Wd.abs() @ h.abs())[:, :, 0]
     assert float(mag.max()) > 0.1 and float(want.abs().max()) <= 1e-12 * float(mag.max())
     assert_within(y, torch.zeros_like(want), 13 * 2.0 ** -24 * mag + TINY[dtype], "y")
+
+
+@pytest.mark.parametrize("lead", [(), (5,), (2, 3), (2, 1, 2)])
+def test_results_can_be_edited_in_place(lead):
+    """A residual added in place, whatever the leading dimensions, with a gradient as without one."""
+    entry, _ = make_entry(4, 24, 64, 4, "32")
+    e, x, res = on(entry, DEV), randn(1, *lead, 64).to(DEV), randn(2, *lead, 24).to(DEV)
+    leaf = x.clone().requires_grad_()
+    y = packed_linear(leaf, e)
+    y += res
+    y.sum().backward()
+    plain = packed_linear(x, e)
+    plain += res
+    assert torch.equal(y.detach(), plain) and y.shape == (*lead, 24)
+    assert torch.equal(leaf.grad, packed_linear_backward(torch.ones_like(plain), e)) and leaf.grad.shape == x.shape

@@ -12,6 +12,7 @@ import re
 from pathlib import Path
 
 import torch
+from torch.autograd import forward_ad
 
 LIB_PATH = Path(os.environ.get("GPTQPLUS_HIP_LIB") or
                 Path(__file__).resolve().parent / "_lib" / "libgptqplus_hip.so").resolve()
@@ -146,6 +147,15 @@ def raw_stream(t):
 def check(name, rc):
     if rc != RQ_OK:
         raise RuntimeError(f"{name} failed with status {rc}")
+
+
+def refuse_tangents(what, *tensors):
+    """The kernels carry no forward-mode tangents on: a tensor with one is refused, not stripped of it."""
+    if getattr(forward_ad, "_current_level", 0) < 0:     # no level is open (spares the calls on one token the rest)
+        return
+    for t in tensors:
+        if isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None:
+            raise NotImplementedError(f"{what} has no forward-mode derivative: call it on tensors without tangents")
 
 
 DTYPE_CODES = {torch.float16: RQ_F16, torch.bfloat16: RQ_BF16, torch.float32: RQ_F32}

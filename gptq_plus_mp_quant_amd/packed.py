@@ -110,7 +110,8 @@ def packed_linear(x: torch.Tensor, entry: Dict[str, object], bias: Optional[torc
     """``x [..., C]`` times the transpose of a packed weight, ``[..., R]`` in x's dtype (fp16, bf16 or
     fp32); ``bias`` [R] of the same dtype is added before the rounding.  Any number of tokens; the
     kernels are made for few (a decoding step, a short prompt).  Differentiable in ``x``; the weight
-    and the bias are constants (a bias that requires grad is refused)."""
+    and the bias are constants (a bias that requires grad is refused).  Forward-mode tangents are refused."""
+    nat.refuse_tangents("packed_linear", x, bias, entry["scales"])
     if torch.is_grad_enabled():
         if bias is not None and bias.requires_grad:
             raise ValueError("packed_linear: the bias of a packed linear is a constant; detach it")
@@ -122,6 +123,7 @@ def packed_linear(x: torch.Tensor, entry: Dict[str, object], bias: Optional[torc
 def packed_linear_backward(grad_y: torch.Tensor, entry: Dict[str, object]) -> torch.Tensor:
     """The gradient of ``packed_linear``'s x: ``grad_y [..., R]`` times the packed weight, ``[..., C]`` in
     grad_y's dtype.  The result does not change from run to run."""
+    nat.refuse_tangents("packed_linear_backward", grad_y, entry["scales"])
     q, nbits, scales, R, C, ng, g_idx, groupsize = _checked(entry, 0)
     g2, T = _tokens(grad_y, R, q, "grad_y")
     return K.packed_linear_grad(g2, q, nbits, scales, T, R, C, ng, g_idx, groupsize, grad_y.shape[:-1])
@@ -156,7 +158,8 @@ def packed_moe(x: torch.Tensor, router: torch.Tensor, gate: Dict[str, object], u
     with ``norm_topk``; an expert is ``down(silu(gate(x)) * up(x))``.  ``gate`` / ``up`` (I x D) and ``down``
     (D x I) are stacked entries, each with bits and groups of its own.  ``return_routing`` adds the
     chosen ids (int32) and weights (fp32), ``[..., top_k]``.  At most 1024 experts, 64 chosen.  It has
-    no backward pass: an x that requires grad is refused."""
+    no backward pass: an x that requires grad is refused, and forward-mode tangents are."""
+    nat.refuse_tangents("packed_moe", x, router, gate["scales"], up["scales"], down["scales"])
     if torch.is_grad_enabled() and isinstance(x, torch.Tensor) and (x.requires_grad or router.requires_grad):
         raise NotImplementedError("packed_moe has no backward pass: call it under torch.no_grad() or on detached tensors")
     g, u, d = _checked(gate, 1), _checked(up, 1), _checked(down, 1)

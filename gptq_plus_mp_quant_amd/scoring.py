@@ -80,7 +80,8 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, top_k: int = 0, 
     ``top_k`` (0 to 64) alternatives are ordered by their logit, equal ones by their index.  Masked
     logits (-inf, or the type's lowest value) have probability 0; a row with nothing but -inf has
     logprob -inf, entropy 0 and no gradient; a row with a NaN or +inf is NaN.  ``logprob`` and
-    ``entropy`` are differentiable in ``logits``, ``top_logprobs`` is not."""
+    ``entropy`` are differentiable in ``logits``, ``top_logprobs`` is not; forward-mode tangents are refused."""
+    nat.refuse_tangents("token_logprobs", logits)
     if torch.is_grad_enabled() and isinstance(logits, torch.Tensor) and logits.requires_grad:
         return TokenLogprobs(*_TokenLogprobs.apply(logits, targets, top_k, ignore_index))
     return _forward(logits, targets, top_k, ignore_index)
@@ -97,6 +98,7 @@ def token_logprobs_backward(logits: torch.Tensor, targets: torch.Tensor, stats: 
                             grad_entropy: Optional[torch.Tensor] = None, ignore_index: int = -100) -> torch.Tensor:
     """The gradient of ``logits`` from the gradients of ``logprob`` and (optionally) ``entropy``, in the
     logits' dtype; ``stats`` is what ``token_logprobs`` returned for the same logits."""
+    nat.refuse_tangents("token_logprobs_backward", logits, stats, grad_logprob, grad_entropy)
     z, t, N, V = _rows(logits, targets)
     gl = _row_grads(grad_logprob, logits, "grad_logprob")
     gh = None if grad_entropy is None else _row_grads(grad_entropy, logits, "grad_entropy")

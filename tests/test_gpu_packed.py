@@ -617,3 +617,24 @@ def test_results_can_be_edited_in_place(lead):
     plain += res
     assert torch.equal(y.detach(), plain) and y.shape == (*lead, 24)
     assert torch.equal(leaf.grad, packed_linear_backward(torch.ones_like(plain), e)) and leaf.grad.shape == x.shape
+
+
+def test_forward_mode_is_refused():
+    """A tangent, which no kernel carries on, is an error, not a result without it."""
+    from torch.autograd import forward_ad
+    entry, _ = make_entry(3, 32, 64, 4, "32")
+    e = on(entry, DEV)
+    x, g = randn(1, 2, 64).to(DEV), randn(2, 2, 32).to(DEV)
+    xm, router, parts = moe_case(1, 2, 64, 32, 4, F32)
+    xm, router, parts = xm.to(DEV), router.to(DEV), [on(p, DEV) for p, _ in parts]
+    with forward_ad.dual_level():
+        def dual(t):
+            return forward_ad.make_dual(t, torch.ones_like(t))
+
+        for call in (lambda: packed_linear(dual(x), e), lambda: packed_linear(x, e, bias=dual(g[0])),
+                     lambda: packed_linear(x, {**e, "scales": dual(e["scales"])}),
+                     lambda: packed_linear_backward(dual(g), e), lambda: packed_moe(dual(xm), router, *parts, 2),
+                     lambda: packed_moe(xm, dual(router), *parts, 2)):
+            with pytest.raises(NotImplementedError):
+                call()
+        assert packed_linear(x, e).shape == (2, 32)          # a level alone changes nothing

@@ -358,3 +358,20 @@ def test_results_can_be_edited_in_place(lead):
     r = token_logprobs(z, t, top_k=2)
     r.logprob.mul_(keep)
     assert torch.equal(r.logprob, want) and bool((r.entropy > 0).all())
+
+
+def test_forward_mode_is_refused():
+    """A tangent, which no kernel carries on, is an error, not a result without it."""
+    from torch.autograd import forward_ad
+    z, t, g = randn(1, 3, 50).to(DEV), ints(2, 50, 3).to(DEV), randn(3, 3).to(DEV)
+    stats = token_logprobs(z, t).stats
+    with forward_ad.dual_level():
+        def dual(x):
+            return forward_ad.make_dual(x, torch.ones_like(x))
+
+        for call in (lambda: token_logprobs(dual(z), t), lambda: token_logprobs_backward(dual(z), t, stats, g),
+                     lambda: token_logprobs_backward(z, t, dual(stats), g), lambda: token_logprobs_backward(z, t, stats, dual(g)),
+                     lambda: token_logprobs_backward(z, t, stats, g, dual(g))):
+            with pytest.raises(NotImplementedError):
+                call()
+        token_logprobs(z, t)                                 # a level alone changes nothing

@@ -584,7 +584,7 @@ def token_logprobs(logits, targets, N, V, top_k, ignore_index, lead):
     """(logprob, entropy, top_ids, top_logprobs, stats) of N = prod(lead) rows: lead, lead, [*lead, k] twice and
     [*lead, 3], none a view of another (so that each may be edited in place); see rq_token_logprobs."""
     lib = nat.load()
-    logprob = logits.new_empty(lead, dtype=_f32)
+    logprob = logits.new_empty((*lead,), dtype=_f32)
     entropy, stats = torch.empty_like(logprob), logprob.new_empty((*lead, 3))
     ids, top = targets.new_empty((*lead, top_k)), logprob.new_empty((*lead, top_k))
     nbytes = lib.rq_token_logprobs_workspace_bytes(N, V, top_k)
@@ -596,9 +596,9 @@ def token_logprobs(logits, targets, N, V, top_k, ignore_index, lead):
     return logprob, entropy, ids, top, stats
 
 
-def token_logprobs_grad(logits, targets, N, V, ignore_index, stats, grad_logprob, grad_entropy=None):
-    """grad_logits [N, V] in the logits' dtype; see rq_token_logprobs_grad."""
-    gz = logits.new_empty((N, V))
+def token_logprobs_grad(logits, targets, N, V, ignore_index, stats, grad_logprob, grad_entropy, lead):
+    """grad_logits [*lead, V], N = prod(lead), in the logits' dtype; see rq_token_logprobs_grad."""
+    gz = logits.new_empty((*lead, V))
     nat.check("rq_token_logprobs_grad", nat.load().rq_token_logprobs_grad(
         logits.data_ptr(), nat.DTYPE_CODES[logits.dtype], N, logits.stride(0), V, targets.data_ptr(), ignore_index,
         stats.data_ptr(), grad_logprob.data_ptr(), _addr(grad_entropy), gz.data_ptr(), V, nat.raw_stream(logits)))

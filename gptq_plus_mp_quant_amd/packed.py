@@ -93,7 +93,7 @@ class _PackedLinear(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, grad_y):
-        return packed_linear_backward(grad_y, ctx.entry), None, None
+        return _backward(grad_y, ctx.entry), None, None
 
 
 def _forward(x, entry, bias):
@@ -120,13 +120,31 @@ def packed_linear(x: torch.Tensor, entry: Dict[str, object], bias: Optional[torc
     return _forward(x, entry, bias)
 
 
-def packed_linear_backward(grad_y: torch.Tensor, entry: Dict[str, object]) -> torch.Tensor:
-    """The gradient of ``packed_linear``'s x: ``grad_y [..., R]`` times the packed weight, ``[..., C]`` in
-    grad_y's dtype.  The result does not change from run to run."""
-    nat.refuse_tangents("packed_linear_backward", grad_y, entry["scales"])
+class _PackedLinearGrad(torch.autograd.Function):
+    """The gradient of a grad_y that requires grad: no constant, so a derivative of it is refused."""
+    @staticmethod
+    def forward(ctx, grad_y, entry):
+        return _backward(grad_y, entry)
+
+    @staticmethod
+    def backward(ctx, _):
+        raise NotImplementedError("packed_linear_backward has no backward pass: call it under torch.no_grad() or on "
+                                  "detached tensors")
+
+
+def _backward(grad_y, entry):
     q, nbits, scales, R, C, ng, g_idx, groupsize = _checked(entry, 0)
     g2, T = _tokens(grad_y, R, q, "grad_y")
     return K.packed_linear_grad(g2, q, nbits, scales, T, R, C, ng, g_idx, groupsize, grad_y.shape[:-1])
+
+
+def packed_linear_backward(grad_y: torch.Tensor, entry: Dict[str, object]) -> torch.Tensor:
+    """The gradient of ``packed_linear``'s x: ``grad_y [..., R]`` times the packed weight, ``[..., C]`` in
+    grad_y's dtype.  The result does not change from run to run.  It cannot be differentiated further."""
+    nat.refuse_tangents("packed_linear_backward", grad_y, entry["scales"])
+    if torch.is_grad_enabled() and isinstance(grad_y, torch.Tensor) and grad_y.requires_grad:
+        return _PackedLinearGrad.apply(grad_y, entry)
+    return _backward(grad_y, entry)
 
 
 def stack_packed(entries: Sequence[Dict[str, object]]) -> Dict[str, object]:

@@ -70,7 +70,7 @@ class _TokenLogprobs(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, grad_logprob, grad_entropy, *_):
         logits, targets, stats = ctx.saved_tensors
-        return token_logprobs_backward(logits, targets, stats, grad_logprob, grad_entropy, ctx.ignore_index), None, None, None
+        return _backward(logits, targets, stats, grad_logprob, grad_entropy, ctx.ignore_index), None, None, None
 
 
 def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, top_k: int = 0, ignore_index: int = -100) -> TokenLogprobs:
@@ -94,17 +94,37 @@ def _row_grads(g, like, name):
     return g if g.is_contiguous() else g.contiguous()
 
 
-def token_logprobs_backward(logits: torch.Tensor, targets: torch.Tensor, stats: torch.Tensor, grad_logprob: torch.Tensor,
-                            grad_entropy: Optional[torch.Tensor] = None, ignore_index: int = -100) -> torch.Tensor:
-    """The gradient of ``logits`` from the gradients of ``logprob`` and (optionally) ``entropy``, in the
-    logits' dtype; ``stats`` is what ``token_logprobs`` returned for the same logits."""
-    nat.refuse_tangents("token_logprobs_backward", logits, stats, grad_logprob, grad_entropy)
+class _TokenLogprobsGrad(torch.autograd.Function):
+    """The gradient from inputs that require grad: no constant, so a derivative of it is refused."""
+    @staticmethod
+    def forward(ctx, *args):
+        return _backward(*args)
+
+    @staticmethod
+    def backward(ctx, _):
+        raise NotImplementedError("token_logprobs_backward has no backward pass: call it under torch.no_grad() or on "
+                                  "detached tensors")
+
+
+def _backward(logits, targets, stats, grad_logprob, grad_entropy, ignore_index):
     z, t, N, V = _rows(logits, targets)
     gl = _row_grads(grad_logprob, logits, "grad_logprob")
     gh = None if grad_entropy is None else _row_grads(grad_entropy, logits, "grad_entropy")
     if not isinstance(stats, torch.Tensor) or stats.dtype != torch.float32 or stats.shape != (*logits.shape[:-1], 3) or \
             stats.device != logits.device:
         raise ValueError(f"stats must be token_logprobs' float32 {list(logits.shape[:-1]) + [3]} on {logits.device}")
-    gz = K.token_logprobs_grad(z, t, N, V, int(ignore_index), stats if stats.is_contiguous() else stats.contiguous(), gl,
-                               gh)
-    return gz if logits.dim() == 2 else gz.view(logits.shape)
+    return K.token_logprobs_grad(z, t, N, V, int(ignore_index), stats if stats.is_contiguous() else stats.contiguous(), gl,
+                                 gh, logits.shape[:-1])
+
+
+def token_logprobs_backward(logits: torch.Tensor, targets: torch.Tensor, stats: torch.Tensor, grad_logprob: torch.Tensor,
+                            grad_entropy: Optional[torch.Tensor] = None, ignore_index: int = -100) -> torch.Tensor:
+    """The gradient of ``logits`` from the gradients of ``logprob`` and (optionally) ``entropy``, in the
+    logits' dtype; ``stats`` is what ``token_logprobs`` returned for the same logits.  It cannot be
+    differentiated further."""
+    nat.refuse_tangents("token_logprobs_backward", logits, stats, grad_logprob, grad_entropy)
+    if torch.is_grad_enabled():
+        for t in (logits, stats, grad_logprob, grad_entropy):
+            if getattr(t, "requires_grad", False):
+                return _TokenLogprobsGrad.apply(logits, targets, stats, grad_logprob, grad_entropy, ignore_index)
+    return _backward(logits, targets, stats, grad_logprob, grad_entropy, ignore_index)

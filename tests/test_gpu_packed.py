@@ -638,3 +638,17 @@ def test_forward_mode_is_refused():
             with pytest.raises(NotImplementedError):
                 call()
         assert packed_linear(x, e).shape == (2, 32)          # a level alone changes nothing
+
+
+def test_gradient_of_the_gradient_call_is_refused():
+    """What packed_linear_backward returns for a grad_y that requires grad is no constant: a gradient through it is
+    an error, as it is through the gradient that autograd takes."""
+    entry, _ = make_entry(3, 32, 64, 4, "32")
+    e, g = on(entry, DEV), randn(2, 2, 32).to(DEV)
+    leaf = g.clone().requires_grad_()
+    gx = packed_linear_backward(leaf, e)
+    assert torch.equal(gx.detach(), packed_linear_backward(g, e)) and gx.requires_grad
+    with pytest.raises(RuntimeError):
+        gx.sum().backward()
+    with torch.no_grad():
+        assert not packed_linear_backward(leaf, e).requires_grad

@@ -375,3 +375,20 @@ def test_forward_mode_is_refused():
             with pytest.raises(NotImplementedError):
                 call()
         token_logprobs(z, t)                                 # a level alone changes nothing
+
+
+def test_gradient_of_the_gradient_call_is_refused():
+    """What token_logprobs_backward returns for inputs that require grad is no constant: a gradient through it is an
+    error, as it is through the gradient that autograd takes."""
+    z, t, g = randn(1, 3, 50).to(DEV), ints(2, 50, 3).to(DEV), randn(3, 3).to(DEV)
+    stats = token_logprobs(z, t).stats
+    want = token_logprobs_backward(z, t, stats, g, g)
+    for k in range(3):
+        args = [z, stats, g]
+        args[k] = args[k].clone().requires_grad_()
+        gz = token_logprobs_backward(args[0], t, args[1], args[2], g)
+        assert torch.equal(gz.detach(), want) and gz.requires_grad
+        with pytest.raises(RuntimeError):
+            gz.sum().backward()
+        with torch.no_grad():
+            assert not token_logprobs_backward(args[0], t, args[1], args[2], g).requires_grad

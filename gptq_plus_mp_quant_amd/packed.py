@@ -87,13 +87,20 @@ def _tokens(x, width, q, name):
 class _PackedLinear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, entry, bias):
-        ctx.entry = entry
-        return _forward(x, entry, bias)
+        y = _forward(x, entry, bias)
+        # the tensors, not the dict: the gradient goes through the weight of this call.  Tensors made in inference
+        # mode cannot be saved (nor changed outside of it).
+        weight = entry["qweight"], entry["scales"], entry["g_idx"]
+        ctx.unsaved = weight if any(t.is_inference() for t in weight) else None
+        ctx.save_for_backward(*(() if ctx.unsaved else weight))
+        ctx.fields = dict(nbits=entry["nbits"], groupsize=entry.get("groupsize", 0))
+        return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad_y):
-        return _backward(grad_y, ctx.entry), None, None
+        q, scales, g_idx = ctx.unsaved or ctx.saved_tensors
+        return _backward(grad_y, dict(qweight=q, scales=scales, g_idx=g_idx, **ctx.fields)), None, None
 
 
 def _forward(x, entry, bias):

@@ -652,3 +652,26 @@ def test_gradient_of_the_gradient_call_is_refused():
         gx.sum().backward()
     with torch.no_grad():
         assert not packed_linear_backward(leaf, e).requires_grad
+
+
+def test_weight_is_what_forward_saw():
+    """The gradient goes through the weight that the product was taken with: an entry whose tensors are
+    exchanged in between does not matter, one changed in place is an error."""
+    entry, _ = make_entry(3, 32, 64, 4, "32")
+    other, _ = make_entry(5, 32, 64, 5, "64")
+    e = on(entry, DEV)
+    x, g = randn(1, 2, 64).to(DEV).requires_grad_(), randn(2, 2, 32).to(DEV)
+    y = packed_linear(x, e)
+    want = packed_linear_backward(g, e)
+    e.update(on(other, DEV))
+    assert torch.equal(torch.autograd.grad(y, x, g)[0], want)
+    e = on(entry, DEV)
+    for name in ("qweight", "scales", "g_idx"):
+        y = packed_linear(x, e)
+        e[name].mul_(1)
+        with pytest.raises(RuntimeError):
+            y.backward(g)
+    with torch.inference_mode():
+        e = on(entry, DEV)
+        inferred = {k: v.clone() if isinstance(v, torch.Tensor) else v for k, v in e.items()}
+    assert torch.equal(torch.autograd.grad(packed_linear(x, inferred), x, g)[0], want)

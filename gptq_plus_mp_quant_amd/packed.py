@@ -62,6 +62,13 @@ def _checked(entry: Dict[str, object], batch: int):
             g_idx if g_idx.is_contiguous() else g_idx.contiguous(), groupsize)
 
 
+def _constant(name, *entries):
+    """Under autograd, scales that require grad are refused: they would get none."""
+    for e in entries:
+        if getattr(e["scales"], "requires_grad", False):
+            raise ValueError(f"{name}: the scales of a packed weight are constants; detach them")
+
+
 def _tokens(x, width, q, name):
     """x as [T, width] with unit column stride (copied only if its strides need it), and T."""
     if not (isinstance(x, torch.Tensor) and x.is_cuda):
@@ -117,10 +124,12 @@ def packed_linear(x: torch.Tensor, entry: Dict[str, object], bias: Optional[torc
     """``x [..., C]`` times the transpose of a packed weight, ``[..., R]`` in x's dtype (fp16, bf16 or
     fp32); ``bias`` [R] of the same dtype is added before the rounding.  Any number of tokens; the
     kernels are made for few (a decoding step, a short prompt).  Differentiable in ``x``; the weight
-    and the bias are constants (a bias that requires grad is refused).  Forward-mode tangents are refused."""
+    and the bias are constants (scales or a bias that require grad are refused).  Forward-mode tangents are
+    refused."""
     nat.refuse_tangents("packed_linear", x, bias, entry["scales"])
     if torch.is_grad_enabled():
-        if bias is not None and bias.requires_grad:
+        _constant("packed_linear", entry)
+        if getattr(bias, "requires_grad", False):
             raise ValueError("packed_linear: the bias of a packed linear is a constant; detach it")
         if isinstance(x, torch.Tensor) and x.requires_grad:
             return _PackedLinear.apply(x, entry, bias)
@@ -149,8 +158,10 @@ def packed_linear_backward(grad_y: torch.Tensor, entry: Dict[str, object]) -> to
     """The gradient of ``packed_linear``'s x: ``grad_y [..., R]`` times the packed weight, ``[..., C]`` in
     grad_y's dtype.  The result does not change from run to run.  It cannot be differentiated further."""
     nat.refuse_tangents("packed_linear_backward", grad_y, entry["scales"])
-    if torch.is_grad_enabled() and isinstance(grad_y, torch.Tensor) and grad_y.requires_grad:
-        return _PackedLinearGrad.apply(grad_y, entry)
+    if torch.is_grad_enabled():
+        _constant("packed_linear_backward", entry)
+        if isinstance(grad_y, torch.Tensor) and grad_y.requires_grad:
+            return _PackedLinearGrad.apply(grad_y, entry)
     return _backward(grad_y, entry)
 
 
@@ -185,8 +196,10 @@ def packed_moe(x: torch.Tensor, router: torch.Tensor, gate: Dict[str, object], u
     chosen ids (int32) and weights (fp32), ``[..., top_k]``.  At most 1024 experts, 64 chosen.  It has
     no backward pass: an x that requires grad is refused, and forward-mode tangents are."""
     nat.refuse_tangents("packed_moe", x, router, gate["scales"], up["scales"], down["scales"])
-    if torch.is_grad_enabled() and isinstance(x, torch.Tensor) and (x.requires_grad or router.requires_grad):
-        raise NotImplementedError("packed_moe has no backward pass: call it under torch.no_grad() or on detached tensors")
+    if torch.is_grad_enabled():
+        _constant("packed_moe", gate, up, down)
+        if isinstance(x, torch.Tensor) and (x.requires_grad or router.requires_grad):
+            raise NotImplementedError("packed_moe has no backward pass: call it under torch.no_grad() or on detached tensors")
     g, u, d = _checked(gate, 1), _checked(up, 1), _checked(down, 1)
     E, I, D = g[0].shape[0], g[3], g[4]
     if u[0].shape[0] != E or d[0].shape[0] != E or u[3] != I or u[4] != D or d[3] != D or d[4] != I:

@@ -675,3 +675,25 @@ def test_weight_is_what_forward_saw():
         e = on(entry, DEV)
         inferred = {k: v.clone() if isinstance(v, torch.Tensor) else v for k, v in e.items()}
     assert torch.equal(torch.autograd.grad(packed_linear(x, inferred), x, g)[0], want)
+
+
+def test_scales_that_require_grad_are_refused():
+    """They would get none, as a bias would."""
+    entry, _ = make_entry(3, 32, 64, 4, "32")
+    e = on(entry, DEV)
+    e["scales"].requires_grad_()
+    x, g = randn(1, 2, 64).to(DEV), randn(2, 2, 32).to(DEV)
+    xm, router, parts = moe_case(1, 2, 64, 32, 4, F32)
+    xm, router, parts = xm.to(DEV), router.to(DEV), [on(p, DEV) for p, _ in parts]
+    for call in (lambda: packed_linear(x, e), lambda: packed_linear(x.clone().requires_grad_(), e), lambda: packed_linear_backward(g, e)):
+        with pytest.raises(ValueError):
+            call()
+    for k in range(3):
+        changed = list(parts)
+        changed[k] = {**parts[k], "scales": parts[k]["scales"].clone().requires_grad_()}
+        with pytest.raises(ValueError):
+            packed_moe(xm, router, *changed, 2)
+        with torch.no_grad():
+            assert torch.equal(packed_moe(xm, router, *changed, 2), packed_moe(xm, router, *parts, 2))
+    with torch.no_grad():
+        assert packed_linear(x, e).shape == (2, 32)

@@ -114,7 +114,7 @@ def _forward(x, entry, bias):
     q, nbits, scales, R, C, ng, g_idx, groupsize = _checked(entry, 0)
     x2, T = _tokens(x, C, q, "x")
     if bias is not None:
-        if bias.dtype != x.dtype or bias.shape != (R,) or bias.device != x.device:
+        if not isinstance(bias, torch.Tensor) or bias.dtype != x.dtype or bias.shape != (R,) or bias.device != x.device:
             raise ValueError(f"bias must be {x.dtype} [{R}] on {x.device}")
         bias = bias.contiguous()
     return K.packed_linear(x2, q, nbits, scales, T, R, C, ng, g_idx, groupsize, bias, x.shape[:-1])
@@ -198,7 +198,7 @@ def packed_moe(x: torch.Tensor, router: torch.Tensor, gate: Dict[str, object], u
     nat.refuse_tangents("packed_moe", x, router, gate["scales"], up["scales"], down["scales"])
     if torch.is_grad_enabled():
         _constant("packed_moe", gate, up, down)
-        if isinstance(x, torch.Tensor) and (x.requires_grad or router.requires_grad):
+        if getattr(x, "requires_grad", False) or getattr(router, "requires_grad", False):
             raise NotImplementedError("packed_moe has no backward pass: call it under torch.no_grad() or on detached tensors")
     g, u, d = _checked(gate, 1), _checked(up, 1), _checked(down, 1)
     E, I, D = g[0].shape[0], g[3], g[4]

@@ -144,3 +144,13 @@ def test_cpu_tensors_are_refused():
         G.stack_packed([e])
     with pytest.raises(RuntimeError):
         G.token_logprobs(torch.zeros(2, 8), torch.zeros(2, dtype=torch.int64))
+
+
+def test_operands_that_are_no_tensors_are_refused():
+    """With the errors that wrong tensors get, not an AttributeError."""
+    e, _ = make_entry(0, 16, 64, 4, "32")
+    for call in (lambda: G.packed_linear([0.0] * 64, e), lambda: G.packed_linear_backward([0.0] * 16, e),
+                 lambda: G.packed_moe(torch.zeros(1, 64), None, e, e, e, 1),
+                 lambda: G.token_logprobs_backward(None, None, None, None)):
+        with pytest.raises((RuntimeError, ValueError, TypeError)):
+            call()

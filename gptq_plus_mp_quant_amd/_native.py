@@ -7,6 +7,7 @@ another build of the same library to load instead (e.g. a variant built for an A
 from __future__ import annotations
 
 import ctypes
+import functools
 import os
 import re
 from pathlib import Path
@@ -115,11 +116,39 @@ def load():
     return lib
 
 
-def call(name, *args):
-    rc = getattr(load(), name)(*args)
+class Stream(ctypes.c_void_p):
+    """A ``hipStream_t`` and the index of its device."""
+    index = None
+
+
+def check(name, rc):
     if rc != RQ_OK:
         raise RuntimeError(f"{name} failed with status {rc}")
     return rc
+
+
+def call(name, *args):
+    """An entry point, on the device of the stream that is its last argument (if it takes one): a kernel goes to
+    the current device, and a default stream's handle names none."""
+    fn = getattr(load(), name)
+    index = args[-1].index if args and isinstance(args[-1], Stream) else None
+    if index is None or index == _current_device():
+        return check(name, fn(*args))
+    with torch.cuda.device(index):
+        return check(name, fn(*args))
+
+
+def on_device_of_first(fn):
+    """fn(tensor, ...) with the tensor's device current, as ``call`` has it, for functions that call entry points
+    themselves."""
+    @functools.wraps(fn)
+    def run(t, *args):
+        index = t.get_device()
+        if index == _current_device():
+            return fn(t, *args)
+        with torch.cuda.device(index):
+            return fn(t, *args)
+    return run
 
 
 def ptr(t):
@@ -128,12 +157,17 @@ def ptr(t):
 
 
 def stream_of(device):
-    return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
+    s = torch.cuda.current_stream(device)
+    out = Stream(s.cuda_stream)
+    out.index = s.device.index
+    return out
 
 
 try:
-    from torch._C import _cuda_getCurrentRawStream as _raw_stream_of
-except ImportError:                                  # a torch without the shortcut
+    from torch._C import _cuda_getCurrentRawStream as _raw_stream_of, _cuda_getDevice as _current_device
+except ImportError:                                  # a torch without the shortcuts
+    _current_device = torch.cuda.current_device
+
     def _raw_stream_of(index):
         return torch.cuda.current_stream(index).cuda_stream
 
@@ -142,11 +176,6 @@ def raw_stream(t):
     """The current stream of a GPU tensor's device as an int, without making a Stream object (the
     calls on single tokens, whose kernels take a few microseconds, are bound by the host)."""
     return _raw_stream_of(t.get_device())
-
-
-def check(name, rc):
-    if rc != RQ_OK:
-        raise RuntimeError(f"{name} failed with status {rc}")
 
 
 def refuse_tangents(what, *tensors):

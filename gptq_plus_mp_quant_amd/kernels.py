@@ -532,6 +532,7 @@ def _addr(t):
     return None if t is None else t.data_ptr()
 
 
+@nat.on_device_of_first
 def packed_linear(x, qweight, nbits, scales, T, R, C, ngroups, g_idx, groupsize, bias, lead):
     """y [*lead, R] = x [T, C] times the transpose of a packed weight, in x's dtype; see rq_packed_linear.  T =
     prod(lead): the result is made in its final shape, for a view could not be edited in place under autograd."""
@@ -543,6 +544,7 @@ def packed_linear(x, qweight, nbits, scales, T, R, C, ngroups, g_idx, groupsize,
     return y
 
 
+@nat.on_device_of_first
 def packed_linear_grad(grad_y, qweight, nbits, scales, T, R, C, ngroups, g_idx, groupsize, lead):
     """grad_x [*lead, C] = grad_y [T, R] times a packed weight, T = prod(lead); see rq_packed_linear_grad."""
     lib = nat.load()
@@ -563,6 +565,7 @@ def _experts(qweight, nbits, scales, ngroups, g_idx, groupsize):
                              groupsize)
 
 
+@nat.on_device_of_first
 def packed_moe(x, router, T, D, I, E, gate, up, down, top_k, norm_topk, want_routing=False):
     """y [T, D] of a mixture-of-experts layer (and the chosen experts' int32 ids and fp32 weights
     [T, top_k]); gate / up / down: (qweight [E, R, words], nbits, scales [E, ngroups, R], ngroups,
@@ -580,6 +583,7 @@ def packed_moe(x, router, T, D, I, E, gate, up, down, top_k, norm_topk, want_rou
     return y, ids, weights
 
 
+@nat.on_device_of_first
 def token_logprobs(logits, targets, N, V, top_k, ignore_index, lead):
     """(logprob, entropy, top_ids, top_logprobs, stats) of N = prod(lead) rows: lead, lead, [*lead, k] twice and
     [*lead, 3], none a view of another (so that each may be edited in place); see rq_token_logprobs."""
@@ -596,6 +600,7 @@ def token_logprobs(logits, targets, N, V, top_k, ignore_index, lead):
     return logprob, entropy, ids, top, stats
 
 
+@nat.on_device_of_first
 def token_logprobs_grad(logits, targets, N, V, ignore_index, stats, grad_logprob, grad_entropy, lead):
     """grad_logits [*lead, V], N = prod(lead), in the logits' dtype; see rq_token_logprobs_grad."""
     gz = logits.new_empty((*lead, V))

@@ -7,6 +7,7 @@ import torch
 
 import gptq_plus_mp_quant_amd as G
 from gptq_plus_mp_quant_amd import _native as nat
+from gptq_plus_mp_quant_amd import kernels as K
 from tests._packed import make_entry
 
 FAKE, NULL = 16, None
@@ -154,3 +155,62 @@ def test_operands_that_are_no_tensors_are_refused():
                  lambda: G.token_logprobs_backward(None, None, None, None)):
         with pytest.raises((RuntimeError, ValueError, TypeError)):
             call()
+
+
+@pytest.fixture
+def two_devices(monkeypatch):
+    """A library that records the current device of every call, on a host with device 0 current of two."""
+    seen, current = [], [0]
+
+    class Library:
+        def __getattr__(self, name):
+            def entry(*args):
+                seen.append((name, current[0], args[-1].value if isinstance(args[-1], ctypes.c_void_p) else args[-1]))
+                return nat.RQ_OK
+            return entry
+
+    class On:
+        def __init__(self, index):
+            self.index = index
+
+        def __enter__(self):
+            self.before, current[0] = current[0], self.index
+
+        def __exit__(self, *_):
+            current[0] = self.before
+
+    monkeypatch.setattr(nat, "load", lambda: Library())
+    monkeypatch.setattr(nat, "_raw_stream_of", lambda index: 100 + index)
+    monkeypatch.setattr(nat, "_current_device", lambda: current[0])
+    monkeypatch.setattr(torch.cuda, "device", On)
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda d: type("S", (), dict(cuda_stream=100 + d.index, device=d)))
+    return seen
+
+
+@pytest.mark.parametrize("index", [0, 1])
+def test_kernels_go_to_the_tensors_device(two_devices, index):
+    """A call on tensors of a device that is not current makes it current for the launch (a default stream's handle
+    is 0 on every device), and leaves the current one as it was."""
+    class T:
+        device = torch.device("cuda", index)
+
+        def get_device(self):
+            return index
+
+    @nat.on_device_of_first
+    def product(t, n):
+        """Twice the number."""
+        nat.check("rq_packed_linear", nat.load().rq_packed_linear(n, nat.raw_stream(t)))
+        return 2 * n
+
+    assert product(T(), 4) == 8 and product.__doc__ == "Twice the number."
+    nat.call("rq_find_params", 1, nat.stream_of(T.device))
+    nat.call("rq_hessian_math", 0)
+    assert two_devices == [("rq_packed_linear", index, 100 + index), ("rq_find_params", index, 100 + index), ("rq_hessian_math", 0, 0)]
+    assert nat._current_device() == 0
+    with pytest.raises(ZeroDivisionError):
+        nat.on_device_of_first(lambda t: 1 // 0)(T())
+    assert nat._current_device() == 0
+    # the wrappers of the packed operators and of scoring are made so
+    for fn in (K.packed_linear, K.packed_linear_grad, K.packed_moe, K.token_logprobs, K.token_logprobs_grad):
+        assert fn.__wrapped__

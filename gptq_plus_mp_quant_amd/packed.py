@@ -34,9 +34,13 @@ def _checked(entry: Dict[str, object], batch: int):
     experts)."""
     q, scales, g_idx, nbits = entry["qweight"], entry["scales"], entry["g_idx"], entry["nbits"]
     groupsize = entry.get("groupsize", 0)
-    if not (q.is_cuda and scales.is_cuda and g_idx.is_cuda):
+    dev = q.get_device()
+    if dev < 0 or scales.get_device() != dev or g_idx.get_device() != dev:
         for t, name in ((q, "qweight"), (scales, "scales"), (g_idx, "g_idx")):
             nat.require_gpu(t, f"packed entry: {name}")
+        raise ValueError("packed entry: qweight, scales and g_idx are on different devices")
+    if scales.requires_grad and torch.is_grad_enabled():
+        raise ValueError("packed entry: the scales are constants and would get no gradient; detach them")
     if q.dtype is not torch.int32 or scales.dtype is not torch.float32 or g_idx.dtype is not torch.int32:
         raise ValueError("packed entry: qweight and g_idx must be int32, scales float32")
     if not 2 <= nbits <= nat.RQ_PACKED_MAXBITS:
@@ -52,9 +56,6 @@ def _checked(entry: Dict[str, object], batch: int):
         raise ValueError("packed entry: qweight, scales and g_idx hold different numbers of experts")
     if groupsize < 0 or (groupsize and ng > 1 and (C - 1) // groupsize >= ng):
         raise ValueError(f"packed entry: groupsize {groupsize} does not fit {ng} groups of {C} columns")
-    dev = q.get_device()
-    if scales.get_device() != dev or g_idx.get_device() != dev:
-        raise ValueError("packed entry: qweight, scales and g_idx are on different devices")
     qst, sst = q.stride(), scales.stride()
     if qst[-1] != 1 or sst[-1] != 1 or (qst[-2] < words and R > 1) or (sst[-2] < R and ng > 1):
         raise ValueError("packed entry: qweight and scales need unit column strides")
@@ -62,15 +63,9 @@ def _checked(entry: Dict[str, object], batch: int):
             g_idx if g_idx.is_contiguous() else g_idx.contiguous(), groupsize)
 
 
-def _constant(name, *entries):
-    """Under autograd, scales that require grad are refused: they would get none."""
-    for e in entries:
-        if getattr(e["scales"], "requires_grad", False):
-            raise ValueError(f"{name}: the scales of a packed weight are constants; detach them")
-
-
 def _tokens(x, width, q, name):
-    """x as [T, width] with unit column stride (copied only if its strides need it), and T."""
+    """x as [T, width] with unit column stride (copied only if its strides need it), T, and x's leading
+    dimensions."""
     if not (isinstance(x, torch.Tensor) and x.is_cuda):
         nat.require_gpu(x, name)
     if x.dtype not in nat.DTYPE_CODES:
@@ -88,7 +83,7 @@ def _tokens(x, width, q, name):
             x2 = x2.contiguous()
         if x2.stride(0) < width:                 # one token: its row stride is never used
             x2 = x2.as_strided((T, width), (width, 1))
-    return x2, T
+    return x2, T, (T,) if x2 is x else shape[:-1]
 
 
 class _PackedLinear(torch.autograd.Function):
@@ -112,12 +107,12 @@ class _PackedLinear(torch.autograd.Function):
 
 def _forward(x, entry, bias):
     q, nbits, scales, R, C, ng, g_idx, groupsize = _checked(entry, 0)
-    x2, T = _tokens(x, C, q, "x")
+    x2, T, lead = _tokens(x, C, q, "x")
     if bias is not None:
         if not isinstance(bias, torch.Tensor) or bias.dtype != x.dtype or bias.shape != (R,) or bias.device != x.device:
             raise ValueError(f"bias must be {x.dtype} [{R}] on {x.device}")
         bias = bias.contiguous()
-    return K.packed_linear(x2, q, nbits, scales, T, R, C, ng, g_idx, groupsize, bias, x.shape[:-1])
+    return K.packed_linear(x2, q, nbits, scales, T, R, C, ng, g_idx, groupsize, bias, lead)
 
 
 def packed_linear(x: torch.Tensor, entry: Dict[str, object], bias: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -128,10 +123,10 @@ def packed_linear(x: torch.Tensor, entry: Dict[str, object], bias: Optional[torc
     refused."""
     nat.refuse_tangents("packed_linear", x, bias, entry["scales"])
     if torch.is_grad_enabled():
-        _constant("packed_linear", entry)
-        if getattr(bias, "requires_grad", False):
+        if bias is not None and getattr(bias, "requires_grad", False):
             raise ValueError("packed_linear: the bias of a packed linear is a constant; detach it")
         if isinstance(x, torch.Tensor) and x.requires_grad:
+            _checked(entry, 0)                       # under autograd; forward runs without
             return _PackedLinear.apply(x, entry, bias)
     return _forward(x, entry, bias)
 
@@ -150,18 +145,17 @@ class _PackedLinearGrad(torch.autograd.Function):
 
 def _backward(grad_y, entry):
     q, nbits, scales, R, C, ng, g_idx, groupsize = _checked(entry, 0)
-    g2, T = _tokens(grad_y, R, q, "grad_y")
-    return K.packed_linear_grad(g2, q, nbits, scales, T, R, C, ng, g_idx, groupsize, grad_y.shape[:-1])
+    g2, T, lead = _tokens(grad_y, R, q, "grad_y")
+    return K.packed_linear_grad(g2, q, nbits, scales, T, R, C, ng, g_idx, groupsize, lead)
 
 
 def packed_linear_backward(grad_y: torch.Tensor, entry: Dict[str, object]) -> torch.Tensor:
     """The gradient of ``packed_linear``'s x: ``grad_y [..., R]`` times the packed weight, ``[..., C]`` in
     grad_y's dtype.  The result does not change from run to run.  It cannot be differentiated further."""
     nat.refuse_tangents("packed_linear_backward", grad_y, entry["scales"])
-    if torch.is_grad_enabled():
-        _constant("packed_linear_backward", entry)
-        if isinstance(grad_y, torch.Tensor) and grad_y.requires_grad:
-            return _PackedLinearGrad.apply(grad_y, entry)
+    if torch.is_grad_enabled() and isinstance(grad_y, torch.Tensor) and grad_y.requires_grad:
+        _checked(entry, 0)
+        return _PackedLinearGrad.apply(grad_y, entry)
     return _backward(grad_y, entry)
 
 
@@ -196,17 +190,15 @@ def packed_moe(x: torch.Tensor, router: torch.Tensor, gate: Dict[str, object], u
     chosen ids (int32) and weights (fp32), ``[..., top_k]``.  At most 1024 experts, 64 chosen.  It has
     no backward pass: an x that requires grad is refused, and forward-mode tangents are."""
     nat.refuse_tangents("packed_moe", x, router, gate["scales"], up["scales"], down["scales"])
-    if torch.is_grad_enabled():
-        _constant("packed_moe", gate, up, down)
-        if getattr(x, "requires_grad", False) or getattr(router, "requires_grad", False):
-            raise NotImplementedError("packed_moe has no backward pass: call it under torch.no_grad() or on detached tensors")
+    if torch.is_grad_enabled() and (getattr(x, "requires_grad", False) or getattr(router, "requires_grad", False)):
+        raise NotImplementedError("packed_moe has no backward pass: call it under torch.no_grad() or on detached tensors")
     g, u, d = _checked(gate, 1), _checked(up, 1), _checked(down, 1)
     E, I, D = g[0].shape[0], g[3], g[4]
     if u[0].shape[0] != E or d[0].shape[0] != E or u[3] != I or u[4] != D or d[3] != D or d[4] != I:
         raise ValueError("packed_moe: gate and up must be [E, I x D] and down [E, D x I]")
     if not u[0].get_device() == d[0].get_device() == g[0].get_device():
         raise ValueError("packed_moe: gate, up and down are on different devices")
-    x2, T = _tokens(x, D, g[0], "x")
+    x2, T, _ = _tokens(x, D, g[0], "x")
     if not isinstance(router, torch.Tensor) or router.shape != (E, D) or router.dtype != x.dtype or router.device != x.device:
         raise ValueError(f"packed_moe: router must be {x.dtype} [{E}, {D}] on {x.device}")
     top_k = int(top_k)

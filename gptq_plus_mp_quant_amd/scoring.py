@@ -28,6 +28,7 @@ class TokenLogprobs(NamedTuple):
 
 
 def _rows(logits, targets):
+    """(logits [N, V] with unit column stride, targets [N], N, V, the leading dimensions)."""
     if not (isinstance(logits, torch.Tensor) and logits.is_cuda):
         nat.require_gpu(logits, "logits")
     if logits.dtype not in nat.DTYPE_CODES:
@@ -35,9 +36,10 @@ def _rows(logits, targets):
     shape = logits.shape
     if len(shape) < 1 or shape[-1] == 0:
         raise ValueError("logits must be [..., V] with V > 0")
-    if not isinstance(targets, torch.Tensor) or targets.dtype is not torch.int64 or targets.shape != shape[:-1] or \
-            targets.device != logits.device:
-        raise ValueError(f"targets must be int64 {list(shape[:-1])} on {logits.device}")
+    lead = shape[:-1]
+    if not isinstance(targets, torch.Tensor) or targets.dtype is not torch.int64 or targets.shape != lead or \
+            targets.get_device() != logits.get_device():
+        raise ValueError(f"targets must be int64 {list(lead)} on {logits.device}")
     V = shape[-1]
     z = logits if len(shape) == 2 else logits.reshape(-1, V)
     s0, s1 = z.stride()
@@ -46,15 +48,15 @@ def _rows(logits, targets):
         if z.stride(0) < V:                      # one row: its stride is never used
             z = z.as_strided((z.shape[0], V), (V, 1))
     t = targets if targets.dim() == 1 else targets.reshape(-1)
-    return z, t if t.is_contiguous() else t.contiguous(), z.shape[0], V
+    return z, t if t.is_contiguous() else t.contiguous(), z.shape[0], V, lead
 
 
 def _forward(logits, targets, top_k, ignore_index):
-    z, t, N, V = _rows(logits, targets)
+    z, t, N, V, lead = _rows(logits, targets)
     top_k = int(top_k)
     if not 0 <= top_k <= min(nat.RQ_SCORE_MAX_TOP, V):
         raise ValueError(f"top_k must be 0 to {min(nat.RQ_SCORE_MAX_TOP, V)}, got {top_k}")
-    return TokenLogprobs(*K.token_logprobs(z, t, N, V, top_k, int(ignore_index), logits.shape[:-1]))
+    return TokenLogprobs(*K.token_logprobs(z, t, N, V, top_k, int(ignore_index), lead))
 
 
 class _TokenLogprobs(torch.autograd.Function):
@@ -87,10 +89,11 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, top_k: int = 0, 
     return _forward(logits, targets, top_k, ignore_index)
 
 
-def _row_grads(g, like, name):
-    if not isinstance(g, torch.Tensor) or g.dtype != torch.float32 or g.shape != like.shape[:-1] or g.device != like.device:
-        raise ValueError(f"{name} must be float32 {list(like.shape[:-1])} on {like.device}")
-    g = g if g.dim() == 1 else g.reshape(-1)
+def _row_values(g, lead, like, name):
+    """A float32 tensor of the given shape on like's device, contiguous."""
+    if not isinstance(g, torch.Tensor) or g.dtype is not torch.float32 or g.shape != lead or \
+            g.get_device() != like.get_device():
+        raise ValueError(f"{name} must be float32 {list(lead)} on {like.device}")
     return g if g.is_contiguous() else g.contiguous()
 
 
@@ -107,14 +110,11 @@ class _TokenLogprobsGrad(torch.autograd.Function):
 
 
 def _backward(logits, targets, stats, grad_logprob, grad_entropy, ignore_index):
-    z, t, N, V = _rows(logits, targets)
-    gl = _row_grads(grad_logprob, logits, "grad_logprob")
-    gh = None if grad_entropy is None else _row_grads(grad_entropy, logits, "grad_entropy")
-    if not isinstance(stats, torch.Tensor) or stats.dtype != torch.float32 or stats.shape != (*logits.shape[:-1], 3) or \
-            stats.device != logits.device:
-        raise ValueError(f"stats must be token_logprobs' float32 {list(logits.shape[:-1]) + [3]} on {logits.device}")
-    return K.token_logprobs_grad(z, t, N, V, int(ignore_index), stats if stats.is_contiguous() else stats.contiguous(), gl,
-                                 gh, logits.shape[:-1])
+    z, t, N, V, lead = _rows(logits, targets)
+    gl = _row_values(grad_logprob, lead, logits, "grad_logprob")
+    gh = None if grad_entropy is None else _row_values(grad_entropy, lead, logits, "grad_entropy")
+    stats = _row_values(stats, (*lead, 3), logits, "stats (token_logprobs')")
+    return K.token_logprobs_grad(z, t, N, V, int(ignore_index), stats, gl, gh, lead)
 
 
 def token_logprobs_backward(logits: torch.Tensor, targets: torch.Tensor, stats: torch.Tensor, grad_logprob: torch.Tensor,

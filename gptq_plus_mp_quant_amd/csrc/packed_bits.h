@@ -16,6 +16,12 @@ struct RqPacked {
   uint32_t run_magic;     // ceil(2^32 / (groupsize / 32)) for rq_run_group; 0: one group, 1: groups of 32
 };
 
+// The groups are runs of a multiple of n columns (n of 32), and rq_run_group may be asked for them.
+inline bool rq_runs_of(const RqPacked& w, int n) {
+  if (w.ngroups == 1) return true;
+  return w.groupsize > 0 && w.groupsize % n == 0 && (int64_t)(w.C / 32 + 1) * (w.groupsize / 32 + 1) < 1ll << 32;
+}
+
 // The weight an entry point was given.  run_magic divides by groupsize / 32 (group sizes that are multiples of
 // 32): n * magic >> 32 is n / d while n * d < 2^32.
 inline RqPacked rq_packed(const uint32_t* q, int64_t ldp, const float* scales, int64_t lds, const int32_t* g_idx, int R,

@@ -257,7 +257,7 @@ __device__ __forceinline__ floatx4 rq_scales4_of(const RqPacked& w, int g, int r
                  d <= 0 ? v[2] : v[3], v[3]};
 }
 
-// The group of column c where groups are runs of a multiple of 32 columns (or there is one).
+// The group of column c where rq_runs_of(w, 32).
 __device__ __forceinline__ int rq_run_group(const RqPacked& w, int c) {
   const uint32_t n = (uint32_t)c >> 5;
   return w.run_magic > 1 ? (int)__umulhi(n, w.run_magic) : w.run_magic ? (int)n : 0;
@@ -535,7 +535,6 @@ constexpr int RQ_STAGED_GROUPS = 1023;      // groups whose scales a workgroup s
 // Which of the three serves a weight.
 inline int rq_mode_of(const RqPacked& w) {
   if ((int64_t)(w.ngroups - 1) * w.lds + w.R < 4) return RQ_ANY;
-  if (w.groupsize > 0 && (int64_t)(w.C / 32 + 1) * (w.groupsize / 32 + 1) >= 1ll << 32 && w.ngroups > 1) return RQ_ANY;
-  if (w.ngroups == 1 || (w.groupsize > 0 && w.groupsize % RQ_CHUNK == 0)) return RQ_RUNS;
-  return w.groupsize > 0 && w.groupsize % 32 == 0 ? RQ_SMALL : RQ_ANY;
+  if (rq_runs_of(w, RQ_CHUNK)) return RQ_RUNS;
+  return rq_runs_of(w, 32) ? RQ_SMALL : RQ_ANY;
 }

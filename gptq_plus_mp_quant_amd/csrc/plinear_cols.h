@@ -303,7 +303,7 @@ void rq_linear_cols(const TX* dy, int T, int64_t ldy, const RqPacked& w, int nbi
       const RqColSplit sp = rq_col_split(n, w.R, w.C);
       const TX* d = dy + t0 * ldy;
       TX* out = dx + t0 * ldx;
-      if (w.ngroups == 1 || (w.groupsize > 0 && w.groupsize % COLS == 0)) linear_cols<TX, NB, RQ_RUNS>(d, n, ldy, w, sp, part, out, ldx, s);
+      if (rq_runs_of(w, COLS)) linear_cols<TX, NB, RQ_RUNS>(d, n, ldy, w, sp, part, out, ldx, s);
       else if (w.groupsize > 0 && w.groupsize % 8 == 0) linear_cols<TX, NB, RQ_SMALL>(d, n, ldy, w, sp, part, out, ldx, s);
       else linear_cols<TX, NB, RQ_ANY>(d, n, ldy, w, sp, part, out, ldx, s);
       if (sp.parts > 1)

@@ -697,3 +697,22 @@ def test_scales_that_require_grad_are_refused():
             assert torch.equal(packed_moe(xm, router, *changed, 2), packed_moe(xm, router, *parts, 2))
     with torch.no_grad():
         assert packed_linear(x, e).shape == (2, 32)
+
+
+def test_groups_of_millions_of_columns():
+    """Group sizes whose division by multiplication would not hold in 32 bits."""
+    size = 32 * 100020                   # a multiple of 128; 100020^2 is past 2^32
+    C = 2 * size
+    r = rng(1)
+    q = torch.from_numpy(r.integers(0, 1 << 32, size=(1, C // 8), dtype=np.uint32).view(np.int32))
+    e = dict(qweight=q.to(DEV), scales=torch.tensor([[0.5], [2.0]], device=DEV), nbits=4,
+             g_idx=(torch.arange(C, device=DEV) // size).to(torch.int32), groupsize=size)
+    nibbles = torch.from_numpy(np.ascontiguousarray(q.numpy().view(np.uint8))).view(-1)
+    codes = torch.stack((nibbles & 15, nibbles >> 4), 1).view(-1).double() - 8
+    W = codes * torch.where(torch.arange(C) < size, 0.5, 2.0)
+    gx = packed_linear_backward(torch.ones((1, 1), device=DEV), e)
+    assert torch.equal(gx.cpu().double(), W[None])
+    x = torch.zeros((2, C))
+    x[0, ::7], x[1, size - 200:size + 200] = 1.0, 1.0
+    want, mag = x.double() @ W, x.double() @ W.abs()
+    assert bool(((packed_linear(x.to(DEV), e).cpu().double()[:, 0] - want).abs() <= sum_eps(C) * mag).all())

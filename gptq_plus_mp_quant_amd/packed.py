@@ -57,7 +57,8 @@ def _checked(entry: Dict[str, object], batch: int):
     if groupsize < 0 or (groupsize and ng > 1 and (C - 1) // groupsize >= ng):
         raise ValueError(f"packed entry: groupsize {groupsize} does not fit {ng} groups of {C} columns")
     qst, sst = q.stride(), scales.stride()
-    if qst[-1] != 1 or sst[-1] != 1 or (qst[-2] < words and R > 1) or (sst[-2] < R and ng > 1):
+    # strides along a dimension of one element are never used, whatever they are
+    if (qst[-1] != 1 and words > 1) or (sst[-1] != 1 and R > 1) or (qst[-2] < words and R > 1) or (sst[-2] < R and ng > 1):
         raise ValueError("packed entry: qweight and scales need unit column strides")
     return (q if qst[-2] >= words else _rows_apart(q), nbits, scales if sst[-2] >= R else _rows_apart(scales), R, C, ng,
             g_idx if g_idx.is_contiguous() else g_idx.contiguous(), groupsize)

@@ -716,3 +716,25 @@ def test_groups_of_millions_of_columns():
     x[0, ::7], x[1, size - 200:size + 200] = 1.0, 1.0
     want, mag = x.double() @ W, x.double() @ W.abs()
     assert bool(((packed_linear(x.to(DEV), e).cpu().double()[:, 0] - want).abs() <= sum_eps(C) * mag).all())
+
+
+def test_strides_that_no_element_needs():
+    """One word a row, or one row: the stride along it is never used, and tables that come transposed have any."""
+    entry, W = make_entry(5, 20, 8, 4, "channel")
+    e = on(entry, DEV)
+    e["qweight"] = e["qweight"].as_strided((20, 1), (1, 20))
+    check_linear(randn(1, 3, 8, dtype=F16), e, W)
+    check_grad(randn(2, 3, 20, dtype=F16), e, W)
+    entry, W = make_entry(6, 1, 96, 4, "32")
+    e = on(entry, DEV)
+    e["scales"] = e["scales"].as_strided((3, 1), (1, 3))
+    check_linear(randn(3, 3, 96, dtype=F16), e, W)
+    check_grad(randn(4, 3, 1, dtype=F16), e, W)
+    parts = [make_entry(7 + k, R, C, 4, "channel", batch=2) for k, (R, C) in enumerate(((1, 8), (1, 8), (8, 1)))]
+    x, router = randn(8, 2, 8, dtype=F16), randn(9, 2, 8, dtype=F16)
+    want = packed_moe(x.to(DEV), router.to(DEV), *(on(e, DEV) for e, _ in parts), 1)
+    odd = [on(e, DEV) for e, _ in parts]
+    odd[0]["qweight"] = odd[0]["qweight"].as_strided((2, 1, 1), (1, 1, 5))
+    odd[1]["scales"] = odd[1]["scales"].as_strided((2, 1, 1), (1, 1, 7))
+    odd[2]["qweight"] = odd[2]["qweight"].as_strided((2, 8, 1), (8, 1, 3))
+    assert torch.equal(packed_moe(x.to(DEV), router.to(DEV), *odd, 1), want)

@@ -738,3 +738,63 @@ def test_strides_that_no_element_needs():
     odd[1]["scales"] = odd[1]["scales"].as_strided((2, 1, 1), (1, 1, 7))
     odd[2]["qweight"] = odd[2]["qweight"].as_strided((2, 8, 1), (8, 1, 3))
     assert torch.equal(packed_moe(x.to(DEV), router.to(DEV), *odd, 1), want)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16, F32])
+@pytest.mark.parametrize("T", [1, 12, 30, 50])
+@pytest.mark.parametrize("R,C,nbits,groups,times", [(48, 17000, 4, "128", 1), (33, 17160, 5, "channel", 1), (41, 8400, 4, "128", 200)])
+def test_many_chunks_a_wave(R, C, nbits, groups, times, T, dtype):
+    """Waves that take eight chunks of 128 columns and more, so that the loop that refills what is in flight
+    runs; with one row tile a wave and (R * times >= 8192) with two."""
+    entry, W = make_entry(R + nbits, R, C, nbits, groups)
+    x = randn(T, T, C, dtype=dtype)
+    y = check_linear(x, entry, W)
+    if times > 1:
+        e = on(entry, DEV)
+        e["qweight"], e["scales"] = e["qweight"].repeat(times, 1), e["scales"].repeat(1, times)
+        many = packed_linear(x.to(DEV), e).view(T, times, R)
+        assert torch.equal(many, many[:, :1].expand_as(many))
+        xd = x.double()
+        want, mag = xd @ W.t(), xd.abs() @ W.abs().t()
+        assert_within(many[:, 0], want, sum_eps(C) * mag + ROUND[dtype] * want.abs() + TINY[dtype], "y")
+    assert y.shape == (T, R)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16, F32])
+@pytest.mark.parametrize("T", [9, 60])
+def test_gradient_many_steps(T, dtype):
+    """Waves that take seven steps of 32 rows and more: 14336 columns, the same 128 over again."""
+    R, times = 9000, 112
+    entry, W = make_entry(T, R, 128, 4, "channel")
+    g = randn(T, T, R, dtype=dtype)
+    e = on(entry, DEV)
+    e["qweight"], e["g_idx"], e["groupsize"] = e["qweight"].repeat(1, times), e["g_idx"].repeat(times), 128 * times
+    many = packed_linear_backward(g.to(DEV), e).view(T, times, 128)
+    assert torch.equal(many, many[:, :1].expand_as(many))
+    gd = g.double()
+    want, mag = gd @ W, gd.abs() @ W.abs()
+    assert_within(many[:, 0], want, sum_eps(R) * mag + ROUND[dtype] * want.abs() + TINY[dtype], "gx")
+
+
+@pytest.mark.parametrize("T", [2, 40])
+@pytest.mark.parametrize("D,I", [(4224, 40), (64, 8448)])
+@pytest.mark.parametrize("nbits,groups", [(3, "128"), (4, "channel"), (5, "128"), (4, "32"), (4, "order128")])
+def test_moe_many_chunks_a_wave(nbits, groups, D, I, T):
+    """Experts of more chunks of 128 columns than waves share them, before the activation and after it."""
+    dtype = (F16, BF16, F32)[(T + nbits) % 3]
+    check_moe(*moe_case(T, T, D, I, 2, dtype, (nbits,) * 3, (groups,) * 3), 1, True)
+
+
+@pytest.mark.parametrize("T", [6, 48])
+@pytest.mark.parametrize("groups", ["128", "32", "order32"])
+def test_moe_tokens_keep_to_themselves_to_the_bit(groups, T):
+    """A NaN token sends itself to other experts, so the units' companions and their order change; the other
+    tokens' results do not, to the last bit."""
+    x, router, parts = moe_case(21, T, 256, 384, 6, BF16, groups=(groups,) * 3)
+    x, router, args = x.to(DEV), router.to(DEV), [on(e, DEV) for e, _ in parts]
+    clean = packed_moe(x, router, *args, 2)
+    x[3, 3] = float("nan")
+    y = packed_moe(x, router, *args, 2)
+    assert bool(torch.isnan(y[3]).all())
+    keep = [t for t in range(T) if t != 3]
+    assert torch.equal(y[keep], clean[keep])

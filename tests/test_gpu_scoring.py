@@ -392,3 +392,24 @@ def test_gradient_of_the_gradient_call_is_refused():
             gz.sum().backward()
         with torch.no_grad():
             assert not token_logprobs_backward(args[0], t, args[1], args[2], g).requires_grad
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16, F32])
+@pytest.mark.parametrize("N,V,k", [(512, 33000, 20), (515, 65541, 8), (512, 140003, 5), (512, 151936, 1), (512, 256000, 64)])
+def test_many_rounds_a_wave(N, V, k, dtype):
+    """A row's four waves take several rounds, several to a block past 131072 columns of a 16-bit type.  The rows
+    are few distinct ones over again, so that the definition in 64 bits needs only those."""
+    z = randn(V, 4, V, dtype=dtype, scale=3.0)
+    z[1] = torch.sort(z[1].float()).values.to(dtype)
+    z[2, : V - 70] = -30.0
+    z[3, ::3] = -INF
+    t = ints(V, V, 4)
+    few = check(z, t, k)                                     # split over workgroups
+    at = (torch.arange(N) % 4).to(DEV)
+    r = token_logprobs(z.to(DEV)[at], t.to(DEV)[at], top_k=k)
+    assert torch.equal(r.top_ids, few.top_ids[at])
+    mine, H, _, top, _, _, _ = reference(z, t, k)
+    u = 2.0 ** -21
+    assert_within(r.logprob, mine[at.cpu()], u * (4 + mine[at.cpu()].abs()), "logprob")
+    assert_within(r.entropy, H[at.cpu()], torch.full((N,), u * (4 + 2 * math.log(V))).double(), "entropy")
+    assert_within(r.top_logprobs, top[at.cpu()], u * (4 + top[at.cpu()].abs()), "top_logprobs")

@@ -79,17 +79,23 @@ void launch_rows(const TX* x, int T, int64_t ldx, const RqPacked& w, const TX* b
 
 template <typename TX, int NB>
 void linear_rows(const TX* x, int T, int64_t ldx, const RqPacked& w, const TX* bias, TX* y, int64_t ldy, hipStream_t s) {
-  constexpr int RT4 = RqOperand<TX>::pieces == 1 ? 2 : 1;       // fp32's pieces leave registers for one row tile
+  constexpr int MORE = RqOperand<TX>::pieces == 1 ? 2 : 1;      // fp32's pieces leave registers for one row tile
   switch (rq_mode_of(w)) {
     case RQ_RUNS:
-      // Two row tiles a wave share their tokens' loads; taken where they still make a workgroup for every CU
-      // (8192 x 28672 4-bit bf16, 1 / 16 tokens: 42 / 71 us with one, 35 / 49 with two).
+      // Two row tiles a wave share their tokens' loads.  Up to 16 tokens they are taken where they still make a workgroup
+      // for every CU (8192 x 28672 4-bit bf16, 1 / 16 tokens: 42 / 71 us with one, 35 / 49 with two); beyond, where a
+      // CU holds one workgroup, as soon as one row tile makes more workgroups than there are CUs (24 / 64 tokens, one
+      // and two: 4096 x 4096 11.0 / 19.7 and 12.0 / 21.9 us, 5120 x 4096 16.9 / 35.8 and 11.6 / 22.0, 8192 x 28672 98 / 216 and
+      // 62 / 121).  Two token tiles up to 32 tokens: 4096 x 4096, 32 tokens 11.4 us for 14.5 with four.
       if (T <= 16 && w.R >= 8192) launch_rows<TX, NB, RQ_RUNS, 2, 1>(x, T, ldx, w, bias, y, ldy, s);
       else if (T <= 16) launch_rows<TX, NB, RQ_RUNS, 1, 1>(x, T, ldx, w, bias, y, ldy, s);
+      else if (T <= 32 && w.R > 4096) launch_rows<TX, NB, RQ_RUNS, MORE, 2>(x, T, ldx, w, bias, y, ldy, s);
       else if (T <= 32) launch_rows<TX, NB, RQ_RUNS, 1, 2>(x, T, ldx, w, bias, y, ldy, s);
-      else launch_rows<TX, NB, RQ_RUNS, RT4, 4>(x, T, ldx, w, bias, y, ldy, s);
+      else if (w.R > 4096) launch_rows<TX, NB, RQ_RUNS, MORE, 4>(x, T, ldx, w, bias, y, ldy, s);
+      else launch_rows<TX, NB, RQ_RUNS, 1, 4>(x, T, ldx, w, bias, y, ldy, s);
       break;
     case RQ_SMALL:
+      // One row tile: with two 4096 x 4096 4-bit bf16 in groups of 64 takes 18.6 us for 11.2 (4 tokens), 29.1 for 21.9 (64).
       if (T <= 16) launch_rows<TX, NB, RQ_SMALL, 1, 1>(x, T, ldx, w, bias, y, ldy, s);
       else launch_rows<TX, NB, RQ_SMALL, 1, 4>(x, T, ldx, w, bias, y, ldy, s);
       break;

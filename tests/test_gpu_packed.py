@@ -798,3 +798,9 @@ def test_moe_tokens_keep_to_themselves_to_the_bit(groups, T):
     assert bool(torch.isnan(y[3]).all())
     keep = [t for t in range(T) if t != 3]
     assert torch.equal(y[keep], clean[keep])
+
+
+def test_moe_most_shared_memory():
+    """The most units (64 tokens, each with 64 of 1024 experts) and the most scales a wave stages, of down along an
+    order, leave least of the 160 KB."""
+    check_moe(*moe_case(9, 64, 48, 62, 1024, BF16, (4, 4, 4), ("channel", "channel", "order1")), 64, True)

@@ -12,9 +12,9 @@
 // that cancel keep fp32's precision.  Where both sides are cut, products that come to at most 2^-22 of a term (2^-24
 // mostly) are left out.
 // Rows are split over workgroups until there are 512, whose sums a second launch joins in their order.
-// Measured: 4096 x 4096 5-bit fp16, 8 tokens 9.1 + 4.1 us, latency; 14336 x 4096 4-bit bf16, 64 tokens 33 + 5.3 us (30.6 with
-// two pieces), where the conversions of codes and of dy on the vector units and three pieces' matrix instructions (7.5
-// GFLOP each) overlap in part, with two waves a SIMD.
+// Measured: 4096 x 4096 5-bit fp16, 8 tokens 9.2 + 4.0 us, latency; 14336 x 4096 4-bit bf16, 64 tokens 33 + 5.4 us (30.6 with
+// two pieces): by the counters 13 us of vector issue, conversions of codes and of dy, and 9 us of matrix instructions
+// (7.5 GFLOP for each piece), overlapped in part by two waves a SIMD, and waits for the one step that is ahead.
 #pragma once
 #include "packed_dot.h"
 
@@ -73,7 +73,7 @@ __device__ __forceinline__ void fp32_of(floatx8 v, floatx8& f) { f = v; }
 constexpr int cols_waves(int nt) { return nt >= 4 ? 4 : 8; }
 
 // Waves of a SIMD that the registers are cut for: with RUNS four token tiles fit 256 (14336 x 4096 4-bit bf16,
-// 64 tokens: 30 us, 37 with one wave a SIMD and 280); the other modes would spill (4096 x 4096 along an order: 54 for
+// 64 tokens, two pieces: 30 us, 37 with one wave a SIMD and 280); the other modes would spill (4096 x 4096 along an order: 54 for
 // 45).
 constexpr int cols_occupancy(int mode, int nt) { return mode == RQ_RUNS && nt >= 4 ? 2 : 1; }
 

@@ -8,10 +8,11 @@ namespace {
 // A workgroup of W waves takes 16 RT rows and 16 NT tokens; its waves take the chunks of 128 columns in
 // turn (rows alone would leave most CUs without work) and are joined through LDS, in their order.
 // Few tokens are bound by the weight's bytes.  Measured, 4 bits in groups of 128, bf16: 4096 x 4096 (8.9 MB), 1
-// token 6.2 us, a launch and three trips to memory; 8192 x 28672 (125 MB), 1 / 16 tokens 35 / 48 us, 3.6 / 2.6 TB/s: 16
-// tokens' loads, twice the words' bytes, share the CU's load path with them, and conversions take a third of the
-// time.  Groups along an order (ANY) 223 us there, a scale from LDS and an fp32 product for every weight; 1026 x 1365 at
-// 5 bits, fp32, 7 tokens 9.7 us, 65 workgroups' latency.
+// token 6.3 us, a launch and three trips to memory; 8192 x 28672 (125 MB), 1 / 16 tokens 35 / 48 us, 3.6 / 2.6 TB/s (with
+// the words in a cache from the call before; from HBM 2 and 1 us more): 16 tokens' loads, twice the words' bytes, share
+// the CU's load path with them, and vector instructions, mostly conversions, take 19 us.  Groups along an order (ANY)
+// 223 us there, a scale from LDS and an fp32 product for every weight; 1026 x 1365 at 5 bits, fp32, 7 tokens 9.7 us, 65
+// workgroups' latency.
 constexpr int rows_threads(int rt, int nt) { return rt * nt >= 2 ? 512 : 1024; }     // 256 or 128 registers a lane
 template <typename TX, int NB, int MODE, int RT, int NT>
 __global__ __launch_bounds__(rows_threads(RT, NT)) void k_packed_rows(const TX* __restrict__ x, int T, int64_t ldx, RqPacked w,

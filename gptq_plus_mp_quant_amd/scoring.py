@@ -80,7 +80,7 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, top_k: int = 0, 
 
     ``logprob`` is 0 where the target is ``ignore_index`` and NaN for another target outside the vocabulary.
     ``top_k`` (0 to 64) alternatives are ordered by their logit, equal ones by their index.  Masked
-    logits (-inf, or the type's lowest value) have probability 0; a row with nothing but -inf has
+    logits (-inf, or a large negative number) have probability 0; a row with nothing but -inf has
     logprob -inf, entropy 0 and no gradient; a row with a NaN or +inf is NaN.  ``logprob`` and
     ``entropy`` are differentiable in ``logits``, ``top_logprobs`` is not; forward-mode tangents are refused."""
     nat.refuse_tangents("token_logprobs", logits)

@@ -356,7 +356,9 @@ int rq_block_gd_step(float* Wp, int64_t ldw, int R, int R_s, int C, int i2, cons
  * [ngroups, lds] fp32 (row r's scale of group g at scales[g * lds + r]) and the group of each column:
  * c / groupsize when groupsize > 0, else g_idx[c] (a column whose g_idx lies outside [0, ngroups)
  * reads as NaN); one group needs neither.  The weight is s * q as it stands, not rounded to a layer's
- * type.  No counterpart in the reference, which multiplies by the dequantized weight. */
+ * type; where the groups are runs of a multiple of 32 columns the sums of x times q come first and
+ * have to stay within fp32's range.  No counterpart in the reference, which multiplies by the
+ * dequantized weight. */
 
 /* y[t, r] = sum_c x[t, c] * s[g(c), r] * q[r, c] (+ bias[r]): x [T, C] (row stride ldx), bias [R] or
  * NULL and y [T, R] (row stride ldy) of type dtype.  fp32 sums, rounded once.  Any T; built for few. */

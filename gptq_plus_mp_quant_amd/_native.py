@@ -30,6 +30,12 @@ RQ_ACT_ORDER_MAXC = 65536      # widest rq_act_order_perm
 RQ_PACKED_MAXBITS = 9          # widest fields the products with packed weights take
 RQ_MOE_MAX_EXPERTS, RQ_MOE_MAX_TOP = 1024, 64
 RQ_SCORE_MAX_TOP = 64          # alternatives of rq_token_logprobs
+RQ_MAX_TOKENS = 1 << 19        # of one call of the products with adapters and of the gated block
+RQ_LORA_MAX_RANK, RQ_LORA_MAX_ADAPTERS = 256, 65535
+RQ_DISTILL_MAX_TOP = 256       # tokens of a teacher's list
+RQ_DISTILL_STATS = 8
+ACTIVATIONS = {"silu": 0, "gelu": 1, "gelu_tanh": 2}
+TAILS = {"renormalise": 0, "bucket": 1}
 # g_update_mode -> (kernel mode of the in-block loop, kernel mode of the trailing update);
 # gptq_plus_utils.py:1190 (inner) and :1500 (outer)
 GMODES = {"frozen": (RQ_GMODE_FROZEN, RQ_GMODE_FROZEN),
@@ -38,12 +44,19 @@ GMODES = {"frozen": (RQ_GMODE_FROZEN, RQ_GMODE_FROZEN),
           "block_gd": (RQ_GMODE_BLOCK_GD, RQ_GMODE_BLOCK_GD),
           "block_backward": (RQ_GMODE_SURROGATE_ONLINE, RQ_GMODE_FROZEN)}
 
-_P, _I, _L, _D = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_double
+_P, _I, _L, _D, _F = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_double, ctypes.c_float
+
 
 class PackedExperts(ctypes.Structure):
     """``rq_packed_experts``: one linear of every expert of a layer."""
     _fields_ = [("qweight", _P), ("scales", _P), ("g_idx", _P), ("ldp", _L), ("lds", _L), ("stride_q", _L),
                 ("stride_scales", _L), ("nbits", _I), ("ngroups", _I), ("groupsize", _I)]
+
+
+class PackedWeight(ctypes.Structure):
+    """``rq_packed_weight``: one packed weight."""
+    _fields_ = [("qweight", _P), ("scales", _P), ("g_idx", _P), ("ldp", _L), ("lds", _L), ("nbits", _I), ("ngroups", _I),
+                ("groupsize", _I)]
 
 
 # name -> (restype, argtypes); mirrors include/gptqplus_hip.h
@@ -85,6 +98,19 @@ SIGNATURES = {
     "rq_packed_linear_grad": (_I, [_P, _I, _I, _L, _I, _P, _L, _I, _I, _P, _L, _I, _P, _I, _P, _L, _P, _L, _P]),
     "rq_packed_moe_workspace_bytes": (_L, [_I, _I, _I, _I, _I]),
     "rq_packed_moe": (_I, [_P, _I, _I, _L, _I, _P, _L, _I, _I, _I, _I, _P, _P, _P, _P, _L, _P, _P, _P, _L, _P]),
+    "rq_packed_linear_lora_workspace_bytes": (_L, [_I, _I, _I]),
+    "rq_packed_linear_lora": (_I, [_P, _I, _I, _L, _I, _P, _L, _I, _I, _P, _L, _I, _P, _I, _P, _P, _P, _I, _I, _P, _P, _F, _P, _L,
+                                   _P, _L, _P]),
+    "rq_packed_linear_lora_grad_workspace_bytes": (_L, [_I, _I, _I, _I]),
+    "rq_packed_linear_lora_grad": (_I, [_P, _I, _I, _L, _P, _L, _I, _P, _L, _I, _I, _P, _L, _I, _P, _I, _P, _P, _I, _I, _P, _P, _F,
+                                        _P, _L, _P, _P, _P, _L, _P]),
+    "rq_packed_gated_workspace_bytes": (_L, [_I, _I, _I, _P, _P]),
+    "rq_packed_gated": (_I, [_P, _I, _I, _L, _I, _I, _P, _P, _I, _P, _P, _L, _P, _L, _P]),
+    "rq_packed_gated_grad_workspace_bytes": (_L, [_I, _I, _I]),
+    "rq_packed_gated_grad": (_I, [_P, _I, _I, _L, _I, _P, _I, _P, _P, _I, _P, _L, _P, _L, _P]),
+    "rq_distill_loss_workspace_bytes": (_L, [_L, _I]),
+    "rq_distill_loss": (_I, [_P, _I, _L, _L, _I, _P, _P, _I, _D, _I, _P, _P, _P, _L, _P]),
+    "rq_distill_loss_grad": (_I, [_P, _I, _L, _L, _I, _P, _P, _I, _D, _I, _P, _P, _P, _L, _P]),
     "rq_token_logprobs_workspace_bytes": (_L, [_L, _I, _I]),
     "rq_token_logprobs": (_I, [_P, _I, _L, _L, _I, _P, _L, _I, _P, _P, _P, _P, _P, _P, _L, _P]),
     "rq_token_logprobs_grad": (_I, [_P, _I, _L, _L, _I, _P, _L, _P, _P, _P, _P, _L, _P]),

@@ -19,14 +19,12 @@
 // where a copy of that size reaches 5.0 (read and written).
 // A row's segments are joined by one wave: in the workgroup that has the whole row, or by k_logprob_join
 // where a row is cut over many workgroups.
-#include "packed_dot.h"
+#include "logits.h"
 
 namespace {
 
 constexpr int MAX_TOP = 64, MAX_V = 1 << 30;
 constexpr int LIST = 320;                  // candidates a wave holds
-constexpr float LOG2E = 1.4426950408889634f;
-
 constexpr float LN2 = 0.6931471805599453f;
 constexpr float LOW = -200.0f;             // 2^LOW is 0 in fp32: stands for any lower exponent where it is a factor
 __device__ __forceinline__ uint64_t top_key(float z, int i) {
@@ -73,7 +71,7 @@ struct Stat {
 __device__ __forceinline__ Stat join(Stat x, Stat y) {
   const float m = fmaxf(x.m, y.m);
   if (m == -INFINITY) return Stat{m, x.s + y.s, x.a + y.a};
-  const float dx = (x.m - m) * LOG2E, dy = (y.m - m) * LOG2E;            // <= 0, -inf for an empty part
+  const float dx = (x.m - m) * RQ_LOG2E, dy = (y.m - m) * RQ_LOG2E;            // <= 0, -inf for an empty part
   const float fx = __builtin_amdgcn_exp2f(dx), fy = __builtin_amdgcn_exp2f(dy);
   Stat r;
   r.m = m;
@@ -216,21 +214,6 @@ __device__ __forceinline__ float above(float v) {
   return __uint_as_float((b & 0x80000000u) ? b - 1 : b + 1);
 }
 
-// The 8 logits from column c on that lie before c1; -inf for the others.
-template <typename TX>
-__device__ __forceinline__ typename RqOperand<TX>::raw load8(const TX* __restrict__ row, int c, int c1) {
-  typename RqOperand<TX>::raw v;
-  if (c + 8 <= c1) return rq_load_x<true>(row + c, 8);
-#pragma unroll
-  for (int k = 0; k < 8; ++k) v[k] = -INFINITY;
-  if (c < c1) {
-#pragma unroll
-    for (int k = 0; k < 8; ++k)
-      if (c + k < c1) __builtin_memcpy((char*)&v + k * sizeof(TX), row + c + k, sizeof(TX));
-  }
-  return v;
-}
-
 // A wave's segment [c0, c1) of a row, in rounds of U loads of 512 columns, blocks of `rounds` rounds each.
 template <typename TX>
 struct Scan {
@@ -248,7 +231,7 @@ __device__ __forceinline__ Stat scan_segment(const Scan<TX>& sc, float* most) {
   const int lane = threadIdx.x & 63, c1 = sc.c1;
   Raw in[U];
 #pragma unroll
-  for (int u = 0; u < U; ++u) in[u] = load8<TX>(sc.row, sc.c0 + 512 * u + 8 * lane, c1);
+  for (int u = 0; u < U; ++u) in[u] = rq_load8<TX>(sc.row, sc.c0 + 512 * u + 8 * lane, c1);
   Stat v = {-INFINITY, 0.0f, 0.0f};
 #pragma unroll
   for (int u = 0; u < U; ++u)
@@ -260,7 +243,7 @@ __device__ __forceinline__ Stat scan_segment(const Scan<TX>& sc, float* most) {
   // (f - m) log2e.
   constexpr float WIDE = 0x1p20f;
   auto is_wide = [](float at) { return __builtin_fabsf(at) > WIDE; };
-  float shift = v.m == -INFINITY ? 0.0f : v.m * LOG2E;
+  float shift = v.m == -INFINITY ? 0.0f : v.m * RQ_LOG2E;
   float block = -INFINITY;
   int round = 0;
   for (int c = sc.c0; c < c1; c += 512 * U) {
@@ -271,19 +254,19 @@ __device__ __forceinline__ Stat scan_segment(const Scan<TX>& sc, float* most) {
       float f[8];
 #pragma unroll
       for (int k = 0; k < 8; ++k) f[k] = (float)in[u][k];
-      in[u] = load8<TX>(sc.row, cu + 512 * U + 8 * lane, c1);
+      in[u] = rq_load8<TX>(sc.row, cu + 512 * U + 8 * lane, c1);
       float big = f[0];
 #pragma unroll
       for (int k = 1; k < 8; ++k) big = fmaxf(big, f[k]);
       block = fmaxf(block, big);
       if (big > v.m) {                     // the maximum grows
-        const float grown = big * LOG2E;
+        const float grown = big * RQ_LOG2E;
         // far: from what the sums' exponents were taken from to what they are taken from now.  One of them is wide only
         // if -shift or grown is (a lane without a maximum so far has shift 0 and sums of 0).
         float far = shift - grown;
         if (__any(__builtin_fmaxf(-shift, grown) > WIDE)) {
-          if (is_wide(shift)) far = is_wide(grown) ? (v.m - big) * LOG2E : __builtin_fmaf(v.m, LOG2E, -grown);
-          else if (is_wide(grown)) far = __builtin_fmaf(-big, LOG2E, shift);
+          if (is_wide(shift)) far = is_wide(grown) ? (v.m - big) * RQ_LOG2E : __builtin_fmaf(v.m, RQ_LOG2E, -grown);
+          else if (is_wide(grown)) far = __builtin_fmaf(-big, RQ_LOG2E, shift);
         }
         const float D = __builtin_amdgcn_fmed3f(far, LOW, 1.0f);
         const float scale = v.m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(D);
@@ -299,10 +282,10 @@ __device__ __forceinline__ Stat scan_segment(const Scan<TX>& sc, float* most) {
       };
       if (__any(is_wide(shift))) {
 #pragma unroll
-        for (int k = 0; k < 8; ++k) add(is_wide(shift) ? (f[k] - v.m) * LOG2E : __builtin_fmaf(f[k], LOG2E, -shift));
+        for (int k = 0; k < 8; ++k) add(is_wide(shift) ? (f[k] - v.m) * RQ_LOG2E : __builtin_fmaf(f[k], RQ_LOG2E, -shift));
       } else {
 #pragma unroll
-        for (int k = 0; k < 8; ++k) add(__builtin_fmaf(f[k], LOG2E, -shift));
+        for (int k = 0; k < 8; ++k) add(__builtin_fmaf(f[k], RQ_LOG2E, -shift));
       }
     }
     if (++round % sc.rounds == 0 || c + 512 * U >= c1) {
@@ -310,7 +293,7 @@ __device__ __forceinline__ Stat scan_segment(const Scan<TX>& sc, float* most) {
       block = -INFINITY;
     }
   }
-  const float off = v.m == -INFINITY || is_wide(shift) ? 0.0f : __builtin_fmaf(v.m, LOG2E, -shift);
+  const float off = v.m == -INFINITY || is_wide(shift) ? 0.0f : __builtin_fmaf(v.m, RQ_LOG2E, -shift);
   const float back = __builtin_amdgcn_exp2f(-off);
   v.a = back * (v.a - off * v.s);
   v.s *= back;
@@ -345,7 +328,7 @@ __device__ __forceinline__ void collect(const Scan<TX>& sc, const float* most, b
     for (int cr = c; cr < end; cr += 512 * U) {
       Raw in[U];
 #pragma unroll
-      for (int u = 0; u < U; ++u) in[u] = load8<TX>(sc.row, cr + 512 * u + 8 * lane, c1);
+      for (int u = 0; u < U; ++u) in[u] = rq_load8<TX>(sc.row, cr + 512 * u + 8 * lane, c1);
       uint32_t passed = 0;
 #pragma unroll
       for (int u = 0; u < U; ++u) {
@@ -496,26 +479,12 @@ inline Split split_of(int64_t N, int V) {
   const int64_t segs = ((fill < most ? fill : most) + W - 1) / W * W;
   return Split{(int)segs, (int)(((V + segs - 1) / segs + 7) / 8 * 8)};
 }
-constexpr int64_t ROWS_PER_LAUNCH = 1 << 20;
 
 // --- the gradient ---------------------------------------------------------------------------
 // A workgroup takes rounds of 8192 columns of a row, 4 x 8 a thread: read once, written once.  z and dz may
 // be the same memory (a thread reads what it writes first).  1024 rows of 128256 bf16: 108 us for 525 MB,
 // 4.9 TB/s, a copy's rate; 12 rows of 32003 fp32 4.8 us, a launch.
 constexpr int GRAD_COLS = 8192;
-
-template <typename TX>
-__device__ __forceinline__ void store8(TX* p, const float (&g)[8]) {
-  typename RqOperand<TX>::raw v;
-#pragma unroll
-  for (int k = 0; k < 8; ++k) {
-    const TX e = rq_cast<TX>(g[k]);
-    typename std::remove_reference<decltype(v[0])>::type w;
-    __builtin_memcpy(&w, &e, sizeof(TX));
-    v[k] = w;
-  }
-  __builtin_memcpy(p, &v, sizeof(v));
-}
 
 template <typename TX>
 __global__ __launch_bounds__(256) void k_logprob_grad(const TX* z, int64_t ldz, int V,
@@ -536,7 +505,7 @@ __global__ __launch_bounds__(256) void k_logprob_grad(const TX* z, int64_t ldz, 
   // -p (gl + gh (log p + H)); 0 where p is 0
   auto gradient = [&](float v, int i) {
     const float lp = (v - m) - ls;
-    const float p = __builtin_amdgcn_exp2f(lp * LOG2E);
+    const float p = __builtin_amdgcn_exp2f(lp * RQ_LOG2E);
     float g = -p * __builtin_fmaf(gh, fmaxf(lp, LOW), c);
     if (i == t) g += gl;
     return empty ? 0.0f : g;
@@ -554,7 +523,7 @@ __global__ __launch_bounds__(256) void k_logprob_grad(const TX* z, int64_t ldz, 
         float g[8];
 #pragma unroll
         for (int k = 0; k < 8; ++k) g[k] = gradient((float)r[u][k], at + k);
-        store8<TX>(out + at, g);
+        rq_store8<TX>(out + at, g);
       } else {
         for (int i = at; i < V; ++i) out[i] = rq_cast<TX>(gradient(rq_load_elem(row + i), i));
       }
@@ -594,8 +563,8 @@ extern "C" int rq_token_logprobs(const void* logits, int dtype, int64_t N, int64
                          ignore_index, top_k, logprob, entropy, top_ids, top_logprobs, stats, st, keys);
       return;
     }
-    for (int64_t n = 0; n < N; n += ROWS_PER_LAUNCH) {
-      const int64_t rows = N - n < ROWS_PER_LAUNCH ? N - n : ROWS_PER_LAUNCH;
+    for (int64_t n = 0; n < N; n += RQ_ROWS_PER_LAUNCH) {
+      const int64_t rows = N - n < RQ_ROWS_PER_LAUNCH ? N - n : RQ_ROWS_PER_LAUNCH;
       hipLaunchKernelGGL((k_logprob_rows<TX, false>), dim3((unsigned)rows), dim3(64 * W), 0, s, (const TX*)logits + n * ldz,
                          ldz, V, sp.segs, sp.cols, targets + n, ignore_index, top_k, logprob + n, entropy + n,
                          top_ids + n * top_k, top_logprobs + n * top_k, stats + 3 * n, nullptr, nullptr);
@@ -617,8 +586,8 @@ extern "C" int rq_token_logprobs_grad(const void* logits, int dtype, int64_t N, 
   const int rounds = (V + GRAD_COLS - 1) / GRAD_COLS, ny = rounds < 64 ? rounds : 64;
   const bool known = rq_with_dtype(dtype, [&](auto* p) {
     typedef typename std::remove_pointer<decltype(p)>::type TX;
-    for (int64_t n = 0; n < N; n += ROWS_PER_LAUNCH) {
-      const int64_t rows = N - n < ROWS_PER_LAUNCH ? N - n : ROWS_PER_LAUNCH;
+    for (int64_t n = 0; n < N; n += RQ_ROWS_PER_LAUNCH) {
+      const int64_t rows = N - n < RQ_ROWS_PER_LAUNCH ? N - n : RQ_ROWS_PER_LAUNCH;
       hipLaunchKernelGGL(k_logprob_grad<TX>, dim3((unsigned)rows, ny), dim3(256), 0, s, (const TX*)logits + n * ldz, ldz, V,
                          targets + n, ignore_index, stats + 3 * n, grad_logprob + n, grad_entropy ? grad_entropy + n : nullptr,
                          (TX*)grad_logits + n * ldd, ldd);

@@ -1,0 +1,141 @@
+// act(x Wg^T) * (x Wu^T) from packed weights, and what its gradient takes beside the gradient of a packed linear: the
+// kernels for one element type.
+#pragma once
+#include "pgated_types.h"
+#include "plinear_rows.h"
+
+namespace {
+
+enum { GATED_BOTH = 0, GATED_GATE = 1, GATED_UP = 2 };
+
+// 16 rows of both weights and 16 NT tokens to a workgroup; the waves take the chunks of 128 columns in turn, multiply a
+// row tile of gate and one of up by the tokens they have loaded once, and are joined through LDS in their order.  GATE
+// and UP (weights of different bits or groups): one of the two, the gate's product goes by way of pre.
+template <typename TX, int NB, int MODE, int NM, int NT>
+__global__ __launch_bounds__(rows_threads(2, NT)) void k_packed_gated(const TX* __restrict__ x, int T, int64_t ldx, RqPacked first,
+                                                                      RqPacked second, int what, int act, bool staged,
+                                                                      float* pre, TX* __restrict__ h, int64_t ldh) {
+  extern __shared__ __attribute__((aligned(16))) float lds[];
+  const int lane = threadIdx.x & 63, wave = rq_wave(), waves = blockDim.x >> 6;
+  const int r0 = blockIdx.x * 16, t0 = blockIdx.y * 16 * NT, I = first.R;
+  RqTokens<TX, NT> xs;
+#pragma unroll
+  for (int b = 0; b < NT; ++b) xs.p[b] = x + (int64_t)min(t0 + 16 * b + (lane & 15), T - 1) * ldx;
+  RqPacked w[NM];
+  w[0] = first;
+  if constexpr (NM == 2) w[1] = second;
+  if (MODE == RQ_ANY && staged) {
+#pragma unroll
+    for (int a = 0; a < NM; ++a) rq_stage_scales(w[a], r0, a, NM, threadIdx.x, blockDim.x, lds);
+    __syncthreads();
+  }
+  floatx4 acc[NM][NT];
+#pragma unroll
+  for (int a = 0; a < NM; ++a)
+#pragma unroll
+    for (int b = 0; b < NT; ++b) acc[a][b] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+  rq_rows_tokens<NB, MODE, NM, NM>(w, r0, xs, wave, waves, MODE == RQ_ANY && staged ? lds : nullptr, acc);
+  if (MODE == RQ_ANY && staged) __syncthreads();
+  floatx4* out = reinterpret_cast<floatx4*>(lds);
+#pragma unroll
+  for (int a = 0; a < NM; ++a)
+#pragma unroll
+    for (int b = 0; b < NT; ++b) out[((wave * NM + a) * NT + b) * 64 + lane] = acc[a][b];
+  __syncthreads();
+  for (int e = threadIdx.x; e < NT * 64; e += blockDim.x) {
+    const int l = e & 63, b = e >> 6;
+    const int t = t0 + 16 * b + (l & 15), r = r0 + 4 * (l >> 4);
+    if (t >= T) continue;
+    floatx4 g = out[e], u = out[(NM - 1) * NT * 64 + e];
+    for (int k = 1; k < waves; ++k) {
+      g += out[k * NM * NT * 64 + e];
+      u += out[(k * NM + NM - 1) * NT * 64 + e];
+    }
+    float* p = pre ? pre + (int64_t)t * 2 * I + r : nullptr;
+    TX* dst = h + (int64_t)t * ldh + r;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if (r + k >= I) continue;
+      if (what == GATED_UP) g[k] = p[k];
+      if (p && what != GATED_UP) p[k] = g[k];
+      if (what == GATED_GATE) continue;
+      if (p) p[I + k] = u[k];
+      dst[k] = rq_cast<TX>(rq_act(act, g[k]).f * u[k]);
+    }
+  }
+}
+
+template <typename TX, int NB, int MODE, int NM, int NT>
+void launch_gated(const TX* x, int T, int64_t ldx, const RqPacked& first, const RqPacked& second, int what, int act, float* pre,
+                  TX* h, int64_t ldh, hipStream_t s) {
+  const int bx = (first.R + 15) / 16, by = (T + 16 * NT - 1) / (16 * NT);
+  const int waves = waves_for(bx * by, (first.C + RQ_CHUNK - 1) / RQ_CHUNK, NM * NT, rows_threads(2, NT) / 64);
+  size_t lds = (size_t)waves * NM * NT * 1024;
+  const size_t scales = (size_t)((first.ngroups > second.ngroups ? first.ngroups : second.ngroups) + 1) * 16 * NM * 4;
+  const bool staged = MODE == RQ_ANY && scales <= 65536;
+  if (staged && lds < scales) lds = scales;
+  hipLaunchKernelGGL((k_packed_gated<TX, NB, MODE, NM, NT>), dim3(bx, by), dim3(64 * waves), lds, s, x, T, ldx, first, second, what,
+                     act, staged, pre, h, ldh);
+}
+
+template <typename TX, int NB, int MODE, int NM>
+void gated_of(const TX* x, int T, int64_t ldx, const RqPacked& first, const RqPacked& second, int what, int act, float* pre, TX* h,
+              int64_t ldh, hipStream_t s) {
+  constexpr int NT = RqOperand<TX>::pieces == 1 ? 4 : 2;
+  if (T <= 16) launch_gated<TX, NB, MODE, NM, 1>(x, T, ldx, first, second, what, act, pre, h, ldh, s);
+  else if (T <= 32) launch_gated<TX, NB, MODE, NM, 2>(x, T, ldx, first, second, what, act, pre, h, ldh, s);
+  else launch_gated<TX, NB, MODE, NM, NT>(x, T, ldx, first, second, what, act, pre, h, ldh, s);
+}
+template <typename TX, int NM>
+void gated_one(const TX* x, int T, int64_t ldx, const RqPacked& first, const RqPacked& second, int bits, int what, int act, float* pre,
+               TX* h, int64_t ldh, hipStream_t s) {
+  rq_with_nbits(bits, [&](auto nb) {
+    constexpr int NB = decltype(nb)::value;
+    switch (rq_mode_of(first)) {
+      case RQ_RUNS: gated_of<TX, NB, RQ_RUNS, NM>(x, T, ldx, first, second, what, act, pre, h, ldh, s); break;
+      case RQ_SMALL: gated_of<TX, NB, RQ_SMALL, NM>(x, T, ldx, first, second, what, act, pre, h, ldh, s); break;
+      default: gated_of<TX, NB, RQ_ANY, NM>(x, T, ldx, first, second, what, act, pre, h, ldh, s);
+    }
+  });
+}
+
+template <typename TX>
+__global__ __launch_bounds__(256) void k_gated_pre_grad(const TX* __restrict__ grad_h, int64_t ldg, int T, int I, int act,
+                                                        const float* __restrict__ pre, float* __restrict__ d) {
+  const int i = blockIdx.x * 256 + threadIdx.x, t = blockIdx.y;
+  if (i >= I) return;
+  const float g = rq_load_elem(grad_h + (int64_t)t * ldg + i);
+  const float a = pre[(int64_t)t * 2 * I + i], b = pre[(int64_t)t * 2 * I + I + i];
+  const RqAct v = rq_act(act, a);
+  d[(int64_t)t * I + i] = g * b * v.df;
+  d[((int64_t)T + t) * I + i] = g * v.f;
+}
+
+template <typename TX>
+__global__ __launch_bounds__(256) void k_gated_join(const float* __restrict__ part, int parts, int T, int C, TX* __restrict__ dx,
+                                                    int64_t ldx) {
+  const int c = blockIdx.x * 256 + threadIdx.x, t = blockIdx.y;
+  if (c >= C) return;
+  float s = 0.0f;
+  for (int p = 0; p < parts; ++p) s += part[((int64_t)p * T + t) * C + c];
+  dx[(int64_t)t * ldx + c] = rq_cast<TX>(s);
+}
+
+}  // namespace
+
+template <typename TX>
+void rq_gated_rows(const TX* x, int T, int64_t ldx, const RqPacked& gate, int gate_bits, const RqPacked& up, int up_bits,
+                   int act, float* pre, TX* h, int64_t ldh, hipStream_t s) {
+  if (rq_gated_together(gate, gate_bits, up, up_bits))
+    return gated_one<TX, 2>(x, T, ldx, gate, up, gate_bits, GATED_BOTH, act, pre, h, ldh, s);
+  gated_one<TX, 1>(x, T, ldx, gate, gate, gate_bits, GATED_GATE, act, pre, h, ldh, s);
+  gated_one<TX, 1>(x, T, ldx, up, up, up_bits, GATED_UP, act, pre, h, ldh, s);
+}
+template <typename TX>
+void rq_gated_pre_grad(const TX* grad_h, int64_t ldg, int T, int I, int act, const float* pre, float* d, hipStream_t s) {
+  hipLaunchKernelGGL(k_gated_pre_grad<TX>, dim3((I + 255) / 256, T), dim3(256), 0, s, grad_h, ldg, T, I, act, pre, d);
+}
+template <typename TX>
+void rq_gated_join(const float* part, int parts, int T, int C, TX* dx, int64_t ldx, hipStream_t s) {
+  hipLaunchKernelGGL(k_gated_join<TX>, dim3((C + 255) / 256, T), dim3(256), 0, s, part, parts, T, C, dx, ldx);
+}

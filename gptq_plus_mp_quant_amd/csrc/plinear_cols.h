@@ -280,7 +280,7 @@ template <typename TX, int NB, int MODE, int NT>
 void launch_cols(const TX* dy, int T, int64_t ldy, const RqPacked& w, const RqColSplit& sp, float* part, TX* dx, int64_t ldx,
                  hipStream_t s) {
   hipLaunchKernelGGL((k_packed_cols<TX, NB, MODE, NT>), dim3((w.C + COLS - 1) / COLS, sp.parts, (T + 16 * NT - 1) / (16 * NT)),
-                     dim3(64 * cols_waves(NT)), 0, s, dy, T, ldy, w, sp.steps_per, sp.parts > 1 ? part : nullptr, dx, ldx);
+                     dim3(64 * cols_waves(NT)), 0, s, dy, T, ldy, w, sp.steps_per, part, dx, ldx);
 }
 template <typename TX, int NB, int MODE>
 void linear_cols(const TX* dy, int T, int64_t ldy, const RqPacked& w, const RqColSplit& sp, float* part, TX* dx, int64_t ldx,
@@ -290,24 +290,35 @@ void linear_cols(const TX* dy, int T, int64_t ldy, const RqPacked& w, const RqCo
   else if (T <= 32) launch_cols<TX, NB, MODE, 2>(dy, T, ldy, w, sp, part, dx, ldx, s);
   else launch_cols<TX, NB, MODE, NT>(dy, T, ldy, w, sp, part, dx, ldx, s);
 }
+// T <= RQ_COL_TOKENS tokens to their parts [sp.parts, T, C], or, without parts, to dx.
+template <typename TX>
+void cols_of(const TX* dy, int T, int64_t ldy, const RqPacked& w, int nbits, const RqColSplit& sp, float* part, TX* dx,
+             int64_t ldx, hipStream_t s) {
+  rq_with_nbits(nbits, [&](auto nb) {
+    constexpr int NB = decltype(nb)::value;
+    if (rq_runs_of(w, COLS)) linear_cols<TX, NB, RQ_RUNS>(dy, T, ldy, w, sp, part, dx, ldx, s);
+    else if (w.groupsize > 0 && w.groupsize % 8 == 0) linear_cols<TX, NB, RQ_SMALL>(dy, T, ldy, w, sp, part, dx, ldx, s);
+    else linear_cols<TX, NB, RQ_ANY>(dy, T, ldy, w, sp, part, dx, ldx, s);
+  });
+}
 
 }  // namespace
 
 template <typename TX>
+void rq_cols_parts(const TX* dy, int T, int64_t ldy, const RqPacked& w, int nbits, const RqColSplit& sp, float* part,
+                   hipStream_t s) {
+  cols_of<TX>(dy, T, ldy, w, nbits, sp, part, nullptr, 0, s);
+}
+
+template <typename TX>
 void rq_linear_cols(const TX* dy, int T, int64_t ldy, const RqPacked& w, int nbits, float* part, TX* dx, int64_t ldx,
                     hipStream_t s) {
-  rq_with_nbits(nbits, [&](auto nb) {
-    constexpr int NB = decltype(nb)::value;
-    for (int64_t t0 = 0; t0 < T; t0 += RQ_COL_TOKENS) {
-      const int n = (int)(T - t0 < RQ_COL_TOKENS ? T - t0 : RQ_COL_TOKENS);
-      const RqColSplit sp = rq_col_split(n, w.R, w.C);
-      const TX* d = dy + t0 * ldy;
-      TX* out = dx + t0 * ldx;
-      if (rq_runs_of(w, COLS)) linear_cols<TX, NB, RQ_RUNS>(d, n, ldy, w, sp, part, out, ldx, s);
-      else if (w.groupsize > 0 && w.groupsize % 8 == 0) linear_cols<TX, NB, RQ_SMALL>(d, n, ldy, w, sp, part, out, ldx, s);
-      else linear_cols<TX, NB, RQ_ANY>(d, n, ldy, w, sp, part, out, ldx, s);
-      if (sp.parts > 1)
-        hipLaunchKernelGGL(k_packed_join<TX>, dim3((w.C + 255) / 256, n), dim3(256), 0, s, part, sp.parts, n, w.C, out, ldx);
-    }
-  });
+  for (int64_t t0 = 0; t0 < T; t0 += RQ_COL_TOKENS) {
+    const int n = (int)(T - t0 < RQ_COL_TOKENS ? T - t0 : RQ_COL_TOKENS);
+    const RqColSplit sp = rq_col_split(n, w.R, w.C);
+    TX* out = dx + t0 * ldx;
+    cols_of<TX>(dy + t0 * ldy, n, ldy, w, nbits, sp, sp.parts > 1 ? part : nullptr, out, ldx, s);
+    if (sp.parts > 1)
+      hipLaunchKernelGGL(k_packed_join<TX>, dim3((w.C + 255) / 256, n), dim3(256), 0, s, part, sp.parts, n, w.C, out, ldx);
+  }
 }

@@ -5,3 +5,4 @@
 
 template void rq_linear_rows<__half>(const __half*, int, int64_t, const RqPacked&, int, const __half*, __half*, int64_t, hipStream_t);
 template void rq_linear_cols<__half>(const __half*, int, int64_t, const RqPacked&, int, float*, __half*, int64_t, hipStream_t);
+template void rq_cols_parts<__half>(const __half*, int, int64_t, const RqPacked&, int, const RqColSplit&, float*, hipStream_t);

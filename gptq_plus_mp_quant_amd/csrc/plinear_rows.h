@@ -13,10 +13,15 @@ namespace {
 // the CU's load path with them, and vector instructions, mostly conversions, take 19 us.  Groups along an order (ANY)
 // 223 us there, a scale from LDS and an fp32 product for every weight; 1026 x 1365 at 5 bits, fp32, 7 tokens 9.7 us, 65
 // workgroups' latency.
+// MORE adds what else a row tile's sums take (RqNothing, or the low-rank term of plora_kernels.h).
 constexpr int rows_threads(int rt, int nt) { return rt * nt >= 2 ? 512 : 1024; }     // 256 or 128 registers a lane
-template <typename TX, int NB, int MODE, int RT, int NT>
+struct RqNothing {
+  template <int RT, int NT>
+  __device__ __forceinline__ void add(int, int, int, int, int, int, floatx4 (&)[RT][NT]) const {}
+};
+template <typename TX, int NB, int MODE, int RT, int NT, typename MORE>
 __global__ __launch_bounds__(rows_threads(RT, NT)) void k_packed_rows(const TX* __restrict__ x, int T, int64_t ldx, RqPacked w,
-                                                      const TX* __restrict__ bias, TX* __restrict__ y, int64_t ldy) {
+                                                      const TX* __restrict__ bias, TX* __restrict__ y, int64_t ldy, MORE more) {
   extern __shared__ __attribute__((aligned(16))) float lds[];
   const int lane = threadIdx.x & 63, wave = rq_wave(), waves = blockDim.x >> 6;
   const int r0 = blockIdx.x * 16 * RT, t0 = blockIdx.y * 16 * NT;
@@ -34,6 +39,7 @@ __global__ __launch_bounds__(rows_threads(RT, NT)) void k_packed_rows(const TX* 
 #pragma unroll
     for (int b = 0; b < NT; ++b) acc[a][b] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
   rq_rows_tokens<NB, MODE, RT, 1>({w}, r0, xs, wave, waves, staged ? lds : nullptr, acc);
+  more.add(r0, w.R, t0, T, wave, waves, acc);
   if (staged) __syncthreads();
   floatx4* out = reinterpret_cast<floatx4*>(lds);
 #pragma unroll
@@ -65,8 +71,9 @@ inline int waves_for(int tiles, int chunks, int per_wave_kb, int most) {
   return waves;
 }
 
-template <typename TX, int NB, int MODE, int RT, int NT>
-void launch_rows(const TX* x, int T, int64_t ldx, const RqPacked& w, const TX* bias, TX* y, int64_t ldy, hipStream_t s) {
+template <typename TX, int NB, int MODE, int RT, int NT, typename MORE>
+void launch_rows(const TX* x, int T, int64_t ldx, const RqPacked& w, const TX* bias, TX* y, int64_t ldy, const MORE& more,
+                 hipStream_t s) {
   const int bx = (w.R + 16 * RT - 1) / (16 * RT), by = (T + 16 * NT - 1) / (16 * NT);
   const int waves = waves_for(bx * by, (w.C + RQ_CHUNK - 1) / RQ_CHUNK, RT * NT, rows_threads(RT, NT) / 64);
   size_t lds = (size_t)waves * RT * NT * 1024;
@@ -74,13 +81,14 @@ void launch_rows(const TX* x, int T, int64_t ldx, const RqPacked& w, const TX* b
     const size_t scales = (size_t)(w.ngroups + 1) * 16 * RT * 4;
     lds = lds > scales ? lds : scales;
   }
-  hipLaunchKernelGGL((k_packed_rows<TX, NB, MODE, RT, NT>), dim3(bx, by), dim3(64 * waves), lds, s, x, T, ldx, w, bias, y,
-                     ldy);
+  hipLaunchKernelGGL((k_packed_rows<TX, NB, MODE, RT, NT, MORE>), dim3(bx, by), dim3(64 * waves), lds, s, x, T, ldx, w,
+                     bias, y, ldy, more);
 }
 
-template <typename TX, int NB>
-void linear_rows(const TX* x, int T, int64_t ldx, const RqPacked& w, const TX* bias, TX* y, int64_t ldy, hipStream_t s) {
-  constexpr int MORE = RqOperand<TX>::pieces == 1 ? 2 : 1;      // fp32's pieces leave registers for one row tile
+template <typename TX, int NB, typename MORE>
+void linear_rows(const TX* x, int T, int64_t ldx, const RqPacked& w, const TX* bias, TX* y, int64_t ldy, const MORE& more,
+                 hipStream_t s) {
+  constexpr int R2 = RqOperand<TX>::pieces == 1 ? 2 : 1;      // fp32's pieces leave registers for one row tile
   switch (rq_mode_of(w)) {
     case RQ_RUNS:
       // Two row tiles a wave share their tokens' loads.  Up to 16 tokens they are taken where they still make a workgroup
@@ -88,21 +96,21 @@ void linear_rows(const TX* x, int T, int64_t ldx, const RqPacked& w, const TX* b
       // CU holds one workgroup, as soon as one row tile makes more workgroups than there are CUs (24 / 64 tokens, one
       // and two: 4096 x 4096 11.0 / 19.7 and 12.0 / 21.9 us, 5120 x 4096 16.9 / 35.8 and 11.6 / 22.0, 8192 x 28672 98 / 216 and
       // 62 / 121).  Two token tiles up to 32 tokens: 4096 x 4096, 32 tokens 11.4 us for 14.5 with four.
-      if (T <= 16 && w.R >= 8192) launch_rows<TX, NB, RQ_RUNS, 2, 1>(x, T, ldx, w, bias, y, ldy, s);
-      else if (T <= 16) launch_rows<TX, NB, RQ_RUNS, 1, 1>(x, T, ldx, w, bias, y, ldy, s);
-      else if (T <= 32 && w.R > 4096) launch_rows<TX, NB, RQ_RUNS, MORE, 2>(x, T, ldx, w, bias, y, ldy, s);
-      else if (T <= 32) launch_rows<TX, NB, RQ_RUNS, 1, 2>(x, T, ldx, w, bias, y, ldy, s);
-      else if (w.R > 4096) launch_rows<TX, NB, RQ_RUNS, MORE, 4>(x, T, ldx, w, bias, y, ldy, s);
-      else launch_rows<TX, NB, RQ_RUNS, 1, 4>(x, T, ldx, w, bias, y, ldy, s);
+      if (T <= 16 && w.R >= 8192) launch_rows<TX, NB, RQ_RUNS, 2, 1>(x, T, ldx, w, bias, y, ldy, more, s);
+      else if (T <= 16) launch_rows<TX, NB, RQ_RUNS, 1, 1>(x, T, ldx, w, bias, y, ldy, more, s);
+      else if (T <= 32 && w.R > 4096) launch_rows<TX, NB, RQ_RUNS, R2, 2>(x, T, ldx, w, bias, y, ldy, more, s);
+      else if (T <= 32) launch_rows<TX, NB, RQ_RUNS, 1, 2>(x, T, ldx, w, bias, y, ldy, more, s);
+      else if (w.R > 4096) launch_rows<TX, NB, RQ_RUNS, R2, 4>(x, T, ldx, w, bias, y, ldy, more, s);
+      else launch_rows<TX, NB, RQ_RUNS, 1, 4>(x, T, ldx, w, bias, y, ldy, more, s);
       break;
     case RQ_SMALL:
       // One row tile: with two 4096 x 4096 4-bit bf16 in groups of 64 takes 18.6 us for 11.2 (4 tokens), 29.1 for 21.9 (64).
-      if (T <= 16) launch_rows<TX, NB, RQ_SMALL, 1, 1>(x, T, ldx, w, bias, y, ldy, s);
-      else launch_rows<TX, NB, RQ_SMALL, 1, 4>(x, T, ldx, w, bias, y, ldy, s);
+      if (T <= 16) launch_rows<TX, NB, RQ_SMALL, 1, 1>(x, T, ldx, w, bias, y, ldy, more, s);
+      else launch_rows<TX, NB, RQ_SMALL, 1, 4>(x, T, ldx, w, bias, y, ldy, more, s);
       break;
     default:
-      if (T <= 16) launch_rows<TX, NB, RQ_ANY, 1, 1>(x, T, ldx, w, bias, y, ldy, s);
-      else launch_rows<TX, NB, RQ_ANY, 1, 4>(x, T, ldx, w, bias, y, ldy, s);
+      if (T <= 16) launch_rows<TX, NB, RQ_ANY, 1, 1>(x, T, ldx, w, bias, y, ldy, more, s);
+      else launch_rows<TX, NB, RQ_ANY, 1, 4>(x, T, ldx, w, bias, y, ldy, more, s);
   }
 }
 
@@ -114,6 +122,6 @@ void rq_linear_rows(const TX* x, int T, int64_t ldx, const RqPacked& w, int nbit
   rq_with_nbits(nbits, [&](auto nb) {
     for (int64_t t0 = 0; t0 < T; t0 += TOKENS_PER_LAUNCH)
       linear_rows<TX, decltype(nb)::value>(x + t0 * ldx, (int)(T - t0 < TOKENS_PER_LAUNCH ? T - t0 : TOKENS_PER_LAUNCH),
-                                           ldx, w, bias, y + t0 * ldy, ldy, s);
+                                           ldx, w, bias, y + t0 * ldy, ldy, RqNothing{}, s);
   });
 }

@@ -23,3 +23,8 @@ inline RqColSplit rq_col_split(int T, int R, int C) {
   const int per = (steps + parts - 1) / parts;
   return RqColSplit{(steps + per - 1) / per, per};
 }
+
+// The gradient's parts [sp.parts, T, C] of T <= RQ_COL_TOKENS tokens, to be joined by the caller in their order.
+template <typename TX>
+void rq_cols_parts(const TX* dy, int T, int64_t ldy, const RqPacked& w, int nbits, const RqColSplit& sp, float* part,
+                   hipStream_t s);

@@ -1,0 +1,53 @@
+// Low-rank adapters beside a packed weight: what the launches share.  Each element type's kernels are a translation
+// unit of their own.
+#pragma once
+#include "plinear_types.h"
+
+constexpr int LORA_MAX_RANK = 256;
+
+// n adapters of rank r: a [n, r, C], b [n, R, r], both contiguous.  Token t's is ids[t] (below 0: none; n or more: one
+// that does not exist, whose results are NaN), or the first where there are no ids.
+template <typename TX>
+struct RqLora {
+  const TX* a;
+  const TX* b;
+  const int64_t* ids;
+  const float* scaling;     // [n] or NULL: scale for all
+  float scale;
+  int n, r;
+  __device__ __forceinline__ int of(int64_t t) const {
+    if (!ids) return 0;
+    const int64_t i = ids[t];
+    return i < 0 ? -1 : i < n ? (int)i : n;
+  }
+  __device__ __forceinline__ float scale_of(int i) const { return scaling ? scaling[i] : scale; }
+};
+
+// What a token's adapter makes of its row: [parts, T, ranks], ranks past the last 0; rows of tokens without an adapter
+// are not written.  Each part sums RQ_LORA_COLS columns.
+struct RqLow {
+  float* u;
+  int parts, T, ranks;
+  __device__ __forceinline__ int64_t at(int p, int64_t t) const { return ((int64_t)p * T + t) * ranks; }
+};
+constexpr int RQ_LORA_COLS = 4096;
+inline RqLow rq_low(float* u, int T, int cols, int r) {
+  return RqLow{u, (cols - 1) / RQ_LORA_COLS + 1, T, (r + 15) / 16 * 16};
+}
+inline int64_t rq_low_floats(const RqLow& l) { return (int64_t)l.parts * l.T * l.ranks; }
+
+// low.u[t] = A x_t (ROWS: x [T, C] with lora.a) or B^T x_t (x [T, R] with lora.b).
+template <typename TX>
+void rq_lora_down(const TX* x, int T, int64_t ldx, int cols, bool rows, const RqLora<TX>& lora, const RqLow& low, hipStream_t s);
+// y = x W^T (+ bias) + s B u
+template <typename TX>
+void rq_lora_rows(const TX* x, int T, int64_t ldx, const RqPacked& w, int nbits, const TX* bias, const RqLora<TX>& lora,
+                  const RqLow& low, TX* y, int64_t ldy, hipStream_t s);
+// dx of tokens t0..t0+T-1 = the sum of parts [parts, T, C] + s A^T v
+template <typename TX>
+void rq_lora_dx(const float* part, int parts, int64_t t0, int T, int C, const RqLora<TX>& lora, const RqLow& v, TX* dx,
+                int64_t ldx, hipStream_t s);
+// da [n, r, C] = s sum_t v_t x_t^T and db [n, R, r] = s sum_t dy_t u_t^T over each adapter's tokens
+template <typename TX>
+void rq_lora_outer(const TX* x, int64_t ldx, int C, const TX* dy, int64_t ldy, int R, int T, const RqLora<TX>& lora,
+                   const RqLow& u, const RqLow& v, TX* da, TX* db, hipStream_t s);

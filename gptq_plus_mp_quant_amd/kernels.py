@@ -584,6 +584,75 @@ def packed_moe(x, router, T, D, I, E, gate, up, down, top_k, norm_topk, want_rou
 
 
 @nat.on_device_of_first
+def packed_linear_lora(x, qweight, nbits, scales, T, R, C, ngroups, g_idx, groupsize, bias, lora_a, lora_b, n, r, ids, scaling,
+                       scale, lead):
+    """y [*lead, R] = x [T, C] times the transpose of a packed weight, with low-rank adapters; see rq_packed_linear_lora."""
+    lib = nat.load()
+    y = x.new_empty((*lead, R))
+    nbytes = lib.rq_packed_linear_lora_workspace_bytes(T, C, r)
+    ws = torch.empty(max(nbytes, 0), dtype=torch.uint8, device=x.device)
+    nat.check("rq_packed_linear_lora", lib.rq_packed_linear_lora(
+        x.data_ptr(), nat.DTYPE_CODES[x.dtype], T, x.stride(0), C, qweight.data_ptr(), qweight.stride(0), nbits, R,
+        scales.data_ptr(), scales.stride(0), ngroups, g_idx.data_ptr(), groupsize, _addr(bias), lora_a.data_ptr(),
+        lora_b.data_ptr(), n, r, _addr(ids), _addr(scaling), scale, y.data_ptr(), R, ws.data_ptr(), nbytes, nat.raw_stream(x)))
+    return y
+
+
+@nat.on_device_of_first
+def packed_linear_lora_grad(grad_y, x, qweight, nbits, scales, T, R, C, ngroups, g_idx, groupsize, lora_a, lora_b, n, r, ids,
+                            scaling, scale, lead, want_x=True, want_lora=True):
+    """(grad_x [*lead, C], grad_a, grad_b in lora_a's and lora_b's shapes), None where not wanted; see
+    rq_packed_linear_lora_grad."""
+    lib = nat.load()
+    gx = grad_y.new_empty((*lead, C)) if want_x else None
+    ga, gb = (torch.empty_like(lora_a), torch.empty_like(lora_b)) if want_lora else (None, None)
+    nbytes = lib.rq_packed_linear_lora_grad_workspace_bytes(T, R, C, r)
+    ws = torch.empty(max(nbytes, 0), dtype=torch.uint8, device=grad_y.device)
+    nat.check("rq_packed_linear_lora_grad", lib.rq_packed_linear_lora_grad(
+        grad_y.data_ptr(), nat.DTYPE_CODES[grad_y.dtype], T, grad_y.stride(0), x.data_ptr(), x.stride(0), C, qweight.data_ptr(),
+        qweight.stride(0), nbits, R, scales.data_ptr(), scales.stride(0), ngroups, g_idx.data_ptr(), groupsize, lora_a.data_ptr(),
+        lora_b.data_ptr(), n, r, _addr(ids), _addr(scaling), scale, _addr(gx), C, _addr(ga), _addr(gb), ws.data_ptr(), nbytes,
+        nat.raw_stream(grad_y)))
+    return gx, ga, gb
+
+
+def _weight(qweight, nbits, scales, ngroups, g_idx, groupsize):
+    return nat.PackedWeight(qweight.data_ptr(), scales.data_ptr(), g_idx.data_ptr(), qweight.stride(0), scales.stride(0), nbits,
+                            ngroups, groupsize)
+
+
+@nat.on_device_of_first
+def packed_gated(x, gate, up, T, I, C, activation, want_pre, lead):
+    """h [*lead, I] of x [T, C] (and the products, fp32 [*lead, 2, I], or None); gate / up: (qweight, nbits, scales, ngroups,
+    g_idx, groupsize); see rq_packed_gated."""
+    lib = nat.load()
+    h = x.new_empty((*lead, I))
+    pre = x.new_empty((*lead, 2, I), dtype=_f32) if want_pre else None
+    g, u = _weight(*gate), _weight(*up)
+    g, u = ctypes.byref(g), ctypes.byref(u)
+    nbytes = 0 if want_pre else lib.rq_packed_gated_workspace_bytes(T, I, C, g, u)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes > 0 else None
+    nat.check("rq_packed_gated", lib.rq_packed_gated(
+        x.data_ptr(), nat.DTYPE_CODES[x.dtype], T, x.stride(0), C, I, g, u, activation, _addr(pre), h.data_ptr(), I, _addr(ws),
+        nbytes, nat.raw_stream(x)))
+    return h, pre
+
+
+@nat.on_device_of_first
+def packed_gated_grad(grad_h, pre, gate, up, T, I, C, activation, lead):
+    """grad_x [*lead, C] in grad_h's dtype; see rq_packed_gated_grad."""
+    lib = nat.load()
+    gx = grad_h.new_empty((*lead, C))
+    nbytes = lib.rq_packed_gated_grad_workspace_bytes(T, I, C)
+    ws = torch.empty(max(nbytes, 0), dtype=torch.uint8, device=grad_h.device)
+    g, u = _weight(*gate), _weight(*up)
+    nat.check("rq_packed_gated_grad", lib.rq_packed_gated_grad(
+        grad_h.data_ptr(), nat.DTYPE_CODES[grad_h.dtype], T, grad_h.stride(0), I, pre.data_ptr(), activation, ctypes.byref(g),
+        ctypes.byref(u), C, gx.data_ptr(), C, ws.data_ptr(), nbytes, nat.raw_stream(grad_h)))
+    return gx
+
+
+@nat.on_device_of_first
 def token_logprobs(logits, targets, N, V, top_k, ignore_index, lead):
     """(logprob, entropy, top_ids, top_logprobs, stats) of N = prod(lead) rows: lead, lead, [*lead, k] twice and
     [*lead, 3], none a view of another (so that each may be edited in place); see rq_token_logprobs."""
@@ -607,4 +676,28 @@ def token_logprobs_grad(logits, targets, N, V, ignore_index, stats, grad_logprob
     nat.check("rq_token_logprobs_grad", nat.load().rq_token_logprobs_grad(
         logits.data_ptr(), nat.DTYPE_CODES[logits.dtype], N, logits.stride(0), V, targets.data_ptr(), ignore_index,
         stats.data_ptr(), grad_logprob.data_ptr(), _addr(grad_entropy), gz.data_ptr(), V, nat.raw_stream(logits)))
+    return gz
+
+
+@nat.on_device_of_first
+def distill_loss(logits, ids, teacher, N, V, K, temperature, tail, lead):
+    """(loss [*lead], stats [*lead, 8]) of N = prod(lead) rows; see rq_distill_loss."""
+    lib = nat.load()
+    loss = logits.new_empty((*lead,), dtype=_f32)
+    stats = loss.new_empty((*lead, nat.RQ_DISTILL_STATS))
+    nbytes = lib.rq_distill_loss_workspace_bytes(N, V)
+    ws = loss.new_empty(nbytes, dtype=torch.uint8) if nbytes > 0 else None
+    nat.check("rq_distill_loss", lib.rq_distill_loss(
+        logits.data_ptr(), nat.DTYPE_CODES[logits.dtype], N, logits.stride(0), V, ids.data_ptr(), teacher.data_ptr(), K, temperature,
+        tail, loss.data_ptr(), stats.data_ptr(), _addr(ws), nbytes, nat.raw_stream(logits)))
+    return loss, stats
+
+
+@nat.on_device_of_first
+def distill_loss_grad(logits, ids, teacher, N, V, K, temperature, tail, stats, grad_loss, lead):
+    """grad_logits [*lead, V], N = prod(lead), in the logits' dtype; see rq_distill_loss_grad."""
+    gz = logits.new_empty((*lead, V))
+    nat.check("rq_distill_loss_grad", nat.load().rq_distill_loss_grad(
+        logits.data_ptr(), nat.DTYPE_CODES[logits.dtype], N, logits.stride(0), V, ids.data_ptr(), teacher.data_ptr(), K, temperature,
+        tail, stats.data_ptr(), grad_loss.data_ptr(), gz.data_ptr(), V, nat.raw_stream(logits)))
     return gz

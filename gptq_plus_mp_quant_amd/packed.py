@@ -5,6 +5,9 @@ here compute with that form; the dequantized weight is never written out:
 
 * ``packed_linear(x, entry)`` -- ``x W^T`` (+ bias) for a few tokens; differentiable in ``x``.
 * ``packed_linear_backward(grad_y, entry)`` -- the gradient of ``x`` alone.
+* ``packed_gated(x, gate, up)`` -- the gated half of a feed-forward block, ``act(gate(x)) * up(x)``; differentiable in
+  ``x``.
+* ``packed_gated_backward(grad_h, pre, gate, up)`` -- the gradient of its ``x`` alone.
 * ``packed_moe(x, router, gate, up, down, top_k)`` -- a mixture-of-experts layer whose experts' linears
   are packed, each of the three stacked over the experts by ``stack_packed``.
 
@@ -29,7 +32,7 @@ def _rows_apart(t):
     return t.clone(memory_format=torch.contiguous_format)
 
 
-def _checked(entry: Dict[str, object], batch: int):
+def checked_entry(entry: Dict[str, object], batch: int):
     """(qweight, nbits, scales, R, C, ngroups, g_idx, groupsize) of an entry (batch = 1: stacked over
     experts)."""
     q, scales, g_idx, nbits = entry["qweight"], entry["scales"], entry["g_idx"], entry["nbits"]
@@ -64,7 +67,7 @@ def _checked(entry: Dict[str, object], batch: int):
             g_idx if g_idx.is_contiguous() else g_idx.contiguous(), groupsize)
 
 
-def _tokens(x, width, q, name):
+def checked_tokens(x, width, q, name):
     """x as [T, width] with unit column stride (copied only if its strides need it), T, and x's leading
     dimensions."""
     if not (isinstance(x, torch.Tensor) and x.is_cuda):
@@ -87,6 +90,14 @@ def _tokens(x, width, q, name):
     return x2, T, (T,) if x2 is x else shape[:-1]
 
 
+def checked_bias(bias, x, R):
+    if bias is None:
+        return None
+    if not isinstance(bias, torch.Tensor) or bias.dtype != x.dtype or bias.shape != (R,) or bias.device != x.device:
+        raise ValueError(f"bias must be {x.dtype} [{R}] on {x.device}")
+    return bias.contiguous()
+
+
 class _PackedLinear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, entry, bias):
@@ -107,13 +118,9 @@ class _PackedLinear(torch.autograd.Function):
 
 
 def _forward(x, entry, bias):
-    q, nbits, scales, R, C, ng, g_idx, groupsize = _checked(entry, 0)
-    x2, T, lead = _tokens(x, C, q, "x")
-    if bias is not None:
-        if not isinstance(bias, torch.Tensor) or bias.dtype != x.dtype or bias.shape != (R,) or bias.device != x.device:
-            raise ValueError(f"bias must be {x.dtype} [{R}] on {x.device}")
-        bias = bias.contiguous()
-    return K.packed_linear(x2, q, nbits, scales, T, R, C, ng, g_idx, groupsize, bias, lead)
+    q, nbits, scales, R, C, ng, g_idx, groupsize = checked_entry(entry, 0)
+    x2, T, lead = checked_tokens(x, C, q, "x")
+    return K.packed_linear(x2, q, nbits, scales, T, R, C, ng, g_idx, groupsize, checked_bias(bias, x, R), lead)
 
 
 def packed_linear(x: torch.Tensor, entry: Dict[str, object], bias: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -127,7 +134,7 @@ def packed_linear(x: torch.Tensor, entry: Dict[str, object], bias: Optional[torc
         if bias is not None and getattr(bias, "requires_grad", False):
             raise ValueError("packed_linear: the bias of a packed linear is a constant; detach it")
         if isinstance(x, torch.Tensor) and x.requires_grad:
-            _checked(entry, 0)                       # under autograd; forward runs without
+            checked_entry(entry, 0)                       # under autograd; forward runs without
             return _PackedLinear.apply(x, entry, bias)
     return _forward(x, entry, bias)
 
@@ -145,8 +152,8 @@ class _PackedLinearGrad(torch.autograd.Function):
 
 
 def _backward(grad_y, entry):
-    q, nbits, scales, R, C, ng, g_idx, groupsize = _checked(entry, 0)
-    g2, T, lead = _tokens(grad_y, R, q, "grad_y")
+    q, nbits, scales, R, C, ng, g_idx, groupsize = checked_entry(entry, 0)
+    g2, T, lead = checked_tokens(grad_y, R, q, "grad_y")
     return K.packed_linear_grad(g2, q, nbits, scales, T, R, C, ng, g_idx, groupsize, lead)
 
 
@@ -155,9 +162,110 @@ def packed_linear_backward(grad_y: torch.Tensor, entry: Dict[str, object]) -> to
     grad_y's dtype.  The result does not change from run to run.  It cannot be differentiated further."""
     nat.refuse_tangents("packed_linear_backward", grad_y, entry["scales"])
     if torch.is_grad_enabled() and isinstance(grad_y, torch.Tensor) and grad_y.requires_grad:
-        _checked(entry, 0)
+        checked_entry(entry, 0)
         return _PackedLinearGrad.apply(grad_y, entry)
     return _backward(grad_y, entry)
+
+
+def _pair(gate, up, name):
+    """The checked tensors of gate and up, I and C."""
+    g, u = checked_entry(gate, 0), checked_entry(up, 0)
+    if g[3:5] != u[3:5]:
+        raise ValueError(f"{name}: gate and up must have one shape, got {g[3]} x {g[4]} and {u[3]} x {u[4]}")
+    if g[0].get_device() != u[0].get_device():
+        raise ValueError(f"{name}: gate and up are on different devices")
+    return (*((q, nbits, scales, ng, gi, gs) for q, nbits, scales, _, _, ng, gi, gs in (g, u)), g[3], g[4])
+
+
+def _activation(activation):
+    if activation not in nat.ACTIVATIONS:
+        raise ValueError(f"activation must be one of {sorted(nat.ACTIVATIONS)}, got {activation!r}")
+    return nat.ACTIVATIONS[activation]
+
+
+def _gated(x, gate, up, activation, want_pre):
+    g, u, I, C = _pair(gate, up, "packed_gated")
+    x2, T, lead = checked_tokens(x, C, g[0], "x")
+    if T > nat.RQ_MAX_TOKENS:
+        raise ValueError(f"packed_gated: {T} tokens, at most {nat.RQ_MAX_TOKENS} in one call")
+    return K.packed_gated(x2, g, u, T, I, C, _activation(activation), want_pre, lead)
+
+
+def _gated_backward(grad_h, pre, gate, up, activation):
+    g, u, I, C = _pair(gate, up, "packed_gated_backward")
+    g2, T, lead = checked_tokens(grad_h, I, g[0], "grad_h")
+    if T > nat.RQ_MAX_TOKENS:
+        raise ValueError(f"packed_gated_backward: {T} tokens, at most {nat.RQ_MAX_TOKENS} in one call")
+    if not isinstance(pre, torch.Tensor) or pre.dtype is not torch.float32 or pre.shape != (*lead, 2, I) or \
+            pre.get_device() != grad_h.get_device():
+        raise ValueError(f"pre (packed_gated's) must be float32 {[*lead, 2, I]} on {grad_h.device}")
+    return K.packed_gated_grad(g2, pre.contiguous(), g, u, T, I, C, _activation(activation), lead)
+
+
+class _PackedGated(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, gate, up, activation):
+        h, pre = _gated(x, gate, up, activation, True)
+        # the tensors, not the dicts, as in _PackedLinear
+        weights = [e[k] for e in (gate, up) for k in ("qweight", "scales", "g_idx")]
+        ctx.unsaved = weights if any(t.is_inference() for t in weights) else None
+        ctx.save_for_backward(pre, *(() if ctx.unsaved else weights))
+        ctx.fields = [dict(nbits=e["nbits"], groupsize=e.get("groupsize", 0)) for e in (gate, up)]
+        ctx.activation = activation
+        ctx.mark_non_differentiable(pre)
+        return h, pre
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_h, _):
+        pre, *weights = ctx.saved_tensors
+        weights = ctx.unsaved or weights
+        gate, up = (dict(zip(("qweight", "scales", "g_idx"), weights[3 * k:]), **f) for k, f in enumerate(ctx.fields))
+        return _gated_backward(grad_h, pre, gate, up, ctx.activation), None, None, None
+
+
+def packed_gated(x: torch.Tensor, gate: Dict[str, object], up: Dict[str, object], activation: str = "silu",
+                 return_pre: bool = False):
+    """The gated half of a feed-forward block in one pass over its weights: ``x [..., C]`` -> ``act(x Wg^T) * (x Wu^T)``,
+    ``[..., I]`` in x's dtype (fp16, bf16 or fp32); ``packed_linear`` with the down projection completes it.
+
+    ``gate`` and ``up`` are entries of one shape, each with bits and groups of its own (one launch where those
+    agree).  ``activation``: "silu", "gelu" (erf) or "gelu_tanh".  Sums and products are fp32, rounded once.  ``return_pre``
+    adds both projections, fp32 ``[..., 2, I]``, for ``packed_gated_backward``.
+
+    Differentiable in ``x`` (not through ``pre``); the weights are constants, forward-mode tangents are refused.  Made for few
+    tokens, as ``packed_linear`` is; at most 2^19."""
+    nat.refuse_tangents("packed_gated", x, gate["scales"], up["scales"])
+    if torch.is_grad_enabled() and isinstance(x, torch.Tensor) and x.requires_grad:
+        _pair(gate, up, "packed_gated")              # under autograd; forward runs without
+        h, pre = _PackedGated.apply(x, gate, up, activation)
+    else:
+        h, pre = _gated(x, gate, up, activation, return_pre)
+    return (h, pre) if return_pre else h
+
+
+class _PackedGatedGrad(torch.autograd.Function):
+    """The gradient from inputs that require grad: no constant, so a derivative of it is refused."""
+    @staticmethod
+    def forward(ctx, grad_h, pre, gate, up, activation):
+        return _gated_backward(grad_h, pre, gate, up, activation)
+
+    @staticmethod
+    def backward(ctx, _):
+        raise NotImplementedError("packed_gated_backward has no backward pass: call it under torch.no_grad() or on "
+                                  "detached tensors")
+
+
+def packed_gated_backward(grad_h: torch.Tensor, pre: torch.Tensor, gate: Dict[str, object], up: Dict[str, object],
+                          activation: str = "silu") -> torch.Tensor:
+    """The gradient of ``packed_gated``'s x from the gradient of its result ``[..., I]``, in grad_h's dtype; ``pre`` is what
+    ``packed_gated(..., return_pre=True)`` returned beside it.  The result does not change from run to run.  It cannot be
+    differentiated further."""
+    nat.refuse_tangents("packed_gated_backward", grad_h, pre, gate["scales"], up["scales"])
+    if torch.is_grad_enabled() and any(getattr(t, "requires_grad", False) for t in (grad_h, pre)):
+        _pair(gate, up, "packed_gated_backward")
+        return _PackedGatedGrad.apply(grad_h, pre, gate, up, activation)
+    return _gated_backward(grad_h, pre, gate, up, activation)
 
 
 def stack_packed(entries: Sequence[Dict[str, object]]) -> Dict[str, object]:
@@ -169,7 +277,7 @@ def stack_packed(entries: Sequence[Dict[str, object]]) -> Dict[str, object]:
         raise ValueError("stack_packed: no entries")
     first = entries[0]
     for e in entries:
-        _checked(e, 0)
+        checked_entry(e, 0)
         if int(e["nbits"]) != int(first["nbits"]) or e["qweight"].shape != first["qweight"].shape or \
                 e["scales"].shape != first["scales"].shape or e["g_idx"].shape != first["g_idx"].shape:
             raise ValueError("stack_packed: the experts' entries differ in bits, shape or groups")
@@ -193,13 +301,13 @@ def packed_moe(x: torch.Tensor, router: torch.Tensor, gate: Dict[str, object], u
     nat.refuse_tangents("packed_moe", x, router, gate["scales"], up["scales"], down["scales"])
     if torch.is_grad_enabled() and (getattr(x, "requires_grad", False) or getattr(router, "requires_grad", False)):
         raise NotImplementedError("packed_moe has no backward pass: call it under torch.no_grad() or on detached tensors")
-    g, u, d = _checked(gate, 1), _checked(up, 1), _checked(down, 1)
+    g, u, d = checked_entry(gate, 1), checked_entry(up, 1), checked_entry(down, 1)
     E, I, D = g[0].shape[0], g[3], g[4]
     if u[0].shape[0] != E or d[0].shape[0] != E or u[3] != I or u[4] != D or d[3] != D or d[4] != I:
         raise ValueError("packed_moe: gate and up must be [E, I x D] and down [E, D x I]")
     if not u[0].get_device() == d[0].get_device() == g[0].get_device():
         raise ValueError("packed_moe: gate, up and down are on different devices")
-    x2, T, _ = _tokens(x, D, g[0], "x")
+    x2, T, _ = checked_tokens(x, D, g[0], "x")
     if not isinstance(router, torch.Tensor) or router.shape != (E, D) or router.dtype != x.dtype or router.device != x.device:
         raise ValueError(f"packed_moe: router must be {x.dtype} [{E}, {D}] on {x.device}")
     top_k = int(top_k)

@@ -27,8 +27,8 @@ class TokenLogprobs(NamedTuple):
     stats: torch.Tensor
 
 
-def _rows(logits, targets):
-    """(logits [N, V] with unit column stride, targets [N], N, V, the leading dimensions)."""
+def logit_rows(logits):
+    """(logits [N, V] with unit column stride, N, V, the leading dimensions)."""
     if not (isinstance(logits, torch.Tensor) and logits.is_cuda):
         nat.require_gpu(logits, "logits")
     if logits.dtype not in nat.DTYPE_CODES:
@@ -36,10 +36,6 @@ def _rows(logits, targets):
     shape = logits.shape
     if len(shape) < 1 or shape[-1] == 0:
         raise ValueError("logits must be [..., V] with V > 0")
-    lead = shape[:-1]
-    if not isinstance(targets, torch.Tensor) or targets.dtype is not torch.int64 or targets.shape != lead or \
-            targets.get_device() != logits.get_device():
-        raise ValueError(f"targets must be int64 {list(lead)} on {logits.device}")
     V = shape[-1]
     z = logits if len(shape) == 2 else logits.reshape(-1, V)
     s0, s1 = z.stride()
@@ -47,8 +43,17 @@ def _rows(logits, targets):
         z = z.contiguous()
         if z.stride(0) < V:                      # one row: its stride is never used
             z = z.as_strided((z.shape[0], V), (V, 1))
+    return z, z.shape[0], V, shape[:-1]
+
+
+def _rows(logits, targets):
+    """(logits [N, V] with unit column stride, targets [N], N, V, the leading dimensions)."""
+    z, N, V, lead = logit_rows(logits)
+    if not isinstance(targets, torch.Tensor) or targets.dtype is not torch.int64 or targets.shape != lead or \
+            targets.get_device() != logits.get_device():
+        raise ValueError(f"targets must be int64 {list(lead)} on {logits.device}")
     t = targets if targets.dim() == 1 else targets.reshape(-1)
-    return z, t if t.is_contiguous() else t.contiguous(), z.shape[0], V, lead
+    return z, t if t.is_contiguous() else t.contiguous(), N, V, lead
 
 
 def _forward(logits, targets, top_k, ignore_index):
@@ -89,7 +94,7 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, top_k: int = 0, 
     return _forward(logits, targets, top_k, ignore_index)
 
 
-def _row_values(g, lead, like, name):
+def row_values(g, lead, like, name):
     """A float32 tensor of the given shape on like's device, contiguous."""
     if not isinstance(g, torch.Tensor) or g.dtype is not torch.float32 or g.shape != lead or \
             g.get_device() != like.get_device():
@@ -111,9 +116,9 @@ class _TokenLogprobsGrad(torch.autograd.Function):
 
 def _backward(logits, targets, stats, grad_logprob, grad_entropy, ignore_index):
     z, t, N, V, lead = _rows(logits, targets)
-    gl = _row_values(grad_logprob, lead, logits, "grad_logprob")
-    gh = None if grad_entropy is None else _row_values(grad_entropy, lead, logits, "grad_entropy")
-    stats = _row_values(stats, (*lead, 3), logits, "stats (token_logprobs')")
+    gl = row_values(grad_logprob, lead, logits, "grad_logprob")
+    gh = None if grad_entropy is None else row_values(grad_entropy, lead, logits, "grad_entropy")
+    stats = row_values(stats, (*lead, 3), logits, "stats (token_logprobs')")
     return K.token_logprobs_grad(z, t, N, V, int(ignore_index), stats, gl, gh, lead)
 
 

@@ -399,6 +399,60 @@ int rq_packed_moe(const void* x, int dtype, int T, int64_t ldx, int D, const voi
                   int* ids_out, float* weights_out, void* workspace, int64_t workspace_bytes,
                   void* stream);
 
+/* y_t = W x_t (+ bias) + s_a B_a (A_a x_t): a packed linear with low-rank adapters of several requests.
+ * lora_a [n, r, C] and lora_b [n, R, r] of type dtype, contiguous, n <= 65535, r <= 256; adapter_ids [T]: the
+ * adapter a of every token, none below 0, NaN results from n on; NULL: adapter 0 for all.  s_a =
+ * scaling[a] (fp32 [n]) or, with scaling NULL, scale.  The rest as rq_packed_linear, T <= 2^19; A x is
+ * fp32.  workspace: rq_packed_linear_lora_workspace_bytes(T, C, r) bytes, any contents. */
+int64_t rq_packed_linear_lora_workspace_bytes(int T, int C, int r);
+int rq_packed_linear_lora(const void* x, int dtype, int T, int64_t ldx, int C, const uint32_t* qweight,
+                          int64_t ldp, int nbits, int R, const float* scales, int64_t lds, int ngroups,
+                          const int32_t* g_idx, int groupsize, const void* bias, const void* lora_a,
+                          const void* lora_b, int n, int r, const int64_t* adapter_ids,
+                          const float* scaling, float scale, void* y, int64_t ldy, void* workspace,
+                          int64_t workspace_bytes, void* stream);
+
+/* Its gradients: grad_x [T, C] = W^T dy + s A^T B^T dy (NULL: not wanted), grad_a [n, r, C] = s sum_t (B^T
+ * dy_t) x_t^T and grad_b [n, R, r] = s sum_t dy_t (A x_t)^T over each adapter's tokens, 0 without any (both
+ * NULL: not wanted), all of type dtype.  Sums are joined in a fixed order.  workspace:
+ * rq_packed_linear_lora_grad_workspace_bytes(T, R, C, r) bytes, any contents. */
+int64_t rq_packed_linear_lora_grad_workspace_bytes(int T, int R, int C, int r);
+int rq_packed_linear_lora_grad(const void* grad_y, int dtype, int T, int64_t ldg, const void* x,
+                               int64_t ldx, int C, const uint32_t* qweight, int64_t ldp, int nbits, int R,
+                               const float* scales, int64_t lds, int ngroups, const int32_t* g_idx,
+                               int groupsize, const void* lora_a, const void* lora_b, int n, int r,
+                               const int64_t* adapter_ids, const float* scaling, float scale,
+                               void* grad_x, int64_t ldgx, void* grad_a, void* grad_b, void* workspace,
+                               int64_t workspace_bytes, void* stream);
+
+/* One packed weight. */
+typedef struct {
+  const uint32_t* qweight;
+  const float* scales;
+  const int32_t* g_idx;
+  int64_t ldp, lds;
+  int nbits, ngroups, groupsize;
+} rq_packed_weight;
+
+/* h [T, I] = act(x Wg^T) * (x Wu^T), the gated half of a feed-forward block: x [T, C] and h of type dtype,
+ * gate and up I x C, each with bits and groups of its own; T <= 2^19.  activation: 0 SiLU, 1 GELU, 2 GELU
+ * with tanh.  pre (optional, fp32 [T, 2, I]) receives both products for rq_packed_gated_grad.  workspace:
+ * rq_packed_gated_workspace_bytes(...) bytes, any contents (0, NULL, where both weights have the same
+ * bits and kind of groups; unused where pre is given). */
+int64_t rq_packed_gated_workspace_bytes(int T, int I, int C, const rq_packed_weight* gate,
+                                        const rq_packed_weight* up);
+int rq_packed_gated(const void* x, int dtype, int T, int64_t ldx, int C, int I,
+                    const rq_packed_weight* gate, const rq_packed_weight* up, int activation, float* pre,
+                    void* h, int64_t ldh, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* grad_x [T, C] = (dh b act'(a)) Wg + (dh act(a)) Wu with (a, b) = pre [T, 2, I]: the gradient of its x,
+ * in dtype (grad_h's).  workspace: rq_packed_gated_grad_workspace_bytes(T, I, C) bytes, any contents (partial
+ * sums, joined in a fixed order). */
+int64_t rq_packed_gated_grad_workspace_bytes(int T, int I, int C);
+int rq_packed_gated_grad(const void* grad_h, int dtype, int T, int64_t ldg, int I, const float* pre,
+                         int activation, const rq_packed_weight* gate, const rq_packed_weight* up, int C,
+                         void* grad_x, int64_t ldx, void* workspace, int64_t workspace_bytes, void* stream);
+
 /* --- Scoring ------------------------------------------------------------------------------
  * Per row of logits [N, V] (V <= 2^30, row stride ldz, type dtype): logprob[n] = log softmax(z)[targets[n]] (0
  * where targets[n] == ignore_index, NaN for any other target outside [0, V)), entropy[n], and the
@@ -421,6 +475,34 @@ int rq_token_logprobs_grad(const void* logits, int dtype, int64_t N, int64_t ldz
                            const int64_t* targets, int64_t ignore_index, const float* stats,
                            const float* grad_logprob, const float* grad_entropy, void* grad_logits,
                            int64_t ldd, void* stream);
+
+/* --- Distillation ------------------------------------------------------------------------
+ * loss[n] = the divergence from a teacher's top tokens to softmax(z / temperature), z = logits [N, V] (V <=
+ * 2^30, row stride ldz, type dtype).  teacher_ids [N, K] and teacher_logprobs [N, K] (contiguous, K <= 256):
+ * its tokens and their log probabilities (at temperature 1), in any order; an id below 0 is no entry.
+ * tail 0: p = softmax(logprobs / temperature) over the list, loss = sum p (log p - log q).
+ * tail 1 (temperature 1 only): p = exp(logprobs), and what is left of 1 is compared with the student's
+ * probability of all other tokens.  A remainder up to 2^-20 (the list's rounding) counts as 0 where the student
+ * leaves nothing to the others.  A row without entries has loss 0; an entry from V on, a NaN or a logit of
+ * +inf makes it NaN; a listed token with p > 0 and a logit of -inf makes it inf.  stats [N, 8] for the gradient:
+ * maximum and log of the sum of exp((z - maximum) / temperature) over all tokens, the same over those that are
+ * not listed (tail 0: over all), the teacher's maximum and log sum, sum p and the remainder, the factor of
+ * the unlisted tokens' probabilities.  temperature: 1e-6 to 1e6.  workspace: rq_distill_loss_workspace_bytes(N,
+ * V) bytes, any contents (NULL where that is 0). */
+int64_t rq_distill_loss_workspace_bytes(int64_t N, int V);
+int rq_distill_loss(const void* logits, int dtype, int64_t N, int64_t ldz, int V,
+                    const int64_t* teacher_ids, const float* teacher_logprobs, int K, double temperature,
+                    int tail, float* loss, float* stats, void* workspace, int64_t workspace_bytes,
+                    void* stream);
+
+/* grad_logits[n, i] = grad_loss[n] / temperature (q_i mass - p_i) for a listed token, grad_loss[n] /
+ * temperature factor w_i for any other, w the softmax over those that are not listed (tail 0: q).  A row
+ * without entries or with nothing but -inf gets 0.  grad_logits [N, V], row stride ldd, type dtype; it may be
+ * the logits themselves (with ldd == ldz). */
+int rq_distill_loss_grad(const void* logits, int dtype, int64_t N, int64_t ldz, int V,
+                         const int64_t* teacher_ids, const float* teacher_logprobs, int K,
+                         double temperature, int tail, const float* stats, const float* grad_loss,
+                         void* grad_logits, int64_t ldd, void* stream);
 
 #ifdef __cplusplus
 }

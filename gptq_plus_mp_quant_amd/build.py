@@ -21,7 +21,7 @@ LIBDIR = PKG / "_lib"
 LIB = LIBDIR / "libgptqplus_hip.so"
 SOURCES = ["hessian.hip", "params.hip", "argsort.hip", "chol.hip", "terms.hip", "colloop.hip", "pack.hip",
            "blockgd.hip", "plinear.hip", "plinear_f16.hip", "plinear_bf16.hip",
-           "plinear_f32.hip", "pmoe.hip", "pmoe_f16.hip", "pmoe_bf16.hip", "pmoe_f32.hip",
+           "plinear_f32.hip", "pcols_f16.hip", "pcols_bf16.hip", "pcols_f32.hip", "pcols_pair.hip", "pmoe.hip", "pmoe_f16.hip", "pmoe_bf16.hip", "pmoe_f32.hip",
            "plora.hip", "plora_f16.hip", "plora_bf16.hip", "plora_f32.hip", "pgated.hip", "pgated_f16.hip", "pgated_bf16.hip",
            "pgated_f32.hip", "logprobs.hip", "distill.hip"]
 

@@ -111,6 +111,30 @@ __device__ __forceinline__ floatx8 rq_codes_of(const uint32_t (&w)[NB], int s) {
   return f;
 }
 
+// The eight 4-bit codes of a word, as they are stored (offset by 8), to fp16 in the order 0 4 1 5 2 6 3 7: a code put into
+// the low bits of 1024, or four bits up of 64, is added to it, and what it is more by is taken off; nine instructions.
+__device__ __forceinline__ half8 rq_half_codes(uint32_t w) {
+  typedef _Float16 half2 __attribute__((ext_vector_type(2)));
+  const uint32_t h = w >> 8;
+  auto put = [](uint32_t v, uint32_t mask, uint32_t in) {          // one instruction: two literals would make it two
+    uint32_t o;
+    asm("v_and_or_b32 %0, %1, %2, %3" : "=v"(o) : "v"(v), "s"(mask), "v"(in));
+    return o;
+  };
+  const uint32_t u[4] = {put(w, 0x000F000Fu, 0x64006400u), put(w, 0x00F000F0u, 0x54005400u), put(h, 0x000F000Fu, 0x64006400u),
+                         put(h, 0x00F000F0u, 0x54005400u)};
+  const half2 low = {(_Float16)1032.0f, (_Float16)1032.0f}, up = {(_Float16)72.0f, (_Float16)72.0f};
+  half2 v[4];
+  __builtin_memcpy(v, u, sizeof(v));
+  v[0] -= low;
+  v[1] -= up;
+  v[2] -= low;
+  v[3] -= up;
+  half8 o;
+  __builtin_memcpy(&o, v, sizeof(o));
+  return o;
+}
+
 // Eight x of a token as they are loaded (FULL: all eight exist; else the first n, which may be none, the rest 0),
 // and the operand's pieces made of them.  Loads past the row's end are moved back to its last element, whose
 // place is p[n - 1], and their values dropped: a mask for every element would take the scalar registers.
@@ -212,6 +236,77 @@ struct RqPieces {
   }
 };
 
+// Tokens laid out once for all rows of a weight with RUNS, as its lanes take them: [tile of 16 tokens][chunk][step][piece][lane],
+// eight elements a lane, columns past the last and tokens past the last 0.  PAIRED (fp16 with 4 bits): the eight in the
+// order 0 4 1 5 2 6 3 7 of rq_half_codes.
+template <typename V, int P>
+struct RqArrangedRow {
+  V v[P];
+};
+template <typename V, int P>
+__device__ __forceinline__ void rq_operand(const RqArrangedRow<V, P>& x, V (&v)[P]) {
+#pragma unroll
+  for (int p = 0; p < P; ++p) v[p] = x.v[p];
+}
+template <typename TX, int NT, bool PAIRED>
+struct RqArranged {
+  typedef typename RqOperand<TX>::vec vec;
+  static constexpr int tiles = NT, pieces = RqOperand<TX>::pieces;
+  static constexpr bool arranged = true, paired = PAIRED, whole = true;
+  typedef RqArrangedRow<vec, pieces> raw;
+  const vec* p[NT];         // the lane's, of each tile
+  template <bool FULL>
+  __device__ __forceinline__ raw load(int b, int c, int) const {
+    const int64_t at = (int64_t)(c >> 5) * pieces * 64;
+    raw r;
+#pragma unroll
+    for (int k = 0; k < pieces; ++k) r.v[k] = p[b][at + k * 64];
+    return r;
+  }
+};
+template <typename TX>
+inline int64_t rq_arranged_bytes(int T, int C) {
+  return (int64_t)((T + 15) / 16) * ((C + RQ_CHUNK - 1) / RQ_CHUNK) * 256 * RqOperand<TX>::pieces * 16;
+}
+template <typename TX>
+constexpr bool rq_pairs(int nbits) {
+  return std::is_same<TX, __half>::value && nbits == 4;
+}
+// The lane's places of the tiles from token t0 on; the last tile again for those past it.
+template <typename TX, int NT>
+__device__ __forceinline__ void rq_arranged_tokens(const void* x, int T, int C, int t0, const typename RqOperand<TX>::vec* (&p)[NT]) {
+  typedef typename RqOperand<TX>::vec vec;
+  const int64_t tile = (int64_t)((C + RQ_CHUNK - 1) / RQ_CHUNK) * 256 * RqOperand<TX>::pieces;
+#pragma unroll
+  for (int b = 0; b < NT; ++b)
+    p[b] = reinterpret_cast<const vec*>(x) + min(t0 / 16 + b, (T - 1) / 16) * tile + (threadIdx.x & 63);
+}
+// Chunks [ch0, ch1) of tile `tile` to their places, by the threads first, first + step, ...
+template <typename TX>
+__device__ __forceinline__ void rq_arrange(const TX* __restrict__ x, int T, int64_t ldx, int C, int tile, int ch0, int ch1, bool paired,
+                                           int first, int step, void* out) {
+  typedef typename RqOperand<TX>::vec vec;
+  typedef typename RqOperand<TX>::raw Raw;
+  constexpr int P = RqOperand<TX>::pieces;
+  const int chunks = (C + RQ_CHUNK - 1) / RQ_CHUNK;
+  for (int e = ch0 * 256 + first; e < ch1 * 256; e += step) {
+    // neighbouring threads read neighbouring columns of a token: within a chunk, (token, q, s) from the thread
+    const int ch = e >> 8, s = e & 3, q = e >> 2 & 3, i = e >> 4 & 15;
+    const int t = tile * 16 + i, c = ch * RQ_CHUNK + 32 * q + 8 * s, n = C - c;
+    Raw r = {};
+    if (t < T && n > 0) r = n >= 8 ? rq_load_x<true>(x + (int64_t)t * ldx + c, 8) : rq_load_x<false>(x + (int64_t)t * ldx + c, n);
+    vec v[P];
+    rq_operand(r, v);
+    vec* to = reinterpret_cast<vec*>(out) + ((((int64_t)tile * chunks + ch) * 4 + s) * P) * 64 + 16 * q + i;
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+      vec o = v[p];
+      if (paired) o = __builtin_shufflevector(v[p], v[p], 0, 4, 1, 5, 2, 6, 3, 7);
+      to[p * 64] = o;
+    }
+  }
+}
+
 // A lane's eight x of any kind as fp32.
 template <typename V>
 __device__ __forceinline__ void rq_floats(const V& x, floatx8& f) { f = __builtin_convertvector(x, floatx8); }
@@ -263,6 +358,9 @@ __device__ __forceinline__ int rq_run_group(const RqPacked& w, int c) {
   return w.run_magic > 1 ? (int)__umulhi(n, w.run_magic) : w.run_magic ? (int)n : 0;
 }
 
+// The group of chunk ch with RUNS, whose group sizes are multiples of 128: run_magic divides by four at least.
+__device__ __forceinline__ int64_t rq_chunk_group(const RqPacked& w, int ch) { return __umulhi((uint32_t)ch * (RQ_CHUNK / 32), w.run_magic); }
+
 // The words of columns c..c+31 of a row (c a multiple of 32); the row's last word again where it has none there,
 // for columns whose x is 0.
 template <int NB>
@@ -272,6 +370,25 @@ __device__ __forceinline__ void rq_words(const uint32_t* row, int c, int C, uint
   for (int k = 0; k < NB; ++k) w[k] = row[first + k < last ? first + k : last];
 }
 
+template <typename X, typename = void>
+struct rq_paired : std::false_type {};
+template <typename X>
+struct rq_paired<X, typename std::enable_if<X::paired>::type> : std::true_type {};
+// WHOLE (X::whole): a row tile that would pass the weight's last row is moved back to end with it, and does the rows
+// before once more; R is 16 at least with RUNS and SMALL.  No lane then has a row or scale to guard.
+template <typename X, typename = void>
+struct rq_whole : std::false_type {};
+template <typename X>
+struct rq_whole<X, typename std::enable_if<X::whole>::type> : std::true_type {};
+template <bool WHOLE>
+__device__ __forceinline__ int rq_tile_row(int r, int R) {
+  return WHOLE ? max(min(r, R - 16), 0) : r;
+}
+template <typename TX, int NT>
+struct RqWholeTokens : RqTokens<TX, NT> {
+  static constexpr bool whole = true;
+};
+
 // What a lane needs of a chunk of 128 columns with RUNS: its words and scales, and its tokens' x.  Row tiles
 // go over NM weights of one shape, tile a being rows r0 + 16 (a / NM) of weight a mod NM.
 template <int NB, int RT>
@@ -279,7 +396,7 @@ struct RqRunsW {
   uint32_t wd[RT][NB];
   floatx4 sc[RT];
 };
-template <bool FULL, int NB, int RT, int NM>
+template <bool FULL, bool WHOLE, int NB, int RT, int NM>
 __device__ __forceinline__ void rq_load_runs(const RqPacked (&w)[NM], const uint32_t* const (&row)[RT], int r0, int ch,
                                              RqRunsW<NB, RT>& f) {
   const int q = (threadIdx.x & 63) >> 4, c = ch * RQ_CHUNK + 32 * q;
@@ -290,7 +407,10 @@ __device__ __forceinline__ void rq_load_runs(const RqPacked (&w)[NM], const uint
     } else {
       rq_words<NB>(row[a], c, w[0].C, f.wd[a]);
     }
-    f.sc[a] = rq_load_scales4(w[a % NM], rq_run_group(w[a % NM], ch * RQ_CHUNK), r0 + 16 * (a / NM) + 4 * q);
+    const RqPacked& wa = w[a % NM];
+    if constexpr (WHOLE)
+      f.sc[a] = rq_load_as<floatx4>(wa.scales + rq_chunk_group(wa, ch) * wa.lds + rq_tile_row<true>(r0 + 16 * (a / NM), wa.R) + 4 * q);
+    else f.sc[a] = rq_load_scales4(wa, rq_run_group(wa, ch * RQ_CHUNK), r0 + 16 * (a / NM) + 4 * q);
   }
 }
 // Step s loads columns 32s + 8q of the chunk, 64 bytes (of a 16-bit type) in a row of each token, and rq_to_runs
@@ -334,9 +454,10 @@ __device__ __forceinline__ void rq_chunk_runs(const RqPacked (&w)[NM], int r0, i
 #pragma unroll
     for (int b = 0; b < NT; ++b) rq_to_runs(x[b]);
   }
+  constexpr bool PAIRED = rq_paired<X>::value;
 #pragma unroll
   for (int a = 0; a < RT; ++a) {
-    rq_to_signed<NB>(f.wd[a]);
+    if constexpr (!PAIRED) rq_to_signed<NB>(f.wd[a]);
 #pragma unroll
     for (int b = 0; b < NT; ++b) part[a][b] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
   }
@@ -348,7 +469,8 @@ __device__ __forceinline__ void rq_chunk_runs(const RqPacked (&w)[NM], int r0, i
 #pragma unroll
     for (int a = 0; a < RT; ++a) {
       V codes;
-      rq_convert(rq_codes_of<NB>(f.wd[a], s), codes);
+      if constexpr (PAIRED) codes = rq_half_codes(f.wd[a][s]);
+      else rq_convert(rq_codes_of<NB>(f.wd[a], s), codes);
 #pragma unroll
       for (int b = 0; b < NT; ++b)
 #pragma unroll
@@ -359,7 +481,9 @@ __device__ __forceinline__ void rq_chunk_runs(const RqPacked (&w)[NM], int r0, i
 #pragma unroll
   for (int a = 0; a < RT; ++a) {
     const RqPacked& wa = w[a % NM];
-    const floatx4 sc = rq_scales4_of(wa, rq_run_group(wa, ch * RQ_CHUNK), r + 16 * (a / NM), f.sc[a]) * rq_unit<NB>();
+    floatx4 sc = f.sc[a];
+    if constexpr (!rq_whole<X>::value) sc = rq_scales4_of(wa, rq_run_group(wa, ch * RQ_CHUNK), r + 16 * (a / NM), sc);
+    if constexpr (!PAIRED) sc *= rq_unit<NB>();
 #pragma unroll
     for (int b = 0; b < NT; ++b)
 #pragma unroll
@@ -385,20 +509,22 @@ __device__ __forceinline__ void rq_rows_tokens(const RqPacked (&w)[NM], int r0, 
   typedef typename X::vec V;
   constexpr int NT = X::tiles, P = X::pieces;
   const int lane = threadIdx.x & 63, i = lane & 15, q = lane >> 4;
+  constexpr bool WHOLE = rq_whole<X>::value;
   const uint32_t* row[RT];
 #pragma unroll
-  for (int a = 0; a < RT; ++a) row[a] = w[a % NM].q + (int64_t)min(r0 + 16 * (a / NM) + i, w[a % NM].R - 1) * w[a % NM].ldp;
+  for (int a = 0; a < RT; ++a)
+    row[a] = w[a % NM].q + (int64_t)min(rq_tile_row<WHOLE>(r0 + 16 * (a / NM), w[a % NM].R) + i, w[a % NM].R - 1) * w[a % NM].ldp;
   const int C = w[0].C, nfull = C / RQ_CHUNK, nch = (C + RQ_CHUNK - 1) / RQ_CHUNK;
   int ch = first;
   if constexpr (MODE == RQ_RUNS) {
     // The words of D chunks and the tokens of DX are in flight, a chunk's place refilled as soon as it has
     // been used.  No load of the loop is conditional: a wait then counts the later loads that may stay
     // in flight, where a branch around one would make it wait for all of them.
-    constexpr int D = NT * P * NM == 1 && NB <= 5 ? 4 : 2, DX = NT == 1 && sizeof(typename X::raw) <= 16 ? 2 : 1;
+    constexpr int D = NT * P * NM == 1 && NB <= 5 ? 4 : 2, DX = (NT == 1 || (X::arranged && NT <= 3)) && sizeof(typename X::raw) <= 16 ? 2 : 1;
     const int n = ch < nfull ? (nfull - ch + step - 1) / step : 0;     // full chunks of this wave
     RqRunsW<NB, RT> f[D];
     typename X::raw x[DX][NT][4];
-    auto words = [&](int k, RqRunsW<NB, RT>& to) { rq_load_runs<true>(w, row, r0, ch + k * step, to); };
+    auto words = [&](int k, RqRunsW<NB, RT>& to) { rq_load_runs<true, WHOLE>(w, row, r0, ch + k * step, to); };
     auto tokens = [&](int k, typename X::raw (&to)[NT][4]) { rq_load_tokens<true>(xs, C, ch + k * step, to); };
     auto compute = [&](int k, RqRunsW<NB, RT>& of, typename X::raw (&xk)[NT][4]) {
       if constexpr (DX == 1) tokens(k, xk);
@@ -437,7 +563,7 @@ __device__ __forceinline__ void rq_rows_tokens(const RqPacked (&w)[NM], int r0, 
         compute(k + u, f[u], x[0]);
       }
     if (nfull < nch && nfull >= first && (nfull - first) % step == 0) {       // the ragged end is this wave's
-      rq_load_runs<false>(w, row, r0, nfull, f[0]);
+      rq_load_runs<false, WHOLE>(w, row, r0, nfull, f[0]);
       rq_load_tokens<false>(xs, C, nfull, x[0]);
       rq_chunk_runs<X, NB, RT, NM>(w, r0, nfull, f[0], x[0], acc);
     }
@@ -468,8 +594,10 @@ __device__ __forceinline__ void rq_rows_tokens(const RqPacked (&w)[NM], int r0, 
           for (int k = 0; k < 8; ++k) f[k] = (float)code[s][a][k];
           rq_convert(f, codes);
           const RqPacked& wa = w[a % NM];
-          const int g = rq_run_group(wa, c0 + 32 * s), r = r0 + 16 * (a / NM) + 4 * q;
-          const floatx4 sc = rq_scales4_of(wa, g, r, rq_load_scales4(wa, g, r));
+          const int g = rq_run_group(wa, c0 + 32 * s), r = rq_tile_row<WHOLE>(r0 + 16 * (a / NM), wa.R) + 4 * q;
+          floatx4 sc;
+          if constexpr (WHOLE) sc = rq_load_as<floatx4>(wa.scales + (int64_t)g * wa.lds + r);
+          else sc = rq_scales4_of(wa, g, r, rq_load_scales4(wa, g, r));
 #pragma unroll
           for (int b = 0; b < NT; ++b) {
             floatx4 part = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -508,7 +636,7 @@ __device__ __forceinline__ void rq_rows_tokens(const RqPacked (&w)[NM], int r0, 
               const RqPacked& wa = w[a % NM];
               const uint32_t ga = g[a % NM][j];
               const float s = lds ? lds[ga * (16 * RT) + 16 * a + i]
-                                  : rq_scale_of(wa, ga, min(r0 + 16 * (a / NM) + i, wa.R - 1));
+                                  : rq_scale_of(wa, ga, min(rq_tile_row<WHOLE>(r0 + 16 * (a / NM), wa.R) + i, wa.R - 1));
               const float v = s * (float)rq_signed_code<NB>(wd[a], 8 * k + j), wv = FULL || j < nk ? v : 0.0f;
 #pragma unroll
               for (int b = 0; b < NT; ++b) acc[a][b] = __builtin_amdgcn_mfma_f32_16x16x4f32(wv, xv[b][j], acc[a][b], 0, 0, 0);
@@ -532,6 +660,9 @@ __device__ __forceinline__ void rq_stage_scales(const RqPacked& w, int r0, int t
 }
 constexpr int RQ_STAGED_GROUPS = 1023;      // groups whose scales a workgroup stages (64 KB for 16 rows)
 
+// Which of the three serves a weight whose row tiles are WHOLE.
+inline int rq_mode_of(const RqPacked& w);
+inline int rq_whole_mode_of(const RqPacked& w) { return w.R < 16 ? RQ_ANY : rq_mode_of(w); }
 // Which of the three serves a weight.
 inline int rq_mode_of(const RqPacked& w) {
   if ((int64_t)(w.ngroups - 1) * w.lds + w.R < 4) return RQ_ANY;

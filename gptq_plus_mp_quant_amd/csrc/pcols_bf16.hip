@@ -1,0 +1,6 @@
+// Gradients of products with packed weights: bf16 tensors.
+#include "plinear_types.h"
+#include "plinear_cols.h"
+
+template void rq_linear_cols<__hip_bfloat16>(const __hip_bfloat16*, int, int64_t, const RqPacked&, int, float*, __hip_bfloat16*, int64_t, hipStream_t);
+template void rq_cols_parts<__hip_bfloat16>(const __hip_bfloat16*, int, int64_t, const RqPacked&, int, const RqColSplit&, float*, hipStream_t);

@@ -12,15 +12,19 @@ enum { GATED_BOTH = 0, GATED_GATE = 1, GATED_UP = 2 };
 // row tile of gate and one of up by the tokens they have loaded once, and are joined through LDS in their order.  GATE
 // and UP (weights of different bits or groups): one of the two, the gate's product goes by way of pre.
 template <typename TX, int NB, int MODE, int NM, int NT>
-__global__ __launch_bounds__(rows_threads(2, NT)) void k_packed_gated(const TX* __restrict__ x, int T, int64_t ldx, RqPacked first,
+__global__ __launch_bounds__(rows_threads(2, NT)) void k_packed_gated(const TX* __restrict__ x, const void* __restrict__ xa, int T, int64_t ldx, RqPacked first,
                                                                       RqPacked second, int what, int act, bool staged,
                                                                       float* pre, TX* __restrict__ h, int64_t ldh) {
   extern __shared__ __attribute__((aligned(16))) float lds[];
   const int lane = threadIdx.x & 63, wave = rq_wave(), waves = blockDim.x >> 6;
-  const int r0 = blockIdx.x * 16, t0 = blockIdx.y * 16 * NT, I = first.R;
-  RqTokens<TX, NT> xs;
+  const int I = first.R, r0 = rq_tile_row<true>(blockIdx.x * 16, I), t0 = blockIdx.y * 16 * NT;
+  constexpr bool ARRANGED = MODE == RQ_RUNS && NT > 1;
+  typename std::conditional<ARRANGED, RqArranged<TX, NT, rq_pairs<TX>(NB)>, RqWholeTokens<TX, NT>>::type xs;
+  if constexpr (ARRANGED) rq_arranged_tokens<TX>(xa, T, first.C, t0, xs.p);
+  else {
 #pragma unroll
-  for (int b = 0; b < NT; ++b) xs.p[b] = x + (int64_t)min(t0 + 16 * b + (lane & 15), T - 1) * ldx;
+    for (int b = 0; b < NT; ++b) xs.p[b] = x + (int64_t)min(t0 + 16 * b + (lane & 15), T - 1) * ldx;
+  }
   RqPacked w[NM];
   w[0] = first;
   if constexpr (NM == 2) w[1] = second;
@@ -65,8 +69,14 @@ __global__ __launch_bounds__(rows_threads(2, NT)) void k_packed_gated(const TX* 
   }
 }
 
+template <typename TX>
+__global__ __launch_bounds__(256) void k_arrange(const TX* __restrict__ x, int T, int64_t ldx, int C, bool paired, void* __restrict__ xa) {
+  const int ch = blockIdx.y * 4;
+  rq_arrange<TX>(x, T, ldx, C, blockIdx.x, ch, min(ch + 4, (C + RQ_CHUNK - 1) / RQ_CHUNK), paired, threadIdx.x, 256, xa);
+}
+
 template <typename TX, int NB, int MODE, int NM, int NT>
-void launch_gated(const TX* x, int T, int64_t ldx, const RqPacked& first, const RqPacked& second, int what, int act, float* pre,
+void launch_gated(const TX* x, void* xa, int T, int64_t ldx, const RqPacked& first, const RqPacked& second, int what, int act, float* pre,
                   TX* h, int64_t ldh, hipStream_t s) {
   const int bx = (first.R + 15) / 16, by = (T + 16 * NT - 1) / (16 * NT);
   const int waves = waves_for(bx * by, (first.C + RQ_CHUNK - 1) / RQ_CHUNK, NM * NT, rows_threads(2, NT) / 64);
@@ -74,27 +84,28 @@ void launch_gated(const TX* x, int T, int64_t ldx, const RqPacked& first, const 
   const size_t scales = (size_t)((first.ngroups > second.ngroups ? first.ngroups : second.ngroups) + 1) * 16 * NM * 4;
   const bool staged = MODE == RQ_ANY && scales <= 65536;
   if (staged && lds < scales) lds = scales;
-  hipLaunchKernelGGL((k_packed_gated<TX, NB, MODE, NM, NT>), dim3(bx, by), dim3(64 * waves), lds, s, x, T, ldx, first, second, what,
+  hipLaunchKernelGGL((k_packed_gated<TX, NB, MODE, NM, NT>), dim3(bx, by), dim3(64 * waves), lds, s, x, xa, T, ldx, first, second, what,
                      act, staged, pre, h, ldh);
 }
 
 template <typename TX, int NB, int MODE, int NM>
-void gated_of(const TX* x, int T, int64_t ldx, const RqPacked& first, const RqPacked& second, int what, int act, float* pre, TX* h,
+void gated_of(const TX* x, void* xa, int T, int64_t ldx, const RqPacked& first, const RqPacked& second, int what, int act, float* pre, TX* h,
               int64_t ldh, hipStream_t s) {
   constexpr int NT = RqOperand<TX>::pieces == 1 ? 4 : 2;
-  if (T <= 16) launch_gated<TX, NB, MODE, NM, 1>(x, T, ldx, first, second, what, act, pre, h, ldh, s);
-  else if (T <= 32) launch_gated<TX, NB, MODE, NM, 2>(x, T, ldx, first, second, what, act, pre, h, ldh, s);
-  else launch_gated<TX, NB, MODE, NM, NT>(x, T, ldx, first, second, what, act, pre, h, ldh, s);
+  if (T <= 16) launch_gated<TX, NB, MODE, NM, 1>(x, xa, T, ldx, first, second, what, act, pre, h, ldh, s);
+  else if (T <= 32) launch_gated<TX, NB, MODE, NM, 2>(x, xa, T, ldx, first, second, what, act, pre, h, ldh, s);
+  else if (MODE == RQ_RUNS && T <= 48 && NT > 3) launch_gated<TX, NB, MODE, NM, NT < 3 ? NT : 3>(x, xa, T, ldx, first, second, what, act, pre, h, ldh, s);
+  else launch_gated<TX, NB, MODE, NM, NT>(x, xa, T, ldx, first, second, what, act, pre, h, ldh, s);
 }
 template <typename TX, int NM>
-void gated_one(const TX* x, int T, int64_t ldx, const RqPacked& first, const RqPacked& second, int bits, int what, int act, float* pre,
+void gated_one(const TX* x, void* xa, int T, int64_t ldx, const RqPacked& first, const RqPacked& second, int bits, int what, int act, float* pre,
                TX* h, int64_t ldh, hipStream_t s) {
   rq_with_nbits(bits, [&](auto nb) {
     constexpr int NB = decltype(nb)::value;
-    switch (rq_mode_of(first)) {
-      case RQ_RUNS: gated_of<TX, NB, RQ_RUNS, NM>(x, T, ldx, first, second, what, act, pre, h, ldh, s); break;
-      case RQ_SMALL: gated_of<TX, NB, RQ_SMALL, NM>(x, T, ldx, first, second, what, act, pre, h, ldh, s); break;
-      default: gated_of<TX, NB, RQ_ANY, NM>(x, T, ldx, first, second, what, act, pre, h, ldh, s);
+    switch (rq_whole_mode_of(first)) {
+      case RQ_RUNS: gated_of<TX, NB, RQ_RUNS, NM>(x, xa, T, ldx, first, second, what, act, pre, h, ldh, s); break;
+      case RQ_SMALL: gated_of<TX, NB, RQ_SMALL, NM>(x, xa, T, ldx, first, second, what, act, pre, h, ldh, s); break;
+      default: gated_of<TX, NB, RQ_ANY, NM>(x, xa, T, ldx, first, second, what, act, pre, h, ldh, s);
     }
   });
 }
@@ -124,12 +135,20 @@ __global__ __launch_bounds__(256) void k_gated_join(const float* __restrict__ pa
 }  // namespace
 
 template <typename TX>
-void rq_gated_rows(const TX* x, int T, int64_t ldx, const RqPacked& gate, int gate_bits, const RqPacked& up, int up_bits,
+void rq_gated_rows(const TX* x, void* xa, int T, int64_t ldx, const RqPacked& gate, int gate_bits, const RqPacked& up, int up_bits,
                    int act, float* pre, TX* h, int64_t ldh, hipStream_t s) {
-  if (rq_gated_together(gate, gate_bits, up, up_bits))
-    return gated_one<TX, 2>(x, T, ldx, gate, up, gate_bits, GATED_BOTH, act, pre, h, ldh, s);
-  gated_one<TX, 1>(x, T, ldx, gate, gate, gate_bits, GATED_GATE, act, pre, h, ldh, s);
-  gated_one<TX, 1>(x, T, ldx, up, up, up_bits, GATED_UP, act, pre, h, ldh, s);
+  auto arrange = [&](int bits) {
+    const int chunks = (gate.C + RQ_CHUNK - 1) / RQ_CHUNK;
+    hipLaunchKernelGGL(k_arrange<TX>, dim3((T + 15) / 16, (chunks + 3) / 4), dim3(256), 0, s, x, T, ldx, gate.C, rq_pairs<TX>(bits), xa);
+  };
+  if (rq_gated_together(gate, gate_bits, up, up_bits)) {
+    if (rq_gated_arranged(T, gate)) arrange(gate_bits);
+    return gated_one<TX, 2>(x, xa, T, ldx, gate, up, gate_bits, GATED_BOTH, act, pre, h, ldh, s);
+  }
+  if (rq_gated_arranged(T, gate)) arrange(gate_bits);
+  gated_one<TX, 1>(x, xa, T, ldx, gate, gate, gate_bits, GATED_GATE, act, pre, h, ldh, s);
+  if (rq_gated_arranged(T, up) && (!rq_gated_arranged(T, gate) || rq_pairs<TX>(gate_bits) != rq_pairs<TX>(up_bits))) arrange(up_bits);
+  gated_one<TX, 1>(x, xa, T, ldx, up, up, up_bits, GATED_UP, act, pre, h, ldh, s);
 }
 template <typename TX>
 void rq_gated_pre_grad(const TX* grad_h, int64_t ldg, int T, int I, int act, const float* pre, float* d, hipStream_t s) {

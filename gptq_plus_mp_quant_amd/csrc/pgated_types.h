@@ -25,12 +25,14 @@ __device__ __forceinline__ RqAct rq_act(int kind, float a) {
 }
 
 // h [T, I] = act(x Wg^T) * (x Wu^T); pre (fp32 [T, 2, I], or NULL where both weights go through one launch): the products.
+// xa: room for x as RqArranged has it, where rq_gated_arranged says so for one of the weights.
 template <typename TX>
-void rq_gated_rows(const TX* x, int T, int64_t ldx, const RqPacked& gate, int gate_bits, const RqPacked& up, int up_bits,
+void rq_gated_rows(const TX* x, void* xa, int T, int64_t ldx, const RqPacked& gate, int gate_bits, const RqPacked& up, int up_bits,
                    int act, float* pre, TX* h, int64_t ldh, hipStream_t s);
 inline bool rq_gated_together(const RqPacked& gate, int gate_bits, const RqPacked& up, int up_bits) {
-  return gate_bits == up_bits && rq_mode_of(gate) == rq_mode_of(up);
+  return gate_bits == up_bits && rq_whole_mode_of(gate) == rq_whole_mode_of(up);
 }
+inline bool rq_gated_arranged(int T, const RqPacked& w) { return T > 16 && rq_whole_mode_of(w) == RQ_RUNS; }
 
 // d [2, T, I] = the gradients of the products from grad_h [T, I] and pre [T, 2, I]
 template <typename TX>

@@ -77,36 +77,177 @@ constexpr int cols_waves(int nt) { return nt >= 4 ? 4 : 8; }
 // 45).
 constexpr int cols_occupancy(int mode, int nt) { return mode == RQ_RUNS && nt >= 4 ? 2 : 1; }
 
+// Where a lane's 8 columns lie in a row of the weight: words from `col` on, of which nw hold its nc columns, shifted by
+// off bits.  A lane past the last column reads the row's first word; words past a row's last field are not read.
+template <int NB>
+struct ColLane {
+  int c, nc, off, nw;                                              // nc <= 0: none
+  const uint32_t* col;
+};
+template <int NB>
+__device__ __forceinline__ ColLane<NB> col_lane(const RqPacked& w) {
+  ColLane<NB> l;
+  l.c = blockIdx.x * COLS + 8 * (threadIdx.x & 15);
+  l.nc = min(8, w.C - l.c);
+  const int64_t bit = (int64_t)l.c * NB;
+  l.off = (int)(bit & 31);
+  l.nw = l.nc > 0 ? (l.off + l.nc * NB + 31) >> 5 : 0;
+  l.col = w.q + (l.nc > 0 ? bit >> 5 : 0);
+  return l;
+}
+// The words of rows r..r+7 (FULL: all exist; else the last row again).
+template <bool FULL, int NB>
+__device__ __forceinline__ void col_words(const RqPacked& w, const ColLane<NB>& l, int r, uint32_t (&wd)[8][Col8<NB>::NW]) {
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    const uint32_t* p = l.col + (int64_t)(FULL ? r + k : min(r + k, w.R - 1)) * w.ldp;
+#pragma unroll
+    for (int m = 0; m < Col8<NB>::NW; ++m) wd[k][m] = p[max(min(m, l.nw - 1), 0)];
+  }
+}
+template <bool FULL>
+__device__ __forceinline__ floatx8 col_scales(const RqPacked& w, uint32_t g, int r) {
+  const float* s = w.scales + (int64_t)g * w.lds + r;
+  if (FULL) return rq_load_as<floatx8>(s);
+  floatx8 v;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) v[k] = r + k < w.R ? s[k] : 0.0f;
+  return v;
+}
+// Fields to bit 0, two's complement; odd: their odd nibbles, for 4 bits.
+template <int NB>
+__device__ __forceinline__ void col_fields(int off, uint32_t (&wd)[8][Col8<NB>::NW], uint32_t (&odd)[8]) {
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+#pragma unroll
+    for (int m = 0; m < Col8<NB>::N; ++m) {
+      const uint32_t hi = m + 1 < Col8<NB>::NW ? wd[k][m + 1] : 0u;
+      const uint32_t v = NB % 4 == 0 ? wd[k][m] : (uint32_t)((((uint64_t)hi << 32) | wd[k][m]) >> off);
+      wd[k][m] = v ^ rq_top_bits<NB>(m);
+    }
+    odd[k] = NB == 4 ? rq_odd_nibbles(wd[k][0]) : 0u;
+  }
+}
+// Eight finite numbers in the three pieces of rq_operand; a number that is not makes its second piece NaN.
+__device__ __forceinline__ void col_pieces(floatx8 x, bf16x8 (&v)[3]) {
+  uint32_t o[3][4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    float a = x[2 * k], b = x[2 * k + 1];
+#pragma unroll
+    for (int p = 0; p < 3; ++p) {
+      const uint32_t ba = __float_as_uint(a), bb = __float_as_uint(b);
+      o[p][k] = __builtin_amdgcn_perm(bb, ba, 0x07060302u);        // the upper halves
+      a -= __uint_as_float(ba & 0xFFFF0000u);
+      b -= __uint_as_float(bb & 0xFFFF0000u);
+    }
+  }
+#pragma unroll
+  for (int p = 0; p < 3; ++p) __builtin_memcpy(&v[p], o[p], 16);
+}
+
+// Steps first, first + W, ... below sb of 32 rows, RUNS: acc[n][b] += tokens of tile b times code n of the lane's columns.
+// A step's words become operands once and serve all token tiles; the next step's words are then loaded, and each
+// tile's place is refilled with the tile after the next as soon as it has been cut into pieces.
+// CAREFUL: infinities and NaN among the tokens give what the formula gives; without it, NaN.
+template <typename TX, int NB, int NT, bool CAREFUL>
+__device__ __forceinline__ void cols_runs(const TX* __restrict__ dy, int T, int64_t ldy, const RqPacked& w, int t0, int first, int sb,
+                                          floatx4 (&acc)[8][NT]) {
+  constexpr int W = cols_waves(NT);
+  typedef typename RqOperand<TX>::raw Raw;
+  const int lane = threadIdx.x & 63, j = lane & 15, q = lane >> 4;
+  const ColLane<NB> l = col_lane<NB>(w);
+  const uint32_t g = rq_run_group(w, blockIdx.x * COLS);
+  const TX* tok[NT];
+#pragma unroll
+  for (int b = 0; b < NT; ++b) tok[b] = dy + (int64_t)min(t0 + 16 * b + j, T - 1) * ldy + 8 * q;
+  auto operands = [&](uint32_t (&wd)[8][Col8<NB>::NW], bf16x8 (&v)[8]) {
+    uint32_t odd[8];
+    col_fields<NB>(l.off, wd, odd);
+#pragma unroll
+    for (int n = 0; n < 8; ++n) rq_convert(col_codes<NB>(wd, odd, n), v[n]);
+  };
+  auto multiply = [&](const Raw& raw, const floatx8& sc, const bf16x8 (&v)[8], int b) {
+    floatx8 f;
+    fp32_of(raw, f);
+    bf16x8 d[3];
+    if constexpr (CAREFUL) rq_operand<3>(f * sc, d);
+    else col_pieces(f * sc, d);
+#pragma unroll
+    for (int p = 0; p < 3; ++p)
+#pragma unroll
+      for (int n = 0; n < 8; ++n) acc[n][b] = rq_mfma(d[p], v[n], acc[n][b]);
+  };
+  const int sf = min(sb, w.R / STEP);                              // up to here steps are full
+  int st = first;
+  if (!CAREFUL && st < sf) {
+    constexpr int AHEAD = 2;
+    auto tile = [&](int item, int from) {                          // token tile item mod NT of its step
+      const int s = min(from + item / NT * W, sf - 1);
+      return rq_load_x<true>(tok[item % NT] + s * STEP, 8);
+    };
+    uint32_t wd[8][Col8<NB>::NW];
+    col_words<true, NB>(w, l, st * STEP + 8 * q, wd);
+    floatx8 sc = col_scales<true>(w, g, st * STEP + 8 * q);
+    Raw raw[AHEAD];
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) raw[k] = tile(k, st);
+    // NT = 1 takes two steps a round, so that a tile's place is known
+    auto step = [&](auto at) {
+      constexpr int AT = decltype(at)::value;
+      bf16x8 v[8];
+      operands(wd, v);
+      const floatx8 s8 = sc * rq_unit<NB>();
+      const int next = min(st + W, sf - 1) * STEP + 8 * q;         // the last one again where there is none
+      col_words<true, NB>(w, l, next, wd);
+      sc = col_scales<true>(w, g, next);
+#pragma unroll
+      for (int b = 0; b < NT; ++b) {
+        constexpr int base = AT % AHEAD;
+        const Raw now = raw[(base + b) % AHEAD];
+        raw[(base + b) % AHEAD] = tile(b + AHEAD, st);
+        multiply(now, s8, v, b);
+      }
+      st += W;
+    };
+    if constexpr (NT == 1) {
+      for (;;) {
+        step(std::integral_constant<int, 0>{});
+        if (st >= sf) break;
+        step(std::integral_constant<int, 1>{});
+        if (st >= sf) break;
+      }
+    } else {
+      while (st < sf) step(std::integral_constant<int, 0>{});
+    }
+  }
+  for (; st < sb; st += W) {                                       // the last rows; CAREFUL: all
+    const int r = st * STEP + 8 * q;
+    uint32_t wd[8][Col8<NB>::NW];
+    col_words<false, NB>(w, l, r, wd);
+    const floatx8 s8 = col_scales<false>(w, g, r) * rq_unit<NB>();
+    bf16x8 v[8];
+    operands(wd, v);
+#pragma unroll
+    for (int b = 0; b < NT; ++b) multiply(rq_load_x<false>(tok[b] + st * STEP, w.R - r), s8, v, b);
+  }
+}
+
+// The same with SMALL and ANY, where a scale multiplies the codes; infinities and NaN as the formula has them.
 template <typename TX, int NB, int MODE, int NT>
-__global__ __launch_bounds__(64 * cols_waves(NT), cols_occupancy(MODE, NT)) void k_packed_cols(
-    const TX* __restrict__ dy, int T, int64_t ldy, RqPacked w, int steps_per, float* __restrict__ part, TX* __restrict__ dx,
-    int64_t ldx) {
+__device__ __forceinline__ void cols_scaled(const TX* __restrict__ dy, int T, int64_t ldy, const RqPacked& w, int t0, int first, int sb,
+                                            floatx4 (&acc)[8][NT]) {
   constexpr int W = cols_waves(NT);
   typedef ColPieces<TX, MODE> P;
   typedef typename RqOperand<TX>::raw Raw;
-  __shared__ floatx4 join[W / 2][8 * NT][64];
-  const int lane = threadIdx.x & 63, wave = rq_wave(), j = lane & 15, q = lane >> 4;
-  const int c0 = blockIdx.x * COLS, c = c0 + 8 * j, t0 = blockIdx.z * 16 * NT;
-  const int nc = min(8, w.C - c);                                  // the lane's columns (<= 0: none)
-  const int nsteps = (w.R + STEP - 1) / STEP;
-  const int sa = blockIdx.y * steps_per, sb = min(nsteps, sa + steps_per);
-  const int64_t bit = (int64_t)c * NB;
-  const int off = (int)(bit & 31), nw = nc > 0 ? (off + nc * NB + 31) >> 5 : 0;
-  // A lane past the last column reads the row's first word; words past a row's last field are not read.
-  const uint32_t* col = w.q + (nc > 0 ? bit >> 5 : 0);
+  const int lane = threadIdx.x & 63, j = lane & 15, q = lane >> 4;
+  const ColLane<NB> l = col_lane<NB>(w);
   uint32_t g[8];
 #pragma unroll
-  for (int k = 0; k < 8; ++k)
-    g[k] = MODE == RQ_RUNS ? rq_run_group(w, c0) : (MODE == RQ_SMALL && k) ? g[0] : k < nc ? rq_group_of(w, c + k) : 0;
+  for (int k = 0; k < 8; ++k) g[k] = (MODE == RQ_SMALL && k) ? g[0] : k < l.nc ? rq_group_of(w, l.c + k) : 0;
   const TX* tok[NT];
 #pragma unroll
   for (int b = 0; b < NT; ++b) tok[b] = dy + (int64_t)min(t0 + 16 * b + j, T - 1) * ldy;
-
-  floatx4 acc[8][NT];
-#pragma unroll
-  for (int n = 0; n < 8; ++n)
-#pragma unroll
-    for (int b = 0; b < NT; ++b) acc[n][b] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
 
   struct Step {
     uint32_t wd[8][Col8<NB>::NW];
@@ -117,23 +258,10 @@ __global__ __launch_bounds__(64 * cols_waves(NT), cols_occupancy(MODE, NT)) void
   auto load = [&](auto full, int st, Step& f) {
     constexpr bool FULL = decltype(full)::value;
     const int r = st * STEP + 8 * q;                               // the lane's rows r..r+7
-#pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      const uint32_t* p = col + (int64_t)(FULL ? r + k : min(r + k, w.R - 1)) * w.ldp;
-#pragma unroll
-      for (int m = 0; m < Col8<NB>::NW; ++m) f.wd[k][m] = p[max(min(m, nw - 1), 0)];
-    }
+    col_words<FULL, NB>(w, l, r, f.wd);
 #pragma unroll
     for (int b = 0; b < NT; ++b) f.dy[b] = rq_load_x<FULL>(tok[b] + r, w.R - r);
-    if (MODE != RQ_ANY) {
-      const float* s = w.scales + (int64_t)g[0] * w.lds + r;
-      if (FULL) {
-        f.sc = rq_load_as<floatx8>(s);
-      } else {
-#pragma unroll
-        for (int k = 0; k < 8; ++k) f.sc[k] = r + k < w.R ? s[k] : 0.0f;
-      }
-    }
+    if (MODE != RQ_ANY) f.sc = col_scales<FULL>(w, g[0], r);
   };
   auto compute = [&](auto full, int st, Step& f) {
     constexpr bool FULL = decltype(full)::value;
@@ -146,67 +274,48 @@ __global__ __launch_bounds__(64 * cols_waves(NT), cols_occupancy(MODE, NT)) void
       } else {
         floatx8 v;
         fp32_of(f.dy[b], v);
-        if (MODE == RQ_RUNS) v *= f.sc * rq_unit<NB>();
         rq_operand<P::dy>(v, d[b]);
       }
     }
     // an inf's product with a piece of 0 would be a NaN that the formula does not have
     bf16x8 low[NT];
-    if constexpr (P::w > 1) {
 #pragma unroll
-      for (int b = 0; b < NT; ++b)
+    for (int b = 0; b < NT; ++b)
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          const float v = (float)d[b][0][k];
-          low[b][k] = __builtin_fabsf(v) == INFINITY ? (__bf16)0.0f : d[b][0][k];
-        }
-    }
-    uint32_t odd[8];
-#pragma unroll
-    for (int k = 0; k < 8; ++k) {                                  // fields to bit 0, two's complement
-#pragma unroll
-      for (int m = 0; m < Col8<NB>::N; ++m) {
-        const uint32_t hi = m + 1 < Col8<NB>::NW ? f.wd[k][m + 1] : 0u;
-        const uint32_t v = NB % 4 == 0 ? f.wd[k][m] : (uint32_t)((((uint64_t)hi << 32) | f.wd[k][m]) >> off);
-        f.wd[k][m] = v ^ rq_top_bits<NB>(m);
+      for (int k = 0; k < 8; ++k) {
+        const float v = (float)d[b][0][k];
+        low[b][k] = __builtin_fabsf(v) == INFINITY ? (__bf16)0.0f : d[b][0][k];
       }
-      odd[k] = NB == 4 ? rq_odd_nibbles(f.wd[k][0]) : 0u;
-    }
+    uint32_t odd[8];
+    col_fields<NB>(l.off, f.wd, odd);
 #pragma unroll
     for (int n = 0; n < 8; ++n) {
       const floatx8 codes = col_codes<NB>(f.wd, odd, n);
       bf16x8 v[P::w];
-      if constexpr (P::w == 1) {
-        rq_convert(codes, v[0]);
-      } else {
-        floatx8 sc = f.sc;
-        if (MODE == RQ_ANY) {
+      floatx8 sc = f.sc;
+      if (MODE == RQ_ANY) {
 #pragma unroll
-          for (int k = 0; k < 8; ++k) sc[k] = rq_scale_of(w, g[n], FULL ? r + k : min(r + k, w.R - 1));
-          if (!FULL) {
+        for (int k = 0; k < 8; ++k) sc[k] = rq_scale_of(w, g[n], FULL ? r + k : min(r + k, w.R - 1));
+        if (!FULL) {
 #pragma unroll
-            for (int k = 0; k < 8; ++k) sc[k] = r + k < w.R ? sc[k] : 0.0f;
-          }
+          for (int k = 0; k < 8; ++k) sc[k] = r + k < w.R ? sc[k] : 0.0f;
         }
-        rq_operand<P::w>(sc * rq_unit<NB>() * codes, v);
       }
+      rq_operand<P::w>(sc * rq_unit<NB>() * codes, v);
 #pragma unroll
       for (int pd = 0; pd < P::dy; ++pd)
 #pragma unroll
         for (int pw = 0; pw < P::w; ++pw)
           if (pd + pw < PIECES_KEPT) {
 #pragma unroll
-            for (int b = 0; b < NT; ++b) {
-              if constexpr (P::w > 1) acc[n][b] = rq_mfma(pd == 0 && pw ? low[b] : d[b][pd], v[pw], acc[n][b]);
-              else acc[n][b] = rq_mfma(d[b][pd], v[pw], acc[n][b]);
-            }
+            for (int b = 0; b < NT; ++b) acc[n][b] = rq_mfma(pd == 0 && pw ? low[b] : d[b][pd], v[pw], acc[n][b]);
           }
     }
   };
   // A step's loads are in flight while the one before is computed.
   const int sf = min(sb, w.R / STEP);                              // up to here steps are full
   Step now, then;
-  int st = sa + wave;
+  int st = first;
   if (st < sf) {
     load(std::true_type{}, st, now);
     for (; st + W < sf; st += W) {
@@ -221,7 +330,16 @@ __global__ __launch_bounds__(64 * cols_waves(NT), cols_occupancy(MODE, NT)) void
     load(std::false_type{}, st, now);
     compute(std::false_type{}, st, now);
   }
-  // The waves' sums, halved together: always in the same order.
+}
+
+// The waves' sums, halved together, always in the same order, and stored: to part [parts, T, C] or, without parts, to dx.
+template <typename TX, int NT>
+__device__ __forceinline__ void cols_store(floatx4 (&acc)[8][NT], int t0, int T, int C, float* __restrict__ part,
+                                           TX* __restrict__ dx, int64_t ldx) {
+  constexpr int W = cols_waves(NT);
+  __shared__ floatx4 join[W / 2][8 * NT][64];
+  const int lane = threadIdx.x & 63, wave = rq_wave(), q = lane >> 4;
+  const int c = blockIdx.x * COLS + 8 * (lane & 15), nc = min(8, C - c);
 #pragma unroll
   for (int half = W / 2; half; half >>= 1) {
     if (wave >= half && wave < 2 * half) {
@@ -250,7 +368,7 @@ __global__ __launch_bounds__(64 * cols_waves(NT), cols_occupancy(MODE, NT)) void
 #pragma unroll
       for (int n = 0; n < 8; ++n) v[n] = acc[n][b][k];
       if (part) {
-        float* to = part + ((int64_t)blockIdx.y * T + t) * w.C + c;
+        float* to = part + ((int64_t)blockIdx.y * T + t) * C + c;
         if (nc >= 8) {
           __builtin_memcpy(to, &v, 32);
         } else {
@@ -266,6 +384,44 @@ __global__ __launch_bounds__(64 * cols_waves(NT), cols_occupancy(MODE, NT)) void
     }
 }
 
+// Grid (tiles of 128 columns, parts, tiles of 16 NT tokens).  NM weights one after the other: dx = dy_0 W_0 + dy_1 W_1,
+// dy_1 lying `plane` elements behind dy_0, and a part is a range of the steps of all.
+template <typename TX, int NB, int MODE, int NT, int NM>
+__global__ __launch_bounds__(64 * cols_waves(NT), cols_occupancy(MODE, NT)) void k_packed_cols(
+    const TX* __restrict__ dy, int T, int64_t ldy, int64_t plane, RqPacked w0, RqPacked w1, int steps_per, float* __restrict__ part,
+    TX* __restrict__ dx, int64_t ldx) {
+  constexpr int W = cols_waves(NT);
+  const int wave = rq_wave(), t0 = blockIdx.z * 16 * NT;
+  const int nsteps = (w0.R + STEP - 1) / STEP;
+  const int sa = blockIdx.y * steps_per, sb = min(NM * nsteps, sa + steps_per);
+  floatx4 acc[8][NT];
+  auto run = [&](auto careful) {
+#pragma unroll
+    for (int n = 0; n < 8; ++n)
+#pragma unroll
+      for (int b = 0; b < NT; ++b) acc[n][b] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 1
+    for (int m = 0; m < NM; ++m) {
+      const int from = max(sa - m * nsteps, 0) + wave, to = min(sb - m * nsteps, nsteps);
+      const RqPacked& w = NM == 2 && m ? w1 : w0;
+      if constexpr (MODE == RQ_RUNS) cols_runs<TX, NB, NT, decltype(careful)::value>(dy + m * plane, T, ldy, w, t0, from, to, acc);
+      else cols_scaled<TX, NB, MODE, NT>(dy + m * plane, T, ldy, w, t0, from, to, acc);
+    }
+  };
+  run(std::false_type{});
+  if constexpr (MODE == RQ_RUNS) {
+    bool nan = false;
+#pragma unroll
+    for (int n = 0; n < 8; ++n)
+#pragma unroll
+      for (int b = 0; b < NT; ++b)
+#pragma unroll
+        for (int k = 0; k < 4; k += 2) nan |= __builtin_isunordered(acc[n][b][k], acc[n][b][k + 1]);
+    if (__any(nan)) run(std::true_type{});
+  }
+  cols_store<TX, NT>(acc, t0, T, w0.C, part, dx, ldx);
+}
+
 template <typename TX>
 __global__ __launch_bounds__(256) void k_packed_join(const float* __restrict__ part, int nparts, int T, int C,
                                                      TX* __restrict__ dx, int64_t ldx) {
@@ -276,29 +432,41 @@ __global__ __launch_bounds__(256) void k_packed_join(const float* __restrict__ p
   dx[(int64_t)t * ldx + c] = rq_cast<TX>(s);
 }
 
-template <typename TX, int NB, int MODE, int NT>
-void launch_cols(const TX* dy, int T, int64_t ldy, const RqPacked& w, const RqColSplit& sp, float* part, TX* dx, int64_t ldx,
-                 hipStream_t s) {
-  hipLaunchKernelGGL((k_packed_cols<TX, NB, MODE, NT>), dim3((w.C + COLS - 1) / COLS, sp.parts, (T + 16 * NT - 1) / (16 * NT)),
-                     dim3(64 * cols_waves(NT)), 0, s, dy, T, ldy, w, sp.steps_per, part, dx, ldx);
-}
-template <typename TX, int NB, int MODE>
-void linear_cols(const TX* dy, int T, int64_t ldy, const RqPacked& w, const RqColSplit& sp, float* part, TX* dx, int64_t ldx,
-                 hipStream_t s) {
-  constexpr int NT = RqOperand<TX>::pieces == 1 ? 4 : 2;        // fp32's pieces leave registers for two token tiles
-  if (T <= 16) launch_cols<TX, NB, MODE, 1>(dy, T, ldy, w, sp, part, dx, ldx, s);
-  else if (T <= 32) launch_cols<TX, NB, MODE, 2>(dy, T, ldy, w, sp, part, dx, ldx, s);
-  else launch_cols<TX, NB, MODE, NT>(dy, T, ldy, w, sp, part, dx, ldx, s);
-}
-// T <= RQ_COL_TOKENS tokens to their parts [sp.parts, T, C], or, without parts, to dx.
+// dy times one weight (w1 NULL) or two: T tokens to part [sp.parts, T, C] or, without, to dx.
 template <typename TX>
-void cols_of(const TX* dy, int T, int64_t ldy, const RqPacked& w, int nbits, const RqColSplit& sp, float* part, TX* dx,
-             int64_t ldx, hipStream_t s) {
+struct Cols {
+  const TX* dy;
+  int T;
+  int64_t ldy, plane;
+  const RqPacked* w1;
+  RqColSplit sp;
+  float* part;
+  TX* dx;
+  int64_t ldx;
+};
+template <typename TX, int NB, int MODE, int NT, int NM>
+void launch_cols(const Cols<TX>& a, const RqPacked& w, hipStream_t s) {
+  hipLaunchKernelGGL((k_packed_cols<TX, NB, MODE, NT, NM>), dim3((w.C + COLS - 1) / COLS, a.sp.parts, (a.T + 16 * NT - 1) / (16 * NT)),
+                     dim3(64 * cols_waves(NT)), 0, s, a.dy, a.T, a.ldy, a.plane, w, NM == 2 ? *a.w1 : w, a.sp.steps_per, a.part, a.dx,
+                     a.ldx);
+}
+template <typename TX, int NB, int MODE, int NM>
+void linear_cols(const Cols<TX>& a, const RqPacked& w, hipStream_t s) {
+  // where codes and fp32 tokens are both cut, registers are left for two token tiles
+  constexpr int NT = RqOperand<TX>::pieces == 1 || MODE == RQ_RUNS ? 4 : 2;
+  if (a.T <= 16) launch_cols<TX, NB, MODE, 1, NM>(a, w, s);
+  else if (a.T <= 32) launch_cols<TX, NB, MODE, 2, NM>(a, w, s);
+  else launch_cols<TX, NB, MODE, NT, NM>(a, w, s);
+}
+template <typename TX, int NM>
+void cols_of(const Cols<TX>& a, const RqPacked& w, int nbits, hipStream_t s) {
   rq_with_nbits(nbits, [&](auto nb) {
     constexpr int NB = decltype(nb)::value;
-    if (rq_runs_of(w, COLS)) linear_cols<TX, NB, RQ_RUNS>(dy, T, ldy, w, sp, part, dx, ldx, s);
-    else if (w.groupsize > 0 && w.groupsize % 8 == 0) linear_cols<TX, NB, RQ_SMALL>(dy, T, ldy, w, sp, part, dx, ldx, s);
-    else linear_cols<TX, NB, RQ_ANY>(dy, T, ldy, w, sp, part, dx, ldx, s);
+    switch (rq_cols_mode_of(w)) {
+      case RQ_RUNS: linear_cols<TX, NB, RQ_RUNS, NM>(a, w, s); break;
+      case RQ_SMALL: linear_cols<TX, NB, RQ_SMALL, NM>(a, w, s); break;
+      default: linear_cols<TX, NB, RQ_ANY, NM>(a, w, s);
+    }
   });
 }
 
@@ -307,7 +475,7 @@ void cols_of(const TX* dy, int T, int64_t ldy, const RqPacked& w, int nbits, con
 template <typename TX>
 void rq_cols_parts(const TX* dy, int T, int64_t ldy, const RqPacked& w, int nbits, const RqColSplit& sp, float* part,
                    hipStream_t s) {
-  cols_of<TX>(dy, T, ldy, w, nbits, sp, part, nullptr, 0, s);
+  cols_of<TX, 1>(Cols<TX>{dy, T, ldy, 0, nullptr, sp, part, nullptr, 0}, w, nbits, s);
 }
 
 template <typename TX>
@@ -317,7 +485,7 @@ void rq_linear_cols(const TX* dy, int T, int64_t ldy, const RqPacked& w, int nbi
     const int n = (int)(T - t0 < RQ_COL_TOKENS ? T - t0 : RQ_COL_TOKENS);
     const RqColSplit sp = rq_col_split(n, w.R, w.C);
     TX* out = dx + t0 * ldx;
-    cols_of<TX>(dy + t0 * ldy, n, ldy, w, nbits, sp, sp.parts > 1 ? part : nullptr, out, ldx, s);
+    cols_of<TX, 1>(Cols<TX>{dy + t0 * ldy, n, ldy, 0, nullptr, sp, sp.parts > 1 ? part : nullptr, out, ldx}, w, nbits, s);
     if (sp.parts > 1)
       hipLaunchKernelGGL(k_packed_join<TX>, dim3((w.C + 255) / 256, n), dim3(256), 0, s, part, sp.parts, n, w.C, out, ldx);
   }

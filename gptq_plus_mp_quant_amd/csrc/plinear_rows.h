@@ -16,21 +16,29 @@ namespace {
 // MORE adds what else a row tile's sums take (RqNothing, or the low-rank term of plora_kernels.h).
 constexpr int rows_threads(int rt, int nt) { return rt * nt >= 2 ? 512 : 1024; }     // 256 or 128 registers a lane
 struct RqNothing {
+  static constexpr bool arranged = false, whole = false;
   template <int RT, int NT>
   __device__ __forceinline__ void add(int, int, int, int, int, int, floatx4 (&)[RT][NT]) const {}
 };
+// ARRANGED (MORE::arranged, more than one token tile, RUNS): x lies as RqArranged has it, at more.arranged_x.
 template <typename TX, int NB, int MODE, int RT, int NT, typename MORE>
 __global__ __launch_bounds__(rows_threads(RT, NT)) void k_packed_rows(const TX* __restrict__ x, int T, int64_t ldx, RqPacked w,
                                                       const TX* __restrict__ bias, TX* __restrict__ y, int64_t ldy, MORE more) {
   extern __shared__ __attribute__((aligned(16))) float lds[];
   const int lane = threadIdx.x & 63, wave = rq_wave(), waves = blockDim.x >> 6;
   const int r0 = blockIdx.x * 16 * RT, t0 = blockIdx.y * 16 * NT;
-  RqTokens<TX, NT> xs;
+  constexpr bool ARRANGED = MORE::arranged && MODE == RQ_RUNS && NT > 1;
+  typename std::conditional<ARRANGED, RqArranged<TX, NT, rq_pairs<TX>(NB)>,
+                            typename std::conditional<MORE::whole, RqWholeTokens<TX, NT>, RqTokens<TX, NT>>::type>::type xs;
+  if constexpr (ARRANGED) rq_arranged_tokens<TX>(more.arranged_x, T, w.C, t0, xs.p);
+  else {
 #pragma unroll
-  for (int b = 0; b < NT; ++b) xs.p[b] = x + (int64_t)min(t0 + 16 * b + (lane & 15), T - 1) * ldx;
+    for (int b = 0; b < NT; ++b) xs.p[b] = x + (int64_t)min(t0 + 16 * b + (lane & 15), T - 1) * ldx;
+  }
   const bool staged = MODE == RQ_ANY && w.ngroups <= RQ_STAGED_GROUPS;
   if (staged) {
-    for (int a = 0; a < RT; ++a) rq_stage_scales(w, r0 + 16 * a, a, RT, threadIdx.x, blockDim.x, lds);
+    for (int a = 0; a < RT; ++a)
+      rq_stage_scales(w, rq_tile_row<MORE::whole>(r0 + 16 * a, w.R), a, RT, threadIdx.x, blockDim.x, lds);
     __syncthreads();
   }
   floatx4 acc[RT][NT];
@@ -49,7 +57,7 @@ __global__ __launch_bounds__(rows_threads(RT, NT)) void k_packed_rows(const TX* 
   __syncthreads();
   for (int e = threadIdx.x; e < RT * NT * 64; e += blockDim.x) {
     const int l = e & 63, b = (e >> 6) % NT, a = (e >> 6) / NT;
-    const int t = t0 + 16 * b + (l & 15), r = r0 + 16 * a + 4 * (l >> 4);
+    const int t = t0 + 16 * b + (l & 15), r = rq_tile_row<MORE::whole>(r0 + 16 * a, w.R) + 4 * (l >> 4);
     if (t >= T) continue;
     floatx4 v = out[e];
     for (int k = 1; k < waves; ++k) v += out[k * RT * NT * 64 + e];
@@ -89,7 +97,7 @@ template <typename TX, int NB, typename MORE>
 void linear_rows(const TX* x, int T, int64_t ldx, const RqPacked& w, const TX* bias, TX* y, int64_t ldy, const MORE& more,
                  hipStream_t s) {
   constexpr int R2 = RqOperand<TX>::pieces == 1 ? 2 : 1;      // fp32's pieces leave registers for one row tile
-  switch (rq_mode_of(w)) {
+  switch (MORE::whole ? rq_whole_mode_of(w) : rq_mode_of(w)) {
     case RQ_RUNS:
       // Two row tiles a wave share their tokens' loads.  Up to 16 tokens they are taken where they still make a workgroup
       // for every CU (8192 x 28672 4-bit bf16, 1 / 16 tokens: 42 / 71 us with one, 35 / 49 with two); beyond, where a
@@ -100,6 +108,8 @@ void linear_rows(const TX* x, int T, int64_t ldx, const RqPacked& w, const TX* b
       else if (T <= 16) launch_rows<TX, NB, RQ_RUNS, 1, 1>(x, T, ldx, w, bias, y, ldy, more, s);
       else if (T <= 32 && w.R > 4096) launch_rows<TX, NB, RQ_RUNS, R2, 2>(x, T, ldx, w, bias, y, ldy, more, s);
       else if (T <= 32) launch_rows<TX, NB, RQ_RUNS, 1, 2>(x, T, ldx, w, bias, y, ldy, more, s);
+      else if (T <= 48 && w.R > 4096) launch_rows<TX, NB, RQ_RUNS, R2, 3>(x, T, ldx, w, bias, y, ldy, more, s);
+      else if (T <= 48) launch_rows<TX, NB, RQ_RUNS, 1, 3>(x, T, ldx, w, bias, y, ldy, more, s);
       else if (w.R > 4096) launch_rows<TX, NB, RQ_RUNS, R2, 4>(x, T, ldx, w, bias, y, ldy, more, s);
       else launch_rows<TX, NB, RQ_RUNS, 1, 4>(x, T, ldx, w, bias, y, ldy, more, s);
       break;

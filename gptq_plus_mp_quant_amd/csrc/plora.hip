@@ -13,26 +13,28 @@ namespace {
 constexpr int TOKENS = 1 << 19;             // of one call: grids hold 65535 x 16 tokens and more
 
 bool lora_ok(const void* a, const void* b, int n, int r) { return a && b && n > 0 && n <= 65535 && r > 0 && r <= LORA_MAX_RANK; }
-// rank tiles times parts are a grid's third dimension
-bool width_ok(int cols, int r) { return (int64_t)((r + 15) / 16) * ((cols - 1) / RQ_LORA_COLS + 1) <= 65535; }
+// rank tiles times parts are a grid's third dimension, of both jobs together
+bool width_ok(int cols, int r) { return (int64_t)((r + 31) / 32 * 2) * ((cols - 1) / RQ_LORA_COLS + 1) <= 32767; }
+// workgroups for da and db
+bool outer_ok(int R, int C, int n, int r) { return ((int64_t)(C + 127) / 128 + (R + 127) / 128) * ((r + 15) / 16) * n <= 1 << 30; }
 
 struct GradSpace {
   int64_t u, v, part;                       // floats
 };
 GradSpace grad_space(int T, int R, int C, int r) {
-  GradSpace g = {rq_low_floats(rq_low(nullptr, T, C, r)), rq_low_floats(rq_low(nullptr, T, R, r)), 0};
-  for (const int n : {T < RQ_COL_TOKENS ? T : RQ_COL_TOKENS, T % RQ_COL_TOKENS}) {
-    const int64_t need = n ? (int64_t)rq_col_split(n, R, C).parts * n * C : 0;
-    g.part = need > g.part ? need : g.part;
-  }
-  return g;
+  return GradSpace{rq_low_floats(rq_low(nullptr, T, C, r)), rq_low_floats(rq_low(nullptr, T, R, r)),
+                   rq_col_parts_floats(T, rq_col_steps(R), C)};
 }
 
 }  // namespace
 
-extern "C" int64_t rq_packed_linear_lora_workspace_bytes(int T, int C, int r) {
+extern "C" int64_t rq_packed_linear_lora_workspace_bytes(int T, int C, int r, int dtype) {
   if (T < 0 || T > TOKENS || C <= 0 || r <= 0 || r > LORA_MAX_RANK || !width_ok(C, r)) return RQ_EINVAL;
-  return 4 * rq_low_floats(rq_low(nullptr, T, C, r));
+  int64_t bytes = 4 * rq_low_floats(rq_low(nullptr, T, C, r));
+  const bool known = rq_with_dtype(dtype, [&](auto* p) {
+    if (T > 16) bytes += rq_arranged_bytes<typename std::remove_pointer<decltype(p)>::type>(T, C);
+  });
+  return known ? bytes : RQ_EINVAL;
 }
 
 extern "C" int rq_packed_linear_lora(const void* x, int dtype, int T, int64_t ldx, int C, const uint32_t* qweight, int64_t ldp,
@@ -45,14 +47,15 @@ extern "C" int rq_packed_linear_lora(const void* x, int dtype, int T, int64_t ld
     return RQ_EINVAL;
   if (T == 0) return RQ_OK;
   if (!x || !y || ldx < C || ldy < R) return RQ_EINVAL;
-  if (!workspace || workspace_bytes < rq_packed_linear_lora_workspace_bytes(T, C, r)) return RQ_EINVAL;
+  if (!workspace || workspace_bytes < rq_packed_linear_lora_workspace_bytes(T, C, r, dtype)) return RQ_EINVAL;
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   const bool known = rq_with_dtype(dtype, [&](auto* p) {
     typedef typename std::remove_pointer<decltype(p)>::type TX;
     const RqLora<TX> lora{(const TX*)lora_a, (const TX*)lora_b, adapter_ids, scaling, scale, n, r};
-    const RqLow low = rq_low((float*)workspace, T, C, r);
-    rq_lora_down<TX>((const TX*)x, T, ldx, C, true, lora, low, s);
-    rq_lora_rows<TX>((const TX*)x, T, ldx, w, nbits, (const TX*)bias, lora, low, (TX*)y, ldy, s);
+    const RqLow low = rq_low((float*)workspace, T, C, r);          // a multiple of 128 bytes
+    void* arranged = rq_lora_arranged(T, w) ? (float*)workspace + rq_low_floats(low) : nullptr;
+    rq_lora_down<TX>(RqDown<TX>{(const TX*)x, ldx, C, 1, low}, nullptr, lora, arranged, nbits, s);
+    rq_lora_rows<TX>((const TX*)x, T, ldx, w, nbits, (const TX*)bias, lora, low, arranged, (TX*)y, ldy, s);
   });
   if (!known) return RQ_EINVAL;
   RQ_CHECK_LAUNCH();
@@ -73,7 +76,7 @@ extern "C" int rq_packed_linear_lora_grad(const void* grad_y, int dtype, int T, 
                                           int64_t workspace_bytes, void* stream) {
   const RqPacked w = rq_packed(qweight, ldp, scales, lds, g_idx, R, C, ngroups, groupsize);
   if (T < 0 || T > TOKENS || rq_packed_check(w, nbits) != RQ_OK || !lora_ok(lora_a, lora_b, n, r) || !width_ok(C, r) ||
-      !width_ok(R, r))
+      !width_ok(R, r) || !outer_ok(R, C, n, r))
     return RQ_EINVAL;
   if (!grad_a != !grad_b || (T && (!grad_y || !x || ldg < R || ldx < C || (grad_x && ldgx < C)))) return RQ_EINVAL;
   const GradSpace g = grad_space(T, R, C, r);
@@ -86,15 +89,17 @@ extern "C" int rq_packed_linear_lora_grad(const void* grad_y, int dtype, int T, 
     const RqLow u = rq_low(ws, T, C, r), v = rq_low(ws + g.u, T, R, r);
     float* part = ws + g.u + g.v;
     const TX* dy = (const TX*)grad_y;
-    if (T) rq_lora_down<TX>(dy, T, ldg, R, false, lora, v, s);
-    if (T && grad_a) rq_lora_down<TX>((const TX*)x, T, ldx, C, true, lora, u, s);
-    for (int t0 = 0; grad_x && t0 < T; t0 += RQ_COL_TOKENS) {
-      const int k = T - t0 < RQ_COL_TOKENS ? T - t0 : RQ_COL_TOKENS;
-      const RqColSplit sp = rq_col_split(k, R, C);
+    const RqDown<TX> ofx{(const TX*)x, ldx, C, 1, u};
+    if (T) rq_lora_down<TX>(RqDown<TX>{dy, ldg, R, 0, v}, grad_a ? &ofx : nullptr, lora, nullptr, nbits, s);
+    RqLoraDx<TX> dx{part, 0, 0, 0, nullptr, ldgx};
+    for (int t0 = 0; grad_x && t0 < T; t0 += RQ_COL_WIDE) {
+      const int k = T - t0 < RQ_COL_WIDE ? T - t0 : RQ_COL_WIDE;
+      const RqColSplit sp = rq_col_split_wide(k, rq_col_steps(R), C);
       rq_cols_parts<TX>(dy + t0 * ldg, k, ldg, w, nbits, sp, part, s);
-      rq_lora_dx<TX>(part, sp.parts, t0, k, C, lora, v, (TX*)grad_x + t0 * ldgx, ldgx, s);
+      dx = RqLoraDx<TX>{part, sp.parts, t0, k, (TX*)grad_x + t0 * ldgx, ldgx};
+      if (t0 + k < T) rq_lora_grads<TX>(dx, (const TX*)x, ldx, C, dy, ldg, R, T, lora, u, v, nullptr, nullptr, s);
     }
-    if (grad_a) rq_lora_outer<TX>((const TX*)x, ldx, C, dy, ldg, R, T, lora, u, v, (TX*)grad_a, (TX*)grad_b, s);
+    rq_lora_grads<TX>(dx, (const TX*)x, ldx, C, dy, ldg, R, T, lora, u, v, (TX*)grad_a, (TX*)grad_b, s);
   });
   if (!known) return RQ_EINVAL;
   RQ_CHECK_LAUNCH();

@@ -20,32 +20,28 @@ __device__ __forceinline__ floatx4 mfma32(floatx8 a, floatx8 b, floatx4 c) {
   return c;
 }
 
-// Four elements from p on as fp32, the first n of them (which may be none; the rest 0).
-template <typename TX>
-__device__ __forceinline__ floatx4 load4(const TX* p, int n) {
-  floatx4 v = {0.0f, 0.0f, 0.0f, 0.0f};
-  if (n >= 4) {
-    TX e[4];
-    __builtin_memcpy(e, p, sizeof(e));
-#pragma unroll
-    for (int k = 0; k < 4; ++k) v[k] = rq_load_elem(e + k);
-  } else {
-#pragma unroll
-    for (int k = 0; k < 4; ++k)
-      if (k < n) v[k] = rq_load_elem(p + k);
-  }
-  return v;
-}
-
 // u = A x or B^T x.  Grid (tiles of 16 tokens, the tile's adapters in the order of their first tokens, rank tiles x
-// parts); the waves take steps of 32 columns in turn and are joined through LDS in their order.
-constexpr int DOWN_WAVES = 8;
-template <typename TX, bool ROWS>
-__global__ __launch_bounds__(64 * DOWN_WAVES) void k_lora_down(const TX* __restrict__ x, int64_t ldx, int cols, RqLora<TX> lora,
-                                                               RqLow low) {
+// parts of one job and then of the other, and behind them chunks of the first's x to be
+// arranged); the waves take steps of 32 columns in turn, all of a full part's in flight at
+// once, and are joined through LDS in their order.
+constexpr int ARRANGED_CHUNKS = 16;
+constexpr int DOWN_WAVES = 16, DOWN_STEPS = RQ_LORA_COLS / (32 * DOWN_WAVES);
+template <typename TX>
+__global__ __launch_bounds__(64 * DOWN_WAVES) void k_lora_down(RqDown<TX> first, RqDown<TX> second, int zfirst, RqLora<TX> lora,
+                                                               RqArrange arrange) {
   typedef typename RqOperand<TX>::raw Raw;
   __shared__ floatx4 join[DOWN_WAVES][64];
   const int lane = threadIdx.x & 63, wave = rq_wave(), i = lane & 15, q = lane >> 4;
+  if ((int)blockIdx.z >= arrange.z) {
+    const int ch = (blockIdx.z - arrange.z) * ARRANGED_CHUNKS, chunks = (first.cols + RQ_CHUNK - 1) / RQ_CHUNK;
+    if (blockIdx.y == 0)
+      rq_arrange<TX>(first.x, first.low.T, first.ldx, first.cols, blockIdx.x, ch, min(ch + ARRANGED_CHUNKS, chunks), arrange.paired,
+                     threadIdx.x, blockDim.x, arrange.out);
+    return;
+  }
+  const RqDown<TX> d = (int)blockIdx.z < zfirst ? first : second;
+  const RqLow& low = d.low;
+  const int z = (int)blockIdx.z < zfirst ? blockIdx.z : blockIdx.z - zfirst;
   const int64_t t = (int64_t)blockIdx.x * 16 + i;
   const int own = t < low.T ? lora.of(t) : -1;
   uint64_t pending = __ballot(lane < 16 && own >= 0 && own < lora.n);
@@ -53,18 +49,17 @@ __global__ __launch_bounds__(64 * DOWN_WAVES) void k_lora_down(const TX* __restr
     pending &= ~__ballot(own == __builtin_amdgcn_readlane(own, __ffsll((unsigned long long)pending) - 1));
   if (!pending) return;
   const int lead = __ffsll((unsigned long long)pending) - 1, a = __builtin_amdgcn_readlane(own, lead);
-  const int tiles = low.ranks / 16, rank = (blockIdx.z % tiles) * 16, part = blockIdx.z / tiles;
-  const int c0 = part * RQ_LORA_COLS, c1 = min(cols, c0 + RQ_LORA_COLS);
-  const TX* xs = x + (own == a ? t : (int64_t)blockIdx.x * 16 + lead) * ldx;
+  const int tiles = low.ranks / 16, rank = z % tiles * 16, part = z / tiles;
+  const int c0 = part * RQ_LORA_COLS, c1 = min(d.cols, c0 + RQ_LORA_COLS);
+  const TX* xs = d.x + (own == a ? t : (int64_t)blockIdx.x * 16 + lead) * d.ldx;
   const int row = min(rank + i, lora.r - 1);
-  const TX* as = ROWS ? lora.a + ((int64_t)a * lora.r + row) * cols : lora.b + (int64_t)a * cols * lora.r + row;
+  const TX* as = d.rows ? lora.a + ((int64_t)a * lora.r + row) * d.cols : lora.b + (int64_t)a * d.cols * lora.r + row;
   floatx4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
-  auto step = [&](auto full, int c) {
+  auto load = [&](auto full, int c, Raw& xv, Raw& av) {
     constexpr bool FULL = decltype(full)::value;
     const int n = c1 - c;                            // the lane's columns (may be none)
-    const Raw xv = rq_load_x<FULL>(xs + c, n);
-    Raw av;
-    if constexpr (ROWS) {
+    xv = rq_load_x<FULL>(xs + c, n);
+    if (d.rows) {
       av = rq_load_x<FULL>(as + c, n);
     } else {
 #pragma unroll
@@ -74,12 +69,27 @@ __global__ __launch_bounds__(64 * DOWN_WAVES) void k_lora_down(const TX* __restr
         av[k] = FULL || k < n ? e : (decltype(e))0.0f;
       }
     }
-    acc = mfma32(av, xv, acc);
   };
-  int c = c0 + 32 * wave;
-#pragma unroll 4
-  for (; c + 32 <= c1; c += 32 * DOWN_WAVES) step(std::true_type{}, c + 8 * q);
-  if (c < c1) step(std::false_type{}, c + 8 * q);
+  if (rank >= lora.r) {
+    // a tile of padding
+  } else if (c0 + RQ_LORA_COLS <= c1) {
+    Raw xv[DOWN_STEPS], av[DOWN_STEPS];
+#pragma unroll
+    for (int k = 0; k < DOWN_STEPS; ++k) load(std::true_type{}, c0 + 32 * (wave + DOWN_WAVES * k) + 8 * q, xv[k], av[k]);
+#pragma unroll
+    for (int k = 0; k < DOWN_STEPS; ++k) acc = mfma32(av[k], xv[k], acc);
+  } else {
+    Raw xv, av;
+    int c = c0 + 32 * wave;
+    for (; c + 32 <= c1; c += 32 * DOWN_WAVES) {
+      load(std::true_type{}, c + 8 * q, xv, av);
+      acc = mfma32(av, xv, acc);
+    }
+    if (c < c1) {
+      load(std::false_type{}, c + 8 * q, xv, av);
+      acc = mfma32(av, xv, acc);
+    }
+  }
   join[wave][lane] = acc;
   __syncthreads();
   if (wave || own != a) return;
@@ -90,21 +100,42 @@ __global__ __launch_bounds__(64 * DOWN_WAVES) void k_lora_down(const TX* __restr
   *reinterpret_cast<floatx4*>(low.u + low.at(part, t) + rank + 4 * q) = acc;
 }
 
-// Four ranks of a token, its parts joined in their order.
-__device__ __forceinline__ floatx4 low4(const RqLow& low, int64_t t, int rank) {
-  floatx4 v = *reinterpret_cast<const floatx4*>(low.u + low.at(0, t) + rank);
-  for (int p = 1; p < low.parts; ++p) v += *reinterpret_cast<const floatx4*>(low.u + low.at(p, t) + rank);
+// Eight ranks of a token, its parts joined in their order.
+__device__ __forceinline__ floatx8 low8(const RqLow& low, int64_t t, int rank) {
+  floatx8 v = rq_load_as<floatx8>(low.u + low.at(0, t) + rank);
+#pragma unroll 2
+  for (int p = 1; p < low.parts; ++p) v += rq_load_as<floatx8>(low.u + low.at(p, t) + rank);
   return v;
 }
 
-// s B u to the sums of a row tile: 16 ranks of an adapter at a time, dealt to the waves by adapter and rank alone, so that
-// a token's bits do not depend on its companions.
+// The adapter's side of s B u as bf16 pieces, exactly: bf16 as it is, fp16's 11 bits in two, fp32 in three.
+template <typename TX> struct LoraPieces;
+template <> struct LoraPieces<__hip_bfloat16> { static constexpr int n = 1; };
+template <> struct LoraPieces<__half> { static constexpr int n = 2; };
+template <> struct LoraPieces<float> { static constexpr int n = 3; };
+__device__ __forceinline__ bf16x8 without_inf(bf16x8 v) {
+  bf16x8 o;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    const float f = (float)v[k];
+    o[k] = __builtin_fabsf(f) == INFINITY ? (__bf16)0.0f : v[k];
+  }
+  return o;
+}
+
+// s B u to the sums of a row tile: 32 ranks of an adapter at a time, dealt to the waves by adapter and rank alone, so that
+// a token's bits do not depend on its companions.  u goes in as three bf16 pieces (24 bits), B in as many as hold it; products of
+// pieces i and j with i + j > 2, at most 2^-22 of a term, are left out.  An inf's product with a piece of 0 would be a
+// NaN that the formula does not have: past a number's first piece the other side's infs are 0.
 template <typename TX>
 struct RqLowRank {
+  static constexpr bool arranged = true, whole = true;
   RqLora<TX> lora;
   RqLow low;
+  const void* arranged_x;
   template <int RT, int NT>
   __device__ __forceinline__ void add(int r0, int R, int t0, int T, int wave, int waves, floatx4 (&acc)[RT][NT]) const {
+    constexpr int PW = LoraPieces<TX>::n;
     const int lane = threadIdx.x & 63, i = lane & 15, q = lane >> 4;
     const int mine = lane < 16 * NT && t0 + lane < T ? lora.of(t0 + lane) : -1;
     int own[NT];
@@ -112,24 +143,47 @@ struct RqLowRank {
     for (int b = 0; b < NT; ++b) own[b] = __shfl(mine, 16 * b + i);
     for (uint64_t pending = __ballot(mine >= 0 && mine < lora.n); pending;) {
       const int a = __builtin_amdgcn_readlane(mine, __ffsll((unsigned long long)pending) - 1);
-      pending &= ~__ballot(mine == a);
-      const float s = lora.scale_of(a);
+      const uint64_t who = __ballot(mine == a);
+      pending &= ~who;
       int turn = wave - a % waves;                   // the first of its rank tiles that this wave takes
-      for (int k0 = 16 * (turn < 0 ? turn + waves : turn); k0 < lora.r; k0 += 16 * waves) {
-        const int k = k0 + 4 * q;
-        floatx4 u[NT], part[RT][NT];
-#pragma unroll
-        for (int b = 0; b < NT; ++b) u[b] = low4(low, min(t0 + 16 * b + i, T - 1), k);
+      turn = turn < 0 ? turn + waves : turn;
+      if (32 * turn >= lora.r) continue;
+      const float s = lora.scale_of(a);
+      for (int k0 = 32 * turn; k0 < lora.r; k0 += 32 * waves) {
+        const int k = k0 + 8 * q;
+        bf16x8 w[RT][PW], first[RT];
 #pragma unroll
         for (int m = 0; m < RT; ++m) {
-          const floatx4 w = load4(lora.b + ((int64_t)a * R + min(r0 + 16 * m + i, R - 1)) * lora.r + k, lora.r - k);
+          const TX* p = lora.b + ((int64_t)a * R + min(rq_tile_row<true>(r0 + 16 * m, R) + i, R - 1)) * lora.r + k;
+          const typename RqOperand<TX>::raw e = k + 8 <= lora.r ? rq_load_x<true>(p, 8) : rq_load_x<false>(p, lora.r - k);
+          if constexpr (PW == 1) {
+            w[m][0] = e;
+          } else {
+            floatx8 f;
+            rq_floats(e, f);
+            rq_operand<PW>(f, w[m]);
+          }
+          first[m] = without_inf(w[m][0]);
+        }
 #pragma unroll
-          for (int b = 0; b < NT; ++b) {
-            part[m][b] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int b = 0; b < NT; ++b) {
+          if (!(who >> (16 * b) & 0xFFFF)) continue;
+          bf16x8 u[3];
+          rq_operand<3>(low8(low, min(t0 + 16 * b + i, T - 1), k), u);
+          bf16x8 lead = u[0];
+          if constexpr (PW > 1) lead = without_inf(lead);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) part[m][b] = mfma4(w[j], u[b][j], part[m][b]);
+          for (int m = 0; m < RT; ++m) {
+            floatx4 part = rq_mfma(w[m][0], u[0], floatx4{0.0f, 0.0f, 0.0f, 0.0f});
+            part = rq_mfma(first[m], u[1], part);
+            part = rq_mfma(first[m], u[2], part);
+            if constexpr (PW > 1) {
+              part = rq_mfma(w[m][1], lead, part);
+              part = rq_mfma(w[m][1], u[1], part);
+            }
+            if constexpr (PW > 2) part = rq_mfma(w[m][2], lead, part);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) acc[m][b][j] = own[b] == a ? __builtin_fmaf(s, part[m][b][j], acc[m][b][j]) : acc[m][b][j];
+            for (int j = 0; j < 4; ++j) acc[m][b][j] = own[b] == a ? __builtin_fmaf(s, part[j], acc[m][b][j]) : acc[m][b][j];
           }
         }
       }
@@ -143,50 +197,114 @@ struct RqLowRank {
   }
 };
 
-// dx: the packed weight's parts and the adapter's term.
+// --- the gradients, once the parts of dy W are there --------------------------------------------
+// One launch: workgroups for da and db and, behind them, for dx.
+constexpr int WINDOW = 512;
+
+// Four elements, of which n exist (which may be none): loads past them are moved back to the last, and their values dropped.
 template <typename TX>
-__global__ __launch_bounds__(256) void k_lora_dx(const float* __restrict__ part, int parts, int64_t t0, int T, int C,
-                                                 RqLora<TX> lora, RqLow v, TX* __restrict__ dx, int64_t ldx) {
-  __shared__ float low[LORA_MAX_RANK];
-  const int c = blockIdx.x * 256 + threadIdx.x;
-  const int64_t t = t0 + blockIdx.y;
-  const int a = lora.of(t);
-  if (a >= 0 && a < lora.n) {
-    for (int k = threadIdx.x; k < lora.r; k += 256) {
-      float s = v.u[v.at(0, t) + k];
-      for (int p = 1; p < v.parts; ++p) s += v.u[v.at(p, t) + k];
-      low[k] = s * lora.scale_of(a);
+__device__ __forceinline__ floatx4 load4(const TX* p, int n) {
+  floatx4 v;
+  if (n >= 4) {
+    TX e[4];
+    __builtin_memcpy(e, p, sizeof(e));
+#pragma unroll
+    for (int k = 0; k < 4; ++k) v[k] = rq_load_elem(e + k);
+  } else {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float e = rq_load_elem(p + min(k, n - 1));
+      v[k] = k < n ? e : 0.0f;
     }
-    __syncthreads();
   }
-  if (c >= C) return;
-  float s = 0.0f;
-  for (int p = 0; p < parts; ++p) s += part[((int64_t)p * T + blockIdx.y) * C + c];
-  if (a >= lora.n) s = __builtin_nanf("");
-  else if (a >= 0) {
-    const TX* w = lora.a + (int64_t)a * lora.r * C + c;
-    for (int k = 0; k < lora.r; ++k) s = __builtin_fmaf(low[k], rq_load_elem(w + (int64_t)k * C), s);
-  }
-  dx[(int64_t)blockIdx.y * ldx + c] = rq_cast<TX>(s);
+  return v;
 }
 
-// da and db.  Grid (tiles of 128 columns of x, then of dy; rank tiles; adapters): the tokens of the adapter, four to a
-// matrix instruction, to the waves in turn.  Lane 16 q + i holds columns 8i..8i+7 of token q, and product n takes
-// the n-th of each, so that D's column i is column 8i + n.
-constexpr int OUTER_WAVES = 4, WINDOW = 512;
+// dx of 16 tokens and 64 columns a workgroup: its waves deal the parts among them, and the adapters' ranks, 32 at a time, by
+// adapter and rank alone; joined through LDS in their order.  Lane 16 q + j has columns 4j..4j+3 of ranks 8q..8q+7,
+// product n takes the n-th of each, so that D's column j is column 4j + n.
+constexpr int DX_COLS = 64, GRAD_WAVES = 4;
 template <typename TX>
-__global__ __launch_bounds__(64 * OUTER_WAVES) void k_lora_outer(const TX* __restrict__ x, int64_t ldx, int C,
-                                                                 const TX* __restrict__ dy, int64_t ldy, int R, int T,
-                                                                 RqLora<TX> lora, RqLow u, RqLow v, TX* __restrict__ da,
-                                                                 TX* __restrict__ db) {
+__device__ __forceinline__ void lora_dx(int block, const float* __restrict__ part, int parts, int64_t t0, int T, int C,
+                                        const RqLora<TX>& lora, const RqLow& v, TX* __restrict__ dx, int64_t ldx, floatx4* lds) {
+  const int lane = threadIdx.x & 63, wave = rq_wave(), j = lane & 15, q = lane >> 4;
+  const int ctiles = (C + DX_COLS - 1) / DX_COLS, c = block % ctiles * DX_COLS + 4 * j, tw = block / ctiles * 16;
+  const int nc = C - c;                            // <= 0: none
+  const int mine = tw + j < T ? lora.of(t0 + tw + j) : -1;
+  int own[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) own[k] = __shfl(mine, 4 * q + k);
+  floatx4 o[4];                                    // of token 4q + k
+#pragma unroll
+  for (int k = 0; k < 4; ++k) o[k] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 2
+  for (int m = wave; m < parts; m += GRAD_WAVES)
+#pragma unroll
+    for (int k = 0; k < 4; ++k) o[k] += load4(part + ((int64_t)m * T + min(tw + 4 * q + k, T - 1)) * C + c, nc);
+  for (uint64_t pending = __ballot(lane < 16 && mine >= 0 && mine < lora.n); pending;) {
+    const int a = __builtin_amdgcn_readlane(mine, __ffsll((unsigned long long)pending) - 1);
+    pending &= ~__ballot(mine == a);
+    const int first = 32 * ((wave - a + 2) & (GRAD_WAVES - 1));
+    if (first >= lora.r) continue;
+    const float s = lora.scale_of(a);
+    floatx4 low[4];
+#pragma unroll
+    for (int n = 0; n < 4; ++n) low[n] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int k0 = first; k0 < lora.r; k0 += 32 * GRAD_WAVES) {
+      const floatx8 vt = low8(v, t0 + min(tw + j, T - 1), k0 + 8 * q);
+      floatx4 row[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) row[k] = load4(lora.a + ((int64_t)a * lora.r + min(k0 + 8 * q + k, lora.r - 1)) * C + c, nc);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const bool is = k0 + 8 * q + k < lora.r;
+#pragma unroll
+        for (int n = 0; n < 4; ++n) low[n] = mfma4(vt[k], is ? row[k][n] : 0.0f, low[n]);
+      }
+    }
+#pragma unroll
+    for (int n = 0; n < 4; ++n)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) o[k][n] = own[k] == a ? __builtin_fmaf(s, low[n][k], o[k][n]) : o[k][n];
+  }
+#pragma unroll
+  for (int k = 0; k < 4; ++k) lds[(wave * 4 + k) * 64 + lane] = o[k];
+  __syncthreads();
+  // wave w: token 4q + w
+  const bool none = __shfl(mine, 4 * q + wave) >= lora.n;
+  const int t = tw + 4 * q + wave;
+  if (t >= T) return;
+  floatx4 r = lds[wave * 64 + lane];
+#pragma unroll
+  for (int w = 1; w < GRAD_WAVES; ++w) r += lds[(w * 4 + wave) * 64 + lane];
+  TX* out = dx + (int64_t)t * ldx + c;
+  TX e[4];
+#pragma unroll
+  for (int n = 0; n < 4; ++n) e[n] = rq_cast<TX>(none ? __builtin_nanf("") : r[n]);
+  if (nc >= 4) {
+    __builtin_memcpy(out, e, sizeof(e));
+  } else {
+#pragma unroll
+    for (int n = 0; n < 4; ++n)
+      if (n < nc) out[n] = e[n];
+  }
+}
+
+// da and db.  Blocks (tiles of 128 columns of x, then of dy; rank tiles; adapters): the tokens of the adapter, four to a
+// matrix instruction, sixteen in flight, to the waves in turn.  Lane 16 q + i holds columns 8i..8i+7 of token q, and product n takes
+// the n-th of each, so that D's column i is column 8i + n.
+template <typename TX>
+__device__ __forceinline__ void lora_outer(int block, const TX* __restrict__ x, int64_t ldx, int C, const TX* __restrict__ dy,
+                                           int64_t ldy, int R, int T, const RqLora<TX>& lora, const RqLow& u, const RqLow& v,
+                                           TX* __restrict__ da, TX* __restrict__ db, floatx4* lds) {
   typedef typename RqOperand<TX>::raw Raw;
-  __shared__ floatx4 join[OUTER_WAVES][8][64];
   __shared__ int list[WINDOW];
   __shared__ int count;
   const int lane = threadIdx.x & 63, wave = rq_wave(), i = lane & 15, q = lane >> 4;
-  const int ctiles = (C + 127) / 128, a = blockIdx.z, rank = blockIdx.y * 16;
-  const bool of_a = (int)blockIdx.x < ctiles;        // da: v with x; db: u with dy
-  const int width = of_a ? C : R, col = (of_a ? blockIdx.x : blockIdx.x - ctiles) * 128 + 8 * i;
+  const int ctiles = (C + 127) / 128, tiles = ctiles + (R + 127) / 128, rtiles = (lora.r + 15) / 16;
+  const int tile = block % tiles, a = block / tiles / rtiles, rank = block / tiles % rtiles * 16;
+  const bool of_a = tile < ctiles;                   // da: v with x; db: u with dy
+  const int width = of_a ? C : R, col = (of_a ? tile : tile - ctiles) * 128 + 8 * i;
   const TX* src = of_a ? x : dy;
   const int64_t ld = of_a ? ldx : ldy;
   const RqLow low = of_a ? v : u;
@@ -206,25 +324,41 @@ __global__ __launch_bounds__(64 * OUTER_WAVES) void k_lora_outer(const TX* __res
     }
     __syncthreads();
     const int n = count;
-    for (int g = 4 * wave; g < n; g += 4 * OUTER_WAVES) {
-      const bool is = g + q < n;
-      const int64_t t = w0 + list[is ? g + q : 0];
-      float m = low.u[low.at(0, t) + rank + i];
-      for (int p = 1; p < low.parts; ++p) m += low.u[low.at(p, t) + rank + i];
-      const Raw r = col + 8 <= width ? rq_load_x<true>(src + t * ld + col, 8) : rq_load_x<false>(src + t * ld + col, width - col);
-      floatx8 f;
-      rq_floats(r, f);
-      if (!is) {
-        m = 0.0f;
-        f = floatx8{0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+    for (int g = 16 * wave; g < n; g += 16 * GRAD_WAVES) {
+      float m[4];
+      Raw r[4];
+      int64_t t[4];
+#pragma unroll
+      for (int h = 0; h < 4; ++h) {
+        t[h] = w0 + list[g + 4 * h + q < n ? g + 4 * h + q : 0];
+        m[h] = 0.0f;
+        r[h] = col + 8 <= width ? rq_load_x<true>(src + t[h] * ld + col, 8) : rq_load_x<false>(src + t[h] * ld + col, width - col);
+      }
+      for (int p0 = 0; p0 < low.parts; p0 += 4) {      // four parts' loads at once, the last again past it
+        float e[4][4];
+#pragma unroll
+        for (int p = 0; p < 4; ++p)
+#pragma unroll
+          for (int h = 0; h < 4; ++h) e[p][h] = low.u[low.at(min(p0 + p, low.parts - 1), t[h]) + rank + i];
+#pragma unroll
+        for (int p = 0; p < 4; ++p)
+#pragma unroll
+          for (int h = 0; h < 4; ++h) m[h] += p0 + p < low.parts ? e[p][h] : 0.0f;
       }
 #pragma unroll
-      for (int k = 0; k < 8; ++k) acc[k] = mfma4(m, f[k], acc[k]);
+      for (int h = 0; h < 4; ++h) {
+        if (g + 4 * h >= n) break;
+        const bool is = g + 4 * h + q < n;
+        floatx8 f;
+        rq_floats(r[h], f);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) acc[k] = mfma4(is ? m[h] : 0.0f, is ? f[k] : 0.0f, acc[k]);
+      }
     }
     __syncthreads();
   }
 #pragma unroll
-  for (int n = 0; n < 8; ++n) join[wave][n][lane] = acc[n];
+  for (int n = 0; n < 8; ++n) lds[(wave * 8 + n) * 64 + lane] = acc[n];
   __syncthreads();
   const float s = lora.scale_of(a);
   if (of_a) {
@@ -235,7 +369,7 @@ __global__ __launch_bounds__(64 * OUTER_WAVES) void k_lora_outer(const TX* __res
 #pragma unroll
     for (int n = 0; n < 8; ++n) {
       float o = 0.0f;
-      for (int w = 0; w < OUTER_WAVES; ++w) o += join[w][n][lane][wave];
+      for (int w = 0; w < GRAD_WAVES; ++w) o += lds[(w * 8 + n) * 64 + lane][wave];
       if (col + n < C) out[n] = rq_cast<TX>(s * o);
     }
   } else {
@@ -243,8 +377,8 @@ __global__ __launch_bounds__(64 * OUTER_WAVES) void k_lora_outer(const TX* __res
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const int n = 2 * wave + h, row = col + n;
-      floatx4 o = join[0][n][lane];
-      for (int w = 1; w < OUTER_WAVES; ++w) o += join[w][n][lane];
+      floatx4 o = lds[n * 64 + lane];
+      for (int w = 1; w < GRAD_WAVES; ++w) o += lds[(w * 8 + n) * 64 + lane];
       if (row >= R) continue;
       TX* out = db + ((int64_t)a * R + row) * lora.r + rank + 4 * q;
 #pragma unroll
@@ -254,32 +388,40 @@ __global__ __launch_bounds__(64 * OUTER_WAVES) void k_lora_outer(const TX* __res
   }
 }
 
+template <typename TX>
+__global__ __launch_bounds__(64 * GRAD_WAVES, 4) void k_lora_grads(RqLoraDx<TX> g, int outer, const TX* x, int64_t ldx, int C,
+                                                                 const TX* dy, int64_t ldy, int R, int T, RqLora<TX> lora, RqLow u,
+                                                                 RqLow v, TX* da, TX* db) {
+  __shared__ floatx4 lds[GRAD_WAVES * 8 * 64];
+  if ((int)blockIdx.x >= outer) lora_dx<TX>(blockIdx.x - outer, g.part, g.parts, g.t0, g.T, C, lora, v, g.dx, g.ldx, lds);
+  else lora_outer<TX>(blockIdx.x, x, ldx, C, dy, ldy, R, T, lora, u, v, da, db, lds);
+}
+
 }  // namespace
 
 template <typename TX>
-void rq_lora_down(const TX* x, int T, int64_t ldx, int cols, bool rows, const RqLora<TX>& lora, const RqLow& low, hipStream_t s) {
-  const dim3 grid((T + 15) / 16, lora.ids ? (lora.n < 16 ? lora.n : 16) : 1, low.ranks / 16 * low.parts), block(64 * DOWN_WAVES);
-  if (rows) hipLaunchKernelGGL((k_lora_down<TX, true>), grid, block, 0, s, x, ldx, cols, lora, low);
-  else hipLaunchKernelGGL((k_lora_down<TX, false>), grid, block, 0, s, x, ldx, cols, lora, low);
+void rq_lora_down(const RqDown<TX>& first, const RqDown<TX>* second, const RqLora<TX>& lora, void* arranged, int nbits, hipStream_t s) {
+  const int z0 = first.low.ranks / 16 * first.low.parts, z1 = second ? second->low.ranks / 16 * second->low.parts : 0;
+  const int chunks = (first.cols + RQ_CHUNK - 1) / RQ_CHUNK, z2 = arranged ? (chunks + ARRANGED_CHUNKS - 1) / ARRANGED_CHUNKS : 0;
+  const dim3 grid((first.low.T + 15) / 16, lora.ids ? (lora.n < 16 ? lora.n : 16) : 1, z0 + z1 + z2), block(64 * DOWN_WAVES);
+  hipLaunchKernelGGL(k_lora_down<TX>, grid, block, 0, s, first, second ? *second : first, z0, lora,
+                     RqArrange{arranged, z0 + z1, rq_pairs<TX>(nbits)});
 }
 
 template <typename TX>
 void rq_lora_rows(const TX* x, int T, int64_t ldx, const RqPacked& w, int nbits, const TX* bias, const RqLora<TX>& lora,
-                  const RqLow& low, TX* y, int64_t ldy, hipStream_t s) {
+                  const RqLow& low, const void* arranged, TX* y, int64_t ldy, hipStream_t s) {
   rq_with_nbits(nbits, [&](auto nb) {
-    linear_rows<TX, decltype(nb)::value>(x, T, ldx, w, bias, y, ldy, RqLowRank<TX>{lora, low}, s);
+    linear_rows<TX, decltype(nb)::value>(x, T, ldx, w, bias, y, ldy, RqLowRank<TX>{lora, low, arranged}, s);
   });
 }
 
 template <typename TX>
-void rq_lora_dx(const float* part, int parts, int64_t t0, int T, int C, const RqLora<TX>& lora, const RqLow& v, TX* dx,
-                int64_t ldx, hipStream_t s) {
-  hipLaunchKernelGGL(k_lora_dx<TX>, dim3((C + 255) / 256, T), dim3(256), 0, s, part, parts, t0, T, C, lora, v, dx, ldx);
-}
-
-template <typename TX>
-void rq_lora_outer(const TX* x, int64_t ldx, int C, const TX* dy, int64_t ldy, int R, int T, const RqLora<TX>& lora,
-                   const RqLow& u, const RqLow& v, TX* da, TX* db, hipStream_t s) {
-  hipLaunchKernelGGL(k_lora_outer<TX>, dim3((C + 127) / 128 + (R + 127) / 128, u.ranks / 16, lora.n), dim3(64 * OUTER_WAVES), 0, s,
-                     x, ldx, C, dy, ldy, R, T, lora, u, v, da, db);
+void rq_lora_grads(const RqLoraDx<TX>& g, const TX* x, int64_t ldx, int C, const TX* dy, int64_t ldy, int R, int T,
+                   const RqLora<TX>& lora, const RqLow& u, const RqLow& v, TX* da, TX* db, hipStream_t s) {
+  const int64_t ndx = g.dx ? (int64_t)((C + DX_COLS - 1) / DX_COLS) * ((g.T + 15) / 16) : 0;
+  const int64_t outer = da ? (int64_t)((C + 127) / 128 + (R + 127) / 128) * ((lora.r + 15) / 16) * lora.n : 0;
+  if (ndx + outer == 0) return;
+  hipLaunchKernelGGL(k_lora_grads<TX>, dim3((unsigned)(ndx + outer)), dim3(64 * GRAD_WAVES), 0, s, g, (int)outer, x, ldx, C, dy, ldy,
+                     R, T, lora, u, v, da, db);
 }

@@ -1,6 +1,7 @@
 // Low-rank adapters beside a packed weight: what the launches share.  Each element type's kernels are a translation
 // unit of their own.
 #pragma once
+#include "packed_dot.h"
 #include "plinear_types.h"
 
 constexpr int LORA_MAX_RANK = 256;
@@ -30,24 +31,42 @@ struct RqLow {
   int parts, T, ranks;
   __device__ __forceinline__ int64_t at(int p, int64_t t) const { return ((int64_t)p * T + t) * ranks; }
 };
-constexpr int RQ_LORA_COLS = 4096;
+constexpr int RQ_LORA_COLS = 2048;
 inline RqLow rq_low(float* u, int T, int cols, int r) {
-  return RqLow{u, (cols - 1) / RQ_LORA_COLS + 1, T, (r + 15) / 16 * 16};
+  return RqLow{u, (cols - 1) / RQ_LORA_COLS + 1, T, (r + 31) / 32 * 32};
 }
 inline int64_t rq_low_floats(const RqLow& l) { return (int64_t)l.parts * l.T * l.ranks; }
 
-// low.u[t] = A x_t (ROWS: x [T, C] with lora.a) or B^T x_t (x [T, R] with lora.b).
+// One of low = A x_t (rows: x [T, C] with lora.a) and low = B^T x_t (x [T, R] with lora.b).
 template <typename TX>
-void rq_lora_down(const TX* x, int T, int64_t ldx, int cols, bool rows, const RqLora<TX>& lora, const RqLow& low, hipStream_t s);
-// y = x W^T (+ bias) + s B u
+struct RqDown {
+  const TX* x;
+  int64_t ldx;
+  int cols, rows;
+  RqLow low;
+};
+template <typename TX>
+void rq_lora_down(const RqDown<TX>& first, const RqDown<TX>* second, const RqLora<TX>& lora, void* arranged, int nbits, hipStream_t s);
+// Beside it (arranged not NULL): the first's x as RqArranged has it, from grid.z = z on.
+struct RqArrange {
+  void* out;
+  int z;
+  bool paired;
+};
+inline bool rq_lora_arranged(int T, const RqPacked& w) { return T > 16 && rq_whole_mode_of(w) == RQ_RUNS; }
+// y = x W^T (+ bias) + s B u; arranged: x once more, where rq_lora_arranged says so.
 template <typename TX>
 void rq_lora_rows(const TX* x, int T, int64_t ldx, const RqPacked& w, int nbits, const TX* bias, const RqLora<TX>& lora,
-                  const RqLow& low, TX* y, int64_t ldy, hipStream_t s);
-// dx of tokens t0..t0+T-1 = the sum of parts [parts, T, C] + s A^T v
+                  const RqLow& low, const void* arranged, TX* y, int64_t ldy, hipStream_t s);
+// dx (NULL: none) of tokens t0..t0+T-1 = the sum of part [parts, T, C] + s A^T v, and with da (else NULL) da [n, r, C] =
+// s sum_t v_t x_t^T and db [n, R, r] = s sum_t dy_t u_t^T over each adapter's tokens of all T.
 template <typename TX>
-void rq_lora_dx(const float* part, int parts, int64_t t0, int T, int C, const RqLora<TX>& lora, const RqLow& v, TX* dx,
-                int64_t ldx, hipStream_t s);
-// da [n, r, C] = s sum_t v_t x_t^T and db [n, R, r] = s sum_t dy_t u_t^T over each adapter's tokens
+struct RqLoraDx {
+  const float* part;
+  int parts, t0, T;
+  TX* dx;                   // token t0's
+  int64_t ldx;
+};
 template <typename TX>
-void rq_lora_outer(const TX* x, int64_t ldx, int C, const TX* dy, int64_t ldy, int R, int T, const RqLora<TX>& lora,
-                   const RqLow& u, const RqLow& v, TX* da, TX* db, hipStream_t s);
+void rq_lora_grads(const RqLoraDx<TX>& g, const TX* x, int64_t ldx, int C, const TX* dy, int64_t ldy, int R, int T,
+                   const RqLora<TX>& lora, const RqLow& u, const RqLow& v, TX* da, TX* db, hipStream_t s);

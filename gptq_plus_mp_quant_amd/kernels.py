@@ -589,7 +589,7 @@ def packed_linear_lora(x, qweight, nbits, scales, T, R, C, ngroups, g_idx, group
     """y [*lead, R] = x [T, C] times the transpose of a packed weight, with low-rank adapters; see rq_packed_linear_lora."""
     lib = nat.load()
     y = x.new_empty((*lead, R))
-    nbytes = lib.rq_packed_linear_lora_workspace_bytes(T, C, r)
+    nbytes = lib.rq_packed_linear_lora_workspace_bytes(T, C, r, nat.DTYPE_CODES[x.dtype])
     ws = torch.empty(max(nbytes, 0), dtype=torch.uint8, device=x.device)
     nat.check("rq_packed_linear_lora", lib.rq_packed_linear_lora(
         x.data_ptr(), nat.DTYPE_CODES[x.dtype], T, x.stride(0), C, qweight.data_ptr(), qweight.stride(0), nbits, R,
@@ -630,7 +630,7 @@ def packed_gated(x, gate, up, T, I, C, activation, want_pre, lead):
     pre = x.new_empty((*lead, 2, I), dtype=_f32) if want_pre else None
     g, u = _weight(*gate), _weight(*up)
     g, u = ctypes.byref(g), ctypes.byref(u)
-    nbytes = 0 if want_pre else lib.rq_packed_gated_workspace_bytes(T, I, C, g, u)
+    nbytes = lib.rq_packed_gated_workspace_bytes(T, I, C, nat.DTYPE_CODES[x.dtype], g, u)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes > 0 else None
     nat.check("rq_packed_gated", lib.rq_packed_gated(
         x.data_ptr(), nat.DTYPE_CODES[x.dtype], T, x.stride(0), C, I, g, u, activation, _addr(pre), h.data_ptr(), I, _addr(ws),

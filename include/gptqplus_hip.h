@@ -403,8 +403,8 @@ int rq_packed_moe(const void* x, int dtype, int T, int64_t ldx, int D, const voi
  * lora_a [n, r, C] and lora_b [n, R, r] of type dtype, contiguous, n <= 65535, r <= 256; adapter_ids [T]: the
  * adapter a of every token, none below 0, NaN results from n on; NULL: adapter 0 for all.  s_a =
  * scaling[a] (fp32 [n]) or, with scaling NULL, scale.  The rest as rq_packed_linear, T <= 2^19; A x is
- * fp32.  workspace: rq_packed_linear_lora_workspace_bytes(T, C, r) bytes, any contents. */
-int64_t rq_packed_linear_lora_workspace_bytes(int T, int C, int r);
+ * fp32.  workspace: rq_packed_linear_lora_workspace_bytes(T, C, r, dtype) bytes, any contents. */
+int64_t rq_packed_linear_lora_workspace_bytes(int T, int C, int r, int dtype);
 int rq_packed_linear_lora(const void* x, int dtype, int T, int64_t ldx, int C, const uint32_t* qweight,
                           int64_t ldp, int nbits, int R, const float* scales, int64_t lds, int ngroups,
                           const int32_t* g_idx, int groupsize, const void* bias, const void* lora_a,
@@ -437,9 +437,8 @@ typedef struct {
 /* h [T, I] = act(x Wg^T) * (x Wu^T), the gated half of a feed-forward block: x [T, C] and h of type dtype,
  * gate and up I x C, each with bits and groups of its own; T <= 2^19.  activation: 0 SiLU, 1 GELU, 2 GELU
  * with tanh.  pre (optional, fp32 [T, 2, I]) receives both products for rq_packed_gated_grad.  workspace:
- * rq_packed_gated_workspace_bytes(...) bytes, any contents (0, NULL, where both weights have the same
- * bits and kind of groups; unused where pre is given). */
-int64_t rq_packed_gated_workspace_bytes(int T, int I, int C, const rq_packed_weight* gate,
+ * rq_packed_gated_workspace_bytes(...) bytes, any contents (NULL where that is 0). */
+int64_t rq_packed_gated_workspace_bytes(int T, int I, int C, int dtype, const rq_packed_weight* gate,
                                         const rq_packed_weight* up);
 int rq_packed_gated(const void* x, int dtype, int T, int64_t ldx, int C, int I,
                     const rq_packed_weight* gate, const rq_packed_weight* up, int activation, float* pre,

@@ -53,15 +53,16 @@ def test_lora_workspaces_and_empty_calls():
     assert _call("rq_packed_linear_lora", LORA, T=0, x=NULL, y=NULL, ws=NULL, nbytes=0) == nat.RQ_OK
     for T in (1, 16, 63, 64, 65, 100, 1000):
         for R, C, r in ((32, 64, 1), (4096, 14336, 64), (100, 28672, 256)):
-            need = lib.rq_packed_linear_lora_workspace_bytes(T, C, r)
+            need = lib.rq_packed_linear_lora_workspace_bytes(T, C, r, nat.RQ_F16)
             assert need >= 4 * T * r
             grad = lib.rq_packed_linear_lora_grad_workspace_bytes(T, R, C, r)
-            assert grad >= need + 4 * T * r + 4 * min(T, 64) * C
+            assert grad >= 8 * T * r + 4 * min(T, 64) * C
             size = dict(T=T, C=C, ldx=C, R=R, ldp=C, lds=R, groupsize=C, r=r)
             assert _call("rq_packed_linear_lora", LORA, **size, ldy=R, nbytes=need - 1) == nat.RQ_EINVAL
             assert _call("rq_packed_linear_lora_grad", LORA_GRAD, **size, ldg=R, ldgx=C, nbytes=grad - 1) == nat.RQ_EINVAL
     for bad in ((-1, 64, 4), (1, 0, 4), (1, 64, 0), (1, 64, 257), ((1 << 19) + 1, 64, 4), (1, 1 << 30, 256)):
-        assert lib.rq_packed_linear_lora_workspace_bytes(*bad) < 0
+        assert lib.rq_packed_linear_lora_workspace_bytes(*bad, nat.RQ_F16) < 0
+    assert lib.rq_packed_linear_lora_workspace_bytes(1, 64, 4, 7) < 0
     for bad in ((-1, 32, 64, 4), (1, 0, 64, 4), (1, 32, 0, 4), (1, 32, 64, 0), (1, 1 << 30, 64, 256)):
         assert lib.rq_packed_linear_lora_grad_workspace_bytes(*bad) < 0
 
@@ -103,11 +104,18 @@ def test_gated_refusals():
 def test_gated_workspaces():
     lib = _lib()
 
-    def need(T, gate, up, I=32, C=64):
-        return lib.rq_packed_gated_workspace_bytes(T, I, C, ctypes.byref(gate), ctypes.byref(up))
+    def need(T, gate, up, I=32, C=64, dtype=nat.RQ_BF16):
+        return lib.rq_packed_gated_workspace_bytes(T, I, C, dtype, ctypes.byref(gate), ctypes.byref(up))
 
     assert need(5, _weight(), _weight()) == 0
-    assert need(5, _weight(), _weight(nbits=3)) == need(5, _weight(), _weight(ngroups=1, groupsize=0)) == 5 * 2 * 32 * 4
+    assert need(5, _weight(), _weight(nbits=3)) == 5 * 2 * 32 * 4
+    assert need(5, _weight(), _weight(ngroups=1, groupsize=0)) == 5 * 2 * 32 * 4
+    # more tokens than a tile: x once more, whole tiles of 16 and chunks of 128, where a weight's groups are runs of 128
+    whole = _weight(ngroups=1, groupsize=0)              # C = 64, one chunk
+    assert need(17, whole, whole) == 32 * 128 * 2 and need(17, whole, whole, dtype=nat.RQ_F32) == 32 * 128 * 6
+    assert need(16, whole, whole) == need(17, _weight(), _weight()) == 0
+    assert _gated(whole, whole, T=17, ws=FAKE, nbytes=32 * 128 * 2 - 1) == nat.RQ_EINVAL
+    assert need(1, whole, whole, dtype=7) < 0
     assert need(-1, _weight(), _weight()) < 0 and need(1, _weight(), _weight(ldp=7)) < 0 and need(1, _weight(), _weight(), I=0) < 0
     for T in (1, 63, 64, 65, 100, 200):
         for I, C in ((32, 64), (14336, 4096), (100, 8192)):

@@ -6,8 +6,7 @@ import numpy as np
 import pytest
 import torch
 
-from gptq_plus_mp_quant_amd import (packed_linear, packed_linear_backward, packed_linear_lora,
-                                    packed_linear_lora_backward)
+from gptq_plus_mp_quant_amd import packed_linear, packed_linear_lora, packed_linear_lora_backward
 from tests._packed import ROUND, TINY, assert_within, make_entry, on, sum_eps
 from tests._util import rng
 
@@ -128,7 +127,7 @@ def test_scaling_and_a_single_adapter():
 
 @pytest.mark.parametrize("dtype", [F16, BF16, F32])
 def test_tokens_without_an_adapter(dtype):
-    """They get packed_linear's result and gradient; adapters that nobody has get zeros, whatever they hold."""
+    """They get packed_linear's result and its gradient; adapters that nobody has get zeros, whatever they hold."""
     entry, W = make_entry(4, 60, 300, 4, "128")
     e = on(entry, DEV)
     x, gy, a, b, s, _ = case(5, 20, 60, 300, 6, 4, dtype)
@@ -141,7 +140,8 @@ def test_tokens_without_an_adapter(dtype):
     none = torch.full((20,), -1, dtype=torch.int64, device=DEV)
     assert torch.equal(packed_linear_lora(dev(x), e, dev(a), dev(b), none, dev(s)), packed_linear(dev(x), e))
     g0, ga0, gb0 = packed_linear_lora_backward(dev(gy), dev(x), e, dev(a), dev(b), none, dev(s))
-    assert torch.equal(g0, packed_linear_backward(dev(gy), e)) and not bool(ga0.any()) and not bool(gb0.any())
+    within(g0, formulas(x, gy, a, b, s, none.cpu(), W)[1], dtype, "gx")
+    assert not bool(ga0.any()) and not bool(gb0.any())
 
 
 @pytest.mark.parametrize("dtype", [F16, BF16, F32])

@@ -20,29 +20,30 @@ from .packed import checked_bias, checked_entry, checked_tokens
 
 def _lora(lora_a, lora_b, ids, scaling, x, R, C, lead):
     """(lora_a, lora_b, n, r, ids or None, scaling tensor or None, scale), each tensor contiguous."""
+    dev, dt = x.get_device(), x.dtype
     for t, name in ((lora_a, "lora_a"), (lora_b, "lora_b")):
-        if not isinstance(t, torch.Tensor) or t.dtype != x.dtype or t.get_device() != x.get_device():
-            raise ValueError(f"{name} must be a {x.dtype} tensor on {x.device}")
-    sa, sb = tuple(lora_a.shape), tuple(lora_b.shape)
-    if len(sa) not in (2, 3) or len(sb) != len(sa) or sa[:-2] != sb[:-2] or sa[-1] != C or sb[-2] != R or sa[-2] != sb[-1]:
-        raise ValueError(f"lora_a and lora_b must be [n, r, {C}] and [n, {R}, r] (or [r, {C}] and [{R}, r]), got {sa} and {sb}")
+        if not isinstance(t, torch.Tensor) or t.dtype is not dt or t.get_device() != dev:
+            raise ValueError(f"{name} must be a {dt} tensor on {x.device}")
+    sa, sb = lora_a.shape, lora_b.shape
+    if len(sa) not in (2, 3) or len(sb) != len(sa) or sa[-1] != C or sb[-2] != R or sa[-2] != sb[-1] or sa[0] != (sb[0] if len(sa) == 3 else sa[0]):
+        raise ValueError(f"lora_a and lora_b must be [n, r, {C}] and [n, {R}, r] (or [r, {C}] and [{R}, r]), got {tuple(sa)} and {tuple(sb)}")
     n, r = sa[0] if len(sa) == 3 else 1, sa[-2]
     if not 1 <= n <= nat.RQ_LORA_MAX_ADAPTERS or not 1 <= r <= nat.RQ_LORA_MAX_RANK:
         raise ValueError(f"{n} adapters of rank {r}: 1 to {nat.RQ_LORA_MAX_ADAPTERS} of rank 1 to {nat.RQ_LORA_MAX_RANK} are supported")
     if ids is None:
         if n != 1:
             raise ValueError(f"adapter_ids are needed to choose between {n} adapters")
-    elif not isinstance(ids, torch.Tensor) or ids.dtype is not torch.int64 or ids.shape != lead or \
-            ids.get_device() != x.get_device():
+    elif not isinstance(ids, torch.Tensor) or ids.dtype is not torch.int64 or ids.shape != lead or ids.get_device() != dev:
         raise ValueError(f"adapter_ids must be int64 {list(lead)} on {x.device}")
-    else:
-        ids = ids.reshape(-1).contiguous()
+    elif not ids.is_contiguous():
+        ids = ids.contiguous()
+    scale = 1.0
     if isinstance(scaling, torch.Tensor):
-        if scaling.dtype is not torch.float32 or tuple(scaling.shape) != (n,) or scaling.get_device() != x.get_device():
+        if scaling.dtype is not torch.float32 or scaling.shape != (n,) or scaling.get_device() != dev:
             raise ValueError(f"scaling must be a number or float32 [{n}] on {x.device}")
         if scaling.requires_grad and torch.is_grad_enabled():
             raise ValueError("scaling is constant and would get no gradient; detach it")
-        scaling, scale = scaling.contiguous(), 1.0
+        scaling = scaling.contiguous()
     else:
         scaling, scale = None, float(scaling)
     return lora_a.contiguous(), lora_b.contiguous(), n, r, ids, scaling, scale
@@ -57,7 +58,7 @@ def _forward(x, entry, lora_a, lora_b, ids, scaling, bias):
     q, nbits, scales, R, C, ng, g_idx, groupsize = checked_entry(entry, 0)
     x2, T, lead = checked_tokens(x, C, q, "x")
     _tokens_ok(T)
-    adapters = _lora(lora_a, lora_b, ids, scaling, x, R, C, tuple(lead))
+    adapters = _lora(lora_a, lora_b, ids, scaling, x, R, C, lead)
     return K.packed_linear_lora(x2, q, nbits, scales, T, R, C, ng, g_idx, groupsize, checked_bias(bias, x, R), *adapters, lead)
 
 
@@ -65,10 +66,10 @@ def _backward(grad_y, x, entry, lora_a, lora_b, ids, scaling, want_x=True, want_
     q, nbits, scales, R, C, ng, g_idx, groupsize = checked_entry(entry, 0)
     g2, T, lead = checked_tokens(grad_y, R, q, "grad_y")
     x2, _, lead_x = checked_tokens(x, C, q, "x")
-    if tuple(lead) != tuple(lead_x) or x.dtype != grad_y.dtype:
+    if lead != lead_x or x.dtype != grad_y.dtype:
         raise ValueError(f"x must be {grad_y.dtype} {[*lead, C]}, got {x.dtype} {list(x.shape)}")
     _tokens_ok(T)
-    a, b, *rest = _lora(lora_a, lora_b, ids, scaling, x, R, C, tuple(lead))
+    a, b, *rest = _lora(lora_a, lora_b, ids, scaling, x, R, C, lead)
     return K.packed_linear_lora_grad(g2, x2, q, nbits, scales, T, R, C, ng, g_idx, groupsize, a, b, *rest, lead, want_x, want_lora)
 
 

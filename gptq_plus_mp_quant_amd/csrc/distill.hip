@@ -15,7 +15,8 @@
 
 namespace {
 
-constexpr int THREADS = 256, MAX_LIST = THREADS, MAX_V = 1 << 30;
+constexpr int MAX_LIST = 256, MAX_V = 1 << 30;
+constexpr int PER_LANE = MAX_LIST / 64;    // entries of a row's list to a lane of its first wave
 constexpr int MAX_COLS = 1 << 18;          // columns of a workgroup that keeps a bit for each (32 KB)
 constexpr int STATS = 8;
 enum { RENORMALISE = 0, BUCKET = 1 };
@@ -26,7 +27,7 @@ struct Teacher {
   const float* t;           // [N, K]
   int K;
   double c;                 // 1 / temperature
-  float k;                  // log2(e) / temperature
+  float k, k_low;           // log2(e) / temperature, and what the first rounds off
 };
 
 // Maximum and sum of exp((z - m) c); nothing: -inf, 0.
@@ -35,87 +36,116 @@ struct Sum {
   double s;
 };
 __device__ __forceinline__ float from(float m) { return m == -INFINITY ? 0.0f : m; }
-__device__ __forceinline__ Sum join(Sum x, Sum y, float k) {
+// exp(d c) for a part's sum: the exponent's rounding, which all of the part would share, is made good.
+__device__ __forceinline__ double power(float d, const Teacher& h) {
+  const float p = d * h.k, low = __builtin_fmaf(d, h.k, -p) + d * h.k_low;
+  const float e = __builtin_amdgcn_exp2f(p);
+  return e == 0.0f || p == -INFINITY ? (double)e : (double)e * (1.0 + 0.6931471805599453 * (double)low);
+}
+__device__ __forceinline__ Sum join(Sum x, Sum y, const Teacher& h) {
   const float m = fmaxf(x.m, y.m), m0 = from(m);
-  return Sum{m, x.s * (double)__builtin_amdgcn_exp2f((x.m - m0) * k) + y.s * (double)__builtin_amdgcn_exp2f((y.m - m0) * k)};
+  return Sum{m, x.s * power(x.m - m0, h) + y.s * power(y.m - m0, h)};
 }
 
-__device__ __forceinline__ double block_sum(double v, double* lds) {
+__device__ __forceinline__ double wave_sum(double v) {
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) v += __shfl_xor(v, o);
+  return v;
+}
+__device__ __forceinline__ float wave_max(float v) {
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) v = fmaxf(v, __shfl_xor(v, o));
+  return v;
+}
+__device__ __forceinline__ Sum wave_join(Sum v, const Teacher& h) {
+  const float m = wave_max(v.m);
+  // 0 times a factor that is 0: a lane without a maximum may still hold a NaN
+  return Sum{m, wave_sum(v.s * power(v.m - from(m), h))};
+}
+// The threads' sums joined in the order of lanes and waves; the first wave's to use.
+template <int THREADS>
+__device__ __forceinline__ Sum block_join(Sum v, const Teacher& h, Sum* lds) {
+  v = wave_join(v, h);
   if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
   __syncthreads();
   v = lds[0];
-  for (int w = 1; w < THREADS / 64; ++w) v += lds[w];
-  __syncthreads();
+  for (int w = 1; w < THREADS / 64; ++w) v = join(v, lds[w], h);
   return v;
-}
-__device__ __forceinline__ float block_max(float v, double* lds) {
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) v = fmaxf(v, __shfl_xor(v, o));
-  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
-  __syncthreads();
-  v = (float)lds[0];
-  for (int w = 1; w < THREADS / 64; ++w) v = fmaxf(v, (float)lds[w]);
-  __syncthreads();
-  return v;
-}
-__device__ __forceinline__ Sum block_join(Sum v, float k, double* lds) {
-  const float m = block_max(v.m, lds), f = __builtin_amdgcn_exp2f((v.m - from(m)) * k);
-  // 0 times a factor that is 0: a lane without a maximum may still hold a NaN
-  return Sum{m, block_sum(v.s * (double)f, lds)};
 }
 
-// The thread's entry of the row's list.
+// Entries of the row's list, of the first wave's lanes: lane l has entries l, l + 64, ...
 struct Entry {
   int id;                   // -1: none, V: outside the vocabulary
   float t, z;
 };
 template <typename TX>
-__device__ __forceinline__ Entry entry_of(const TX* __restrict__ row, int V, int64_t n, const Teacher& h) {
-  Entry e = {-1, 0.0f, 0.0f};
-  if ((int)threadIdx.x < h.K) {
-    const int64_t id = h.ids[n * h.K + threadIdx.x];
-    e.t = h.t[n * h.K + threadIdx.x];
-    e.id = id < 0 ? -1 : id < V ? (int)id : V;
-    if (id >= 0 && id < V) e.z = rq_load_elem(row + id);
+__device__ __forceinline__ void entries_of(const TX* __restrict__ row, int V, int64_t n, const Teacher& h, Entry (&e)[PER_LANE]) {
+#pragma unroll
+  for (int k = 0; k < PER_LANE; ++k) {
+    e[k] = Entry{-1, 0.0f, 0.0f};
+    const int at = threadIdx.x + 64 * k;
+    if (threadIdx.x < 64 && at < h.K) {
+      const int64_t id = h.ids[n * h.K + at];
+      e[k].t = h.t[n * h.K + at];
+      e[k].id = id < 0 ? -1 : id < V ? (int)id : V;
+      if (id >= 0 && id < V) e[k].z = rq_load_elem(row + id);
+    }
   }
-  return e;
 }
 
-// A row's loss and statistics from the sums over the rest (RENORMALISE: over everything) and over the list.
+// A row's loss and statistics from the sums over the rest (RENORMALISE: over everything) and over the list, by its first
+// wave.
 template <int TAIL>
-__device__ __forceinline__ void finish_row(int64_t n, int V, const Entry& e, const Teacher& h, Sum rest, Sum list, double* lds,
+__device__ __forceinline__ void finish_row(int64_t n, int V, const Entry (&e)[PER_LANE], const Teacher& h, Sum rest, Sum list,
                                            float* __restrict__ loss_out, float* __restrict__ stats) {
-  const bool used = e.id >= 0;
   float mt = 0.0f;
-  if (TAIL == RENORMALISE) mt = from(block_max(used ? e.t : -INFINITY, lds));
-  const double at = ((double)e.t - mt) * h.c, x = used ? exp(at) : 0.0;
-  const double total = block_sum(x, lds), count = block_sum(used ? 1.0 : 0.0, lds);
-  const double bad = block_sum(e.id == V ? 1.0 : 0.0, lds);
-  const double lt = TAIL == RENORMALISE && total != 0.0 ? log(total) : 0.0;
+  if (TAIL == RENORMALISE) {
+    mt = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < PER_LANE; ++k) mt = fmaxf(mt, e[k].id >= 0 ? e[k].t : -INFINITY);
+    mt = from(wave_max(mt));
+  }
+  double at[PER_LANE], x[PER_LANE], total = 0.0;
+  bool used = false, outside = false;
+#pragma unroll
+  for (int k = 0; k < PER_LANE; ++k) {
+    at[k] = ((double)e[k].t - mt) * h.c;
+    x[k] = e[k].id >= 0 ? exp(at[k]) : 0.0;
+    total += x[k];
+    used |= e[k].id >= 0;
+    outside |= e[k].id == V;
+  }
+  total = wave_sum(total);
   const double P = TAIL == RENORMALISE ? (total == 0.0 ? 0.0 : total / total) : total;
-  const double p = TAIL == RENORMALISE && total != 0.0 ? x / total : x;
-  const Sum all = TAIL == BUCKET ? join(rest, list, h.k) : rest;
-  const bool empty = all.m == -INFINITY && all.s == 0.0;
-  const double m = from(all.m), ls = empty ? 0.0 : log(all.s);
-  const double lq = empty ? -(double)INFINITY : ((double)e.z - m) * h.c - ls;
-  double loss = block_sum(p == 0.0 ? 0.0 : p * (at - lt - lq), lds);
+  const Sum all = TAIL == BUCKET ? join(rest, list, h) : rest;
+  const bool empty = all.m == -INFINITY && all.s == 0.0, none = rest.m == -INFINITY && rest.s == 0.0;
+  double r = TAIL == BUCKET && !(1.0 - P < 0.0) ? 1.0 - P : 0.0;
+  if (none && r <= NO_REST) r = 0.0;
+  // four logarithms at once, by four lanes
+  const int lane = threadIdx.x & 63;
+  const double logs = log(lane == 0 ? all.s : lane == 1 ? rest.s : lane == 2 ? total : r);
+  const double m = from(all.m), ls = empty ? 0.0 : __shfl(logs, 0);
+  const double lt = TAIL == RENORMALISE && total != 0.0 ? __shfl(logs, 2) : 0.0;
+  double loss = 0.0;
+#pragma unroll
+  for (int k = 0; k < PER_LANE; ++k) {
+    const double lq = empty ? -(double)INFINITY : ((double)e[k].z - m) * h.c - ls;
+    const double p = TAIL == RENORMALISE && total != 0.0 ? x[k] / total : x[k];
+    loss += p == 0.0 ? 0.0 : p * (at[k] - lt - lq);
+  }
+  loss = wave_sum(loss);
   double mass = P, factor = P, mr = m, lr = ls;
   if (TAIL == BUCKET) {
-    const bool none = rest.m == -INFINITY && rest.s == 0.0;
     mr = from(rest.m);
-    lr = none ? 0.0 : log(rest.s);
-    double r = 1.0 - P < 0.0 ? 0.0 : 1.0 - P;
-    if (none && r <= NO_REST) r = 0.0;
+    lr = none ? 0.0 : __shfl(logs, 1);
     const double lrest = none ? -(double)INFINITY : (mr - m) * h.c + lr - ls;
-    if (r != 0.0) loss += r * (log(r) - lrest);
+    if (r != 0.0) loss += r * (__shfl(logs, 3) - lrest);
     mass = P + r;
     factor = exp(lrest) * mass - r;
   }
   if (empty) mass = factor = 0.0;
-  if (bad != 0.0) loss = mass = factor = __builtin_nan("");
-  if (count == 0.0) loss = mass = factor = 0.0;
+  if (__any(outside)) loss = mass = factor = __builtin_nan("");
+  if (!__any(used)) loss = mass = factor = 0.0;
   if (threadIdx.x == 0) {
     loss_out[n] = (float)loss;
     float* o = stats + n * STATS;
@@ -132,26 +162,28 @@ __device__ __forceinline__ void finish_row(int64_t n, int V, const Entry& e, con
 
 // A workgroup sums columns [c0, c0 + seg_cols) of row blockIdx.x.  SPLIT: c0 = seg_cols blockIdx.y, and k_distill_join
 // finishes the row; else that is the row.
-template <typename TX, int TAIL, bool SPLIT>
+template <typename TX, int TAIL, bool SPLIT, int THREADS>
 __global__ __launch_bounds__(THREADS) void k_distill_rows(const TX* __restrict__ z, int64_t ldz, int V, int seg_cols, Teacher h,
                                                           float* __restrict__ loss, float* __restrict__ stats,
                                                           float* __restrict__ seg) {
   typedef typename RqOperand<TX>::raw Raw;
   constexpr int U = sizeof(TX) == 2 ? 8 : 4;
   extern __shared__ __attribute__((aligned(16))) uint32_t listed[];     // BUCKET: a bit for every column
-  __shared__ double lds[THREADS / 64];
+  __shared__ Sum lds[THREADS / 64];
   const int64_t n = blockIdx.x;
   const TX* row = z + n * ldz;
   const int c0 = SPLIT ? blockIdx.y * seg_cols : 0, c1 = min(V, c0 + seg_cols);
-  Entry e = {-1, 0.0f, 0.0f};
-  if (!SPLIT || TAIL == BUCKET) e = entry_of(row, V, n, h);
-  bool first = false;                      // of the entries with this id, which lies here
+  Entry e[PER_LANE];
+  if (!SPLIT || TAIL == BUCKET) entries_of(row, V, n, h, e);
+  uint32_t first = 0;                      // entries that are the first with their id, which lies here
   if (TAIL == BUCKET) {
     for (int w = threadIdx.x; w < (c1 - c0 + 31) / 32; w += THREADS) listed[w] = 0u;
     __syncthreads();
-    if (e.id >= c0 && e.id < c1) {
-      const uint32_t bit = 1u << ((e.id - c0) & 31);
-      first = !(atomicOr(&listed[(e.id - c0) >> 5], bit) & bit);
+#pragma unroll
+    for (int k = 0; k < PER_LANE; ++k) {
+      if (e[k].id < c0 || e[k].id >= c1) continue;
+      const uint32_t bit = 1u << ((e[k].id - c0) & 31);
+      if (!(atomicOr(&listed[(e[k].id - c0) >> 5], bit) & bit)) first |= 1u << k;
     }
     __syncthreads();
   }
@@ -182,12 +214,17 @@ __global__ __launch_bounds__(THREADS) void k_distill_rows(const TX* __restrict__
 #pragma unroll
       for (int k = 0; k < 8; ++k) s += __builtin_amdgcn_exp2f((f[u][k] - m0) * h.k);
   }
-  const Sum rest = block_join(Sum{m, s}, h.k, lds);
+  const Sum rest = block_join<THREADS>(Sum{m, s}, h, lds);
+  if (threadIdx.x >= 64) return;
   Sum list = {-INFINITY, 0.0};
   if (TAIL == BUCKET) {
-    // a listed NaN or inf makes the row NaN as any other does
-    const float lm = first ? fmaxf(e.z, -INFINITY) : -INFINITY;
-    list = block_join(Sum{lm, first ? (double)__builtin_amdgcn_exp2f((e.z - from(lm)) * h.k) : 0.0}, h.k, lds);
+#pragma unroll
+    for (int k = 0; k < PER_LANE; ++k)     // a listed NaN or inf makes the row NaN as any other does
+      list.m = fmaxf(list.m, first >> k & 1 ? e[k].z : -INFINITY);
+#pragma unroll
+    for (int k = 0; k < PER_LANE; ++k)
+      if (first >> k & 1) list.s += power(e[k].z - from(list.m), h);
+    list = wave_join(list, h);
   }
   if (SPLIT) {
     if (threadIdx.x == 0) {
@@ -198,31 +235,31 @@ __global__ __launch_bounds__(THREADS) void k_distill_rows(const TX* __restrict__
       o[3] = (float)list.s;
     }
   } else {
-    finish_row<TAIL>(n, V, e, h, rest, list, lds, loss, stats);
+    finish_row<TAIL>(n, V, e, h, rest, list, loss, stats);
   }
 }
 
 template <typename TX, int TAIL>
-__global__ __launch_bounds__(THREADS) void k_distill_join(const TX* __restrict__ z, int64_t ldz, int V, Teacher h,
-                                                          const float* __restrict__ seg, int segs, float* __restrict__ loss,
-                                                          float* __restrict__ stats) {
-  __shared__ double lds[THREADS / 64];
+__global__ __launch_bounds__(64) void k_distill_join(const TX* __restrict__ z, int64_t ldz, int V, Teacher h,
+                                                     const float* __restrict__ seg, int segs, float* __restrict__ loss,
+                                                     float* __restrict__ stats) {
   const int64_t n = blockIdx.x;
-  const Entry e = entry_of(z + n * ldz, V, n, h);
+  Entry e[PER_LANE];
+  entries_of(z + n * ldz, V, n, h, e);
   Sum rest = {-INFINITY, 0.0}, list = {-INFINITY, 0.0};
-  for (int p = threadIdx.x; p < segs; p += THREADS) {
-    const float* o = seg + (n * segs + p) * 4;
-    rest = join(rest, Sum{o[0], o[1]}, h.k);
-    if (TAIL == BUCKET) list = join(list, Sum{o[2], o[3]}, h.k);
+  for (int p = threadIdx.x; p < segs; p += 64) {
+    const floatx4 o = *reinterpret_cast<const floatx4*>(seg + (n * segs + p) * 4);
+    rest = join(rest, Sum{o[0], o[1]}, h);
+    if (TAIL == BUCKET) list = join(list, Sum{o[2], o[3]}, h);
   }
-  rest = block_join(rest, h.k, lds);
-  if (TAIL == BUCKET) list = block_join(list, h.k, lds);
-  finish_row<TAIL>(n, V, e, h, rest, list, lds, loss, stats);
+  rest = wave_join(rest, h);
+  if (TAIL == BUCKET) list = wave_join(list, h);
+  finish_row<TAIL>(n, V, e, h, rest, list, loss, stats);
 }
 
 // The gradient: every column as if it were outside the list, then the listed ones of the workgroup's columns over
 // them.  z and dz may be the same memory: a thread reads what it writes first, and listed logits before anything is written.
-constexpr int GRAD_COLS = 8 * THREADS * 4;
+constexpr int THREADS = MAX_LIST, GRAD_COLS = 8 * THREADS * 4;
 
 template <typename TX, int TAIL>
 __global__ __launch_bounds__(THREADS) void k_distill_grad(const TX* z, int64_t ldz, int V, Teacher h,
@@ -238,28 +275,24 @@ __global__ __launch_bounds__(THREADS) void k_distill_grad(const TX* z, int64_t l
   const float m = st[0], ls = st[1], mr = st[2], lr = st[3], mt = st[4], lt = st[5], mass = st[6], factor = st[7];
   const bool none = mass == 0.0f;                  // nothing to learn from this row
   const float g = none ? 0.0f : gl[n] * (float)h.c;
-  int id = -1;
-  float zi = 0.0f;
-  if ((int)threadIdx.x < h.K) {
-    const int64_t i = h.ids[n * h.K + threadIdx.x];
-    id = i < 0 || i >= V ? -1 : (int)i;
-    ids[threadIdx.x] = id;
-    ps[threadIdx.x] = expf((h.t[n * h.K + threadIdx.x] - mt) * (float)h.c - lt);
-  }
-  const bool mine = id >= 0 && id / GRAD_COLS % (int)gridDim.y == (int)blockIdx.y;
-  if (mine) zi = rq_load_elem(row + id);
-  __syncthreads();
-  float p = 0.0f;                                  // of all entries with this id
-  if (mine)
-    for (int j = 0; j < h.K; ++j) p += ids[j] == id ? ps[j] : 0.0f;
   const float ls2 = lr * RQ_LOG2E, scale = g * factor;
   auto gradient = [&](float v) { return none ? 0.0f : __builtin_amdgcn_exp2f((v - mr) * h.k - ls2) * scale; };
+  int id = -1;
+  float zi = 0.0f;
   for (int c0 = blockIdx.y * GRAD_COLS; c0 < V; c0 += GRAD_COLS * gridDim.y) {
     const int at0 = c0 + 8 * (int)threadIdx.x;
     Raw r[4];
 #pragma unroll
     for (int u = 0; u < 4; ++u)
       if (at0 + 8 * THREADS * u + 8 <= V) r[u] = rq_load_x<true>(row + at0 + 8 * THREADS * u, 8);
+    if (c0 == (int)blockIdx.y * GRAD_COLS && (int)threadIdx.x < h.K) {        // the list, while they are on their way
+      const int64_t i = h.ids[n * h.K + threadIdx.x];
+      id = i < 0 || i >= V ? -1 : (int)i;
+      if (id >= 0) zi = rq_load_elem(row + id);
+      ids[threadIdx.x] = id;
+      ps[threadIdx.x] = expf((h.t[n * h.K + threadIdx.x] - mt) * (float)h.c - lt);
+    }
+    if (z == dz) __syncthreads();                  // listed logits are read before they are written over
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
       const int at = at0 + 8 * THREADS * u;
@@ -274,19 +307,26 @@ __global__ __launch_bounds__(THREADS) void k_distill_grad(const TX* z, int64_t l
     }
   }
   __syncthreads();
-  if (mine) out[id] = rq_cast<TX>(none ? 0.0f : g * (__builtin_amdgcn_exp2f((zi - m) * h.k - ls * RQ_LOG2E) * mass - p));
+  if (id < 0 || id / GRAD_COLS % (int)gridDim.y != (int)blockIdx.y) return;
+  float p = 0.0f;                                  // of all entries with this id
+  for (int j = 0; j < h.K; ++j) p += ids[j] == id ? ps[j] : 0.0f;
+  out[id] = rq_cast<TX>(none ? 0.0f : g * (__builtin_amdgcn_exp2f((zi - m) * h.k - ls * RQ_LOG2E) * mass - p));
 }
 
-// How a row is cut: into one workgroup where the rows alone fill the GPU, fewer rows over more.
+// How a row is cut: into one workgroup where the rows alone fill the GPU, and where a large one reads it in the
+// time that a second launch takes; fewer and longer rows over more.
+constexpr int LARGE = 1024, ALONE = 1 << 16;
 struct Cut {
   int segs, cols;
+  bool large;
 };
 inline Cut cut_of(int64_t N, int V) {
+  if (N < 512 && V <= ALONE) return Cut{1, (V + 31) / 32 * 32, V > 8 * THREADS};
   const int64_t fill = N >= 512 ? 1 : (1024 + N - 1) / N, most = ((int64_t)V + 4095) / 4096, least = ((int64_t)V + MAX_COLS - 1) / MAX_COLS;
   int64_t segs = fill < most ? fill : most;
   segs = segs > least ? segs : least;
   const int cols = (int)(((V + segs - 1) / segs + 31) / 32 * 32);
-  return Cut{(V + cols - 1) / cols, cols};
+  return Cut{(V + cols - 1) / cols, cols, false};
 }
 
 inline bool bad_sizes(int64_t N, int V, int K, double temperature, int tail) {
@@ -294,7 +334,8 @@ inline bool bad_sizes(int64_t N, int V, int K, double temperature, int tail) {
          (tail != RENORMALISE && (tail != BUCKET || temperature != 1.0));
 }
 inline Teacher teacher(const int64_t* ids, const float* t, int K, double temperature) {
-  return Teacher{ids, t, K, 1.0 / temperature, (float)(1.4426950408889634 / temperature)};
+  const double k = 1.4426950408889634 / temperature;
+  return Teacher{ids, t, K, 1.0 / temperature, (float)k, (float)(k - (float)k)};
 }
 template <typename F>
 inline bool with_tail(int dtype, int tail, F&& f) {
@@ -332,14 +373,18 @@ extern "C" int rq_distill_loss(const void* logits, int dtype, int64_t N, int64_t
       const Teacher h = teacher(teacher_ids + n * K, teacher_logprobs + n * K, K, temperature);
       const TX* z = (const TX*)logits + n * ldz;
       float* seg = (float*)workspace + n * cut.segs * 4;
+      auto rows_of = [&](auto split, auto threads) {
+        hipLaunchKernelGGL((k_distill_rows<TX, TAIL, decltype(split)::value, decltype(threads)::value>), dim3(rows, cut.segs),
+                           dim3(decltype(threads)::value), lds, s, z, ldz, V, cut.cols, h, loss + n, stats + n * STATS, seg);
+      };
       if (cut.segs > 1) {
-        hipLaunchKernelGGL((k_distill_rows<TX, TAIL, true>), dim3(rows, cut.segs), dim3(THREADS), lds, s, z, ldz, V, cut.cols, h,
-                           nullptr, nullptr, seg);
-        hipLaunchKernelGGL((k_distill_join<TX, TAIL>), dim3(rows), dim3(THREADS), 0, s, z, ldz, V, h, seg, cut.segs, loss + n,
+        rows_of(std::true_type{}, std::integral_constant<int, 256>{});
+        hipLaunchKernelGGL((k_distill_join<TX, TAIL>), dim3(rows), dim3(64), 0, s, z, ldz, V, h, seg, cut.segs, loss + n,
                            stats + n * STATS);
+      } else if (cut.large) {
+        rows_of(std::false_type{}, std::integral_constant<int, LARGE>{});
       } else {
-        hipLaunchKernelGGL((k_distill_rows<TX, TAIL, false>), dim3(rows), dim3(THREADS), lds, s, z, ldz, V, cut.cols, h, loss + n,
-                           stats + n * STATS, nullptr);
+        rows_of(std::false_type{}, std::integral_constant<int, 256>{});
       }
     }
   });

@@ -194,6 +194,25 @@ __device__ __forceinline__ void rq_operand(floatx8 x, bf16x8 (&v)[P]) {
   }
 }
 
+// Four elements, of which n exist (which may be none): loads past them are moved back to the last, and their values dropped.
+template <typename TX>
+__device__ __forceinline__ floatx4 rq_load4(const TX* p, int n) {
+  floatx4 v;
+  if (n >= 4) {
+    TX e[4];
+    __builtin_memcpy(e, p, sizeof(e));
+#pragma unroll
+    for (int k = 0; k < 4; ++k) v[k] = rq_load_elem(e + k);
+  } else {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float e = rq_load_elem(p + min(k, n - 1));
+      v[k] = k < n ? e : 0.0f;
+    }
+  }
+  return v;
+}
+
 // A lane's tokens, one for each of NT tiles: rows of x.
 template <typename TX, int NT>
 struct RqTokens {

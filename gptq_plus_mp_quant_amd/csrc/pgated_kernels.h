@@ -8,16 +8,17 @@ namespace {
 
 enum { GATED_BOTH = 0, GATED_GATE = 1, GATED_UP = 2 };
 
-// 16 rows of both weights and 16 NT tokens to a workgroup; the waves take the chunks of 128 columns in turn, multiply a
-// row tile of gate and one of up by the tokens they have loaded once, and are joined through LDS in their order.  GATE
+// 16 RP rows of both weights and 16 NT tokens to a workgroup; the waves take the chunks of 128 columns in turn, multiply RP
+// row tiles of gate and of up by the tokens they have loaded once, and are joined through LDS in their order.  GATE
 // and UP (weights of different bits or groups): one of the two, the gate's product goes by way of pre.
-template <typename TX, int NB, int MODE, int NM, int NT>
+template <typename TX, int NB, int MODE, int NM, int NT, int RP>
 __global__ __launch_bounds__(rows_threads(2, NT)) void k_packed_gated(const TX* __restrict__ x, const void* __restrict__ xa, int T, int64_t ldx, RqPacked first,
                                                                       RqPacked second, int what, int act, bool staged,
                                                                       float* pre, TX* __restrict__ h, int64_t ldh) {
   extern __shared__ __attribute__((aligned(16))) float lds[];
   const int lane = threadIdx.x & 63, wave = rq_wave(), waves = blockDim.x >> 6;
-  const int I = first.R, r0 = rq_tile_row<true>(blockIdx.x * 16, I), t0 = blockIdx.y * 16 * NT;
+  const int I = first.R, r0 = blockIdx.x * 16 * RP, t0 = blockIdx.y * 16 * NT;
+  constexpr int RT = NM * RP;
   constexpr bool ARRANGED = MODE == RQ_RUNS && NT > 1;
   typename std::conditional<ARRANGED, RqArranged<TX, NT, rq_pairs<TX>(NB)>, RqWholeTokens<TX, NT>>::type xs;
   if constexpr (ARRANGED) rq_arranged_tokens<TX>(xa, T, first.C, t0, xs.p);
@@ -30,30 +31,31 @@ __global__ __launch_bounds__(rows_threads(2, NT)) void k_packed_gated(const TX* 
   if constexpr (NM == 2) w[1] = second;
   if (MODE == RQ_ANY && staged) {
 #pragma unroll
-    for (int a = 0; a < NM; ++a) rq_stage_scales(w[a], r0, a, NM, threadIdx.x, blockDim.x, lds);
+    for (int a = 0; a < RT; ++a) rq_stage_scales(w[a % NM], rq_tile_row<true>(r0 + 16 * (a / NM), I), a, RT, threadIdx.x, blockDim.x, lds);
     __syncthreads();
   }
-  floatx4 acc[NM][NT];
+  floatx4 acc[RT][NT];
 #pragma unroll
-  for (int a = 0; a < NM; ++a)
+  for (int a = 0; a < RT; ++a)
 #pragma unroll
     for (int b = 0; b < NT; ++b) acc[a][b] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
-  rq_rows_tokens<NB, MODE, NM, NM>(w, r0, xs, wave, waves, MODE == RQ_ANY && staged ? lds : nullptr, acc);
+  rq_rows_tokens<NB, MODE, RT, NM>(w, r0, xs, wave, waves, MODE == RQ_ANY && staged ? lds : nullptr, acc);
   if (MODE == RQ_ANY && staged) __syncthreads();
   floatx4* out = reinterpret_cast<floatx4*>(lds);
 #pragma unroll
-  for (int a = 0; a < NM; ++a)
+  for (int a = 0; a < RT; ++a)
 #pragma unroll
-    for (int b = 0; b < NT; ++b) out[((wave * NM + a) * NT + b) * 64 + lane] = acc[a][b];
+    for (int b = 0; b < NT; ++b) out[((wave * RT + a) * NT + b) * 64 + lane] = acc[a][b];
   __syncthreads();
-  for (int e = threadIdx.x; e < NT * 64; e += blockDim.x) {
-    const int l = e & 63, b = e >> 6;
-    const int t = t0 + 16 * b + (l & 15), r = r0 + 4 * (l >> 4);
+  for (int e = threadIdx.x; e < RP * NT * 64; e += blockDim.x) {
+    const int l = e & 63, b = (e >> 6) % NT, m = (e >> 6) / NT;      // row tiles m NM and m NM + NM - 1
+    const int t = t0 + 16 * b + (l & 15), r = rq_tile_row<true>(r0 + 16 * m, I) + 4 * (l >> 4);
     if (t >= T) continue;
-    floatx4 g = out[e], u = out[(NM - 1) * NT * 64 + e];
+    const floatx4 *at = out + (m * NM * NT + b) * 64 + l, *up = at + (NM - 1) * NT * 64;
+    floatx4 g = *at, u = *up;
     for (int k = 1; k < waves; ++k) {
-      g += out[k * NM * NT * 64 + e];
-      u += out[(k * NM + NM - 1) * NT * 64 + e];
+      g += at[k * RT * NT * 64];
+      u += up[k * RT * NT * 64];
     }
     float* p = pre ? pre + (int64_t)t * 2 * I + r : nullptr;
     TX* dst = h + (int64_t)t * ldh + r;
@@ -75,27 +77,37 @@ __global__ __launch_bounds__(256) void k_arrange(const TX* __restrict__ x, int T
   rq_arrange<TX>(x, T, ldx, C, blockIdx.x, ch, min(ch + 4, (C + RQ_CHUNK - 1) / RQ_CHUNK), paired, threadIdx.x, 256, xa);
 }
 
-template <typename TX, int NB, int MODE, int NM, int NT>
+template <typename TX, int NB, int MODE, int NM, int NT, int RP>
 void launch_gated(const TX* x, void* xa, int T, int64_t ldx, const RqPacked& first, const RqPacked& second, int what, int act, float* pre,
                   TX* h, int64_t ldh, hipStream_t s) {
-  const int bx = (first.R + 15) / 16, by = (T + 16 * NT - 1) / (16 * NT);
-  const int waves = waves_for(bx * by, (first.C + RQ_CHUNK - 1) / RQ_CHUNK, NM * NT, rows_threads(2, NT) / 64);
-  size_t lds = (size_t)waves * NM * NT * 1024;
-  const size_t scales = (size_t)((first.ngroups > second.ngroups ? first.ngroups : second.ngroups) + 1) * 16 * NM * 4;
+  constexpr int RT = NM * RP;
+  const int bx = (first.R + 16 * RP - 1) / (16 * RP), by = (T + 16 * NT - 1) / (16 * NT);
+  const int waves = waves_for(bx * by, (first.C + RQ_CHUNK - 1) / RQ_CHUNK, RT * NT, rows_threads(2, NT) / 64);
+  size_t lds = (size_t)waves * RT * NT * 1024;
+  const size_t scales = (size_t)((first.ngroups > second.ngroups ? first.ngroups : second.ngroups) + 1) * 16 * RT * 4;
   const bool staged = MODE == RQ_ANY && scales <= 65536;
   if (staged && lds < scales) lds = scales;
-  hipLaunchKernelGGL((k_packed_gated<TX, NB, MODE, NM, NT>), dim3(bx, by), dim3(64 * waves), lds, s, x, xa, T, ldx, first, second, what,
-                     act, staged, pre, h, ldh);
+  hipLaunchKernelGGL((k_packed_gated<TX, NB, MODE, NM, NT, RP>), dim3(bx, by), dim3(64 * waves), lds, s, x, xa, T, ldx, first, second,
+                     what, act, staged, pre, h, ldh);
 }
 
 template <typename TX, int NB, int MODE, int NM>
-void gated_of(const TX* x, void* xa, int T, int64_t ldx, const RqPacked& first, const RqPacked& second, int what, int act, float* pre, TX* h,
-              int64_t ldh, hipStream_t s) {
+void gated_of(const TX* x, void* xa, int T, int64_t ldx, const RqPacked& first, const RqPacked& second, int what, int act, float* pre,
+              TX* h, int64_t ldh, hipStream_t s) {
   constexpr int NT = RqOperand<TX>::pieces == 1 ? 4 : 2;
-  if (T <= 16) launch_gated<TX, NB, MODE, NM, 1>(x, xa, T, ldx, first, second, what, act, pre, h, ldh, s);
-  else if (T <= 32) launch_gated<TX, NB, MODE, NM, 2>(x, xa, T, ldx, first, second, what, act, pre, h, ldh, s);
-  else if (MODE == RQ_RUNS && T <= 48 && NT > 3) launch_gated<TX, NB, MODE, NM, NT < 3 ? NT : 3>(x, xa, T, ldx, first, second, what, act, pre, h, ldh, s);
-  else launch_gated<TX, NB, MODE, NM, NT>(x, xa, T, ldx, first, second, what, act, pre, h, ldh, s);
+  auto run = [&](auto nt, auto rp) {
+    launch_gated<TX, NB, MODE, NM, decltype(nt)::value, decltype(rp)::value>(x, xa, T, ldx, first, second, what, act, pre, h, ldh, s);
+  };
+  typedef std::integral_constant<int, 1> One;
+  if (T <= 16) return run(One{}, One{});
+  if constexpr (MODE == RQ_RUNS) {
+    // 28672 x 8192 4-bit fp16, 24 tokens: 97 us with one row tile of each weight a wave, 81 with two
+    if constexpr (NM == 2 && NT == 4)
+      if (T <= 32 && first.R >= 16384) return run(std::integral_constant<int, 2>{}, std::integral_constant<int, 2>{});
+    if (T <= 32) return run(std::integral_constant<int, 2>{}, One{});
+    if (NT == 4 && T <= 48) return run(std::integral_constant<int, NT == 4 ? 3 : NT>{}, One{});
+  }
+  run(std::integral_constant<int, NT>{}, One{});
 }
 template <typename TX, int NM>
 void gated_one(const TX* x, void* xa, int T, int64_t ldx, const RqPacked& first, const RqPacked& second, int bits, int what, int act, float* pre,
@@ -122,13 +134,23 @@ __global__ __launch_bounds__(256) void k_gated_pre_grad(const TX* __restrict__ g
   d[((int64_t)T + t) * I + i] = g * v.f;
 }
 
+// Sixteen parts' loads in flight (they lie in other XCDs' caches or beyond); summed in their order.
 template <typename TX>
 __global__ __launch_bounds__(256) void k_gated_join(const float* __restrict__ part, int parts, int T, int C, TX* __restrict__ dx,
                                                     int64_t ldx) {
   const int c = blockIdx.x * 256 + threadIdx.x, t = blockIdx.y;
   if (c >= C) return;
+  const float* p = part + (int64_t)t * C + c;
+  const int64_t plane = (int64_t)T * C;
   float s = 0.0f;
-  for (int p = 0; p < parts; ++p) s += part[((int64_t)p * T + t) * C + c];
+  for (int m = 0; m < parts; m += 16) {
+    float e[16];
+#pragma unroll
+    for (int k = 0; k < 16; ++k) e[k] = p[min(m + k, parts - 1) * plane];
+#pragma unroll
+    for (int k = 0; k < 16; ++k)
+      if (m + k < parts) s += e[k];
+  }
   dx[(int64_t)t * ldx + c] = rq_cast<TX>(s);
 }
 

@@ -294,11 +294,10 @@ __device__ __forceinline__ void cols_scaled(const TX* __restrict__ dy, int T, in
       bf16x8 v[P::w];
       floatx8 sc = f.sc;
       if (MODE == RQ_ANY) {
+        sc = col_scales<FULL>(w, g[n] < (uint32_t)w.ngroups ? g[n] : 0, r);
+        if (g[n] >= (uint32_t)w.ngroups) {
 #pragma unroll
-        for (int k = 0; k < 8; ++k) sc[k] = rq_scale_of(w, g[n], FULL ? r + k : min(r + k, w.R - 1));
-        if (!FULL) {
-#pragma unroll
-          for (int k = 0; k < 8; ++k) sc[k] = r + k < w.R ? sc[k] : 0.0f;
+          for (int k = 0; k < 8; ++k) sc[k] = FULL || r + k < w.R ? __builtin_nanf("") : 0.0f;
         }
       }
       rq_operand<P::w>(sc * rq_unit<NB>() * codes, v);
@@ -450,22 +449,24 @@ void launch_cols(const Cols<TX>& a, const RqPacked& w, hipStream_t s) {
                      dim3(64 * cols_waves(NT)), 0, s, a.dy, a.T, a.ldy, a.plane, w, NM == 2 ? *a.w1 : w, a.sp.steps_per, a.part, a.dx,
                      a.ldx);
 }
-template <typename TX, int NB, int MODE, int NM>
+// WIDE: the caller joins the parts.
+template <typename TX, int NB, int MODE, int NM, bool WIDE>
 void linear_cols(const Cols<TX>& a, const RqPacked& w, hipStream_t s) {
-  // where codes and fp32 tokens are both cut, registers are left for two token tiles
-  constexpr int NT = RqOperand<TX>::pieces == 1 || MODE == RQ_RUNS ? 4 : 2;
+  // Where codes and fp32 tokens are both cut, registers are left for two token tiles; with RUNS four fit, which
+  // packed_linear_backward does not use: other waves would make other sums of what it has always returned.
+  constexpr int NT = RqOperand<TX>::pieces == 1 || (MODE == RQ_RUNS && WIDE) ? 4 : 2;
   if (a.T <= 16) launch_cols<TX, NB, MODE, 1, NM>(a, w, s);
   else if (a.T <= 32) launch_cols<TX, NB, MODE, 2, NM>(a, w, s);
   else launch_cols<TX, NB, MODE, NT, NM>(a, w, s);
 }
-template <typename TX, int NM>
+template <typename TX, int NM, bool WIDE>
 void cols_of(const Cols<TX>& a, const RqPacked& w, int nbits, hipStream_t s) {
   rq_with_nbits(nbits, [&](auto nb) {
     constexpr int NB = decltype(nb)::value;
     switch (rq_cols_mode_of(w)) {
-      case RQ_RUNS: linear_cols<TX, NB, RQ_RUNS, NM>(a, w, s); break;
-      case RQ_SMALL: linear_cols<TX, NB, RQ_SMALL, NM>(a, w, s); break;
-      default: linear_cols<TX, NB, RQ_ANY, NM>(a, w, s);
+      case RQ_RUNS: linear_cols<TX, NB, RQ_RUNS, NM, WIDE>(a, w, s); break;
+      case RQ_SMALL: linear_cols<TX, NB, RQ_SMALL, NM, WIDE>(a, w, s); break;
+      default: linear_cols<TX, NB, RQ_ANY, NM, WIDE>(a, w, s);
     }
   });
 }
@@ -475,7 +476,7 @@ void cols_of(const Cols<TX>& a, const RqPacked& w, int nbits, hipStream_t s) {
 template <typename TX>
 void rq_cols_parts(const TX* dy, int T, int64_t ldy, const RqPacked& w, int nbits, const RqColSplit& sp, float* part,
                    hipStream_t s) {
-  cols_of<TX, 1>(Cols<TX>{dy, T, ldy, 0, nullptr, sp, part, nullptr, 0}, w, nbits, s);
+  cols_of<TX, 1, true>(Cols<TX>{dy, T, ldy, 0, nullptr, sp, part, nullptr, 0}, w, nbits, s);
 }
 
 template <typename TX>
@@ -485,7 +486,7 @@ void rq_linear_cols(const TX* dy, int T, int64_t ldy, const RqPacked& w, int nbi
     const int n = (int)(T - t0 < RQ_COL_TOKENS ? T - t0 : RQ_COL_TOKENS);
     const RqColSplit sp = rq_col_split(n, w.R, w.C);
     TX* out = dx + t0 * ldx;
-    cols_of<TX, 1>(Cols<TX>{dy + t0 * ldy, n, ldy, 0, nullptr, sp, sp.parts > 1 ? part : nullptr, out, ldx}, w, nbits, s);
+    cols_of<TX, 1, false>(Cols<TX>{dy + t0 * ldy, n, ldy, 0, nullptr, sp, sp.parts > 1 ? part : nullptr, out, ldx}, w, nbits, s);
     if (sp.parts > 1)
       hipLaunchKernelGGL(k_packed_join<TX>, dim3((w.C + 255) / 256, n), dim3(256), 0, s, part, sp.parts, n, w.C, out, ldx);
   }

@@ -201,25 +201,6 @@ struct RqLowRank {
 // One launch: workgroups for da and db and, behind them, for dx.
 constexpr int WINDOW = 512;
 
-// Four elements, of which n exist (which may be none): loads past them are moved back to the last, and their values dropped.
-template <typename TX>
-__device__ __forceinline__ floatx4 load4(const TX* p, int n) {
-  floatx4 v;
-  if (n >= 4) {
-    TX e[4];
-    __builtin_memcpy(e, p, sizeof(e));
-#pragma unroll
-    for (int k = 0; k < 4; ++k) v[k] = rq_load_elem(e + k);
-  } else {
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const float e = rq_load_elem(p + min(k, n - 1));
-      v[k] = k < n ? e : 0.0f;
-    }
-  }
-  return v;
-}
-
 // dx of 16 tokens and 64 columns a workgroup: its waves deal the parts among them, and the adapters' ranks, 32 at a time, by
 // adapter and rank alone; joined through LDS in their order.  Lane 16 q + j has columns 4j..4j+3 of ranks 8q..8q+7,
 // product n takes the n-th of each, so that D's column j is column 4j + n.
@@ -240,7 +221,7 @@ __device__ __forceinline__ void lora_dx(int block, const float* __restrict__ par
 #pragma unroll 2
   for (int m = wave; m < parts; m += GRAD_WAVES)
 #pragma unroll
-    for (int k = 0; k < 4; ++k) o[k] += load4(part + ((int64_t)m * T + min(tw + 4 * q + k, T - 1)) * C + c, nc);
+    for (int k = 0; k < 4; ++k) o[k] += rq_load4(part + ((int64_t)m * T + min(tw + 4 * q + k, T - 1)) * C + c, nc);
   for (uint64_t pending = __ballot(lane < 16 && mine >= 0 && mine < lora.n); pending;) {
     const int a = __builtin_amdgcn_readlane(mine, __ffsll((unsigned long long)pending) - 1);
     pending &= ~__ballot(mine == a);
@@ -254,7 +235,7 @@ __device__ __forceinline__ void lora_dx(int block, const float* __restrict__ par
       const floatx8 vt = low8(v, t0 + min(tw + j, T - 1), k0 + 8 * q);
       floatx4 row[8];
 #pragma unroll
-      for (int k = 0; k < 8; ++k) row[k] = load4(lora.a + ((int64_t)a * lora.r + min(k0 + 8 * q + k, lora.r - 1)) * C + c, nc);
+      for (int k = 0; k < 8; ++k) row[k] = rq_load4(lora.a + ((int64_t)a * lora.r + min(k0 + 8 * q + k, lora.r - 1)) * C + c, nc);
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
         const bool is = k0 + 8 * q + k < lora.r;

@@ -395,3 +395,28 @@ def test_results_can_be_edited_in_place(lead):
     r2.stats.zero_()
     with pytest.raises(RuntimeError):
         r2.loss.sum().backward()
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16, F32])
+@pytest.mark.parametrize("N,V", [(3, 40), (5, 8199), (2, 600001)])
+def test_the_gradient_may_take_the_logits_place(N, V, dtype):
+    """The C entry's grad_logits may be the logits: listed ones are read before they are written over, also where a
+    workgroup goes over several rounds of columns."""
+    from gptq_plus_mp_quant_amd import _native as nat
+    z = randn(1, N, V, dtype=dtype)
+    ids, t = (v.to(DEV) for v in teacher(2, z, 30))
+    z, gl = z.to(DEV), randn(3, N).to(DEV)
+    r = distillation_loss(z, ids, t, tail="bucket")
+    want = distillation_loss_backward(z, ids, t, r.stats, gl, tail="bucket")
+    nat.check("rq_distill_loss_grad", nat.load().rq_distill_loss_grad(
+        z.data_ptr(), nat.DTYPE_CODES[dtype], N, V, V, ids.data_ptr(), t.data_ptr(), 30, 1.0, nat.TAILS["bucket"], r.stats.data_ptr(),
+        gl.data_ptr(), z.data_ptr(), V, nat.raw_stream(z)))
+    assert torch.equal(z, want)
+
+
+@pytest.mark.parametrize("tail,temperature", TAILS)
+@pytest.mark.parametrize("N,V", [(1, 2048), (1, 2049), (2, 8192), (511, 600), (3, 65536), (3, 65537), (2, 262145), (512, 70001)])
+def test_every_way_a_row_is_cut(N, V, tail, temperature):
+    """One small workgroup, one large one, several and a join; rows that end on the borders between them."""
+    z = randn(N + V, N, V, dtype=BF16, scale=2.0)
+    check(z, *teacher(V, z, 70), temperature, tail, grad=N * V < 1 << 20)

@@ -10,6 +10,7 @@ import ctypes
 import functools
 import os
 import re
+import struct
 from pathlib import Path
 
 import torch
@@ -53,10 +54,9 @@ class PackedExperts(ctypes.Structure):
                 ("stride_scales", _L), ("nbits", _I), ("ngroups", _I), ("groupsize", _I)]
 
 
-class PackedWeight(ctypes.Structure):
-    """``rq_packed_weight``: one packed weight."""
-    _fields_ = [("qweight", _P), ("scales", _P), ("g_idx", _P), ("ldp", _L), ("lds", _L), ("nbits", _I), ("ngroups", _I),
-                ("groupsize", _I)]
+# rq_packed_weight, one packed weight, as bytes (made faster than a Structure): qweight, scales, g_idx, ldp, lds, nbits,
+# ngroups, groupsize
+PACKED_WEIGHT = struct.Struct("PPPqqiii4x")
 
 
 # name -> (restype, argtypes); mirrors include/gptqplus_hip.h

@@ -308,9 +308,9 @@ __device__ __forceinline__ void rq_arrange(const TX* __restrict__ x, int T, int6
   typedef typename RqOperand<TX>::raw Raw;
   constexpr int P = RqOperand<TX>::pieces;
   const int chunks = (C + RQ_CHUNK - 1) / RQ_CHUNK;
-  for (int e = ch0 * 256 + first; e < ch1 * 256; e += step) {
+  for (int64_t e = (int64_t)ch0 * 256 + first; e < (int64_t)ch1 * 256; e += step) {
     // neighbouring threads read neighbouring columns of a token: within a chunk, (token, q, s) from the thread
-    const int ch = e >> 8, s = e & 3, q = e >> 2 & 3, i = e >> 4 & 15;
+    const int ch = (int)(e >> 8), s = (int)(e & 3), q = (int)(e >> 2 & 3), i = (int)(e >> 4 & 15);
     const int t = tile * 16 + i, c = ch * RQ_CHUNK + 32 * q + 8 * s, n = C - c;
     Raw r = {};
     if (t < T && n > 0) r = n >= 8 ? rq_load_x<true>(x + (int64_t)t * ldx + c, 8) : rq_load_x<false>(x + (int64_t)t * ldx + c, n);
@@ -393,8 +393,8 @@ template <typename X, typename = void>
 struct rq_paired : std::false_type {};
 template <typename X>
 struct rq_paired<X, typename std::enable_if<X::paired>::type> : std::true_type {};
-// WHOLE (X::whole): a row tile that would pass the weight's last row is moved back to end with it, and does the rows
-// before once more; R is 16 at least with RUNS and SMALL.  No lane then has a row or scale to guard.
+// WHOLE (X::whole): a row tile that would pass the weight's last row is moved back to end with it, and does rows of the
+// tile before once more, which it does not store; R is 16 at least with RUNS and SMALL.  No lane then has a row or scale to guard.
 template <typename X, typename = void>
 struct rq_whole : std::false_type {};
 template <typename X>
@@ -406,6 +406,21 @@ __device__ __forceinline__ int rq_tile_row(int r, int R) {
 template <typename TX, int NT>
 struct RqWholeTokens : RqTokens<TX, NT> {
   static constexpr bool whole = true;
+};
+
+// A few tokens with RUNS: each lane loads what goes with its codes, four times as many lines of the cache, which few tokens
+// do not feel, and spares the 16 swaps of rq_to_runs.  PAIRED as RqArranged has it.
+template <typename TX, bool PAIRED>
+struct RqDirect : RqTokens<TX, 1> {
+  typedef typename RqTokens<TX, 1>::raw raw;
+  static constexpr bool arranged = true, whole = true, paired = PAIRED;
+  template <bool FULL>
+  __device__ __forceinline__ raw load(int b, int c, int n) const {
+    const int q = (threadIdx.x & 63) >> 4, d = (c & ~(RQ_CHUNK - 1)) + 32 * q + (c >> 5 & 3) * 8;
+    raw r = RqTokens<TX, 1>::template load<FULL>(b, d, n + c - d);
+    if constexpr (PAIRED) r = __builtin_shufflevector(r, r, 0, 4, 1, 5, 2, 6, 3, 7);
+    return r;
+  }
 };
 
 // What a lane needs of a chunk of 128 columns with RUNS: its words and scales, and its tokens' x.  Row tiles

@@ -17,6 +17,7 @@
 // (7.5 GFLOP for each piece), overlapped in part by two waves a SIMD, and waits for the one step that is ahead.
 #pragma once
 #include "packed_dot.h"
+#include "plora_down.h"
 
 namespace {
 
@@ -333,10 +334,9 @@ __device__ __forceinline__ void cols_scaled(const TX* __restrict__ dy, int T, in
 
 // The waves' sums, halved together, always in the same order, and stored: to part [parts, T, C] or, without parts, to dx.
 template <typename TX, int NT>
-__device__ __forceinline__ void cols_store(floatx4 (&acc)[8][NT], int t0, int T, int C, float* __restrict__ part,
-                                           TX* __restrict__ dx, int64_t ldx) {
+__device__ __forceinline__ void cols_store(floatx4 (&acc)[8][NT], int y, int t0, int T, int C, float* __restrict__ part,
+                                           TX* __restrict__ dx, int64_t ldx, floatx4 (*join)[8 * NT][64]) {
   constexpr int W = cols_waves(NT);
-  __shared__ floatx4 join[W / 2][8 * NT][64];
   const int lane = threadIdx.x & 63, wave = rq_wave(), q = lane >> 4;
   const int c = blockIdx.x * COLS + 8 * (lane & 15), nc = min(8, C - c);
 #pragma unroll
@@ -367,7 +367,7 @@ __device__ __forceinline__ void cols_store(floatx4 (&acc)[8][NT], int t0, int T,
 #pragma unroll
       for (int n = 0; n < 8; ++n) v[n] = acc[n][b][k];
       if (part) {
-        float* to = part + ((int64_t)blockIdx.y * T + t) * C + c;
+        float* to = part + ((int64_t)y * T + t) * C + c;
         if (nc >= 8) {
           __builtin_memcpy(to, &v, 32);
         } else {
@@ -383,16 +383,26 @@ __device__ __forceinline__ void cols_store(floatx4 (&acc)[8][NT], int t0, int T,
     }
 }
 
-// Grid (tiles of 128 columns, parts, tiles of 16 NT tokens).  NM weights one after the other: dx = dy_0 W_0 + dy_1 W_1,
+// Grid (tiles of 128 columns, rows of jobs and then parts, tiles of 16 NT tokens).  The jobs (of packed linears with
+// adapters: what does not wait for this product) come first and spare a launch.  NM weights one after the other: dx = dy_0 W_0 + dy_1 W_1,
 // dy_1 lying `plane` elements behind dy_0, and a part is a range of the steps of all.
 template <typename TX, int NB, int MODE, int NT, int NM>
 __global__ __launch_bounds__(64 * cols_waves(NT), cols_occupancy(MODE, NT)) void k_packed_cols(
     const TX* __restrict__ dy, int T, int64_t ldy, int64_t plane, RqPacked w0, RqPacked w1, int steps_per, float* __restrict__ part,
-    TX* __restrict__ dx, int64_t ldx) {
+    TX* __restrict__ dx, int64_t ldx, RqDownJobs<TX> jobs, int job_rows) {
   constexpr int W = cols_waves(NT);
+  __shared__ floatx4 join[W / 2][8 * NT][64];
+  const int y = (int)blockIdx.y - job_rows;
+  if (y < 0) {
+    const int64_t id = ((int64_t)blockIdx.z * job_rows + blockIdx.y) * gridDim.x + blockIdx.x;
+    const int z = (int)(id % jobs.z), nth = (int)(id / jobs.z % jobs.adapters);
+    const int64_t tile = id / jobs.z / jobs.adapters;
+    if (tile < jobs.tiles) rq_lora_down_job<TX, W>(jobs, (int)tile, nth, z, &join[0][0][0]);
+    return;
+  }
   const int wave = rq_wave(), t0 = blockIdx.z * 16 * NT;
   const int nsteps = (w0.R + STEP - 1) / STEP;
-  const int sa = blockIdx.y * steps_per, sb = min(NM * nsteps, sa + steps_per);
+  const int sa = y * steps_per, sb = min(NM * nsteps, sa + steps_per);
   floatx4 acc[8][NT];
   auto run = [&](auto careful) {
 #pragma unroll
@@ -418,7 +428,7 @@ __global__ __launch_bounds__(64 * cols_waves(NT), cols_occupancy(MODE, NT)) void
         for (int k = 0; k < 4; k += 2) nan |= __builtin_isunordered(acc[n][b][k], acc[n][b][k + 1]);
     if (__any(nan)) run(std::true_type{});
   }
-  cols_store<TX, NT>(acc, t0, T, w0.C, part, dx, ldx);
+  cols_store<TX, NT>(acc, y, t0, T, w0.C, part, dx, ldx, join);
 }
 
 template <typename TX>
@@ -442,12 +452,14 @@ struct Cols {
   float* part;
   TX* dx;
   int64_t ldx;
+  RqDownJobs<TX> jobs;      // z = 0: none
 };
 template <typename TX, int NB, int MODE, int NT, int NM>
 void launch_cols(const Cols<TX>& a, const RqPacked& w, hipStream_t s) {
-  hipLaunchKernelGGL((k_packed_cols<TX, NB, MODE, NT, NM>), dim3((w.C + COLS - 1) / COLS, a.sp.parts, (a.T + 16 * NT - 1) / (16 * NT)),
-                     dim3(64 * cols_waves(NT)), 0, s, a.dy, a.T, a.ldy, a.plane, w, NM == 2 ? *a.w1 : w, a.sp.steps_per, a.part, a.dx,
-                     a.ldx);
+  const int rows = a.jobs.z ? rq_jobs_rows(a.jobs, a.T, w.C) : 0;      // for tiles of 64 tokens: smaller ones leave some idle
+  hipLaunchKernelGGL((k_packed_cols<TX, NB, MODE, NT, NM>),
+                     dim3((w.C + COLS - 1) / COLS, rows + a.sp.parts, (a.T + 16 * NT - 1) / (16 * NT)), dim3(64 * cols_waves(NT)), 0, s,
+                     a.dy, a.T, a.ldy, a.plane, w, NM == 2 ? *a.w1 : w, a.sp.steps_per, a.part, a.dx, a.ldx, a.jobs, rows);
 }
 // WIDE: the caller joins the parts.
 template <typename TX, int NB, int MODE, int NM, bool WIDE>
@@ -476,7 +488,12 @@ void cols_of(const Cols<TX>& a, const RqPacked& w, int nbits, hipStream_t s) {
 template <typename TX>
 void rq_cols_parts(const TX* dy, int T, int64_t ldy, const RqPacked& w, int nbits, const RqColSplit& sp, float* part,
                    hipStream_t s) {
-  cols_of<TX, 1, true>(Cols<TX>{dy, T, ldy, 0, nullptr, sp, part, nullptr, 0}, w, nbits, s);
+  cols_of<TX, 1, true>(Cols<TX>{dy, T, ldy, 0, nullptr, sp, part, nullptr, 0, {}}, w, nbits, s);
+}
+template <typename TX>
+void rq_lora_cols(const TX* dy, int T, int64_t ldy, const RqPacked& w, int nbits, const RqColSplit& sp, float* part,
+                  const RqDownJobs<TX>& jobs, hipStream_t s) {
+  cols_of<TX, 1, true>(Cols<TX>{dy, T, ldy, 0, nullptr, sp, part, nullptr, 0, jobs}, w, nbits, s);
 }
 
 template <typename TX>
@@ -486,7 +503,7 @@ void rq_linear_cols(const TX* dy, int T, int64_t ldy, const RqPacked& w, int nbi
     const int n = (int)(T - t0 < RQ_COL_TOKENS ? T - t0 : RQ_COL_TOKENS);
     const RqColSplit sp = rq_col_split(n, w.R, w.C);
     TX* out = dx + t0 * ldx;
-    cols_of<TX, 1, false>(Cols<TX>{dy + t0 * ldy, n, ldy, 0, nullptr, sp, sp.parts > 1 ? part : nullptr, out, ldx}, w, nbits, s);
+    cols_of<TX, 1, false>(Cols<TX>{dy + t0 * ldy, n, ldy, 0, nullptr, sp, sp.parts > 1 ? part : nullptr, out, ldx, {}}, w, nbits, s);
     if (sp.parts > 1)
       hipLaunchKernelGGL(k_packed_join<TX>, dim3((w.C + 255) / 256, n), dim3(256), 0, s, part, sp.parts, n, w.C, out, ldx);
   }

@@ -54,7 +54,7 @@ extern "C" int rq_packed_linear_lora(const void* x, int dtype, int T, int64_t ld
     const RqLora<TX> lora{(const TX*)lora_a, (const TX*)lora_b, adapter_ids, scaling, scale, n, r};
     const RqLow low = rq_low((float*)workspace, T, C, r);          // a multiple of 128 bytes
     void* arranged = rq_lora_arranged(T, w) ? (float*)workspace + rq_low_floats(low) : nullptr;
-    rq_lora_down<TX>(RqDown<TX>{(const TX*)x, ldx, C, 1, low}, nullptr, lora, arranged, nbits, s);
+    rq_lora_down<TX>(rq_down_jobs<TX>(RqDown<TX>{(const TX*)x, ldx, C, 1, low}, nullptr, lora), arranged, nbits, s);
     rq_lora_rows<TX>((const TX*)x, T, ldx, w, nbits, (const TX*)bias, lora, low, arranged, (TX*)y, ldy, s);
   });
   if (!known) return RQ_EINVAL;
@@ -90,12 +90,17 @@ extern "C" int rq_packed_linear_lora_grad(const void* grad_y, int dtype, int T, 
     float* part = ws + g.u + g.v;
     const TX* dy = (const TX*)grad_y;
     const RqDown<TX> ofx{(const TX*)x, ldx, C, 1, u};
-    if (T) rq_lora_down<TX>(RqDown<TX>{dy, ldg, R, 0, v}, grad_a ? &ofx : nullptr, lora, nullptr, nbits, s);
+    RqDownJobs<TX> jobs = rq_down_jobs<TX>(RqDown<TX>{dy, ldg, R, 0, v}, grad_a ? &ofx : nullptr, lora);
+    if (T && (!grad_x || !rq_jobs_rows(jobs, T < RQ_COL_WIDE ? T : RQ_COL_WIDE, C))) {
+      rq_lora_down<TX>(jobs, nullptr, nbits, s);
+      jobs.z = 0;
+    }
     RqLoraDx<TX> dx{part, 0, 0, 0, nullptr, ldgx};
     for (int t0 = 0; grad_x && t0 < T; t0 += RQ_COL_WIDE) {
       const int k = T - t0 < RQ_COL_WIDE ? T - t0 : RQ_COL_WIDE;
       const RqColSplit sp = rq_col_split_wide(k, rq_col_steps(R), C);
-      rq_cols_parts<TX>(dy + t0 * ldg, k, ldg, w, nbits, sp, part, s);
+      rq_lora_cols<TX>(dy + t0 * ldg, k, ldg, w, nbits, sp, part, jobs, s);
+      jobs.z = 0;
       dx = RqLoraDx<TX>{part, sp.parts, t0, k, (TX*)grad_x + t0 * ldgx, ldgx};
       if (t0 + k < T) rq_lora_grads<TX>(dx, (const TX*)x, ldx, C, dy, ldg, R, T, lora, u, v, nullptr, nullptr, s);
     }

@@ -4,100 +4,25 @@
 // cores' columns are tokens, so what another adapter makes of a token is dropped, not added as 0 (an adapter that holds an
 // inf or NaN spoils its own tokens only).
 #pragma once
-#include "plora_types.h"
+#include "plora_down.h"
 #include "plinear_rows.h"
 
 namespace {
 
-__device__ __forceinline__ floatx4 mfma4(float a, float b, floatx4 c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
-
-// acc += A[.][32 k] B[32 k][.]: lane 16 q + i holds A[i][8q..8q+7] and B[8q..8q+7][i].
-__device__ __forceinline__ floatx4 mfma32(half8 a, half8 b, floatx4 c) { return rq_mfma(a, b, c); }
-__device__ __forceinline__ floatx4 mfma32(bf16x8 a, bf16x8 b, floatx4 c) { return rq_mfma(a, b, c); }
-__device__ __forceinline__ floatx4 mfma32(floatx8 a, floatx8 b, floatx4 c) {
-#pragma unroll
-  for (int k = 0; k < 8; ++k) c = mfma4(a[k], b[k], c);
-  return c;
-}
-
-// u = A x or B^T x.  Grid (tiles of 16 tokens, the tile's adapters in the order of their first tokens, rank tiles x
-// parts of one job and then of the other, and behind them chunks of the first's x to be
-// arranged); the waves take steps of 32 columns in turn, all of a full part's in flight at
-// once, and are joined through LDS in their order.
-constexpr int ARRANGED_CHUNKS = 16;
-constexpr int DOWN_WAVES = 16, DOWN_STEPS = RQ_LORA_COLS / (32 * DOWN_WAVES);
+constexpr int ARRANGED_CHUNKS = 16, DOWN_WAVES = 16;
+// Both jobs, and behind them chunks of the first's x to be arranged.
 template <typename TX>
-__global__ __launch_bounds__(64 * DOWN_WAVES) void k_lora_down(RqDown<TX> first, RqDown<TX> second, int zfirst, RqLora<TX> lora,
-                                                               RqArrange arrange) {
-  typedef typename RqOperand<TX>::raw Raw;
-  __shared__ floatx4 join[DOWN_WAVES][64];
-  const int lane = threadIdx.x & 63, wave = rq_wave(), i = lane & 15, q = lane >> 4;
-  if ((int)blockIdx.z >= arrange.z) {
-    const int ch = (blockIdx.z - arrange.z) * ARRANGED_CHUNKS, chunks = (first.cols + RQ_CHUNK - 1) / RQ_CHUNK;
+__global__ __launch_bounds__(64 * DOWN_WAVES) void k_lora_down(RqDownJobs<TX> jobs, RqArrange arrange) {
+  __shared__ floatx4 join[DOWN_WAVES * 64];
+  if ((int)blockIdx.z >= jobs.z) {
+    const RqDown<TX>& d = jobs.first;
+    const int ch = (blockIdx.z - jobs.z) * ARRANGED_CHUNKS, chunks = (d.cols + RQ_CHUNK - 1) / RQ_CHUNK;
     if (blockIdx.y == 0)
-      rq_arrange<TX>(first.x, first.low.T, first.ldx, first.cols, blockIdx.x, ch, min(ch + ARRANGED_CHUNKS, chunks), arrange.paired,
-                     threadIdx.x, blockDim.x, arrange.out);
+      rq_arrange<TX>(d.x, d.low.T, d.ldx, d.cols, blockIdx.x, ch, min(ch + ARRANGED_CHUNKS, chunks), arrange.paired, threadIdx.x,
+                     blockDim.x, arrange.out);
     return;
   }
-  const RqDown<TX> d = (int)blockIdx.z < zfirst ? first : second;
-  const RqLow& low = d.low;
-  const int z = (int)blockIdx.z < zfirst ? blockIdx.z : blockIdx.z - zfirst;
-  const int64_t t = (int64_t)blockIdx.x * 16 + i;
-  const int own = t < low.T ? lora.of(t) : -1;
-  uint64_t pending = __ballot(lane < 16 && own >= 0 && own < lora.n);
-  for (int k = 0; k < (int)blockIdx.y && pending; ++k)
-    pending &= ~__ballot(own == __builtin_amdgcn_readlane(own, __ffsll((unsigned long long)pending) - 1));
-  if (!pending) return;
-  const int lead = __ffsll((unsigned long long)pending) - 1, a = __builtin_amdgcn_readlane(own, lead);
-  const int tiles = low.ranks / 16, rank = z % tiles * 16, part = z / tiles;
-  const int c0 = part * RQ_LORA_COLS, c1 = min(d.cols, c0 + RQ_LORA_COLS);
-  const TX* xs = d.x + (own == a ? t : (int64_t)blockIdx.x * 16 + lead) * d.ldx;
-  const int row = min(rank + i, lora.r - 1);
-  const TX* as = d.rows ? lora.a + ((int64_t)a * lora.r + row) * d.cols : lora.b + (int64_t)a * d.cols * lora.r + row;
-  floatx4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
-  auto load = [&](auto full, int c, Raw& xv, Raw& av) {
-    constexpr bool FULL = decltype(full)::value;
-    const int n = c1 - c;                            // the lane's columns (may be none)
-    xv = rq_load_x<FULL>(xs + c, n);
-    if (d.rows) {
-      av = rq_load_x<FULL>(as + c, n);
-    } else {
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        typename std::remove_reference<decltype(av[0])>::type e;
-        __builtin_memcpy(&e, as + (int64_t)(c + (FULL ? k : min(k, n - 1))) * lora.r, sizeof(e));
-        av[k] = FULL || k < n ? e : (decltype(e))0.0f;
-      }
-    }
-  };
-  if (rank >= lora.r) {
-    // a tile of padding
-  } else if (c0 + RQ_LORA_COLS <= c1) {
-    Raw xv[DOWN_STEPS], av[DOWN_STEPS];
-#pragma unroll
-    for (int k = 0; k < DOWN_STEPS; ++k) load(std::true_type{}, c0 + 32 * (wave + DOWN_WAVES * k) + 8 * q, xv[k], av[k]);
-#pragma unroll
-    for (int k = 0; k < DOWN_STEPS; ++k) acc = mfma32(av[k], xv[k], acc);
-  } else {
-    Raw xv, av;
-    int c = c0 + 32 * wave;
-    for (; c + 32 <= c1; c += 32 * DOWN_WAVES) {
-      load(std::true_type{}, c + 8 * q, xv, av);
-      acc = mfma32(av, xv, acc);
-    }
-    if (c < c1) {
-      load(std::false_type{}, c + 8 * q, xv, av);
-      acc = mfma32(av, xv, acc);
-    }
-  }
-  join[wave][lane] = acc;
-  __syncthreads();
-  if (wave || own != a) return;
-  for (int w = 1; w < DOWN_WAVES; ++w) acc += join[w][lane];
-#pragma unroll
-  for (int k = 0; k < 4; ++k)
-    if (rank + 4 * q + k >= lora.r) acc[k] = 0.0f;
-  *reinterpret_cast<floatx4*>(low.u + low.at(part, t) + rank + 4 * q) = acc;
+  rq_lora_down_job<TX, DOWN_WAVES>(jobs, blockIdx.x, blockIdx.y, blockIdx.z, join);
 }
 
 // Eight ranks of a token, its parts joined in their order.
@@ -240,7 +165,7 @@ __device__ __forceinline__ void lora_dx(int block, const float* __restrict__ par
       for (int k = 0; k < 8; ++k) {
         const bool is = k0 + 8 * q + k < lora.r;
 #pragma unroll
-        for (int n = 0; n < 4; ++n) low[n] = mfma4(vt[k], is ? row[k][n] : 0.0f, low[n]);
+        for (int n = 0; n < 4; ++n) low[n] = rq_mfma4(vt[k], is ? row[k][n] : 0.0f, low[n]);
       }
     }
 #pragma unroll
@@ -292,6 +217,7 @@ __device__ __forceinline__ void lora_outer(int block, const TX* __restrict__ x, 
   floatx4 acc[8];
 #pragma unroll
   for (int n = 0; n < 8; ++n) acc[n] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+  bool any = false;                                // tokens with this adapter
   for (int64_t w0 = 0; w0 < T; w0 += WINDOW) {
     if (wave == 0) {
       int n = 0;
@@ -305,6 +231,7 @@ __device__ __forceinline__ void lora_outer(int block, const TX* __restrict__ x, 
     }
     __syncthreads();
     const int n = count;
+    any |= n > 0;
     for (int g = 16 * wave; g < n; g += 16 * GRAD_WAVES) {
       float m[4];
       Raw r[4];
@@ -333,7 +260,7 @@ __device__ __forceinline__ void lora_outer(int block, const TX* __restrict__ x, 
         floatx8 f;
         rq_floats(r[h], f);
 #pragma unroll
-        for (int k = 0; k < 8; ++k) acc[k] = mfma4(is ? m[h] : 0.0f, is ? f[k] : 0.0f, acc[k]);
+        for (int k = 0; k < 8; ++k) acc[k] = rq_mfma4(is ? m[h] : 0.0f, is ? f[k] : 0.0f, acc[k]);
       }
     }
     __syncthreads();
@@ -341,7 +268,7 @@ __device__ __forceinline__ void lora_outer(int block, const TX* __restrict__ x, 
 #pragma unroll
   for (int n = 0; n < 8; ++n) lds[(wave * 8 + n) * 64 + lane] = acc[n];
   __syncthreads();
-  const float s = lora.scale_of(a);
+  const float s = any ? lora.scale_of(a) : 0.0f;   // 0, whatever the scaling of an adapter that nobody has
   if (of_a) {
     // wave w: rank 4q + w, eight columns
     const int k = rank + 4 * q + wave;
@@ -381,12 +308,10 @@ __global__ __launch_bounds__(64 * GRAD_WAVES, 4) void k_lora_grads(RqLoraDx<TX> 
 }  // namespace
 
 template <typename TX>
-void rq_lora_down(const RqDown<TX>& first, const RqDown<TX>* second, const RqLora<TX>& lora, void* arranged, int nbits, hipStream_t s) {
-  const int z0 = first.low.ranks / 16 * first.low.parts, z1 = second ? second->low.ranks / 16 * second->low.parts : 0;
-  const int chunks = (first.cols + RQ_CHUNK - 1) / RQ_CHUNK, z2 = arranged ? (chunks + ARRANGED_CHUNKS - 1) / ARRANGED_CHUNKS : 0;
-  const dim3 grid((first.low.T + 15) / 16, lora.ids ? (lora.n < 16 ? lora.n : 16) : 1, z0 + z1 + z2), block(64 * DOWN_WAVES);
-  hipLaunchKernelGGL(k_lora_down<TX>, grid, block, 0, s, first, second ? *second : first, z0, lora,
-                     RqArrange{arranged, z0 + z1, rq_pairs<TX>(nbits)});
+void rq_lora_down(const RqDownJobs<TX>& jobs, void* arranged, int nbits, hipStream_t s) {
+  const int chunks = (jobs.first.cols + RQ_CHUNK - 1) / RQ_CHUNK, more = arranged ? (chunks + ARRANGED_CHUNKS - 1) / ARRANGED_CHUNKS : 0;
+  hipLaunchKernelGGL(k_lora_down<TX>, dim3(jobs.tiles, jobs.adapters, jobs.z + more), dim3(64 * DOWN_WAVES), 0, s, jobs,
+                     RqArrange{arranged, rq_pairs<TX>(nbits)});
 }
 
 template <typename TX>

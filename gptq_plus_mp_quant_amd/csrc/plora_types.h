@@ -45,15 +45,38 @@ struct RqDown {
   int cols, rows;
   RqLow low;
 };
+// One or two of them (z >= zfirst: the second), of the same tokens; z = 0: none.
 template <typename TX>
-void rq_lora_down(const RqDown<TX>& first, const RqDown<TX>* second, const RqLora<TX>& lora, void* arranged, int nbits, hipStream_t s);
-// Beside it (arranged not NULL): the first's x as RqArranged has it, from grid.z = z on.
+struct RqDownJobs {
+  RqDown<TX> first, second;
+  RqLora<TX> lora;
+  int tiles, adapters, zfirst, z;
+};
+template <typename TX>
+inline RqDownJobs<TX> rq_down_jobs(const RqDown<TX>& first, const RqDown<TX>* second, const RqLora<TX>& lora) {
+  const int z0 = first.low.ranks / 16 * first.low.parts, z1 = second ? second->low.ranks / 16 * second->low.parts : 0;
+  return RqDownJobs<TX>{first, second ? *second : first, lora, (first.low.T + 15) / 16, lora.ids ? (lora.n < 16 ? lora.n : 16) : 1, z0,
+                        z0 + z1};
+}
+// Beside them: the first's x as RqArranged has it.
 struct RqArrange {
   void* out;
-  int z;
   bool paired;
 };
+template <typename TX>
+void rq_lora_down(const RqDownJobs<TX>& jobs, void* arranged, int nbits, hipStream_t s);
 inline bool rq_lora_arranged(int T, const RqPacked& w) { return T > 16 && rq_whole_mode_of(w) == RQ_RUNS; }
+// The gradient's parts of T <= RQ_COL_WIDE tokens as rq_cols_parts has them, and in the same launch the jobs.
+template <typename TX>
+void rq_lora_cols(const TX* dy, int T, int64_t ldy, const RqPacked& w, int nbits, const RqColSplit& sp, float* part,
+                  const RqDownJobs<TX>& jobs, hipStream_t s);
+// Rows of the grid that the jobs take there; 0: too many, they need a launch of their own.
+template <typename TX>
+inline int rq_jobs_rows(const RqDownJobs<TX>& jobs, int T, int C) {
+  const int64_t row = (int64_t)((C + 127) / 128) * ((T + 63) / 64);
+  const int64_t rows = ((int64_t)jobs.tiles * jobs.adapters * jobs.z + row - 1) / row;
+  return rows <= 4096 ? (int)rows : 0;
+}
 // y = x W^T (+ bias) + s B u; arranged: x once more, where rq_lora_arranged says so.
 template <typename TX>
 void rq_lora_rows(const TX* x, int T, int64_t ldx, const RqPacked& w, int nbits, const TX* bias, const RqLora<TX>& lora,

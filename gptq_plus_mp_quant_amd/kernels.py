@@ -617,8 +617,9 @@ def packed_linear_lora_grad(grad_y, x, qweight, nbits, scales, T, R, C, ngroups,
 
 
 def _weight(qweight, nbits, scales, ngroups, g_idx, groupsize):
-    return nat.PackedWeight(qweight.data_ptr(), scales.data_ptr(), g_idx.data_ptr(), qweight.stride(0), scales.stride(0), nbits,
-                            ngroups, groupsize)
+    """A rq_packed_weight's bytes, which an entry point takes as a pointer."""
+    return nat.PACKED_WEIGHT.pack(qweight.data_ptr(), scales.data_ptr(), g_idx.data_ptr(), qweight.stride(0), scales.stride(0), nbits,
+                                  ngroups, groupsize)
 
 
 @nat.on_device_of_first
@@ -629,7 +630,6 @@ def packed_gated(x, gate, up, T, I, C, activation, want_pre, lead):
     h = x.new_empty((*lead, I))
     pre = x.new_empty((*lead, 2, I), dtype=_f32) if want_pre else None
     g, u = _weight(*gate), _weight(*up)
-    g, u = ctypes.byref(g), ctypes.byref(u)
     nbytes = lib.rq_packed_gated_workspace_bytes(T, I, C, nat.DTYPE_CODES[x.dtype], g, u)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes > 0 else None
     nat.check("rq_packed_gated", lib.rq_packed_gated(
@@ -645,10 +645,9 @@ def packed_gated_grad(grad_h, pre, gate, up, T, I, C, activation, lead):
     gx = grad_h.new_empty((*lead, C))
     nbytes = lib.rq_packed_gated_grad_workspace_bytes(T, I, C)
     ws = torch.empty(max(nbytes, 0), dtype=torch.uint8, device=grad_h.device)
-    g, u = _weight(*gate), _weight(*up)
     nat.check("rq_packed_gated_grad", lib.rq_packed_gated_grad(
-        grad_h.data_ptr(), nat.DTYPE_CODES[grad_h.dtype], T, grad_h.stride(0), I, pre.data_ptr(), activation, ctypes.byref(g),
-        ctypes.byref(u), C, gx.data_ptr(), C, ws.data_ptr(), nbytes, nat.raw_stream(grad_h)))
+        grad_h.data_ptr(), nat.DTYPE_CODES[grad_h.dtype], T, grad_h.stride(0), I, pre.data_ptr(), activation, _weight(*gate),
+        _weight(*up), C, gx.data_ptr(), C, ws.data_ptr(), nbytes, nat.raw_stream(grad_h)))
     return gx
 
 

@@ -1,7 +1,5 @@
 """The C entries and Python checks of the adapters, the gated block and the distillation loss, without a device: bad
 arguments are refused before any launch, sizes of workspaces, tensors on the CPU."""
-import ctypes
-
 import pytest
 import torch
 
@@ -68,19 +66,18 @@ def test_lora_workspaces_and_empty_calls():
 
 
 def _weight(**over):
-    f = {**dict(qweight=FAKE, scales=FAKE, g_idx=None, ldp=8, lds=32, nbits=4, ngroups=2, groupsize=32), **over}
-    return nat.PackedWeight(*(f[n] for n, _ in nat.PackedWeight._fields_))
+    f = {**dict(qweight=FAKE, scales=FAKE, g_idx=0, ldp=8, lds=32, nbits=4, ngroups=2, groupsize=32), **over}
+    return nat.PACKED_WEIGHT.pack(*(v or 0 for v in f.values()))
 
 
 def _gated(gate=_weight(), up=_weight(), **over):
-    base = dict(x=FAKE, dtype=nat.RQ_BF16, T=1, ldx=64, C=64, I=32, gate=gate and ctypes.byref(gate), up=up and ctypes.byref(up), act=0,
+    base = dict(x=FAKE, dtype=nat.RQ_BF16, T=1, ldx=64, C=64, I=32, gate=gate, up=up, act=0,
                 pre=NULL, h=FAKE, ldh=32, ws=NULL, nbytes=0, stream=NULL)
     return _call("rq_packed_gated", base, **over)
 
 
 def _gated_grad(gate=_weight(), up=_weight(), **over):
-    base = dict(gh=FAKE, dtype=nat.RQ_BF16, T=1, ldg=32, I=32, pre=FAKE, act=0, gate=gate and ctypes.byref(gate),
-                up=up and ctypes.byref(up), C=64, gx=FAKE, ldx=64, ws=FAKE, nbytes=MUCH, stream=NULL)
+    base = dict(gh=FAKE, dtype=nat.RQ_BF16, T=1, ldg=32, I=32, pre=FAKE, act=0, gate=gate, up=up, C=64, gx=FAKE, ldx=64, ws=FAKE, nbytes=MUCH, stream=NULL)
     return _call("rq_packed_gated_grad", base, **over)
 
 
@@ -105,7 +102,7 @@ def test_gated_workspaces():
     lib = _lib()
 
     def need(T, gate, up, I=32, C=64, dtype=nat.RQ_BF16):
-        return lib.rq_packed_gated_workspace_bytes(T, I, C, dtype, ctypes.byref(gate), ctypes.byref(up))
+        return lib.rq_packed_gated_workspace_bytes(T, I, C, dtype, gate, up)
 
     assert need(5, _weight(), _weight()) == 0
     assert need(5, _weight(), _weight(nbits=3)) == 5 * 2 * 32 * 4

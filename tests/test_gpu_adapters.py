@@ -135,6 +135,7 @@ def test_tokens_without_an_adapter(dtype):
     whose[3::5] = 2
     whose[4] = -(1 << 40)
     a[0], b[1], b[3, 0, 0] = float("nan"), float("inf"), float("nan")
+    s[1], s[3] = float("nan"), float("inf")
     y, (gx, ga, gb) = check(x, gy, a, b, s, whose, entry, W)
     assert bool((ga.cpu()[[0, 1, 3]] == 0).all()) and bool((gb.cpu()[[0, 1, 3]] == 0).all())
     none = torch.full((20,), -1, dtype=torch.int64, device=DEV)

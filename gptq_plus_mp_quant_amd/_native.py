@@ -98,7 +98,7 @@ SIGNATURES = {
     "rq_packed_linear_grad": (_I, [_P, _I, _I, _L, _I, _P, _L, _I, _I, _P, _L, _I, _P, _I, _P, _L, _P, _L, _P]),
     "rq_packed_moe_workspace_bytes": (_L, [_I, _I, _I, _I, _I]),
     "rq_packed_moe": (_I, [_P, _I, _I, _L, _I, _P, _L, _I, _I, _I, _I, _P, _P, _P, _P, _L, _P, _P, _P, _L, _P]),
-    "rq_packed_linear_lora_workspace_bytes": (_L, [_I, _I, _I, _I]),
+    "rq_packed_linear_lora_workspace_bytes": (_L, [_I, _I, _I, _I, _I]),
     "rq_packed_linear_lora": (_I, [_P, _I, _I, _L, _I, _P, _L, _I, _I, _P, _L, _I, _P, _I, _P, _P, _P, _I, _I, _P, _P, _F, _P, _L,
                                    _P, _L, _P]),
     "rq_packed_linear_lora_grad_workspace_bytes": (_L, [_I, _I, _I, _I]),

@@ -18,7 +18,7 @@ constexpr int rows_threads(int rt, int nt) { return rt * nt >= 2 ? 512 : 1024; }
 struct RqNothing {
   static constexpr bool arranged = false, whole = false;
   template <int RT, int NT>
-  __device__ __forceinline__ void add(int, int, int, int, int, int, floatx4 (&)[RT][NT]) const {}
+  __device__ __forceinline__ void add(int, int, int, int, int, int, const float*, floatx4 (&)[RT][NT]) const {}
 };
 // ARRANGED (MORE::arranged, more than one token tile, RUNS): x lies as RqArranged has it, at more.arranged_x.
 template <typename TX, int NB, int MODE, int RT, int NT, typename MORE>
@@ -35,6 +35,7 @@ __global__ __launch_bounds__(rows_threads(RT, NT)) void k_packed_rows(const TX* 
 #pragma unroll
     for (int b = 0; b < NT; ++b) xs.p[b] = x + (int64_t)min(t0 + 16 * b + (lane & 15), T - 1) * ldx;
   }
+  if constexpr (MORE::whole && NT == 1) more.prepare(x, T, ldx, w.C, wave, waves, lds);
   const bool staged = MODE == RQ_ANY && w.ngroups <= RQ_STAGED_GROUPS;
   if (staged) {
     for (int a = 0; a < RT; ++a)
@@ -47,7 +48,7 @@ __global__ __launch_bounds__(rows_threads(RT, NT)) void k_packed_rows(const TX* 
 #pragma unroll
     for (int b = 0; b < NT; ++b) acc[a][b] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
   rq_rows_tokens<NB, MODE, RT, 1>({w}, r0, xs, wave, waves, staged ? lds : nullptr, acc);
-  more.add(r0, w.R, t0, T, wave, waves, acc);
+  more.add(r0, w.R, t0, T, wave, waves, lds, acc);
   if (staged) __syncthreads();
   floatx4* out = reinterpret_cast<floatx4*>(lds);
 #pragma unroll
@@ -92,8 +93,10 @@ void launch_rows(const TX* x, int T, int64_t ldx, const RqPacked& w, const TX* b
     const size_t scales = (size_t)(w.ngroups + 1) * 16 * RT * 4;
     lds = lds > scales ? lds : scales;
   }
+  MORE with = more;
+  if constexpr (MORE::whole && NT == 1) lds = with.own_lds(lds);
   hipLaunchKernelGGL((k_packed_rows<TX, NB, MODE, RT, NT, MORE>), dim3(bx, by), dim3(64 * waves), lds, s, x, T, ldx, w,
-                     bias, y, ldy, more);
+                     bias, y, ldy, with);
 }
 
 template <typename TX, int NB, typename MORE>

@@ -28,11 +28,12 @@ GradSpace grad_space(int T, int R, int C, int r) {
 
 }  // namespace
 
-extern "C" int64_t rq_packed_linear_lora_workspace_bytes(int T, int C, int r, int dtype) {
-  if (T < 0 || T > TOKENS || C <= 0 || r <= 0 || r > LORA_MAX_RANK || !width_ok(C, r)) return RQ_EINVAL;
+extern "C" int64_t rq_packed_linear_lora_workspace_bytes(int T, int R, int C, int r, int dtype) {
+  if (T < 0 || T > TOKENS || R <= 0 || C <= 0 || r <= 0 || r > LORA_MAX_RANK || !width_ok(C, r)) return RQ_EINVAL;
   int64_t bytes = 4 * rq_low_floats(rq_low(nullptr, T, C, r));
   const bool known = rq_with_dtype(dtype, [&](auto* p) {
-    if (T > 16) bytes += rq_arranged_bytes<typename std::remove_pointer<decltype(p)>::type>(T, C);
+    if (rq_lora_own(T, R, C, r, sizeof(*p))) bytes = 0;
+    else if (T > 16) bytes += rq_arranged_bytes<typename std::remove_pointer<decltype(p)>::type>(T, C);
   });
   return known ? bytes : RQ_EINVAL;
 }
@@ -47,14 +48,15 @@ extern "C" int rq_packed_linear_lora(const void* x, int dtype, int T, int64_t ld
     return RQ_EINVAL;
   if (T == 0) return RQ_OK;
   if (!x || !y || ldx < C || ldy < R) return RQ_EINVAL;
-  if (!workspace || workspace_bytes < rq_packed_linear_lora_workspace_bytes(T, C, r, dtype)) return RQ_EINVAL;
+  const int64_t need = rq_packed_linear_lora_workspace_bytes(T, R, C, r, dtype);
+  if (need < 0 || (need && (!workspace || workspace_bytes < need))) return RQ_EINVAL;
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   const bool known = rq_with_dtype(dtype, [&](auto* p) {
     typedef typename std::remove_pointer<decltype(p)>::type TX;
     const RqLora<TX> lora{(const TX*)lora_a, (const TX*)lora_b, adapter_ids, scaling, scale, n, r};
-    const RqLow low = rq_low((float*)workspace, T, C, r);          // a multiple of 128 bytes
+    const RqLow low = rq_low(need ? (float*)workspace : nullptr, T, C, r);         // a multiple of 128 bytes
     void* arranged = rq_lora_arranged(T, w) ? (float*)workspace + rq_low_floats(low) : nullptr;
-    rq_lora_down<TX>(rq_down_jobs<TX>(RqDown<TX>{(const TX*)x, ldx, C, 1, low}, nullptr, lora), arranged, nbits, s);
+    if (need) rq_lora_down<TX>(rq_down_jobs<TX>(RqDown<TX>{(const TX*)x, ldx, C, 1, low}, nullptr, lora), arranged, nbits, s);
     rq_lora_rows<TX>((const TX*)x, T, ldx, w, nbits, (const TX*)bias, lora, low, arranged, (TX*)y, ldy, s);
   });
   if (!known) return RQ_EINVAL;

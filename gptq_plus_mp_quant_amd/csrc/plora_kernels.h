@@ -58,14 +58,67 @@ struct RqLowRank {
   RqLora<TX> lora;
   RqLow low;
   const void* arranged_x;
+  bool own;                 // no launch made u: each workgroup makes it for itself, in LDS from float own_at on
+  int own_at;
+  size_t own_lds(size_t lds) {
+    own_at = (int)(lds / 4);
+    return own ? lds + (size_t)low.T * low.ranks * 4 : lds;
+  }
+  // u of at most 16 tokens: the waves take steps of 32 columns in turn, eight in flight, and are joined in their order.
+  __device__ __forceinline__ void prepare(const TX* __restrict__ x, int T, int64_t ldx, int C, int wave, int waves, float* lds) const {
+    typedef typename RqOperand<TX>::raw Raw;
+    if (!own) return;
+    floatx4* join = reinterpret_cast<floatx4*>(lds);
+    const int lane = threadIdx.x & 63, i = lane & 15, q = lane >> 4;
+    const int mine = i < T ? lora.of(i) : -1;
+    for (uint64_t pending = __ballot(lane < 16 && mine >= 0 && mine < lora.n); pending;) {
+      const int lead = __ffsll((unsigned long long)pending) - 1, a = __builtin_amdgcn_readlane(mine, lead);
+      pending &= ~__ballot(mine == a);
+      const TX* xs = x + (int64_t)(mine == a ? i : lead) * ldx;
+      for (int rank = 0; rank < low.ranks; rank += 16) {
+        const TX* as = lora.a + ((int64_t)a * lora.r + min(rank + i, lora.r - 1)) * C;
+        floatx4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+        int c = 32 * wave;
+        if (rank < lora.r) {
+          for (; c + 32 * (7 * waves + 1) <= C; c += 32 * 8 * waves) {
+            Raw xv[8], av[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+              xv[k] = rq_load_x<true>(xs + c + 32 * k * waves + 8 * q, 8);
+              av[k] = rq_load_x<true>(as + c + 32 * k * waves + 8 * q, 8);
+            }
+#pragma unroll
+            for (int k = 0; k < 8; ++k) acc = rq_mfma32(av[k], xv[k], acc);
+          }
+          for (; c + 32 <= C; c += 32 * waves)
+            acc = rq_mfma32(rq_load_x<true>(as + c + 8 * q, 8), rq_load_x<true>(xs + c + 8 * q, 8), acc);
+          if (c < C) {
+            const int n = C - c - 8 * q;             // the lane's columns (may be none)
+            acc = rq_mfma32(rq_load_x<false>(as + c + 8 * q, n), rq_load_x<false>(xs + c + 8 * q, n), acc);
+          }
+        }
+        join[wave * 64 + lane] = acc;
+        __syncthreads();
+        if (wave == 0) {
+          for (int w = 1; w < waves; ++w) acc += join[w * 64 + lane];
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            if (rank + 4 * q + k >= lora.r) acc[k] = 0.0f;
+          if (mine == a) *reinterpret_cast<floatx4*>(lds + own_at + i * low.ranks + rank + 4 * q) = acc;
+        }
+        __syncthreads();
+      }
+    }
+  }
   template <int RT, int NT>
-  __device__ __forceinline__ void add(int r0, int R, int t0, int T, int wave, int waves, floatx4 (&acc)[RT][NT]) const {
+  __device__ __forceinline__ void add(int r0, int R, int t0, int T, int wave, int waves, const float* lds,
+                                      floatx4 (&acc)[RT][NT]) const {
     constexpr int PW = LoraPieces<TX>::n;
     const int lane = threadIdx.x & 63, i = lane & 15, q = lane >> 4;
     const int mine = lane < 16 * NT && t0 + lane < T ? lora.of(t0 + lane) : -1;
-    int own[NT];
+    int whose[NT];
 #pragma unroll
-    for (int b = 0; b < NT; ++b) own[b] = __shfl(mine, 16 * b + i);
+    for (int b = 0; b < NT; ++b) whose[b] = __shfl(mine, 16 * b + i);
     for (uint64_t pending = __ballot(mine >= 0 && mine < lora.n); pending;) {
       const int a = __builtin_amdgcn_readlane(mine, __ffsll((unsigned long long)pending) - 1);
       const uint64_t who = __ballot(mine == a);
@@ -94,7 +147,11 @@ struct RqLowRank {
         for (int b = 0; b < NT; ++b) {
           if (!(who >> (16 * b) & 0xFFFF)) continue;
           bf16x8 u[3];
-          rq_operand<3>(low8(low, min(t0 + 16 * b + i, T - 1), k), u);
+          const int t = min(t0 + 16 * b + i, T - 1);
+          floatx8 f;
+          if (NT == 1 && own) f = rq_load_as<floatx8>(lds + own_at + t * low.ranks + k);
+          else f = low8(low, t, k);
+          rq_operand<3>(f, u);
           bf16x8 lead = u[0];
           if constexpr (PW > 1) lead = without_inf(lead);
 #pragma unroll
@@ -108,14 +165,14 @@ struct RqLowRank {
             }
             if constexpr (PW > 2) part = rq_mfma(w[m][2], lead, part);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) acc[m][b][j] = own[b] == a ? __builtin_fmaf(s, part[j], acc[m][b][j]) : acc[m][b][j];
+            for (int j = 0; j < 4; ++j) acc[m][b][j] = whose[b] == a ? __builtin_fmaf(s, part[j], acc[m][b][j]) : acc[m][b][j];
           }
         }
       }
     }
 #pragma unroll
     for (int b = 0; b < NT; ++b)
-      if (own[b] == lora.n) {
+      if (whose[b] == lora.n) {
 #pragma unroll
         for (int m = 0; m < RT; ++m) acc[m][b] = floatx4{1.0f, 1.0f, 1.0f, 1.0f} * __builtin_nanf("");
       }
@@ -318,7 +375,7 @@ template <typename TX>
 void rq_lora_rows(const TX* x, int T, int64_t ldx, const RqPacked& w, int nbits, const TX* bias, const RqLora<TX>& lora,
                   const RqLow& low, const void* arranged, TX* y, int64_t ldy, hipStream_t s) {
   rq_with_nbits(nbits, [&](auto nb) {
-    linear_rows<TX, decltype(nb)::value>(x, T, ldx, w, bias, y, ldy, RqLowRank<TX>{lora, low, arranged}, s);
+    linear_rows<TX, decltype(nb)::value>(x, T, ldx, w, bias, y, ldy, RqLowRank<TX>{lora, low, arranged, low.u == nullptr, 0}, s);
   });
 }
 

@@ -77,7 +77,13 @@ inline int rq_jobs_rows(const RqDownJobs<TX>& jobs, int T, int C) {
   const int64_t rows = ((int64_t)jobs.tiles * jobs.adapters * jobs.z + row - 1) / row;
   return rows <= 4096 ? (int)rows : 0;
 }
-// y = x W^T (+ bias) + s B u; arranged: x once more, where rq_lora_arranged says so.
+// Whether the workgroups make u for themselves: one or two tokens, 16 ranks, and little enough of A for all of them
+// together (one token of 4096 x 4096 with 16 ranks: 13.0 us a call, 17.1 with a launch that makes u
+// first; on the GPU 13.7 for 11.8, which a host that launches in time would notice).
+inline bool rq_lora_own(int T, int R, int C, int r, int bytes) {
+  return T <= 2 && r <= 16 && (int64_t)((R + 15) / 16) * T * r * C * bytes <= 40 << 20;
+}
+// y = x W^T (+ bias) + s B u (low.u NULL: made there); arranged: x once more, where rq_lora_arranged says so.
 template <typename TX>
 void rq_lora_rows(const TX* x, int T, int64_t ldx, const RqPacked& w, int nbits, const TX* bias, const RqLora<TX>& lora,
                   const RqLow& low, const void* arranged, TX* y, int64_t ldy, hipStream_t s);

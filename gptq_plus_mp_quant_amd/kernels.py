@@ -589,12 +589,12 @@ def packed_linear_lora(x, qweight, nbits, scales, T, R, C, ngroups, g_idx, group
     """y [*lead, R] = x [T, C] times the transpose of a packed weight, with low-rank adapters; see rq_packed_linear_lora."""
     lib = nat.load()
     y = x.new_empty((*lead, R))
-    nbytes = lib.rq_packed_linear_lora_workspace_bytes(T, C, r, nat.DTYPE_CODES[x.dtype])
-    ws = torch.empty(max(nbytes, 0), dtype=torch.uint8, device=x.device)
+    nbytes = lib.rq_packed_linear_lora_workspace_bytes(T, R, C, r, nat.DTYPE_CODES[x.dtype])
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes > 0 else None
     nat.check("rq_packed_linear_lora", lib.rq_packed_linear_lora(
         x.data_ptr(), nat.DTYPE_CODES[x.dtype], T, x.stride(0), C, qweight.data_ptr(), qweight.stride(0), nbits, R,
         scales.data_ptr(), scales.stride(0), ngroups, g_idx.data_ptr(), groupsize, _addr(bias), lora_a.data_ptr(),
-        lora_b.data_ptr(), n, r, _addr(ids), _addr(scaling), scale, y.data_ptr(), R, ws.data_ptr(), nbytes, nat.raw_stream(x)))
+        lora_b.data_ptr(), n, r, _addr(ids), _addr(scaling), scale, y.data_ptr(), R, _addr(ws), nbytes, nat.raw_stream(x)))
     return y
 
 

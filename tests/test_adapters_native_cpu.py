@@ -21,7 +21,7 @@ def _call(entry, base, **over):
     return getattr(_lib(), entry)(*{**base, **over}.values())
 
 
-LORA = dict(x=FAKE, dtype=nat.RQ_F16, T=1, ldx=64, C=64, q=FAKE, ldp=8, nbits=4, R=32, scales=FAKE, lds=32, ngroups=2, g_idx=NULL,
+LORA = dict(x=FAKE, dtype=nat.RQ_F16, T=3, ldx=64, C=64, q=FAKE, ldp=8, nbits=4, R=32, scales=FAKE, lds=32, ngroups=2, g_idx=NULL,
             groupsize=32, bias=NULL, a=FAKE, b=FAKE, n=2, r=4, ids=FAKE, scaling=NULL, scale=1.0, y=FAKE, ldy=32, ws=FAKE,
             nbytes=MUCH, stream=NULL)
 WEIGHT_BAD = [dict(q=NULL), dict(ldp=7), dict(nbits=1), dict(nbits=10), dict(R=0), dict(C=0), dict(scales=NULL), dict(lds=31),
@@ -51,16 +51,17 @@ def test_lora_workspaces_and_empty_calls():
     assert _call("rq_packed_linear_lora", LORA, T=0, x=NULL, y=NULL, ws=NULL, nbytes=0) == nat.RQ_OK
     for T in (1, 16, 63, 64, 65, 100, 1000):
         for R, C, r in ((32, 64, 1), (4096, 14336, 64), (100, 28672, 256)):
-            need = lib.rq_packed_linear_lora_workspace_bytes(T, C, r, nat.RQ_F16)
-            assert need >= 4 * T * r
+            need = lib.rq_packed_linear_lora_workspace_bytes(T, R, C, r, nat.RQ_F16)
+            assert need >= 4 * T * r or (need == 0 and T == r == 1)            # one token of few ranks needs none
             grad = lib.rq_packed_linear_lora_grad_workspace_bytes(T, R, C, r)
             assert grad >= 8 * T * r + 4 * min(T, 64) * C
             size = dict(T=T, C=C, ldx=C, R=R, ldp=C, lds=R, groupsize=C, r=r)
-            assert _call("rq_packed_linear_lora", LORA, **size, ldy=R, nbytes=need - 1) == nat.RQ_EINVAL
+            assert need == 0 or _call("rq_packed_linear_lora", LORA, **size, ldy=R, nbytes=need - 1) == nat.RQ_EINVAL
             assert _call("rq_packed_linear_lora_grad", LORA_GRAD, **size, ldg=R, ldgx=C, nbytes=grad - 1) == nat.RQ_EINVAL
-    for bad in ((-1, 64, 4), (1, 0, 4), (1, 64, 0), (1, 64, 257), ((1 << 19) + 1, 64, 4), (1, 1 << 30, 256)):
-        assert lib.rq_packed_linear_lora_workspace_bytes(*bad, nat.RQ_F16) < 0
-    assert lib.rq_packed_linear_lora_workspace_bytes(1, 64, 4, 7) < 0
+    for T, C, r in ((-1, 64, 4), (1, 0, 4), (1, 64, 0), (1, 64, 257), ((1 << 19) + 1, 64, 4), (1, 1 << 30, 256)):
+        assert lib.rq_packed_linear_lora_workspace_bytes(T, 32, C, r, nat.RQ_F16) < 0
+    assert lib.rq_packed_linear_lora_workspace_bytes(1, 0, 64, 4, nat.RQ_F16) < 0
+    assert lib.rq_packed_linear_lora_workspace_bytes(1, 32, 64, 4, 7) < 0
     for bad in ((-1, 32, 64, 4), (1, 0, 64, 4), (1, 32, 0, 4), (1, 32, 64, 0), (1, 1 << 30, 64, 256)):
         assert lib.rq_packed_linear_lora_grad_workspace_bytes(*bad) < 0
 

@@ -87,7 +87,8 @@ def check(x, gy, a, b, s, whose, entry, W, bias=None, x_dev=None, gy_dev=None):
     (1, 1, 1, 1, 1, "one"), (1, 16, 128, 16, 1, "one"), (1, 40, 200, 5, 3, "mixed"), (3, 64, 31, 4, 2, "mixed"),
     (7, 130, 1365, 5, 3, "mixed"), (16, 33, 520, 8, 16, "mixed"), (17, 48, 384, 24, 40, "mixed"), (17, 100, 96, 17, 1, "one"),
     (33, 65, 250, 64, 5, "runs"), (64, 128, 512, 16, 64, "mixed"), (65, 31, 136, 100, 2, "runs"), (130, 20, 200, 32, 7, "mixed"),
-    (40, 24, 64, 256, 3, "mixed"), (5, 300, 4200, 16, 2, "mixed"), (600, 16, 40, 3, 2, "mixed"), (9, 8200, 130, 20, 4, "mixed")])
+    (2, 33, 4200, 16, 3, "mixed"), (2, 40, 5000, 16, 1, "one"), (1, 8200, 96, 7, 5, "mixed"), (2, 20, 300, 9, 2, "runs"),
+    (1, 4096, 8300, 16, 2, "mixed"), (40, 24, 64, 256, 3, "mixed"), (5, 300, 4200, 16, 2, "mixed"), (600, 16, 40, 3, 2, "mixed"), (9, 8200, 130, 20, 4, "mixed")])
 @pytest.mark.parametrize("nbits,groups", [(4, "128"), (5, "64"), (3, "order32")])
 def test_shapes(T, R, C, r, n, ids, nbits, groups, dtype):
     entry, W = make_entry(T * 7 + R + C, R, C, nbits, groups)
@@ -189,6 +190,25 @@ def test_a_token_does_not_depend_on_its_companions(T, dtype):
     back = torch.arange(T - 1, -1, -1, device=DEV)
     assert torch.equal(packed_linear_lora(x[back], e, a, b, whose[back], s), y[back])
     assert torch.equal(packed_linear_lora_backward(gy[back], x[back], e, a, b, whose[back], s)[0], gx[back])
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16, F32])
+@pytest.mark.parametrize("groups", ["128", "32", "order32"])
+def test_two_tokens_with_an_adapter_each(groups, dtype):
+    """What one or two tokens take (their low-rank values are made where they are used): the same adapter, two, one and
+    none, one that does not exist; a NaN stays with its token."""
+    entry, W = make_entry(11, 70, 1100, 4, groups)
+    e = on(entry, DEV)
+    x, _, a, b, s, _ = case(12, 2, 70, 1100, 13, 3, dtype)
+    for ids in ((1, 1), (2, 0), (-1, 2), (0, -7), (-1, -1), (1, 3)):
+        whose = torch.tensor(ids)
+        y = formulas(x, torch.zeros(2, 70), a, b, s, whose, W)[0]
+        got = packed_linear_lora(dev(x), e, dev(a), dev(b), dev(whose), dev(s))
+        within(got, y, dtype, "y")
+        assert torch.equal(got[1:], packed_linear_lora(dev(x).flip(0), e, dev(a), dev(b), dev(whose).flip(0), dev(s))[:1]) or ids[1] == 3
+    a[2, 4, 1099] = float("nan")
+    y = packed_linear_lora(dev(x), e, dev(a), dev(b), torch.tensor([2, 0], device=DEV), dev(s))
+    assert bool(torch.isnan(y[0]).all()) and bool(torch.isfinite(y[1]).all())
 
 
 @pytest.mark.parametrize("dtype", [F16, BF16, F32])

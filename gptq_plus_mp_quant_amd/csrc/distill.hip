@@ -11,6 +11,9 @@
 // it has a maximum of its own for the same reason.  Terms with p = 0 are 0.  A row without entries, or without a logit
 // above -inf, has no gradient.  Differences from a maximum are formed first, in fp32; a lane's sums are fp32, what is joined
 // from them and the sums over the list, a few values a row, 64 bits.
+// The rows are bound by the logits' bytes: 2048 x 128256 bf16 95 us, 5.5 TB/s; a few short ones by latency (3 x 32003 fp32, one
+// large workgroup each: 10.2 us; cut over several and joined by a second launch 4.9 + 5.6).  The gradient reads and writes them
+// once: 1024 x 128256 bf16 114 us, 4.6 TB/s, where a copy reaches 5.1.
 #include "logits.h"
 
 namespace {

@@ -17,6 +17,7 @@ namespace {
 constexpr int rows_threads(int rt, int nt) { return rt * nt >= 2 ? 512 : 1024; }     // 256 or 128 registers a lane
 struct RqNothing {
   static constexpr bool arranged = false, whole = false;
+  static constexpr int staged_groups = RQ_STAGED_GROUPS;
   template <int RT, int NT>
   __device__ __forceinline__ void add(int, int, int, int, int, int, const float*, floatx4 (&)[RT][NT]) const {}
 };
@@ -36,7 +37,7 @@ __global__ __launch_bounds__(rows_threads(RT, NT)) void k_packed_rows(const TX* 
     for (int b = 0; b < NT; ++b) xs.p[b] = x + (int64_t)min(t0 + 16 * b + (lane & 15), T - 1) * ldx;
   }
   if constexpr (MORE::whole && NT == 1) more.prepare(x, T, ldx, w.C, wave, waves, lds);
-  const bool staged = MODE == RQ_ANY && w.ngroups <= RQ_STAGED_GROUPS;
+  const bool staged = MODE == RQ_ANY && w.ngroups <= MORE::staged_groups;
   if (staged) {
     for (int a = 0; a < RT; ++a)
       rq_stage_scales(w, rq_tile_row<MORE::whole>(r0 + 16 * a, w.R), a, RT, threadIdx.x, blockDim.x, lds);
@@ -89,7 +90,7 @@ void launch_rows(const TX* x, int T, int64_t ldx, const RqPacked& w, const TX* b
   // 4096 39.2 -> 34.7 us.  (Without adapters the sums stay as they are.)
   if (MORE::whole && RT * NT >= 4 && bx * by > 256 && bx * by <= 512 && waves > 4) waves = 4;
   size_t lds = (size_t)waves * RT * NT * 1024;
-  if (MODE == RQ_ANY && w.ngroups <= RQ_STAGED_GROUPS) {
+  if (MODE == RQ_ANY && w.ngroups <= MORE::staged_groups) {
     const size_t scales = (size_t)(w.ngroups + 1) * 16 * RT * 4;
     lds = lds > scales ? lds : scales;
   }

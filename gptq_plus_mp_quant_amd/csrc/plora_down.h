@@ -15,7 +15,8 @@ __device__ __forceinline__ floatx4 rq_mfma32(floatx8 a, floatx8 b, floatx4 c) {
 
 // A workgroup takes 16 tokens, one of their adapters (the nth in the order of their first tokens) and 16 ranks of one
 // part of one of the jobs (z); its waves take steps of 32 columns in turn, four in flight, and are joined through LDS (64 for
-// each wave) in their order.
+// each wave) in their order.  Latency: a part of 2048 columns is one round of loads for 16 waves (one token of 4096
+// columns 4.8 us, 7.7 with parts of 4096 for 8 waves).
 template <typename TX, int WAVES>
 __device__ __forceinline__ void rq_lora_down_job(const RqDownJobs<TX>& jobs, int tile, int nth, int z, floatx4* join) {
   typedef typename RqOperand<TX>::raw Raw;

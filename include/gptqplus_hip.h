@@ -403,8 +403,8 @@ int rq_packed_moe(const void* x, int dtype, int T, int64_t ldx, int D, const voi
  * lora_a [n, r, C] and lora_b [n, R, r] of type dtype, contiguous, n <= 65535, r <= 256; adapter_ids [T]: the
  * adapter a of every token, none below 0, NaN results from n on; NULL: adapter 0 for all.  s_a =
  * scaling[a] (fp32 [n]) or, with scaling NULL, scale.  The rest as rq_packed_linear, T <= 2^19; A x is
- * fp32.  workspace: rq_packed_linear_lora_workspace_bytes(T, R, C, r, dtype) bytes, any contents
- * (NULL where that is 0). */
+ * fp32.  workspace: rq_packed_linear_lora_workspace_bytes(T, R, C, r, dtype) bytes, any contents,
+ * aligned to 16 bytes as those below (NULL where that is 0). */
 int64_t rq_packed_linear_lora_workspace_bytes(int T, int R, int C, int r, int dtype);
 int rq_packed_linear_lora(const void* x, int dtype, int T, int64_t ldx, int C, const uint32_t* qweight,
                           int64_t ldp, int nbits, int R, const float* scales, int64_t lds, int ngroups,

@@ -211,6 +211,16 @@ def test_two_tokens_with_an_adapter_each(groups, dtype):
     assert bool(torch.isnan(y[0]).all()) and bool(torch.isfinite(y[1]).all())
 
 
+@pytest.mark.parametrize("T", [1, 2, 3, 20])
+@pytest.mark.parametrize("size,C", [(8, 8056), (8, 8064), (8, 8184), (8, 8192), (8, 8400)])
+def test_as_many_groups_as_are_staged(size, C, T):
+    """Along an order, on both sides of the number of groups whose scales lie in LDS beside the low-rank values."""
+    entry, W = make_entry(C, 24, C, 4, f"order{size}")
+    x, gy, a, b, s, whose = case(T, T, 24, C, 16, 2, BF16)
+    y = formulas(x, gy, a, b, s, whose, W)[0]
+    within(packed_linear_lora(dev(x), on(entry, DEV), dev(a), dev(b), dev(whose), dev(s)), y, BF16, "y")
+
+
 @pytest.mark.parametrize("dtype", [F16, BF16, F32])
 def test_strides_and_views(dtype):
     R, C, r, n = 50, 260, 12, 3

@@ -103,7 +103,7 @@ def test_bits_and_groups(nbits, groups, dtype):
     check(*case(nbits, 9, 70, 777, 12, 3, dtype), entry, W)
 
 
-@pytest.mark.parametrize("T", [1, 5, 40])
+@pytest.mark.parametrize("T", [1, 5, 20, 40, 60, 260])
 def test_rows_shared_by_many_waves(T):
     """Every number of waves a workgroup and row tiles a wave, with fewer and more rank tiles than waves."""
     for R, C, r in ((8200, 64, 256), (4100, 700, 100), (40, 5000, 256), (40, 64, 33)):

@@ -161,6 +161,24 @@ def test_gradient_many_steps(T, dtype):
     check_grad(randn(T, T, 9000, dtype=dtype), pre_of(T, T, 9000), weights, "silu")
 
 
+@pytest.mark.parametrize("dtype", [F16, BF16, F32])
+@pytest.mark.parametrize("T", [3, 17, 32, 48, 50])
+@pytest.mark.parametrize("nbits", [4, 7])
+def test_many_rows(nbits, T, dtype):
+    """Two row tiles of each weight a wave, the last of them moved back; every number of token tiles."""
+    weights = pair(T, 16408, 200, (nbits,) * 2, ("channel", "channel"))
+    check(randn(T, T, 200, dtype=dtype), weights, "silu")
+
+
+@pytest.mark.parametrize("groups", [("128", "128"), ("32", "order32")])
+@pytest.mark.parametrize("T", [256, 257, 300, 600])
+def test_more_tokens_than_a_launch(T, groups):
+    dtype = (F16, BF16, F32)[T % 3]
+    weights = pair(T, 40, 300, (4, 4), groups)
+    check(randn(T, T, 300, dtype=dtype), weights, "gelu")
+    check_grad(randn(T + 1, T, 40, dtype=dtype), pre_of(T, T, 40), weights, "gelu")
+
+
 @pytest.mark.parametrize("groups", ["128", "32", "order32"])
 @pytest.mark.parametrize("dtype", [F16, BF16, F32])
 def test_non_finite_inputs_stay_in_their_row(dtype, groups):

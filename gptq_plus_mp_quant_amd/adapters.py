@@ -49,6 +49,13 @@ def _lora(lora_a, lora_b, ids, scaling, x, R, C, lead):
     return lora_a.contiguous(), lora_b.contiguous(), n, r, ids, scaling, scale
 
 
+def _needs_grad(*tensors):
+    for t in tensors:                                # a loop: any() over a generator takes three times as long
+        if getattr(t, "requires_grad", False):
+            return True
+    return False
+
+
 def _tokens_ok(T):
     if T > nat.RQ_MAX_TOKENS:
         raise ValueError(f"{T} tokens: at most {nat.RQ_MAX_TOKENS} in one call")
@@ -115,7 +122,7 @@ def packed_linear_lora(x: torch.Tensor, entry: Dict[str, object], lora_a: torch.
             raise ValueError("packed_linear_lora: the bias of a packed linear is a constant; detach it")
         if isinstance(scaling, torch.Tensor) and scaling.requires_grad:
             raise ValueError("scaling is constant and would get no gradient; detach it")
-        if any(getattr(t, "requires_grad", False) for t in (x, lora_a, lora_b)):
+        if _needs_grad(x, lora_a, lora_b):
             checked_entry(entry, 0)                  # under autograd; forward runs without
             return _PackedLinearLora.apply(x, lora_a, lora_b, entry, adapter_ids, scaling, bias)
     return _forward(x, entry, lora_a, lora_b, adapter_ids, scaling, bias)
@@ -140,7 +147,7 @@ def packed_linear_lora_backward(grad_y: torch.Tensor, x: torch.Tensor, entry: Di
     dtype; an adapter that no token has gets 0.  The results do not change from run to run.  They cannot be
     differentiated further."""
     nat.refuse_tangents("packed_linear_lora_backward", grad_y, x, lora_a, lora_b, scaling, entry["scales"])
-    if torch.is_grad_enabled() and any(getattr(t, "requires_grad", False) for t in (grad_y, x, lora_a, lora_b)):
+    if torch.is_grad_enabled() and _needs_grad(grad_y, x, lora_a, lora_b):
         checked_entry(entry, 0)
         return _PackedLinearLoraGrad.apply(grad_y, x, lora_a, lora_b, entry, adapter_ids, scaling)
     return _backward(grad_y, x, entry, lora_a, lora_b, adapter_ids, scaling)

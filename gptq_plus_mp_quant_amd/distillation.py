@@ -111,7 +111,8 @@ def distillation_loss_backward(logits: torch.Tensor, teacher_ids: torch.Tensor, 
     returned for the same arguments.  It cannot be differentiated further."""
     nat.refuse_tangents("distillation_loss_backward", logits, teacher_logprobs, stats, grad_loss)
     args = logits, teacher_ids, teacher_logprobs, stats, grad_loss, temperature, tail
-    if torch.is_grad_enabled() and any(getattr(t, "requires_grad", False) for t in (logits, stats, grad_loss)):
+    if torch.is_grad_enabled() and (getattr(logits, "requires_grad", False) or getattr(stats, "requires_grad", False) or
+                                    getattr(grad_loss, "requires_grad", False)):
         _checked(logits, teacher_ids, teacher_logprobs, temperature, tail)
         return _DistillationLossGrad.apply(*args)
     return _backward(*args)

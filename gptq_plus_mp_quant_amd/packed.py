@@ -170,11 +170,11 @@ def packed_linear_backward(grad_y: torch.Tensor, entry: Dict[str, object]) -> to
 def _pair(gate, up, name):
     """The checked tensors of gate and up, I and C."""
     g, u = checked_entry(gate, 0), checked_entry(up, 0)
-    if g[3:5] != u[3:5]:
+    if g[3] != u[3] or g[4] != u[4]:
         raise ValueError(f"{name}: gate and up must have one shape, got {g[3]} x {g[4]} and {u[3]} x {u[4]}")
     if g[0].get_device() != u[0].get_device():
         raise ValueError(f"{name}: gate and up are on different devices")
-    return (*((q, nbits, scales, ng, gi, gs) for q, nbits, scales, _, _, ng, gi, gs in (g, u)), g[3], g[4])
+    return (*g[:3], *g[5:]), (*u[:3], *u[5:]), g[3], g[4]
 
 
 def _activation(activation):
@@ -262,7 +262,7 @@ def packed_gated_backward(grad_h: torch.Tensor, pre: torch.Tensor, gate: Dict[st
     ``packed_gated(..., return_pre=True)`` returned beside it.  The result does not change from run to run.  It cannot be
     differentiated further."""
     nat.refuse_tangents("packed_gated_backward", grad_h, pre, gate["scales"], up["scales"])
-    if torch.is_grad_enabled() and any(getattr(t, "requires_grad", False) for t in (grad_h, pre)):
+    if torch.is_grad_enabled() and (getattr(grad_h, "requires_grad", False) or getattr(pre, "requires_grad", False)):
         _pair(gate, up, "packed_gated_backward")
         return _PackedGatedGrad.apply(grad_h, pre, gate, up, activation)
     return _gated_backward(grad_h, pre, gate, up, activation)

@@ -320,6 +320,46 @@ def test_in_a_graph(groups):
             assert torch.equal(got, want)
 
 
+def test_two_graphs_in_turn():
+    """A training step through the block and its adapter, captured twice for different numbers of tokens, the graphs
+    replayed in turn and between eager steps: neither's workspaces are the other's."""
+    g, u = (on(e, DEV) for e, _ in pair(8, 96, 512, (4, 4), ("128", "128")))
+    d = on(make_entry(9, 64, 96, 4, "channel")[0], DEV)
+    a, b = randn(3, 2, 8, 96, dtype=BF16, scale=0.1).to(DEV), randn(4, 2, 64, 8, dtype=BF16, scale=0.1).to(DEV)
+    leaves = [t.requires_grad_() for t in (a, b)]
+
+    def step(x, ids, gy):
+        y = packed_linear_lora(packed_gated(x, g, u), d, *leaves, ids)
+        return (y.detach(), *torch.autograd.grad(y, leaves, gy))
+
+    def inputs(seed, T):
+        return (randn(seed, T, 512, dtype=BF16, scale=0.1), torch.from_numpy(rng(seed).integers(-1, 2, T)), randn(seed + 1, T, 64, dtype=BF16))
+
+    states, graphs, outs = [], [], []
+    for T in (20, 40):
+        state = [t.to(DEV) for t in inputs(T, T)]
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            step(*state)
+        torch.cuda.current_stream().wait_stream(side)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = step(*state)
+        states.append(state), graphs.append(graph), outs.append(out)
+    for seed in range(3):
+        for state in states:
+            for t, new in zip(state, inputs(100 + 10 * seed, state[0].shape[0])):
+                t.copy_(new)
+        graphs[0].replay()
+        graphs[1].replay()
+        torch.cuda.synchronize()
+        for state, out in zip(states, outs):
+            for got, want in zip(out, step(*state)):
+                assert torch.equal(got, want)
+
+
 def test_refusals():
     (e, _), (f, _) = pair(1, 16, 64, (4, 4), ("32", "32"))
     g, u = on(e, DEV), on(f, DEV)

@@ -4,5 +4,5 @@
 
 void rq_cols_parts2(const float* dy, int T, int64_t ldy, int64_t plane, const RqPacked& w0, const RqPacked& w1, int nbits,
                     const RqColSplit& sp, float* part, hipStream_t s) {
-  cols_of<float, 2, true>(Cols<float>{dy, T, ldy, plane, &w1, sp, part, nullptr, 0, {}}, w0, nbits, s);
+  cols_of<float, 2>(Cols<float>{dy, T, ldy, plane, &w1, sp, part, {}}, w0, nbits, s);
 }

@@ -236,7 +236,9 @@ __device__ __forceinline__ void cols_runs(const TX* __restrict__ dy, int T, int6
   }
 }
 
-// The same with SMALL and ANY, where a scale multiplies the codes; infinities and NaN as the formula has them.
+// The same with SMALL and ANY, where a scale multiplies the codes, and with RUNS for packed_linear_backward, whose waves
+// have a few steps each, too few for the loads further ahead and the second pass of cols_runs to pay (64 tokens,
+// 4096 x 4096 4-bit bf16: 19.3 us for 21.0; 14336 x 4096 34.5 for 35.3).  Infinities and NaN as the formula has them.
 template <typename TX, int NB, int MODE, int NT>
 __device__ __forceinline__ void cols_scaled(const TX* __restrict__ dy, int T, int64_t ldy, const RqPacked& w, int t0, int first, int sb,
                                             floatx4 (&acc)[8][NT]) {
@@ -247,7 +249,8 @@ __device__ __forceinline__ void cols_scaled(const TX* __restrict__ dy, int T, in
   const ColLane<NB> l = col_lane<NB>(w);
   uint32_t g[8];
 #pragma unroll
-  for (int k = 0; k < 8; ++k) g[k] = (MODE == RQ_SMALL && k) ? g[0] : k < l.nc ? rq_group_of(w, l.c + k) : 0;
+  for (int k = 0; k < 8; ++k)
+    g[k] = MODE == RQ_RUNS ? rq_run_group(w, blockIdx.x * COLS) : (MODE == RQ_SMALL && k) ? g[0] : k < l.nc ? rq_group_of(w, l.c + k) : 0;
   const TX* tok[NT];
 #pragma unroll
   for (int b = 0; b < NT; ++b) tok[b] = dy + (int64_t)min(t0 + 16 * b + j, T - 1) * ldy;
@@ -277,18 +280,21 @@ __device__ __forceinline__ void cols_scaled(const TX* __restrict__ dy, int T, in
       } else {
         floatx8 v;
         fp32_of(f.dy[b], v);
+        if (MODE == RQ_RUNS) v *= f.sc * rq_unit<NB>();
         rq_operand<P::dy>(v, d[b]);
       }
     }
     // an inf's product with a piece of 0 would be a NaN that the formula does not have
     bf16x8 low[NT];
+    if constexpr (P::w > 1) {
 #pragma unroll
-    for (int b = 0; b < NT; ++b)
+      for (int b = 0; b < NT; ++b)
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const float v = (float)d[b][0][k];
-        low[b][k] = __builtin_fabsf(v) == INFINITY ? (__bf16)0.0f : d[b][0][k];
-      }
+        for (int k = 0; k < 8; ++k) {
+          const float v = (float)d[b][0][k];
+          low[b][k] = __builtin_fabsf(v) == INFINITY ? (__bf16)0.0f : d[b][0][k];
+        }
+    }
     uint32_t odd[8];
     col_fields<NB>(l.off, f.wd, odd);
 #pragma unroll
@@ -303,14 +309,18 @@ __device__ __forceinline__ void cols_scaled(const TX* __restrict__ dy, int T, in
           for (int k = 0; k < 8; ++k) sc[k] = FULL || r + k < w.R ? __builtin_nanf("") : 0.0f;
         }
       }
-      rq_operand<P::w>(sc * rq_unit<NB>() * codes, v);
+      if constexpr (P::w == 1) rq_convert(codes, v[0]);
+      else rq_operand<P::w>(sc * rq_unit<NB>() * codes, v);
 #pragma unroll
       for (int pd = 0; pd < P::dy; ++pd)
 #pragma unroll
         for (int pw = 0; pw < P::w; ++pw)
           if (pd + pw < PIECES_KEPT) {
 #pragma unroll
-            for (int b = 0; b < NT; ++b) acc[n][b] = rq_mfma(pd == 0 && pw ? low[b] : d[b][pd], v[pw], acc[n][b]);
+            for (int b = 0; b < NT; ++b) {
+              if constexpr (P::w > 1) acc[n][b] = rq_mfma(pd == 0 && pw ? low[b] : d[b][pd], v[pw], acc[n][b]);
+              else acc[n][b] = rq_mfma(d[b][pd], v[pw], acc[n][b]);
+            }
           }
     }
   };
@@ -385,13 +395,30 @@ __device__ __forceinline__ void cols_store(floatx4 (&acc)[8][NT], int y, int t0,
     }
 }
 
+// packed_linear_backward: grid (tiles of 128 columns, parts, tiles of 16 NT tokens).  A kernel of its own: the arguments of
+// the next one's jobs and second weight cost groups of 64 up to 3 % (one token, 4096 x 4096 4-bit bf16: 11.5 us for 11.9).
+template <typename TX, int NB, int MODE, int NT>
+__global__ __launch_bounds__(64 * cols_waves(NT), cols_occupancy(MODE, NT)) void k_linear_cols(
+    const TX* __restrict__ dy, int T, int64_t ldy, RqPacked w, int steps_per, float* __restrict__ part, TX* __restrict__ dx,
+    int64_t ldx) {
+  __shared__ floatx4 join[cols_waves(NT) / 2][8 * NT][64];
+  const int t0 = blockIdx.z * 16 * NT, nsteps = (w.R + STEP - 1) / STEP, sa = blockIdx.y * steps_per;
+  floatx4 acc[8][NT];
+#pragma unroll
+  for (int n = 0; n < 8; ++n)
+#pragma unroll
+    for (int b = 0; b < NT; ++b) acc[n][b] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+  cols_scaled<TX, NB, MODE, NT>(dy, T, ldy, w, t0, sa + rq_wave(), min(nsteps, sa + steps_per), acc);
+  cols_store<TX, NT>(acc, blockIdx.y, t0, T, w.C, part, dx, ldx, join);
+}
+
 // Grid (tiles of 128 columns, rows of jobs and then parts, tiles of 16 NT tokens).  The jobs (of packed linears with
 // adapters: what does not wait for this product) come first and spare a launch.  NM weights one after the other: dx = dy_0 W_0 + dy_1 W_1,
 // dy_1 lying `plane` elements behind dy_0, and a part is a range of the steps of all.
 template <typename TX, int NB, int MODE, int NT, int NM>
 __global__ __launch_bounds__(64 * cols_waves(NT), cols_occupancy(MODE, NT)) void k_packed_cols(
     const TX* __restrict__ dy, int T, int64_t ldy, int64_t plane, RqPacked w0, RqPacked w1, int steps_per, float* __restrict__ part,
-    TX* __restrict__ dx, int64_t ldx, RqDownJobs<TX> jobs, int job_rows) {
+    RqDownJobs<TX> jobs, int job_rows) {
   constexpr int W = cols_waves(NT);
   __shared__ floatx4 join[W / 2][8 * NT][64];
   const int y = (int)blockIdx.y - job_rows;
@@ -430,7 +457,7 @@ __global__ __launch_bounds__(64 * cols_waves(NT), cols_occupancy(MODE, NT)) void
         for (int k = 0; k < 4; k += 2) nan |= __builtin_isunordered(acc[n][b][k], acc[n][b][k + 1]);
     if (__any(nan)) run(std::true_type{});
   }
-  cols_store<TX, NT>(acc, y, t0, T, w0.C, part, dx, ldx, join);
+  cols_store<TX, NT>(acc, y, t0, T, w0.C, part, nullptr, 0, join);
 }
 
 template <typename TX>
@@ -443,7 +470,7 @@ __global__ __launch_bounds__(256) void k_packed_join(const float* __restrict__ p
   dx[(int64_t)t * ldx + c] = rq_cast<TX>(s);
 }
 
-// dy times one weight (w1 NULL) or two: T tokens to part [sp.parts, T, C] or, without, to dx.
+// dy times one weight (w1 NULL) or two: T tokens to part [sp.parts, T, C].
 template <typename TX>
 struct Cols {
   const TX* dy;
@@ -452,8 +479,6 @@ struct Cols {
   const RqPacked* w1;
   RqColSplit sp;
   float* part;
-  TX* dx;
-  int64_t ldx;
   RqDownJobs<TX> jobs;      // z = 0: none
 };
 template <typename TX, int NB, int MODE, int NT, int NM>
@@ -461,27 +486,28 @@ void launch_cols(const Cols<TX>& a, const RqPacked& w, hipStream_t s) {
   const int rows = a.jobs.z ? rq_jobs_rows(a.jobs, a.T, w.C) : 0;      // for tiles of 64 tokens: smaller ones leave some idle
   hipLaunchKernelGGL((k_packed_cols<TX, NB, MODE, NT, NM>),
                      dim3((w.C + COLS - 1) / COLS, rows + a.sp.parts, (a.T + 16 * NT - 1) / (16 * NT)), dim3(64 * cols_waves(NT)), 0, s,
-                     a.dy, a.T, a.ldy, a.plane, w, NM == 2 ? *a.w1 : w, a.sp.steps_per, a.part, a.dx, a.ldx, a.jobs, rows);
+                     a.dy, a.T, a.ldy, a.plane, w, NM == 2 ? *a.w1 : w, a.sp.steps_per, a.part, a.jobs, rows);
 }
-// WIDE: the caller joins the parts.
-template <typename TX, int NB, int MODE, int NM, bool WIDE>
-void linear_cols(const Cols<TX>& a, const RqPacked& w, hipStream_t s) {
-  // Where codes and fp32 tokens are both cut, registers are left for two token tiles; with RUNS four fit, which
-  // packed_linear_backward does not use: other waves would make other sums of what it has always returned.
-  constexpr int NT = RqOperand<TX>::pieces == 1 || (MODE == RQ_RUNS && WIDE) ? 4 : 2;
-  if (a.T <= 16) launch_cols<TX, NB, MODE, 1, NM>(a, w, s);
-  else if (a.T <= 32) launch_cols<TX, NB, MODE, 2, NM>(a, w, s);
-  else launch_cols<TX, NB, MODE, NT, NM>(a, w, s);
-}
-template <typename TX, int NM, bool WIDE>
-void cols_of(const Cols<TX>& a, const RqPacked& w, int nbits, hipStream_t s) {
+// The mode that serves a weight, as a constant, and its number of bits.
+template <typename F>
+void with_cols_mode(const RqPacked& w, int nbits, F&& f) {
   rq_with_nbits(nbits, [&](auto nb) {
-    constexpr int NB = decltype(nb)::value;
     switch (rq_cols_mode_of(w)) {
-      case RQ_RUNS: linear_cols<TX, NB, RQ_RUNS, NM, WIDE>(a, w, s); break;
-      case RQ_SMALL: linear_cols<TX, NB, RQ_SMALL, NM, WIDE>(a, w, s); break;
-      default: linear_cols<TX, NB, RQ_ANY, NM, WIDE>(a, w, s);
+      case RQ_RUNS: f(nb, std::integral_constant<int, RQ_RUNS>{}); break;
+      case RQ_SMALL: f(nb, std::integral_constant<int, RQ_SMALL>{}); break;
+      default: f(nb, std::integral_constant<int, RQ_ANY>{});
     }
+  });
+}
+template <typename TX, int NM>
+void cols_of(const Cols<TX>& a, const RqPacked& w, int nbits, hipStream_t s) {
+  with_cols_mode(w, nbits, [&](auto nb, auto mode) {
+    constexpr int NB = decltype(nb)::value, MODE = decltype(mode)::value;
+    // Where codes and fp32 tokens are both cut, registers are left for two token tiles; with RUNS four fit.
+    constexpr int NT = RqOperand<TX>::pieces == 1 || MODE == RQ_RUNS ? 4 : 2;
+    if (a.T <= 16) launch_cols<TX, NB, MODE, 1, NM>(a, w, s);
+    else if (a.T <= 32) launch_cols<TX, NB, MODE, 2, NM>(a, w, s);
+    else launch_cols<TX, NB, MODE, NT, NM>(a, w, s);
   });
 }
 
@@ -490,23 +516,34 @@ void cols_of(const Cols<TX>& a, const RqPacked& w, int nbits, hipStream_t s) {
 template <typename TX>
 void rq_cols_parts(const TX* dy, int T, int64_t ldy, const RqPacked& w, int nbits, const RqColSplit& sp, float* part,
                    hipStream_t s) {
-  cols_of<TX, 1, true>(Cols<TX>{dy, T, ldy, 0, nullptr, sp, part, nullptr, 0, {}}, w, nbits, s);
+  cols_of<TX, 1>(Cols<TX>{dy, T, ldy, 0, nullptr, sp, part, {}}, w, nbits, s);
 }
 template <typename TX>
 void rq_lora_cols(const TX* dy, int T, int64_t ldy, const RqPacked& w, int nbits, const RqColSplit& sp, float* part,
                   const RqDownJobs<TX>& jobs, hipStream_t s) {
-  cols_of<TX, 1, true>(Cols<TX>{dy, T, ldy, 0, nullptr, sp, part, nullptr, 0, jobs}, w, nbits, s);
+  cols_of<TX, 1>(Cols<TX>{dy, T, ldy, 0, nullptr, sp, part, jobs}, w, nbits, s);
 }
 
 template <typename TX>
 void rq_linear_cols(const TX* dy, int T, int64_t ldy, const RqPacked& w, int nbits, float* part, TX* dx, int64_t ldx,
                     hipStream_t s) {
-  for (int64_t t0 = 0; t0 < T; t0 += RQ_COL_TOKENS) {
-    const int n = (int)(T - t0 < RQ_COL_TOKENS ? T - t0 : RQ_COL_TOKENS);
-    const RqColSplit sp = rq_col_split(n, w.R, w.C);
-    TX* out = dx + t0 * ldx;
-    cols_of<TX, 1, false>(Cols<TX>{dy + t0 * ldy, n, ldy, 0, nullptr, sp, sp.parts > 1 ? part : nullptr, out, ldx, {}}, w, nbits, s);
-    if (sp.parts > 1)
-      hipLaunchKernelGGL(k_packed_join<TX>, dim3((w.C + 255) / 256, n), dim3(256), 0, s, part, sp.parts, n, w.C, out, ldx);
-  }
+  with_cols_mode(w, nbits, [&](auto nb, auto mode) {
+    for (int64_t t0 = 0; t0 < T; t0 += RQ_COL_TOKENS) {
+      const int n = (int)(T - t0 < RQ_COL_TOKENS ? T - t0 : RQ_COL_TOKENS);
+      const RqColSplit sp = rq_col_split(n, w.R, w.C);
+      TX* out = dx + t0 * ldx;
+      auto launch = [&](auto nt) {
+        constexpr int NT = decltype(nt)::value;
+        hipLaunchKernelGGL((k_linear_cols<TX, decltype(nb)::value, decltype(mode)::value, NT>),
+                           dim3((w.C + COLS - 1) / COLS, sp.parts, (n + 16 * NT - 1) / (16 * NT)), dim3(64 * cols_waves(NT)), 0, s,
+                           dy + t0 * ldy, n, ldy, w, sp.steps_per, sp.parts > 1 ? part : nullptr, out, ldx);
+      };
+      // fp32's pieces leave registers for two token tiles
+      if (n <= 16) launch(std::integral_constant<int, 1>{});
+      else if (n <= 32) launch(std::integral_constant<int, 2>{});
+      else launch(std::integral_constant<int, RqOperand<TX>::pieces == 1 ? 4 : 2>{});
+      if (sp.parts > 1)
+        hipLaunchKernelGGL(k_packed_join<TX>, dim3((w.C + 255) / 256, n), dim3(256), 0, s, part, sp.parts, n, w.C, out, ldx);
+    }
+  });
 }

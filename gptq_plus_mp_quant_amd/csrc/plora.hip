@@ -15,8 +15,6 @@ constexpr int TOKENS = 1 << 19;             // of one call: grids hold 65535 x 1
 bool lora_ok(const void* a, const void* b, int n, int r) { return a && b && n > 0 && n <= 65535 && r > 0 && r <= LORA_MAX_RANK; }
 // rank tiles times parts are a grid's third dimension, of both jobs together
 bool width_ok(int cols, int r) { return (int64_t)((r + 31) / 32 * 2) * ((cols - 1) / RQ_LORA_COLS + 1) <= 32767; }
-// workgroups for da and db
-bool outer_ok(int R, int C, int n, int r) { return ((int64_t)(C + 127) / 128 + (R + 127) / 128) * ((r + 15) / 16) * n <= 1 << 30; }
 
 struct GradSpace {
   int64_t u, v, part;                       // floats
@@ -78,7 +76,7 @@ extern "C" int rq_packed_linear_lora_grad(const void* grad_y, int dtype, int T, 
                                           int64_t workspace_bytes, void* stream) {
   const RqPacked w = rq_packed(qweight, ldp, scales, lds, g_idx, R, C, ngroups, groupsize);
   if (T < 0 || T > TOKENS || rq_packed_check(w, nbits) != RQ_OK || !lora_ok(lora_a, lora_b, n, r) || !width_ok(C, r) ||
-      !width_ok(R, r) || !outer_ok(R, C, n, r))
+      !width_ok(R, r))
     return RQ_EINVAL;
   if (!grad_a != !grad_b || (T && (!grad_y || !x || ldg < R || ldx < C || (grad_x && ldgx < C)))) return RQ_EINVAL;
   const GradSpace g = grad_space(T, R, C, r);

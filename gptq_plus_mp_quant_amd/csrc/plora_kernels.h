@@ -261,11 +261,11 @@ __device__ __forceinline__ void lora_dx(int block, const float* __restrict__ par
   }
 }
 
-// da and db.  Blocks (tiles of 128 columns of x, then of dy; rank tiles; adapters): the tokens of the adapter, four to a
+// da and db.  Blocks (tiles of 128 columns of x, then of dy; rank tiles; adapters from a0 on): the tokens of the adapter, four to a
 // matrix instruction, sixteen in flight, to the waves in turn.  Lane 16 q + i holds columns 8i..8i+7 of token q, and product n takes
 // the n-th of each, so that D's column i is column 8i + n.
 template <typename TX>
-__device__ __forceinline__ void lora_outer(int block, const TX* __restrict__ x, int64_t ldx, int C, const TX* __restrict__ dy,
+__device__ __forceinline__ void lora_outer(int block, int a0, const TX* __restrict__ x, int64_t ldx, int C, const TX* __restrict__ dy,
                                            int64_t ldy, int R, int T, const RqLora<TX>& lora, const RqLow& u, const RqLow& v,
                                            TX* __restrict__ da, TX* __restrict__ db, floatx4* lds) {
   typedef typename RqOperand<TX>::raw Raw;
@@ -273,7 +273,7 @@ __device__ __forceinline__ void lora_outer(int block, const TX* __restrict__ x, 
   __shared__ int count;
   const int lane = threadIdx.x & 63, wave = rq_wave(), i = lane & 15, q = lane >> 4;
   const int ctiles = (C + 127) / 128, tiles = ctiles + (R + 127) / 128, rtiles = (lora.r + 15) / 16;
-  const int tile = block % tiles, a = block / tiles / rtiles, rank = block / tiles % rtiles * 16;
+  const int tile = block % tiles, a = a0 + block / tiles / rtiles, rank = block / tiles % rtiles * 16;
   const bool of_a = tile < ctiles;                   // da: v with x; db: u with dy
   const int width = of_a ? C : R, col = (of_a ? tile : tile - ctiles) * 128 + 8 * i;
   const TX* src = of_a ? x : dy;
@@ -362,12 +362,12 @@ __device__ __forceinline__ void lora_outer(int block, const TX* __restrict__ x, 
 }
 
 template <typename TX>
-__global__ __launch_bounds__(64 * GRAD_WAVES, 4) void k_lora_grads(RqLoraDx<TX> g, int outer, const TX* x, int64_t ldx, int C,
+__global__ __launch_bounds__(64 * GRAD_WAVES, 4) void k_lora_grads(RqLoraDx<TX> g, int outer, int a0, const TX* x, int64_t ldx, int C,
                                                                  const TX* dy, int64_t ldy, int R, int T, RqLora<TX> lora, RqLow u,
                                                                  RqLow v, TX* da, TX* db) {
   __shared__ floatx4 lds[GRAD_WAVES * 8 * 64];
   if ((int)blockIdx.x >= outer) lora_dx<TX>(blockIdx.x - outer, g.part, g.parts, g.t0, g.T, C, lora, v, g.dx, g.ldx, lds);
-  else lora_outer<TX>(blockIdx.x, x, ldx, C, dy, ldy, R, T, lora, u, v, da, db, lds);
+  else lora_outer<TX>(blockIdx.x, a0, x, ldx, C, dy, ldy, R, T, lora, u, v, da, db, lds);
 }
 
 }  // namespace
@@ -390,9 +390,17 @@ void rq_lora_rows(const TX* x, int T, int64_t ldx, const RqPacked& w, int nbits,
 template <typename TX>
 void rq_lora_grads(const RqLoraDx<TX>& g, const TX* x, int64_t ldx, int C, const TX* dy, int64_t ldy, int R, int T,
                    const RqLora<TX>& lora, const RqLow& u, const RqLow& v, TX* da, TX* db, hipStream_t s) {
-  const int64_t ndx = g.dx ? (int64_t)((C + DX_COLS - 1) / DX_COLS) * ((g.T + 15) / 16) : 0;
-  const int64_t outer = da ? (int64_t)((C + 127) / 128 + (R + 127) / 128) * ((lora.r + 15) / 16) * lora.n : 0;
-  if (ndx + outer == 0) return;
-  hipLaunchKernelGGL(k_lora_grads<TX>, dim3((unsigned)(ndx + outer)), dim3(64 * GRAD_WAVES), 0, s, g, (int)outer, x, ldx, C, dy, ldy,
-                     R, T, lora, u, v, da, db);
+  // A launch holds fewer than 2^32 threads along a dimension: adapters past that go into further launches.  One adapter's
+  // workgroups, at most 2^20 (by width_ok), and dx's, at most 2^23 of 256 tokens, always fit.
+  constexpr int64_t MOST = ((1ll << 32) - 1) / (64 * GRAD_WAVES);
+  int64_t ndx = g.dx ? (int64_t)((C + DX_COLS - 1) / DX_COLS) * ((g.T + 15) / 16) : 0;
+  const int64_t each = da ? (int64_t)((C + 127) / 128 + (R + 127) / 128) * ((lora.r + 15) / 16) : 0;
+  const int n = da ? lora.n : 0;
+  for (int a0 = 0; ndx || a0 < n; ndx = 0) {
+    const int64_t fit = each ? (MOST - ndx) / each : 0;
+    const int adapters = (int)(fit < n - a0 ? fit : n - a0);
+    hipLaunchKernelGGL(k_lora_grads<TX>, dim3((unsigned)(ndx + adapters * each)), dim3(64 * GRAD_WAVES), 0, s, g, (int)(adapters * each),
+                       a0, x, ldx, C, dy, ldy, R, T, lora, u, v, da, db);
+    a0 += adapters;
+  }
 }

@@ -430,3 +430,26 @@ def test_results_can_be_edited_in_place(lead):
     plain = packed_linear_lora(x, e, a, b)
     plain += res
     assert torch.equal(y.detach(), plain) and y.shape == (*lead, 24) and leaf.grad.shape == x.shape
+
+
+def test_more_adapters_than_a_launch_holds():
+    """65535 adapters of 257 tiles are more workgroups than one launch takes (2^32 threads): those on both sides of the
+    cut, the first and the last, and all others 0 whatever they hold."""
+    n, R, C, used = 65535, 1, 32768, [0, 65278, 65279, 65534]
+    entry, W = make_entry(3, R, C, 4, "128")
+    e = on(entry, DEV)
+    x, gy, a, b, s, _ = case(5, 6, R, C, 1, 4, BF16)
+    whose = torch.tensor([2, 0, -1, 3, 1, 2])
+    y, gx, ga, gb = formulas(x, gy, a, b, s, whose, W)
+    many = torch.full((n, 1, C), float("nan"), dtype=BF16, device=DEV), torch.full((n, R, 1), float("nan"), dtype=BF16, device=DEV)
+    scaling = torch.full((n,), float("nan"), device=DEV)
+    for t, values in zip((*many, scaling), (a, b, s)):
+        t[used] = dev(values)
+    ids = torch.tensor([*used, -1])[whose].to(DEV)
+    within(packed_linear_lora(dev(x), e, *many, ids, scaling), y, BF16, "y")
+    got = packed_linear_lora_backward(dev(gy), dev(x), e, *many, ids, scaling)
+    within(got[0], gx, BF16, "gx")
+    for g, want in zip(got[1:], (ga, gb)):
+        within(g[used], want, BF16, "gradient")
+        g[used] = 0
+        assert not bool(g.any())

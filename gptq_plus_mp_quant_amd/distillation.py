@@ -62,11 +62,14 @@ class _DistillationLoss(torch.autograd.Function):
         ctx.save_for_backward(logits, ids, teacher, r.stats)
         ctx.how = temperature, tail
         ctx.mark_non_differentiable(r.stats)
+        ctx.set_materialize_grads(False)                 # or backward gets zeros of the statistics' size
         return tuple(r)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad_loss, _):
+        if grad_loss is None:
+            return None, None, None, None, None
         logits, ids, teacher, stats = ctx.saved_tensors
         return _backward(logits, ids, teacher, stats, grad_loss, *ctx.how), None, None, None, None
 

@@ -213,11 +213,14 @@ class _PackedGated(torch.autograd.Function):
         ctx.fields = [dict(nbits=e["nbits"], groupsize=e.get("groupsize", 0)) for e in (gate, up)]
         ctx.activation = activation
         ctx.mark_non_differentiable(pre)
+        ctx.set_materialize_grads(False)                 # or backward gets zeros of pre's size
         return h, pre
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad_h, _):
+        if grad_h is None:
+            return None, None, None, None
         pre, *weights = ctx.saved_tensors
         weights = ctx.unsaved or weights
         gate, up = (dict(zip(("qweight", "scales", "g_idx"), weights[3 * k:]), **f) for k, f in enumerate(ctx.fields))

@@ -5,7 +5,9 @@ import torch
 
 import gptq_plus_mp_quant_amd as G
 from gptq_plus_mp_quant_amd import _native as nat
+from gptq_plus_mp_quant_amd import distillation as D
 from gptq_plus_mp_quant_amd import kernels as K
+from gptq_plus_mp_quant_amd import packed as P
 from tests._packed import make_entry
 
 FAKE, NULL, MUCH = 16, None, 1 << 50
@@ -181,3 +183,43 @@ def test_autograd_checks_what_needs_a_gradient_on_any_device():
         G.packed_linear_lora(torch.zeros(1, 64, requires_grad=True), e, torch.zeros(1, 2, 64), torch.zeros(1, 16, 2))
     with pytest.raises(RuntimeError):
         G.distillation_loss(torch.zeros(2, 8, requires_grad=True), torch.zeros((2, 3), dtype=torch.int64), torch.zeros(2, 3))
+
+
+class _Drops(torch.autograd.Function):
+    """Passes on no gradient."""
+    @staticmethod
+    def forward(ctx, x):
+        return x.clone()
+
+    @staticmethod
+    def backward(ctx, g):
+        return None
+
+
+def _stand_ins(monkeypatch):
+    """The gated block and the loss with the launches left out, as (Function, arguments, leaf), and what their backward is given."""
+    e, seen = make_entry(0, 16, 64, 4, "32")[0], []
+    monkeypatch.setattr(P, "_gated", lambda x, *a: (x[:, :16].clone(), x.new_zeros((2, 2, 16))))
+    monkeypatch.setattr(P, "_gated_backward", lambda g, *a: g.new_ones((2, 64)))
+    monkeypatch.setattr(D, "_forward", lambda z, *a: D.Distillation(z.sum(-1), z.new_zeros((2, 8))))
+    monkeypatch.setattr(D, "_backward", lambda z, *a: torch.ones_like(z))
+    x, z = torch.zeros((2, 64), requires_grad=True), torch.zeros((2, 8), requires_grad=True)
+    ids, t = torch.zeros((2, 3), dtype=torch.int64), torch.zeros((2, 3))
+    for cls in (P._PackedGated, D._DistillationLoss):
+        def backward(ctx, *grads, real=cls.backward):
+            seen.append(grads)
+            return real(ctx, *grads)
+        monkeypatch.setattr(cls, "backward", staticmethod(backward))
+    return ((P._PackedGated, (x, e, e, "silu"), x), (D._DistillationLoss, (z, ids, t, 1.0, "bucket"), z)), seen
+
+
+def test_no_zeros_are_filled_for_what_takes_no_gradient(monkeypatch):
+    """pre and the statistics are results without a gradient: none is made for them on the way back, and none of the
+    input where the result's own is missing."""
+    cases, seen = _stand_ins(monkeypatch)
+    for fn, args, leaf in cases:
+        fn.apply(*args)[0].sum().backward()
+        assert seen[-1][0] is not None and seen[-1][1] is None and bool((leaf.grad == 1).all())
+        leaf.grad = None
+        _Drops.apply(fn.apply(*args)[0]).sum().backward()
+        assert leaf.grad is None

@@ -213,6 +213,18 @@ def refuse_tangents(what, *tensors):
             raise NotImplementedError(f"{what} has no forward-mode derivative: call it on tensors without tangents")
 
 
+def save_for_backward(ctx, *tensors):
+    """Tensors (or None) that a backward pass takes by saved_for_backward.  Autograd refuses to save those made in inference
+    mode; they cannot be changed outside of it and are kept as they are."""
+    kept = [t if t is not None and t.is_inference() else None for t in tensors]
+    ctx.save_for_backward(*(t if k is None else None for t, k in zip(tensors, kept)))
+    ctx.kept = kept
+
+
+def saved_for_backward(ctx):
+    return [t if k is None else k for t, k in zip(ctx.saved_tensors, ctx.kept)]
+
+
 DTYPE_CODES = {torch.float16: RQ_F16, torch.bfloat16: RQ_BF16, torch.float32: RQ_F32}
 
 

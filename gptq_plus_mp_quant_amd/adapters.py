@@ -84,10 +84,9 @@ class _PackedLinearLora(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, lora_a, lora_b, entry, ids, scaling, bias):
         y = _forward(x, entry, lora_a, lora_b, ids, scaling, bias)
-        # the tensors, not the dict, as packed_linear saves them; ones made in inference mode cannot be saved
-        fixed = entry["qweight"], entry["scales"], entry["g_idx"], ids, scaling if isinstance(scaling, torch.Tensor) else None
-        ctx.unsaved = fixed if any(t is not None and t.is_inference() for t in fixed) else None
-        ctx.save_for_backward(x, lora_a, lora_b, *(() if ctx.unsaved else fixed))
+        # the tensors, not the dict, as packed_linear saves them
+        nat.save_for_backward(ctx, x, lora_a, lora_b, entry["qweight"], entry["scales"], entry["g_idx"], ids,
+                              scaling if isinstance(scaling, torch.Tensor) else None)
         ctx.scaling = scaling if not isinstance(scaling, torch.Tensor) else None
         ctx.fields = dict(nbits=entry["nbits"], groupsize=entry.get("groupsize", 0))
         return y
@@ -95,8 +94,7 @@ class _PackedLinearLora(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, grad_y):
-        x, lora_a, lora_b, *fixed = ctx.saved_tensors
-        q, scales, g_idx, ids, scaling = ctx.unsaved or fixed
+        x, lora_a, lora_b, q, scales, g_idx, ids, scaling = nat.saved_for_backward(ctx)
         need = ctx.needs_input_grad
         gx, ga, gb = _backward(grad_y, x, dict(qweight=q, scales=scales, g_idx=g_idx, **ctx.fields), lora_a, lora_b, ids,
                                ctx.scaling if scaling is None else scaling, need[0], need[1] or need[2])

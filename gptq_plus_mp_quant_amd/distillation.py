@@ -59,7 +59,7 @@ class _DistillationLoss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, ids, teacher, temperature, tail):
         r = _forward(logits, ids, teacher, temperature, tail)
-        ctx.save_for_backward(logits, ids, teacher, r.stats)
+        nat.save_for_backward(ctx, logits, ids, teacher, r.stats)
         ctx.how = temperature, tail
         ctx.mark_non_differentiable(r.stats)
         ctx.set_materialize_grads(False)                 # or backward gets zeros of the statistics' size
@@ -70,7 +70,7 @@ class _DistillationLoss(torch.autograd.Function):
     def backward(ctx, grad_loss, _):
         if grad_loss is None:
             return None, None, None, None, None
-        logits, ids, teacher, stats = ctx.saved_tensors
+        logits, ids, teacher, stats = nat.saved_for_backward(ctx)
         return _backward(logits, ids, teacher, stats, grad_loss, *ctx.how), None, None, None, None
 
 

@@ -5,6 +5,7 @@ import torch
 
 import gptq_plus_mp_quant_amd as G
 from gptq_plus_mp_quant_amd import _native as nat
+from gptq_plus_mp_quant_amd import adapters as A
 from gptq_plus_mp_quant_amd import distillation as D
 from gptq_plus_mp_quant_amd import kernels as K
 from gptq_plus_mp_quant_amd import packed as P
@@ -223,3 +224,28 @@ def test_no_zeros_are_filled_for_what_takes_no_gradient(monkeypatch):
         leaf.grad = None
         _Drops.apply(fn.apply(*args)[0]).sum().backward()
         assert leaf.grad is None
+
+
+def test_constants_made_in_inference_mode_have_a_backward_pass(monkeypatch):
+    """A teacher's list, a frozen part's activations, another's adapters: what needs no gradient may come from there, and
+    what is changed in place between the passes is still noticed."""
+    (_, (dist, (z, *_), _)), _ = _stand_ins(monkeypatch)
+    e = make_entry(0, 16, 64, 4, "32")[0]
+    monkeypatch.setattr(A, "_forward", lambda x, *a: x[:, :16] * 1)
+    monkeypatch.setattr(A, "_backward", lambda *a: (torch.ones(2, 64), torch.ones(1, 2, 64), torch.ones(1, 16, 2)))
+    with torch.inference_mode():
+        ids, t = torch.zeros((2, 3), dtype=torch.int64), torch.zeros((2, 3))
+        x, b, s = torch.zeros((2, 64)), torch.zeros((1, 16, 2)), torch.ones(1)
+        inferred = {k: v.clone() if isinstance(v, torch.Tensor) else v for k, v in e.items()}
+    dist.apply(z, ids, t, 1.0, "bucket")[0].sum().backward()
+    assert bool((z.grad == 1).all())
+    leaf = torch.zeros((1, 2, 64), requires_grad=True)
+    for entry in (e, inferred):
+        leaf.grad = None
+        A._PackedLinearLora.apply(x, leaf, b, entry, None, s, None).sum().backward()
+        assert bool((leaf.grad == 1).all())
+        y = A._PackedLinearLora.apply(x, leaf, b, entry, None, s, None).sum()
+        with torch.no_grad():
+            leaf.add_(1)
+        with pytest.raises(RuntimeError):
+            y.backward()

@@ -453,3 +453,16 @@ def test_more_adapters_than_a_launch_holds():
         within(g[used], want, BF16, "gradient")
         g[used] = 0
         assert not bool(g.any())
+
+
+def test_constants_made_in_inference_mode():
+    """A frozen part's activations and half an adapter from there: the other half is trained as ever."""
+    entry, _ = make_entry(3, 32, 64, 4, "32")
+    e = on(entry, DEV)
+    x, gy, a, b, s, whose = (dev(t) for t in case(1, 4, 32, 64, 4, 3, F32))
+    want = packed_linear_lora_backward(gy, x, e, a, b, whose, s)
+    with torch.inference_mode():
+        xi, ai, bi = x.clone(), a.clone(), b.clone()
+    for args, leaf, k in (((xi, e, a.clone().requires_grad_(), bi), 2, 1), ((xi, e, ai, b.clone().requires_grad_()), 3, 2),
+                          ((x.clone().requires_grad_(), e, ai, bi), 0, 0)):
+        assert torch.equal(torch.autograd.grad(packed_linear_lora(*args, whose, s), args[leaf], gy)[0], want[k])

@@ -420,3 +420,19 @@ def test_every_way_a_row_is_cut(N, V, tail, temperature):
     """One small workgroup, one large one, several and a join; rows that end on the borders between them."""
     z = randn(N + V, N, V, dtype=BF16, scale=2.0)
     check(z, *teacher(V, z, 70), temperature, tail, grad=N * V < 1 << 20)
+
+
+@pytest.mark.parametrize("tail,temperature", TAILS)
+def test_a_teacher_scored_in_inference_mode(tail, temperature):
+    """Its list trains a student as one from elsewhere does."""
+    z, best = randn(1, 6, 500).to(DEV), randn(2, 6, 500).to(DEV)
+    target = torch.zeros(6, dtype=torch.int64, device=DEV)
+    with torch.inference_mode():
+        scored = token_logprobs(best, target, top_k=9)
+    plain = token_logprobs(best, target, top_k=9)
+    grads = []
+    for r in (plain, scored):
+        leaf = z.clone().requires_grad_()
+        distillation_loss(leaf, r.top_ids, r.top_logprobs, temperature, tail).loss.sum().backward()
+        grads.append(leaf.grad)
+    assert scored.top_ids.is_inference() and torch.equal(*grads) and bool(grads[0].any())

@@ -466,3 +466,14 @@ def test_constants_made_in_inference_mode():
     for args, leaf, k in (((xi, e, a.clone().requires_grad_(), bi), 2, 1), ((xi, e, ai, b.clone().requires_grad_()), 3, 2),
                           ((x.clone().requires_grad_(), e, ai, bi), 0, 0)):
         assert torch.equal(torch.autograd.grad(packed_linear_lora(*args, whose, s), args[leaf], gy)[0], want[k])
+
+
+@pytest.mark.parametrize("T", [512, 513, 1100])
+def test_as_many_low_rank_products_as_ride_along(T):
+    """On both sides of the number of tokens from which the gradients' low-rank products get a launch of their own beside
+    dx (4096 rows of its grid), with dx in one launch of 256 tokens after the other: all three gradients, and dx alone."""
+    entry, W = make_entry(T, 64, 64, 4, "32")
+    x, gy, a, b, s, whose = case(T, T, 64, 64, 256, 16, BF16)
+    e, back = on(entry, DEV), check(x, gy, a, b, s, whose, entry, W)[1]
+    leaf = dev(x).requires_grad_()
+    assert torch.equal(torch.autograd.grad(packed_linear_lora(leaf, e, dev(a), dev(b), dev(whose), dev(s)), leaf, dev(gy))[0], back[0])

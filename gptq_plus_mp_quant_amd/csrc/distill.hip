@@ -9,8 +9,9 @@
 //   student's distribution over the others and F = q_rest mass - r (RENORMALISE: w = q, F = mass).
 // For q_rest listed tokens are left out of the sum, not subtracted from it, so that a small rest keeps its digits;
 // it has a maximum of its own for the same reason.  Terms with p = 0 are 0.  A row without entries, or without a logit
-// above -inf, has no gradient.  Differences from a maximum are formed first, in fp32; a lane's sums are fp32, what is joined
-// from them and the sums over the list, a few values a row, 64 bits.
+// above -inf, has no gradient.  Differences from a maximum are formed first, in fp32; a lane's sums are fp32.  They are
+// joined in 64 bits, as the sums over the list are, a few values a row; the sums that the parts of a cut row hand on are
+// rounded to fp32 in between, half a unit beside what the lanes' sums are off by, for half the bytes.
 // The rows are bound by the logits' bytes: 2048 x 128256 bf16 95 us, 5.5 TB/s; a few short ones by latency (3 x 32003 fp32, one
 // large workgroup each: 10.2 us; cut over several and joined by a second launch 4.9 + 5.6).  The gradient reads and writes them
 // once: 1024 x 128256 bf16 114 us, 4.6 TB/s, where a copy reaches 5.1.
@@ -264,7 +265,7 @@ __global__ __launch_bounds__(64) void k_distill_join(const TX* __restrict__ z, i
 // them.  z and dz may be the same memory: a thread reads what it writes first, and listed logits before anything is written.
 constexpr int THREADS = MAX_LIST, GRAD_COLS = 8 * THREADS * 4;
 
-template <typename TX, int TAIL>
+template <typename TX>
 __global__ __launch_bounds__(THREADS) void k_distill_grad(const TX* z, int64_t ldz, int V, Teacher h,
                                                           const float* __restrict__ stats, const float* __restrict__ gl,
                                                           TX* dz, int64_t ldd) {
@@ -404,11 +405,11 @@ extern "C" int rq_distill_loss_grad(const void* logits, int dtype, int64_t N, in
   if (!logits || !teacher_ids || !teacher_logprobs || !stats || !grad_loss || !grad_logits) return RQ_EINVAL;
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   const int rounds = (V + GRAD_COLS - 1) / GRAD_COLS, ny = rounds < 64 ? rounds : 64;
-  const bool known = with_tail(dtype, tail, [&](auto* ptr, auto of) {
+  const bool known = rq_with_dtype(dtype, [&](auto* ptr) {
     typedef typename std::remove_pointer<decltype(ptr)>::type TX;
     for (int64_t n = 0; n < N; n += RQ_ROWS_PER_LAUNCH) {
       const unsigned rows = (unsigned)(N - n < RQ_ROWS_PER_LAUNCH ? N - n : RQ_ROWS_PER_LAUNCH);
-      hipLaunchKernelGGL((k_distill_grad<TX, decltype(of)::value>), dim3(rows, ny), dim3(THREADS), 0, s, (const TX*)logits + n * ldz,
+      hipLaunchKernelGGL(k_distill_grad<TX>, dim3(rows, ny), dim3(THREADS), 0, s, (const TX*)logits + n * ldz,
                          ldz, V, teacher(teacher_ids + n * K, teacher_logprobs + n * K, K, temperature), stats + n * STATS,
                          grad_loss + n, (TX*)grad_logits + n * ldd, ldd);
     }

@@ -344,8 +344,9 @@ __device__ __forceinline__ void cols_scaled(const TX* __restrict__ dy, int T, in
   }
 }
 
-// The waves' sums, halved together, always in the same order, and stored: to part [parts, T, C] or, without parts, to dx.
-template <typename TX, int NT>
+// The waves' sums, halved together, always in the same order, and stored: to part [parts, T, C] or, without parts (PARTS:
+// there are), to dx.
+template <bool PARTS, typename TX, int NT>
 __device__ __forceinline__ void cols_store(floatx4 (&acc)[8][NT], int y, int t0, int T, int C, float* __restrict__ part,
                                            TX* __restrict__ dx, int64_t ldx, floatx4 (*join)[8 * NT][64]) {
   constexpr int W = cols_waves(NT);
@@ -378,7 +379,7 @@ __device__ __forceinline__ void cols_store(floatx4 (&acc)[8][NT], int y, int t0,
       floatx8 v;
 #pragma unroll
       for (int n = 0; n < 8; ++n) v[n] = acc[n][b][k];
-      if (part) {
+      if (PARTS || part) {
         float* to = part + ((int64_t)y * T + t) * C + c;
         if (nc >= 8) {
           __builtin_memcpy(to, &v, 32);
@@ -409,7 +410,7 @@ __global__ __launch_bounds__(64 * cols_waves(NT), cols_occupancy(MODE, NT)) void
 #pragma unroll
     for (int b = 0; b < NT; ++b) acc[n][b] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
   cols_scaled<TX, NB, MODE, NT>(dy, T, ldy, w, t0, sa + rq_wave(), min(nsteps, sa + steps_per), acc);
-  cols_store<TX, NT>(acc, blockIdx.y, t0, T, w.C, part, dx, ldx, join);
+  cols_store<false, TX, NT>(acc, blockIdx.y, t0, T, w.C, part, dx, ldx, join);
 }
 
 // Grid (tiles of 128 columns, rows of jobs and then parts, tiles of 16 NT tokens).  The jobs (of packed linears with
@@ -417,8 +418,8 @@ __global__ __launch_bounds__(64 * cols_waves(NT), cols_occupancy(MODE, NT)) void
 // dy_1 lying `plane` elements behind dy_0, and a part is a range of the steps of all.
 template <typename TX, int NB, int MODE, int NT, int NM>
 __global__ __launch_bounds__(64 * cols_waves(NT), cols_occupancy(MODE, NT)) void k_packed_cols(
-    const TX* __restrict__ dy, int T, int64_t ldy, int64_t plane, RqPacked w0, RqPacked w1, int steps_per, float* __restrict__ part,
-    RqDownJobs<TX> jobs, int job_rows) {
+    const TX* __restrict__ dy, int T, int64_t ldy, int64_t plane, RqPacked w0, RqPacked w1, RqDownJobs<TX> jobs,
+    int job_rows, int steps_per, float* __restrict__ part) {
   constexpr int W = cols_waves(NT);
   __shared__ floatx4 join[W / 2][8 * NT][64];
   const int y = (int)blockIdx.y - job_rows;
@@ -457,7 +458,7 @@ __global__ __launch_bounds__(64 * cols_waves(NT), cols_occupancy(MODE, NT)) void
         for (int k = 0; k < 4; k += 2) nan |= __builtin_isunordered(acc[n][b][k], acc[n][b][k + 1]);
     if (__any(nan)) run(std::true_type{});
   }
-  cols_store<TX, NT>(acc, y, t0, T, w0.C, part, nullptr, 0, join);
+  cols_store<true, TX, NT>(acc, y, t0, T, w0.C, part, nullptr, 0, join);
 }
 
 template <typename TX>
@@ -486,7 +487,7 @@ void launch_cols(const Cols<TX>& a, const RqPacked& w, hipStream_t s) {
   const int rows = a.jobs.z ? rq_jobs_rows(a.jobs, a.T, w.C) : 0;      // for tiles of 64 tokens: smaller ones leave some idle
   hipLaunchKernelGGL((k_packed_cols<TX, NB, MODE, NT, NM>),
                      dim3((w.C + COLS - 1) / COLS, rows + a.sp.parts, (a.T + 16 * NT - 1) / (16 * NT)), dim3(64 * cols_waves(NT)), 0, s,
-                     a.dy, a.T, a.ldy, a.plane, w, NM == 2 ? *a.w1 : w, a.sp.steps_per, a.part, a.jobs, rows);
+                     a.dy, a.T, a.ldy, a.plane, w, NM == 2 ? *a.w1 : w, a.jobs, rows, a.sp.steps_per, a.part);
 }
 // The mode that serves a weight, as a constant, and its number of bits.
 template <typename F>

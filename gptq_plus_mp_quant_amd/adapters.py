@@ -107,7 +107,7 @@ def packed_linear_lora(x: torch.Tensor, entry: Dict[str, object], lora_a: torch.
     """``packed_linear(x, entry, bias)`` with a low-rank adapter for every token: ``x [..., C]`` -> ``[..., R]``,
     ``W x + bias + s B (A x)``, in x's dtype (fp16, bf16 or fp32).
 
-    ``lora_a`` [n, r, C] and ``lora_b`` [n, R, r] (x's dtype; r up to 256) hold n adapters, ``adapter_ids`` [...] (int64) says
+    ``lora_a`` [n, r, C] and ``lora_b`` [n, R, r] (x's dtype; r up to 256, n up to 65535) hold n adapters, ``adapter_ids`` [...] (int64) says
     which is whose: a token with an id below 0 has none, one with an id from n on gets NaN.  Without ids there is one
     adapter (which may come as [r, C] and [R, r]) for all tokens.  ``scaling``: a number, or fp32 [n].
 

@@ -12,8 +12,9 @@ enum { GATED_BOTH = 0, GATED_GATE = 1, GATED_UP = 2 };
 // row tiles of gate and of up by the tokens they have loaded once, and are joined through LDS in their order.  GATE
 // and UP (weights of different bits or groups): one of the two, the gate's product goes by way of pre.
 // Bound by the weights' bytes and the path that brings them and the tokens to a CU.  Measured, 4-bit: 14336 x 4096 bf16, 1
-// token 18.8 us (3.3 TB/s), 28672 x 8192 fp16, 24 tokens 84.5 us (2.8 TB/s; of 100 us 27 went without the tokens' loads, 45 without
-// the words'); there 127 us with tokens as they lie, 97 with tokens laid out once (k_arrange, 5 us), codes to fp16 in 9 instructions and unguarded rows.
+// token 18.7 us (3.3 TB/s), 28672 x 8192 fp16, 24 tokens 84.7 us (2.8 TB/s).  With one row tile of each weight, a call there:
+// 127 us with tokens as they lie, 97 to 100 with tokens laid out once (k_arrange, 5 us), codes to fp16 in 9 instructions and
+// unguarded rows; of those 27 went without the tokens' loads, 45 without the words'.
 template <typename TX, int NB, int MODE, int NM, int NT, int RP, bool DIRECT>
 __global__ __launch_bounds__(rows_threads(2, NT)) void k_packed_gated(const TX* __restrict__ x, const void* __restrict__ xa, int T, int64_t ldx, RqPacked first,
                                                                       RqPacked second, int what, int act, bool staged,
@@ -106,12 +107,14 @@ void gated_of(const TX* x, void* xa, int T, int64_t ldx, const RqPacked& first, 
   };
   auto run = [&](auto nt, auto rp) { launch(nt, rp, std::false_type{}); };
   typedef std::integral_constant<int, 1> One;
-  // 14336 x 4096 4-bit bf16, 1 token: 19.0 us, 20.1 without
+  // 14336 x 4096 4-bit bf16, 1 / 4 tokens: 17.0 / 18.9 us a call, 18.6 / 20.3 without; 4096 x 4096 6.8 / 7.4 and 7.2 / 7.6.
   if constexpr (MODE == RQ_RUNS && NM == 2)
     if (T <= 4) return launch(One{}, One{}, std::true_type{});
   if (T <= 16) return run(One{}, One{});
   if constexpr (MODE == RQ_RUNS) {
-    // 28672 x 8192 4-bit fp16, 24 tokens: 97 us with one row tile of each weight a wave, 81 with two
+    // 4-bit fp16, 24 tokens, one row tile of each weight a wave and two, us a call on the same weights: 28672 x 8192 73.4 and
+    // 69.9, 20480 x 8192 53.6 and 51.7, 16384 x 8192 44.4 and 38.6.  With fewer rows it is how the workgroups fall on
+    // the CUs that decides: 14336 x 8192 43.3 and 38.9, 11008 x 8192 34.1 and 37.8, 14336 x 4096 (32 tokens) 24.2 and 25.3.
     if constexpr (NM == 2 && NT == 4)
       if (T <= 32 && first.R >= 16384) return run(std::integral_constant<int, 2>{}, std::integral_constant<int, 2>{});
     if (T <= 32) return run(std::integral_constant<int, 2>{}, One{});

@@ -14,9 +14,10 @@
 // Rows are split over workgroups until there are 512, whose sums a second launch joins in their order.
 // Measured: 4096 x 4096 5-bit fp16, 8 tokens 9.2 + 4.0 us, latency; 14336 x 4096 4-bit bf16, 64 tokens 33 + 5.4 us (30.6 with
 // two pieces): by the counters 13 us of vector issue, conversions of codes and of dy, and 9 us of matrix instructions
-// (7.5 GFLOP for each piece), overlapped in part by two waves a SIMD, and waits for the loads ahead.  128 tokens of 4096 x
-// 14336 in one launch 59 us, of which 40 are issue: on a SIMD 24 matrix instructions (480 cycles) and 96 vector ones (506)
-// of two waves take 739 together.  Two weights of 14336 x 4096 from fp32, 64 tokens: 50 us.
+// (7.5 GFLOP for each piece), overlapped in part by two waves a SIMD, and waits for the one step of loads that is ahead.
+// With the parts left to the caller, 128 tokens of 4096 x 14336 in one launch: 58 us (66 with an adapter's jobs), of which 40
+// are issue: on a SIMD 24 matrix instructions (480 cycles) and 96 vector ones (506) of two waves take 739 together.  Two
+// weights of 14336 x 4096 from fp32, 64 tokens: 50 us.
 #pragma once
 #include "packed_dot.h"
 #include "plora_down.h"

@@ -86,8 +86,9 @@ void launch_rows(const TX* x, int T, int64_t ldx, const RqPacked& w, const TX* b
                  hipStream_t s) {
   const int bx = (w.R + 16 * RT - 1) / (16 * RT), by = (T + 16 * NT - 1) / (16 * NT);
   int waves = waves_for(bx * by, (w.C + RQ_CHUNK - 1) / RQ_CHUNK, RT * NT, rows_threads(RT, NT) / 64);
-  // Workgroups of eight waves go one to a CU there, in two rounds; of four two to a CU, in one: adapters of 48 tokens, 14336 x
-  // 4096 39.2 -> 34.7 us.  (Without adapters the sums stay as they are.)
+  // Workgroups of eight waves go one to a CU there, in two rounds; of four two to a CU, in one: adapters of 24 / 48 / 64
+  // tokens, 14336 x 4096, 29.1 / 37.3 / 43.3 us a call with eight, 26.1 / 32.8 / 39.5 with four.  (Without adapters the
+  // sums stay as they are.)
   if (MORE::whole && RT * NT >= 4 && bx * by > 256 && bx * by <= 512 && waves > 4) waves = 4;
   size_t lds = (size_t)waves * RT * NT * 1024;
   if (MODE == RQ_ANY && w.ngroups <= MORE::staged_groups) {
@@ -116,7 +117,8 @@ void linear_rows(const TX* x, int T, int64_t ldx, const RqPacked& w, const TX* b
       else if (T <= 32 && w.R > 4096) launch_rows<TX, NB, RQ_RUNS, R2, 2>(x, T, ldx, w, bias, y, ldy, more, s);
       else if (T <= 32) launch_rows<TX, NB, RQ_RUNS, 1, 2>(x, T, ldx, w, bias, y, ldy, more, s);
       else if (MORE::whole && T <= 48) {
-        // Three token tiles, with adapters: 48 tokens of 14336 x 4096 46.9 us for 49.8 with four.
+        // Three token tiles, with adapters: 33 / 48 tokens of 14336 x 4096 29.8 / 32.8 us a call for 32.7 / 35.9 with four,
+        // 48 of 4096 x 4096 18.3 for 21.6.
         if constexpr (MORE::whole) {
           if (w.R > 4096) launch_rows<TX, NB, RQ_RUNS, R2, 3>(x, T, ldx, w, bias, y, ldy, more, s);
           else launch_rows<TX, NB, RQ_RUNS, 1, 3>(x, T, ldx, w, bias, y, ldy, more, s);

@@ -3,7 +3,7 @@
 // Bound, for few tokens, by the packed weight's bytes and by latency: what the adapters add is a few operations and a
 // launch.  Hence their products ride in the packed weight's launches, and what precedes them is one short launch (or
 // none).  Measured, 4-bit bf16: 48 tokens of 16 adapters of rank 32, 14336 x 4096, 5.8 + 28.2 us; one token, 4096 x 4096, rank 16,
-// 13.5 us; gradients of 128 tokens, 4096 x 14336, rank 64, 65.7 + 19.7 us, 7 tokens of 1026 x 1365 along an order 10.8 + 6.6.
+// 13.5 us; gradients of 128 tokens, 4096 x 14336, rank 64, 65.8 + 19.8 us, 7 tokens of 1026 x 1365 along an order 11.0 + 6.5.
 //
 // A tile is 16 tokens, as with the packed weight, and goes once over every adapter that one of them has: the matrix
 // cores' columns are tokens, so what another adapter makes of a token is dropped, not added as 0 (an adapter that holds an
@@ -56,8 +56,8 @@ __device__ __forceinline__ bf16x8 without_inf(bf16x8 v) {
 // s B u to the sums of a row tile: 32 ranks of an adapter at a time, dealt to the waves by adapter and rank alone, so that
 // a token's bits do not depend on its companions.  u goes in as three bf16 pieces (24 bits), B in as many as hold it; products of
 // pieces i and j with i + j > 2, at most 2^-22 of a term, are left out.  An inf's product with a piece of 0 would be a
-// NaN that the formula does not have: past a number's first piece the other side's infs are 0.  With fp32 matrix
-// instructions the 48 tokens above took 59.9 us where they took 49.9 with these, and 38 without adapters.
+// NaN that the formula does not have: past a number's first piece the other side's infs are 0.  Of the 28.2 us
+// above they take 10 (18.0 with no adapter for any token); as fp32 matrix instructions they took nearly twice as long.
 template <typename TX>
 struct RqLowRank {
   static constexpr bool arranged = true, whole = true;

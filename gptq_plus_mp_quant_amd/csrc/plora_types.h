@@ -78,8 +78,9 @@ inline int rq_jobs_rows(const RqDownJobs<TX>& jobs, int T, int C) {
   return rows <= 4096 ? (int)rows : 0;
 }
 // Whether the workgroups make u for themselves: one or two tokens, 16 ranks, and little enough of A for all of them
-// together (one token of 4096 x 4096 with 16 ranks: 13.0 us a call, 17.1 with a launch that makes u
-// first; on the GPU 13.7 for 11.8, which a host that launches in time would notice).
+// together.  One token of 4096 x 4096 with 16 ranks: 13.0 us a call, 17.1 with a launch that makes u first.  That is
+// the host's time: replayed in a graph it is 12.0 for 10.4, with few long rows more (2048 x 8192 19.7 for 13.0), and only for
+// small weights less (1024 x 1024 7.1 for 7.8).
 inline bool rq_lora_own(int T, int R, int C, int r, int bytes) {
   return T <= 2 && r <= 16 && (int64_t)((R + 15) / 16) * T * r * C * bytes <= 40 << 20;
 }
